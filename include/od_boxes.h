@@ -381,6 +381,37 @@ int od_preprocess_images(const float* const* images, const int32_t* image_h, con
                          const float* mean, const float* std, float* out, int32_t out_h, int32_t out_w, void* stream);
 
 /*
+ * Group norm with an activation on channels-last maps: the [GroupNorm, ReLU] pair between the convolutions of the head
+ * towers (torchvision's FCOS head; the RetinaNet head with norm_layer=partial(nn.GroupNorm, 32), reference
+ * retinanet_model.py:47-52), forward and backward.
+ *   x, y, dy, dx : [batch, pixels, channels] of element type dtype (OD_DTYPE_*), dense, channels contiguous (a
+ *                  channels_last [batch, channels, height, width] map is that memory); x is read twice: y must not
+ *                  overlap it, nor dx overlap x or dy
+ *   weight, bias : [channels] of element type param_dtype, either may be null (one, zero); groups divides channels
+ *   activation   : OD_ACT_*: identity, max(u, 0), u * sigmoid(u)
+ *   forward  -> y, and mean / rstd fp32 [batch, groups] for the backward pass
+ *   backward -> dx (may be null), dweight / dbias [channels] of param_dtype (either may be null)
+ * Arithmetic is fp32 with sums merged in a fixed order; 16-bit results are rounded once, to nearest even.
+ * Nothing is done for batch = 0 or pixels = 0 (dweight / dbias are then left as they are).
+ *   workspace: od_group_norm_act_workspace_bytes (0: shape outside the limits), 256-byte aligned, for both directions
+ */
+#define OD_ACT_NONE 0
+#define OD_ACT_RELU 1
+#define OD_ACT_SILU 2
+#define OD_MAX_NORM_CHANNELS 2048
+#define OD_MAX_NORM_PIXELS 2147483647
+#define OD_MAX_NORM_BATCH 65535
+size_t od_group_norm_act_workspace_bytes(int64_t batch, int64_t pixels, int32_t channels, int32_t groups);
+int od_group_norm_act_forward(const void* x, int32_t dtype, int64_t batch, int64_t pixels, int32_t channels,
+                              int32_t groups, const void* weight, const void* bias, int32_t param_dtype, float eps,
+                              int32_t activation, void* y, float* mean, float* rstd, void* workspace,
+                              size_t workspace_bytes, void* stream);
+int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int64_t batch, int64_t pixels,
+                               int32_t channels, int32_t groups, const void* weight, const void* bias,
+                               int32_t param_dtype, int32_t activation, const float* mean, const float* rstd, void* dx,
+                               void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Per-kernel timing aid.  No counterpart in the reference (it has no profiling hooks); used by
  * bench.py to measure a kernel's own duration on the stream it runs on.  od_profile_select makes the
  * library launch that kernel (or all kernels) with a start and a stop event that receive the dispatch's own
@@ -412,7 +443,11 @@ int od_preprocess_images(const float* const* images, const int32_t* image_h, con
 #define OD_KERNEL_PACK 19           /* od_pack_detections */
 #define OD_KERNEL_NMS_ORDER 20      /* od_batched_nms: global order of unsorted candidates */
 #define OD_KERNEL_PREDICT_TAIL 21   /* od_predict_tail */
-#define OD_KERNEL_COUNT 22
+#define OD_KERNEL_NORM_STATS 22     /* od_group_norm_act_forward: statistics of large maps */
+#define OD_KERNEL_NORM_APPLY 23     /* od_group_norm_act_forward: normalise + activation (small maps: all of it) */
+#define OD_KERNEL_NORM_BWD_SUMS 24  /* od_group_norm_act_backward: channel sums of large maps */
+#define OD_KERNEL_NORM_BWD_APPLY 25 /* od_group_norm_act_backward: gradient of the map (small maps: sums as well) */
+#define OD_KERNEL_COUNT 26
 int od_profile_select(int32_t kernel_id);
 /* Time only every `every`-th launch of a selected kernel (default 1): a timed launch costs the host tens of
  * microseconds, which a throughput measurement should not pay on every step. */

@@ -77,6 +77,11 @@ SIGNATURES = {
     "od_box_loss_backward": (c_int32, [_P, c_int32, c_int64, _P, c_int64, c_int64, _P, _P, _P, c_int32, c_int32, c_float,
                                        _P, c_float, c_float, _P, _P, _P, _P]),
     "od_preprocess_images": (c_int32, [_P, _P, _P, _P, _P, c_int32, c_int32, _P, _P, _P, c_int32, c_int32, _P]),
+    "od_group_norm_act_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32, c_int32]),
+    "od_group_norm_act_forward": (c_int32, [_P, c_int32, c_int64, c_int64, c_int32, c_int32, _P, _P, c_int32, c_float,
+                                            c_int32, _P, _P, _P, _P, c_size_t, _P]),
+    "od_group_norm_act_backward": (c_int32, [_P, _P, c_int32, c_int64, c_int64, c_int32, c_int32, _P, _P, c_int32, c_int32,
+                                             _P, _P, _P, _P, _P, _P, c_size_t, _P]),
     "od_match_restore_groups": (c_int32, [c_int32]),
     "od_profile_select": (c_int32, [c_int32]),
     "od_profile_stride": (c_int32, [c_int32]),
@@ -86,9 +91,12 @@ SIGNATURES = {
 PROFILE_OFF, PROFILE_ALL = -1, -2
 KERNEL_NAMES = ["anchor", "match_assign", "match_restore", "match_fcos", "box_iou", "matcher", "decode", "filter",
                 "select", "nms", "match_heavy", "match_init", "focal_fwd", "focal_bwd", "box_loss_fwd", "box_loss_bwd", "preprocess", "sample", "filter_redo",
-                "pack", "nms_order", "predict_tail"]
+                "pack", "nms_order", "predict_tail", "norm_stats", "norm_apply", "norm_bwd_sums", "norm_bwd_apply"]
 BOX_LOSS_L1, BOX_LOSS_SMOOTH_L1, BOX_LOSS_GIOU = 0, 1, 2
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
+OD_MAX_NORM_CHANNELS = 2048
+OD_MAX_NORM_BATCH = 65535
 LOSS_NORM_PER_IMAGE, LOSS_NORM_BATCH = 0, 1
 
 _lib = None

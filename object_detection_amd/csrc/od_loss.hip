@@ -18,6 +18,7 @@
 // and double across workgroups (deterministic: no atomics).
 #include "od_common.h"
 #include "../../include/od_boxes.h"
+#include "od_elem.h"
 
 namespace {
 
@@ -27,42 +28,6 @@ constexpr int LT = 256;                 // threads per workgroup
 constexpr int LPT = 16;                 // elements per thread (four 16-byte groups)
 constexpr int LCHUNK = LT * LPT;        // elements per workgroup
 
-typedef float vec4f __attribute__((ext_vector_type(4)));
-
-// Element types of the head outputs and of their gradients: fp32, or the 16-bit types a head produces under autocast
-// (the reference trains with use_amp, reference object_detection/configs/config_all.py:16, train.py:61).  All
-// arithmetic is fp32; a 16-bit gradient is rounded once, to nearest even.
-struct bf16_t { unsigned short bits; };
-template <typename T> struct Elem;
-template <> struct Elem<float> {
-    typedef vec4f V;
-    static __device__ __forceinline__ float to_float(float v) { return v; }
-    static __device__ __forceinline__ float from_float(float v) { return v; }
-    static __device__ __forceinline__ float4 unpack(V v) { return make_float4(v.x, v.y, v.z, v.w); }
-    static __device__ __forceinline__ V pack(float4 f) { V v; v.x = f.x; v.y = f.y; v.z = f.z; v.w = f.w; return v; }
-};
-template <> struct Elem<_Float16> {
-    typedef _Float16 V __attribute__((ext_vector_type(4)));
-    static __device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
-    static __device__ __forceinline__ _Float16 from_float(float v) { return (_Float16)v; }
-    static __device__ __forceinline__ float4 unpack(V v) { return make_float4((float)v.x, (float)v.y, (float)v.z, (float)v.w); }
-    static __device__ __forceinline__ V pack(float4 f) {
-        V v; v.x = (_Float16)f.x; v.y = (_Float16)f.y; v.z = (_Float16)f.z; v.w = (_Float16)f.w; return v;
-    }
-};
-template <> struct Elem<bf16_t> {
-    typedef unsigned short V __attribute__((ext_vector_type(4)));
-    static __device__ __forceinline__ float up(unsigned short h) { return u2f((uint32_t)h << 16); }
-    static __device__ __forceinline__ unsigned short down(float f) {
-        const uint32_t u = f2u(f);
-        if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)((u >> 16) | 0x40u);      // NaN stays NaN
-        return (unsigned short)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-    }
-    static __device__ __forceinline__ float to_float(bf16_t v) { return up(v.bits); }
-    static __device__ __forceinline__ bf16_t from_float(float v) { bf16_t r; r.bits = down(v); return r; }
-    static __device__ __forceinline__ float4 unpack(V v) { return make_float4(up(v.x), up(v.y), up(v.z), up(v.w)); }
-    static __device__ __forceinline__ V pack(float4 f) { V v; v.x = down(f.x); v.y = down(f.y); v.z = down(f.z); v.w = down(f.w); return v; }
-};
 template <typename T> constexpr uintptr_t vec_mask() { return 4 * sizeof(T) - 1; }   // alignment of a group of four
 
 struct FocalTerms {

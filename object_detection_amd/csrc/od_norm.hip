@@ -1,0 +1,796 @@
+// Group norm with an activation on channels-last maps, forward and backward: the [GroupNorm, ReLU] pair between the
+// convolutions of the head towers (reference object_detection/retinanet/retinanet_model.py:47-52 passes
+// partial(nn.GroupNorm, 32); torchvision's FCOS head has the same pair).
+//
+//   x, y: [batch, pixels, channels], channels contiguous;  a group is channels/groups neighbouring channels
+//   mean, rstd over the pixels * channels/groups values of one (image, group);  xhat = (x - mean) * rstd
+//   u = xhat * gamma + beta;  y = act(u), act = identity, max(u, 0) or u * sigmoid(u)
+//   backward, du = dy * act'(u):  dbeta_c = sum du,  dgamma_c = sum du * xhat  (over images and pixels),
+//   dx = rstd * (gamma du - mean_g(gamma du) - xhat * mean_g(gamma du * xhat))
+//
+// Both directions are HBM streams; the arithmetic is fp32 for every element type and a 16-bit result is rounded once.
+// A thread owns one 16-byte column vector (8 or 4 channels) and walks down the pixels, so a row of the map is read in
+// whole cache lines and the per-channel coefficients stay in registers.
+//
+// Statistics: a thread sums x - k and (x - k)^2 with k its own first value of the channel, which bounds what the
+// subtraction of the two sums can lose by the number of its pixels whatever the mean of the map is; everything above a
+// thread is merged as (count, mean, M2) in two passes, M2 = sum M2_i + n_i (mean_i - mean)^2.  Fixed order, no atomics.
+#include "od_common.h"
+#include "../../include/od_boxes.h"
+#include "od_elem.h"
+
+#pragma clang fp contract(fast)
+
+namespace {
+
+using namespace od;
+
+constexpr int NT = 256;                 // threads per workgroup
+constexpr int MAX_CHUNKS = 256;         // pixel chunks per image of the two-pass form
+
+struct NormShape {
+    long long batch, pixels;            // images, pixels per image
+    int channels, groups, per_group;    // per_group = channels / groups
+    int chunks;                         // workgroups per image (two-pass form)
+    long long chunk_pixels;
+    float eps;
+};
+
+// weight or bias of channel c in the parameters' own type; a missing table is the constant `none`
+__device__ __forceinline__ float param(const void* p, int dtype, int c, float none) {
+    if (!p) return none;
+    if (dtype == OD_DTYPE_F32) return ((const float*)p)[c];
+    if (dtype == OD_DTYPE_F16) return (float)((const _Float16*)p)[c];
+    return Elem<bf16_t>::to_float(((const bf16_t*)p)[c]);
+}
+__device__ __forceinline__ void store_param(void* p, int dtype, int c, float v) {
+    if (dtype == OD_DTYPE_F32) ((float*)p)[c] = v;
+    else if (dtype == OD_DTYPE_F16) ((_Float16*)p)[c] = (_Float16)v;
+    else ((bf16_t*)p)[c] = Elem<bf16_t>::from_float(v);
+}
+
+// 1 / (1 + exp(-u)) with the hardware exponential and reciprocal: relative error below 1e-6 for |u| < 16
+template <int ACT>
+__device__ __forceinline__ float act_value(float u) {
+    if (ACT == OD_ACT_RELU) return u < 0.0f ? 0.0f : u;              // NaN stays NaN
+    if (ACT == OD_ACT_SILU) return u * __builtin_amdgcn_rcpf(1.0f + __expf(-u));
+    return u;
+}
+// dy * act'(u)
+template <int ACT>
+__device__ __forceinline__ float act_grad(float u, float dy) {
+    if (ACT == OD_ACT_RELU) return u <= 0.0f ? 0.0f : dy;
+    if (ACT == OD_ACT_SILU) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-u));
+        return dy * s * (1.0f + u * (1.0f - s));
+    }
+    return dy;
+}
+
+// Threads of a workgroup laid over a window of `cols` column vectors: `width` of them side by side (all of them, or NT
+// at a time), NT / width pixel rows below each other; threads left over idle.
+struct Lay {
+    int width, rows, tx, ty;
+    bool active;
+    __device__ __forceinline__ explicit Lay(int cols) {
+        width = cols < NT ? cols : NT;
+        rows = NT / width;
+        tx = threadIdx.x % width;
+        ty = threadIdx.x / width;
+        active = ty < rows;
+    }
+};
+
+// pixels that row ty of `rows` takes out of n: ty, ty + rows, ...
+__device__ __forceinline__ int taken(long long n, int ty, int rows) {
+    return ty < n ? (int)((n - ty + rows - 1) / rows) : 0;
+}
+
+// Statistics of channels [c0, c0 + nc) over `n` pixels at src (row stride `channels`), by the whole workgroup.
+// Leaves (mean, M2) of each channel in ch[0 .. nc).  red: 2 * NT * VEC floats.
+template <typename T, int VEC>
+__device__ __forceinline__ void channel_stats(const T* src, int channels, int c0, int nc, long long n, float2* ch,
+                                              float* red) {
+    const int cols = nc / VEC;
+    const Lay lay(cols);
+    for (int base = 0; base < cols; base += lay.width) {
+        const int col = base + lay.tx;
+        const bool on = lay.active && col < cols;
+        float k[VEC], s1[VEC], s2[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) k[i] = s1[i] = s2[i] = 0.0f;
+        const int mine = on ? taken(n, lay.ty, lay.rows) : 0;
+        if (mine > 0) {
+            const T* p = src + (long long)lay.ty * channels + c0 + col * VEC;
+            const long long step = (long long)lay.rows * channels;
+            load_vec<T, VEC>(p, k);
+            p += step;
+            int j = 1;
+            for (; j + 4 <= mine; j += 4) {             // four loads in flight
+                float v[4][VEC];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) load_vec<T, VEC>(p + q * step, v[q]);
+                p += 4 * step;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float d = v[q][i] - k[i];
+                        s1[i] += d;
+                        s2[i] = fmaf(d, d, s2[i]);
+                    }
+            }
+            for (; j < mine; ++j, p += step) {
+                float v[VEC];
+                load_vec<T, VEC>(p, v);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = v[i] - k[i];
+                    s1[i] += d;
+                    s2[i] = fmaf(d, d, s2[i]);
+                }
+            }
+        }
+        __syncthreads();                                // red may still be read for the previous columns
+        if (on) {
+            const float inv = mine > 0 ? 1.0f / (float)mine : 0.0f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float m = s1[i] * inv;
+                red[(lay.ty * lay.width + lay.tx) * VEC + i] = k[i] + m;
+                red[NT * VEC + (lay.ty * lay.width + lay.tx) * VEC + i] = s2[i] - s1[i] * m;
+            }
+        }
+        __syncthreads();
+        const int here = min(lay.width, cols - base) * VEC;              // channels of this window
+        for (int c = threadIdx.x; c < here; c += NT) {
+            float mean = 0.0f;
+            for (int r = 0; r < lay.rows; ++r)
+                mean += (float)taken(n, r, lay.rows) * red[r * lay.width * VEC + c];
+            mean /= (float)n;
+            float m2 = 0.0f;
+            for (int r = 0; r < lay.rows; ++r) {
+                const float cnt = (float)taken(n, r, lay.rows);
+                const float d = cnt > 0.0f ? red[r * lay.width * VEC + c] - mean : 0.0f;
+                m2 += red[NT * VEC + r * lay.width * VEC + c] + cnt * d * d;
+            }
+            ch[base * VEC + c] = make_float2(mean, m2);
+        }
+    }
+    __syncthreads();
+}
+
+// lanes that share one group of `per` values: the power of two not below it, at most a wave
+__device__ __forceinline__ int lanes_of(int per) {
+    int l = 1;
+    while (l < per && l < 64) l <<= 1;
+    return l;
+}
+__device__ __forceinline__ float lane_sum(float v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// (mean, M2) of group g over n pixels out of its channels' values ch[g * per ..); f(g, mean, M2) once per group
+template <typename F>
+__device__ __forceinline__ void merge_groups(const float2* ch, int groups, int per, long long n, F f) {
+    const int lanes = lanes_of(per);
+    const int at = threadIdx.x % lanes;
+    for (int g0 = 0; g0 < groups; g0 += NT / lanes) {
+        const int g = g0 + threadIdx.x / lanes;
+        float mean = 0.0f, m2 = 0.0f;
+        if (g < groups)
+            for (int c = at; c < per; c += lanes) mean += ch[g * per + c].x;
+        mean = lane_sum(mean, lanes) / (float)per;
+        if (g < groups)
+            for (int c = at; c < per; c += lanes) {
+                const float d = ch[g * per + c].x - mean;
+                m2 += ch[g * per + c].y + (float)n * d * d;
+            }
+        m2 = lane_sum(m2, lanes);
+        if (g < groups && at == 0) f(g, mean, m2);
+    }
+}
+
+// ---- two-pass form ------------------------------------------------------------------------------------------
+// part[(image * chunks + chunk) * groups + g] = (mean, M2) of the chunk
+template <typename T, int VEC>
+__global__ __launch_bounds__(NT) void norm_stats_kernel(NormShape s, const T* __restrict__ x, float2* __restrict__ part) {
+    extern __shared__ float smem[];
+    float* red = smem;
+    float2* ch = reinterpret_cast<float2*>(smem + 2 * NT * VEC);
+    const long long b = blockIdx.x / s.chunks;
+    const int chunk = blockIdx.x % s.chunks;
+    const long long p0 = chunk * s.chunk_pixels;
+    const long long n = min(s.chunk_pixels, s.pixels - p0);
+    channel_stats<T, VEC>(x + (b * s.pixels + p0) * s.channels, s.channels, 0, s.channels, n, ch, red);
+    float2* out = part + (long long)blockIdx.x * s.groups;
+    merge_groups(ch, s.groups, s.per_group, n, [&](int g, float mean, float m2) { out[g] = make_float2(mean, m2); });
+}
+
+// y of one window of channels and pixels; s_mean / s_rstd: per group, g counted from the window's first channel
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void apply_window(const NormShape& s, const T* src, T* dst, int c0, int nc, long long n,
+                                             const float* s_mean, const float* s_rstd, const void* weight,
+                                             const void* bias, int pdtype) {
+    const int cols = nc / VEC;
+    const Lay lay(cols);
+    for (int base = 0; base < cols; base += lay.width) {
+        const int col = base + lay.tx;
+        if (!lay.active || col >= cols) continue;
+        float mean[VEC], a[VEC], beta[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int c = col * VEC + i, g = c / s.per_group;
+            mean[i] = s_mean[g];
+            a[i] = s_rstd[g] * param(weight, pdtype, c0 + c, 1.0f);
+            beta[i] = param(bias, pdtype, c0 + c, 0.0f);
+        }
+        const int mine = taken(n, lay.ty, lay.rows);
+        const long long off = (long long)lay.ty * s.channels + c0 + col * VEC;
+        const long long step = (long long)lay.rows * s.channels;
+        const T* p = src + off;
+        T* q = dst + off;
+        int j = 0;
+        for (; j + 4 <= mine; j += 4) {
+            float v[4][VEC];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load_vec<T, VEC>(p + u * step, v[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[u][i] = act_value<ACT>(fmaf(v[u][i] - mean[i], a[i], beta[i]));
+                store_vec<T, VEC>(q + u * step, v[u]);
+            }
+            p += 4 * step;
+            q += 4 * step;
+        }
+        for (; j < mine; ++j, p += step, q += step) {
+            float v[VEC];
+            load_vec<T, VEC>(p, v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = act_value<ACT>(fmaf(v[i] - mean[i], a[i], beta[i]));
+            store_vec<T, VEC>(q, v);
+        }
+    }
+}
+
+// Every workgroup merges the chunks of its image again (at most 256 x groups pairs out of L2) instead of waiting for a
+// launch of its own that would do it once.
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(NT) void norm_apply_kernel(NormShape s, const T* __restrict__ x, T* __restrict__ y,
+                                                        const float2* __restrict__ part, const void* __restrict__ weight,
+                                                        const void* __restrict__ bias, int pdtype,
+                                                        float* __restrict__ mean_out, float* __restrict__ rstd_out) {
+    extern __shared__ float smem[];
+    float* s_mean = smem;
+    float* s_rstd = smem + s.groups;
+    float* red = smem + 2 * s.groups;                   // NT floats
+    const long long b = blockIdx.x / s.chunks;
+    const int chunk = blockIdx.x % s.chunks;
+    const float2* mine = part + b * s.chunks * s.groups;
+    const int slices = s.groups < NT ? NT / s.groups : 1;
+    const int slice = s.groups < NT ? threadIdx.x / s.groups : 0;
+    for (int g0 = 0; g0 < s.groups; g0 += NT) {         // one turn unless there are more groups than threads
+        const int g = s.groups < NT ? threadIdx.x % s.groups : g0 + threadIdx.x;
+        const bool on = slice < slices && g < s.groups;
+        float mean = 0.0f, m2 = 0.0f;
+        if (on)
+            for (int k = slice; k < s.chunks; k += slices)
+                mean += (float)min(s.chunk_pixels, s.pixels - k * s.chunk_pixels) * mine[k * s.groups + g].x;
+        __syncthreads();
+        red[threadIdx.x] = mean;
+        __syncthreads();
+        if (on) {
+            mean = 0.0f;
+            for (int r = 0; r < slices; ++r) mean += red[slices > 1 ? r * s.groups + g : threadIdx.x];
+            mean /= (float)s.pixels;
+            for (int k = slice; k < s.chunks; k += slices) {
+                const float2 v = mine[k * s.groups + g];
+                const float d = v.x - mean;
+                m2 += v.y + (float)(min(s.chunk_pixels, s.pixels - k * s.chunk_pixels) * s.per_group) * d * d;
+            }
+        }
+        __syncthreads();
+        red[threadIdx.x] = m2;
+        __syncthreads();
+        if (on && slice == 0) {
+            m2 = 0.0f;
+            for (int r = 0; r < slices; ++r) m2 += red[slices > 1 ? r * s.groups + g : threadIdx.x];
+            const float rstd = 1.0f / sqrtf(m2 / ((float)s.pixels * (float)s.per_group) + s.eps);
+            s_mean[g] = mean;
+            s_rstd[g] = rstd;
+            if (chunk == 0) {
+                mean_out[b * s.groups + g] = mean;
+                rstd_out[b * s.groups + g] = rstd;
+            }
+        }
+    }
+    __syncthreads();
+    const long long p0 = chunk * s.chunk_pixels;
+    const long long first = (b * s.pixels + p0) * s.channels;
+    apply_window<T, VEC, ACT>(s, x + first, y + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0), s_mean, s_rstd,
+                              weight, bias, pdtype);
+}
+
+// ---- one-launch form: a workgroup takes `slab` channels (whole groups) of one image over all its pixels -----------
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(NT) void norm_small_kernel(NormShape s, int slab, const T* __restrict__ x, T* __restrict__ y,
+                                                        const void* __restrict__ weight, const void* __restrict__ bias,
+                                                        int pdtype, float* __restrict__ mean_out,
+                                                        float* __restrict__ rstd_out) {
+    extern __shared__ float smem[];
+    float* red = smem;
+    float2* ch = reinterpret_cast<float2*>(smem + 2 * NT * VEC);
+    float* s_mean = smem + 2 * NT * VEC + 2 * slab;
+    float* s_rstd = s_mean + slab;                      // at most one group per channel
+    const int slabs = (s.channels + slab - 1) / slab;
+    const long long b = blockIdx.x / slabs;
+    const int c0 = (int)(blockIdx.x % slabs) * slab;
+    const int nc = min(slab, s.channels - c0);
+    const long long first = b * s.pixels * s.channels;
+    channel_stats<T, VEC>(x + first, s.channels, c0, nc, s.pixels, ch, red);
+    const long long g0 = b * s.groups + c0 / s.per_group;
+    merge_groups(ch, nc / s.per_group, s.per_group, s.pixels, [&](int g, float mean, float m2) {
+        const float rstd = 1.0f / sqrtf(m2 / ((float)s.pixels * (float)s.per_group) + s.eps);
+        s_mean[g] = mean;
+        s_rstd[g] = rstd;
+        mean_out[g0 + g] = mean;
+        rstd_out[g0 + g] = rstd;
+    });
+    __syncthreads();
+    apply_window<T, VEC, ACT>(s, x + first, y + first, c0, nc, s.pixels, s_mean, s_rstd, weight, bias, pdtype);
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------
+// Per-channel sums (du, du * xhat) of `n` pixels of channels [c0, c0 + nc); into out[0 .. nc).  red: 2 * NT * VEC floats.
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void channel_sums(const NormShape& s, const T* x, const T* dy, int c0, int nc, long long n,
+                                             const float* mean_b, const float* rstd_b, const void* weight,
+                                             const void* bias, int pdtype, float2* out, float* red) {
+    const int cols = nc / VEC;
+    const Lay lay(cols);
+    for (int base = 0; base < cols; base += lay.width) {
+        const int col = base + lay.tx;
+        const bool on = lay.active && col < cols;
+        float s1[VEC], s2[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = 0.0f;
+        if (on) {
+            float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int c = c0 + col * VEC + i, g = c / s.per_group;
+                mean[i] = mean_b[g];
+                rstd[i] = rstd_b[g];
+                gamma[i] = param(weight, pdtype, c, 1.0f);
+                beta[i] = param(bias, pdtype, c, 0.0f);
+            }
+            const int mine = taken(n, lay.ty, lay.rows);
+            const long long step = (long long)lay.rows * s.channels;
+            long long off = (long long)lay.ty * s.channels + c0 + col * VEC;
+            auto add = [&](const float* v, const float* g) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    const float d = v[i] - mean[i];
+                    // the forward's own expression, so that the mask of a rectified value is the forward's
+                    const float du = act_grad<ACT>(fmaf(d, rstd[i] * gamma[i], beta[i]), g[i]);
+                    s1[i] += du;
+                    s2[i] = fmaf(du, d * rstd[i], s2[i]);
+                }
+            };
+            int j = 0;
+            for (; j + 2 <= mine; j += 2, off += 2 * step) {
+                float v0[VEC], v1[VEC], g0[VEC], g1[VEC];
+                load_vec<T, VEC>(x + off, v0);
+                load_vec<T, VEC>(dy + off, g0);
+                load_vec<T, VEC>(x + off + step, v1);
+                load_vec<T, VEC>(dy + off + step, g1);
+                add(v0, g0);
+                add(v1, g1);
+            }
+            if (j < mine) {
+                float v0[VEC], g0[VEC];
+                load_vec<T, VEC>(x + off, v0);
+                load_vec<T, VEC>(dy + off, g0);
+                add(v0, g0);
+            }
+        }
+        __syncthreads();
+        if (on)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                red[(lay.ty * lay.width + lay.tx) * VEC + i] = s1[i];
+                red[NT * VEC + (lay.ty * lay.width + lay.tx) * VEC + i] = s2[i];
+            }
+        __syncthreads();
+        const int here = min(lay.width, cols - base) * VEC;
+        for (int c = threadIdx.x; c < here; c += NT) {
+            float a = 0.0f, q = 0.0f;
+            for (int r = 0; r < lay.rows; ++r) {
+                a += red[r * lay.width * VEC + c];
+                q += red[NT * VEC + r * lay.width * VEC + c];
+            }
+            out[base * VEC + c] = make_float2(a, q);
+        }
+    }
+}
+
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void grad_window(const NormShape& s, const T* x, const T* dy, T* dx, int c0, int nc, long long n,
+                                            const float* mean_b, const float* rstd_b, const float2* s_avg, int g_first,
+                                            const void* weight, const void* bias, int pdtype) {
+    const int cols = nc / VEC;
+    const Lay lay(cols);
+    for (int base = 0; base < cols; base += lay.width) {
+        const int col = base + lay.tx;
+        if (!lay.active || col >= cols) continue;
+        float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC], avg1[VEC], avg2[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int c = c0 + col * VEC + i, g = c / s.per_group;
+            mean[i] = mean_b[g];
+            rstd[i] = rstd_b[g];
+            gamma[i] = param(weight, pdtype, c, 1.0f);
+            beta[i] = param(bias, pdtype, c, 0.0f);
+            avg1[i] = s_avg[g - g_first].x;
+            avg2[i] = s_avg[g - g_first].y;
+        }
+        const int mine = taken(n, lay.ty, lay.rows);
+        const long long step = (long long)lay.rows * s.channels;
+        long long off = (long long)lay.ty * s.channels + c0 + col * VEC;
+        auto grad = [&](float* v, const float* g) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float d = v[i] - mean[i];
+                const float du = act_grad<ACT>(fmaf(d, rstd[i] * gamma[i], beta[i]), g[i]);
+                v[i] = rstd[i] * (fmaf(gamma[i], du, -avg1[i]) - d * rstd[i] * avg2[i]);
+            }
+        };
+        int j = 0;
+        for (; j + 2 <= mine; j += 2, off += 2 * step) {
+            float v0[VEC], v1[VEC], g0[VEC], g1[VEC];
+            load_vec<T, VEC>(x + off, v0);
+            load_vec<T, VEC>(dy + off, g0);
+            load_vec<T, VEC>(x + off + step, v1);
+            load_vec<T, VEC>(dy + off + step, g1);
+            grad(v0, g0);
+            store_vec<T, VEC>(dx + off, v0);
+            grad(v1, g1);
+            store_vec<T, VEC>(dx + off + step, v1);
+        }
+        if (j < mine) {
+            float v0[VEC], g0[VEC];
+            load_vec<T, VEC>(x + off, v0);
+            load_vec<T, VEC>(dy + off, g0);
+            grad(v0, g0);
+            store_vec<T, VEC>(dx + off, v0);
+        }
+    }
+}
+
+// group means of (gamma du, gamma du xhat) from the channel sums ch[0 .. groups * per)
+template <typename F>
+__device__ __forceinline__ void group_averages(const float2* ch, int groups, int per, int c0, double count,
+                                               const void* weight, int pdtype, F f) {
+    const int lanes = lanes_of(per);
+    const int at = threadIdx.x % lanes;
+    const float inv = (float)(1.0 / count);
+    for (int g0 = 0; g0 < groups; g0 += NT / lanes) {
+        const int g = g0 + threadIdx.x / lanes;
+        float a = 0.0f, q = 0.0f;
+        if (g < groups)
+            for (int c = at; c < per; c += lanes) {
+                const float w = param(weight, pdtype, c0 + g * per + c, 1.0f);
+                a += w * ch[g * per + c].x;
+                q += w * ch[g * per + c].y;
+            }
+        a = lane_sum(a, lanes);
+        q = lane_sum(q, lanes);
+        if (g < groups && at == 0) f(g, a * inv, q * inv);
+    }
+}
+
+// part[(image * chunks + chunk) * channels + c] = channel sums of the chunk
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(NT) void norm_bwd_sums_kernel(NormShape s, const T* __restrict__ x, const T* __restrict__ dy,
+                                                           const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                           const void* __restrict__ weight, const void* __restrict__ bias,
+                                                           int pdtype, float2* __restrict__ part) {
+    extern __shared__ float smem[];
+    const long long b = blockIdx.x / s.chunks;
+    const int chunk = blockIdx.x % s.chunks;
+    const long long p0 = chunk * s.chunk_pixels;
+    const long long first = (b * s.pixels + p0) * s.channels;
+    channel_sums<T, VEC, ACT>(s, x + first, dy + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0),
+                              mean + b * s.groups, rstd + b * s.groups, weight, bias, pdtype,
+                              part + (long long)blockIdx.x * s.channels, smem);
+}
+
+// sums[image * channels + c] = the chunks of one image joined.  A workgroup: 64 channels x 4 slices of the chunks.
+__global__ __launch_bounds__(NT) void norm_bwd_join_kernel(NormShape s, const float2* __restrict__ part,
+                                                           float2* __restrict__ sums) {
+    __shared__ float2 red[NT];
+    const int blocks = (s.channels + 63) / 64;
+    const long long b = blockIdx.x / blocks;
+    const int c = (int)(blockIdx.x % blocks) * 64 + (threadIdx.x & 63);
+    float2 v = make_float2(0.0f, 0.0f);
+    if (c < s.channels)
+        for (int k = threadIdx.x >> 6; k < s.chunks; k += NT / 64) {
+            const float2 t = part[(b * s.chunks + k) * s.channels + c];
+            v.x += t.x;
+            v.y += t.y;
+        }
+    red[threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.x < 64 && c < s.channels) {
+        for (int k = 1; k < NT / 64; ++k) {
+            v.x += red[k * 64 + threadIdx.x].x;
+            v.y += red[k * 64 + threadIdx.x].y;
+        }
+        sums[b * s.channels + c] = v;
+    }
+}
+
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(NT) void norm_bwd_apply_kernel(NormShape s, const T* __restrict__ x, const T* __restrict__ dy,
+                                                            T* __restrict__ dx, const float* __restrict__ mean,
+                                                            const float* __restrict__ rstd, const void* __restrict__ weight,
+                                                            const void* __restrict__ bias, int pdtype,
+                                                            const float2* __restrict__ sums) {
+    extern __shared__ float smem[];
+    float2* avg = reinterpret_cast<float2*>(smem);
+    const long long b = blockIdx.x / s.chunks;
+    const int chunk = blockIdx.x % s.chunks;
+    group_averages(sums + b * s.channels, s.groups, s.per_group, 0, (double)s.pixels * s.per_group, weight, pdtype,
+                   [&](int g, float a, float q) { avg[g] = make_float2(a, q); });
+    __syncthreads();
+    const long long p0 = chunk * s.chunk_pixels;
+    const long long first = (b * s.pixels + p0) * s.channels;
+    grad_window<T, VEC, ACT>(s, x + first, dy + first, dx + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0),
+                             mean + b * s.groups, rstd + b * s.groups, avg, 0, weight, bias, pdtype);
+}
+
+template <typename T, int VEC, int ACT>
+__global__ __launch_bounds__(NT) void norm_bwd_small_kernel(NormShape s, int slab, const T* __restrict__ x,
+                                                            const T* __restrict__ dy, T* __restrict__ dx,
+                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                            const void* __restrict__ weight, const void* __restrict__ bias,
+                                                            int pdtype, float2* __restrict__ sums) {
+    extern __shared__ float smem[];
+    float* red = smem;
+    float2* ch = reinterpret_cast<float2*>(smem + 2 * NT * VEC);
+    float2* avg = ch + slab;
+    const int slabs = (s.channels + slab - 1) / slab;
+    const long long b = blockIdx.x / slabs;
+    const int c0 = (int)(blockIdx.x % slabs) * slab;
+    const int nc = min(slab, s.channels - c0);
+    const long long first = b * s.pixels * s.channels;
+    channel_sums<T, VEC, ACT>(s, x + first, dy + first, c0, nc, s.pixels, mean + b * s.groups, rstd + b * s.groups, weight,
+                              bias, pdtype, ch, red);
+    __syncthreads();
+    for (int c = threadIdx.x; c < nc; c += NT) sums[b * s.channels + c0 + c] = ch[c];
+    if (dx) {
+        group_averages(ch, nc / s.per_group, s.per_group, c0, (double)s.pixels * s.per_group, weight, pdtype,
+                       [&](int g, float a, float q) { avg[g] = make_float2(a, q); });
+        __syncthreads();
+        grad_window<T, VEC, ACT>(s, x + first, dy + first, dx + first, c0, nc, s.pixels, mean + b * s.groups,
+                                 rstd + b * s.groups, avg, c0 / s.per_group, weight, bias, pdtype);
+    }
+}
+
+// dgamma, dbeta: the images' channel sums joined, 64 channels x 4 slices of the images a workgroup
+__global__ __launch_bounds__(NT) void norm_param_grads_kernel(long long batch, int channels, const float2* __restrict__ sums,
+                                                              void* __restrict__ dweight, void* __restrict__ dbias,
+                                                              int pdtype) {
+    __shared__ float2 red[NT];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63);
+    float2 v = make_float2(0.0f, 0.0f);
+    if (c < channels)
+        for (long long b = threadIdx.x >> 6; b < batch; b += NT / 64) {
+            const float2 t = sums[b * channels + c];
+            v.x += t.x;
+            v.y += t.y;
+        }
+    red[threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.x < 64 && c < channels) {
+        for (int k = 1; k < NT / 64; ++k) {
+            v.x += red[k * 64 + threadIdx.x].x;
+            v.y += red[k * 64 + threadIdx.x].y;
+        }
+        if (dbias) store_param(dbias, pdtype, c, v.x);
+        if (dweight) store_param(dweight, pdtype, c, v.y);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------
+int elem_size(int dtype) { return dtype == OD_DTYPE_F32 ? 4 : 2; }
+
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// channels per workgroup of the one-launch form: whole groups, whole vectors, at least 64 bytes of a row
+int slab_channels(int channels, int per_group, int vec, int size) {
+    const int unit = per_group / gcd(per_group, vec) * vec;
+    const int want = (64 / size + unit - 1) / unit * unit;
+    return want < channels ? want : channels;
+}
+
+// The one-launch form reads its slab twice, the second time out of the caches, with one workgroup per slab of an image.
+bool small_form(const NormShape& s, int slab, int size) {
+    return s.pixels * slab * size <= (64 << 10);
+}
+
+NormShape shape_of(long long batch, long long pixels, int channels, int groups, float eps) {
+    NormShape s;
+    s.batch = batch;
+    s.pixels = pixels;
+    s.channels = channels;
+    s.groups = groups;
+    s.per_group = channels / groups;
+    s.eps = eps;
+    // enough workgroups for 256 compute units several times over, at most MAX_CHUNKS per image, at least 16 pixels each
+    long long chunks = batch > 0 ? (2048 + batch - 1) / batch : 1;
+    if (chunks > MAX_CHUNKS) chunks = MAX_CHUNKS;
+    if (chunks > (pixels + 15) / 16) chunks = (pixels + 15) / 16;
+    if (chunks < 1) chunks = 1;
+    s.chunk_pixels = (pixels + chunks - 1) / chunks;
+    if (s.chunk_pixels < 1) s.chunk_pixels = 1;
+    s.chunks = (int)((pixels + s.chunk_pixels - 1) / s.chunk_pixels);
+    if (s.chunks < 1) s.chunks = 1;
+    return s;
+}
+
+int check_shape(int32_t dtype, int64_t batch, int64_t pixels, int32_t channels, int32_t groups, int32_t param_dtype,
+                int32_t activation) {
+    if (dtype < OD_DTYPE_F32 || dtype > OD_DTYPE_BF16 || param_dtype < OD_DTYPE_F32 || param_dtype > OD_DTYPE_BF16)
+        return OD_ERR_ARG;
+    if (activation < OD_ACT_NONE || activation > OD_ACT_SILU) return OD_ERR_ARG;
+    if (batch < 0 || pixels < 0 || channels <= 0 || groups <= 0 || channels % groups) return OD_ERR_ARG;
+    if (channels > OD_MAX_NORM_CHANNELS || pixels > OD_MAX_NORM_PIXELS || batch > OD_MAX_NORM_BATCH) return OD_ERR_LIMIT;
+    return OD_OK;
+}
+
+struct FwdCall {
+    NormShape s;
+    const void *x, *weight, *bias;
+    void* y;
+    int pdtype;
+    float *mean, *rstd;
+    void* ws;
+    hipStream_t stream;
+};
+
+template <typename T, int VEC, int ACT>
+int forward_typed(const FwdCall& c) {
+    const int slab = slab_channels(c.s.channels, c.s.per_group, VEC, sizeof(T));
+    const T* x = (const T*)c.x;
+    T* y = (T*)c.y;
+    if (small_form(c.s, slab, sizeof(T))) {
+        const long long grid = c.s.batch * ((c.s.channels + slab - 1) / slab);
+        const size_t lds = (2 * NT * VEC + 4 * (size_t)slab) * sizeof(float);
+        OD_LAUNCH_KERNEL(OD_KERNEL_NORM_APPLY, (norm_small_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT), lds, c.stream,
+                         c.s, slab, x, y, c.weight, c.bias, c.pdtype, c.mean, c.rstd);
+        return OD_OK;
+    }
+    float2* part = (float2*)c.ws;
+    const long long grid = c.s.batch * c.s.chunks;
+    OD_LAUNCH_KERNEL(OD_KERNEL_NORM_STATS, (norm_stats_kernel<T, VEC>), dim3((unsigned)grid), dim3(NT),
+                     (2 * NT * VEC + 2 * (size_t)c.s.channels) * sizeof(float), c.stream, c.s, x, part);
+    OD_LAUNCH_KERNEL(OD_KERNEL_NORM_APPLY, (norm_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
+                     (2 * (size_t)c.s.groups + NT) * sizeof(float), c.stream, c.s, x, y, (const float2*)part, c.weight, c.bias,
+                     c.pdtype, c.mean, c.rstd);
+    return OD_OK;
+}
+
+struct BwdCall {
+    NormShape s;
+    const void *x, *dy, *weight, *bias;
+    void *dx, *dweight, *dbias;
+    int pdtype;
+    const float *mean, *rstd;
+    void* ws;
+    hipStream_t stream;
+};
+
+template <typename T, int VEC, int ACT>
+int backward_typed(const BwdCall& c) {
+    const int slab = slab_channels(c.s.channels, c.s.per_group, VEC, sizeof(T));
+    const T *x = (const T*)c.x, *dy = (const T*)c.dy;
+    T* dx = (T*)c.dx;
+    float2* sums = (float2*)c.ws;
+    if (small_form(c.s, slab, sizeof(T))) {
+        const long long grid = c.s.batch * ((c.s.channels + slab - 1) / slab);
+        const size_t lds = (2 * NT * VEC + 4 * (size_t)slab) * sizeof(float);
+        OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_APPLY, (norm_bwd_small_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT), lds,
+                         c.stream, c.s, slab, x, dy, dx, c.mean, c.rstd, c.weight, c.bias, c.pdtype, sums);
+    } else {
+        float2* part = sums + c.s.batch * c.s.channels;
+        const long long grid = c.s.batch * c.s.chunks;
+        OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_SUMS, (norm_bwd_sums_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
+                         2 * NT * VEC * sizeof(float), c.stream, c.s, x, dy, c.mean, c.rstd, c.weight, c.bias, c.pdtype, part);
+        hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(c.s.batch * ((c.s.channels + 63) / 64))), dim3(NT), 0,
+                           c.stream, c.s, (const float2*)part, sums);
+        OD_LAUNCH_CHECK();
+        if (dx) {
+            OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_APPLY, (norm_bwd_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
+                             2 * (size_t)c.s.groups * sizeof(float), c.stream, c.s, x, dy, dx, c.mean, c.rstd, c.weight,
+                             c.bias, c.pdtype, (const float2*)sums);
+        }
+    }
+    if (c.dweight || c.dbias) {
+        hipLaunchKernelGGL(norm_param_grads_kernel, dim3((c.s.channels + 63) / 64), dim3(NT), 0, c.stream, c.s.batch,
+                           c.s.channels, (const float2*)sums, c.dweight, c.dbias, c.pdtype);
+        OD_LAUNCH_CHECK();
+    }
+    return OD_OK;
+}
+
+// The vector width follows from the channel count and the addresses; the activation and the type are compiled in.
+#define OD_NORM_DISPATCH(fn, call, aligned)                                                              \
+    do {                                                                                                 \
+        auto by_act = [&](auto vec, auto elem) -> int {                                                  \
+            using T = decltype(elem);                                                                    \
+            constexpr int V = decltype(vec)::value;                                                      \
+            if (activation == OD_ACT_RELU) return fn<T, V, OD_ACT_RELU>(call);                           \
+            if (activation == OD_ACT_SILU) return fn<T, V, OD_ACT_SILU>(call);                           \
+            return fn<T, V, OD_ACT_NONE>(call);                                                          \
+        };                                                                                               \
+        const int width_ = (aligned);                                                                    \
+        using V1 = std::integral_constant<int, 1>;                                                       \
+        using V4 = std::integral_constant<int, 4>;                                                       \
+        using V8 = std::integral_constant<int, 8>;                                                       \
+        if (dtype == OD_DTYPE_F32) return width_ >= 4 ? by_act(V4{}, float{}) : by_act(V1{}, float{});   \
+        if (dtype == OD_DTYPE_F16)                                                                       \
+            return width_ >= 8 ? by_act(V8{}, _Float16{}) : width_ >= 4 ? by_act(V4{}, _Float16{})       \
+                                                                        : by_act(V1{}, _Float16{});      \
+        return width_ >= 8 ? by_act(V8{}, bf16_t{}) : width_ >= 4 ? by_act(V4{}, bf16_t{})               \
+                                                                  : by_act(V1{}, bf16_t{});              \
+    } while (0)
+
+// elements per access: what divides the channel count and keeps every pointer aligned
+int vector_width(int dtype, int channels, uintptr_t addresses) {
+    const int size = elem_size(dtype);
+    for (int v = 16 / size; v >= 4; v /= 2)
+        if (channels % v == 0 && addresses % (uintptr_t)(v * size) == 0) return v;
+    return 1;
+}
+
+}  // namespace
+
+extern "C" size_t od_group_norm_act_workspace_bytes(int64_t batch, int64_t pixels, int32_t channels, int32_t groups) {
+    if (check_shape(OD_DTYPE_F32, batch, pixels, channels, groups, OD_DTYPE_F32, OD_ACT_NONE) != OD_OK) return 0;
+    const NormShape s = shape_of(batch, pixels, channels, groups, 0.0f);
+    return (size_t)(batch * (s.chunks + 1)) * channels * sizeof(float2) + 256;
+}
+
+extern "C" int od_group_norm_act_forward(const void* x, int32_t dtype, int64_t batch, int64_t pixels, int32_t channels,
+                                         int32_t groups, const void* weight, const void* bias, int32_t param_dtype,
+                                         float eps, int32_t activation, void* y, float* mean, float* rstd,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = check_shape(dtype, batch, pixels, channels, groups, param_dtype, activation);
+    if (rc != OD_OK) return rc;
+    if (batch == 0 || pixels == 0) return OD_OK;
+    if (!x || !y || !mean || !rstd || !workspace || ((uintptr_t)workspace & 255)) return OD_ERR_ARG;
+    if (((uintptr_t)x | (uintptr_t)y) % elem_size(dtype)) return OD_ERR_ARG;
+    if (workspace_bytes < od_group_norm_act_workspace_bytes(batch, pixels, channels, groups)) return OD_ERR_WORKSPACE;
+    const FwdCall call = {shape_of(batch, pixels, channels, groups, eps), x, weight, bias, y, param_dtype, mean, rstd,
+                          workspace, (hipStream_t)stream};
+    OD_NORM_DISPATCH(forward_typed, call, vector_width(dtype, channels, (uintptr_t)x | (uintptr_t)y));
+}
+
+extern "C" int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int64_t batch, int64_t pixels,
+                                          int32_t channels, int32_t groups, const void* weight, const void* bias,
+                                          int32_t param_dtype, int32_t activation, const float* mean, const float* rstd,
+                                          void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                                          void* stream) {
+    const int rc = check_shape(dtype, batch, pixels, channels, groups, param_dtype, activation);
+    if (rc != OD_OK) return rc;
+    if (batch == 0 || pixels == 0) return OD_OK;
+    if (!x || !dy || !mean || !rstd || !workspace || ((uintptr_t)workspace & 255)) return OD_ERR_ARG;
+    if (((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx) % elem_size(dtype)) return OD_ERR_ARG;
+    if (workspace_bytes < od_group_norm_act_workspace_bytes(batch, pixels, channels, groups)) return OD_ERR_WORKSPACE;
+    const BwdCall call = {shape_of(batch, pixels, channels, groups, 0.0f), x, dy, weight, bias, dx, dweight, dbias,
+                          param_dtype, mean, rstd, workspace, (hipStream_t)stream};
+    OD_NORM_DISPATCH(backward_typed, call, vector_width(dtype, channels, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx));
+}

@@ -14,6 +14,7 @@ from torch import Tensor, nn
 
 from . import _C, det_utils, kernels
 from .anchor_utils import AnchorGenerator
+from .norm import activates
 from .retinanet import _to_anchor_major, postprocess_batched
 from .transform import GeneralizedRCNNTransform
 
@@ -21,7 +22,8 @@ from .transform import GeneralizedRCNNTransform
 def _gn_tower(in_channels: int, num_convs: int, norm_layer) -> nn.Sequential:
     layers: List[nn.Module] = []
     for _ in range(num_convs):
-        layers += [nn.Conv2d(in_channels, in_channels, 3, 1, 1), norm_layer(in_channels), nn.ReLU()]
+        layers += [nn.Conv2d(in_channels, in_channels, 3, 1, 1), norm_layer(in_channels)]
+        layers.append(nn.Identity() if activates(layers[-1]) else nn.ReLU())     # same keys either way
     tower = nn.Sequential(*layers)
     for m in tower.modules():
         if isinstance(m, nn.Conv2d):
@@ -73,11 +75,12 @@ class FCOSRegressionHead(nn.Module):
 
 
 class FCOSHead(nn.Module):
-    def __init__(self, in_channels, num_anchors, num_classes, num_convs: Optional[int] = 4):
+    def __init__(self, in_channels, num_anchors, num_classes, num_convs: Optional[int] = 4, norm_layer=None):
         super().__init__()
         self.box_coder = det_utils.BoxLinearCoder(normalize_by_size=True)
-        self.classification_head = FCOSClassificationHead(in_channels, num_anchors, num_classes, num_convs)
-        self.regression_head = FCOSRegressionHead(in_channels, num_anchors, num_convs)
+        self.classification_head = FCOSClassificationHead(in_channels, num_anchors, num_classes, num_convs,
+                                                          norm_layer=norm_layer)
+        self.regression_head = FCOSRegressionHead(in_channels, num_anchors, num_convs, norm_layer=norm_layer)
 
     def compute_loss(self, targets, head_outputs, anchors, matched_idxs) -> Dict[str, Tensor]:
         cls_logits = head_outputs["cls_logits"]

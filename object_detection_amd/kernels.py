@@ -6,6 +6,7 @@ a GPU; none of them has a CPU implementation.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Dict, Optional, Sequence, Tuple
 
@@ -45,6 +46,13 @@ def _raw_stream(device: torch.device) -> int:
 
 def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(_raw_stream(device))
+
+
+def _on(device: torch.device):
+    """Makes ``device`` the current one for a launch (a stream belongs to its device); free where it already is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _ptr(t: Optional[Tensor]) -> ctypes.c_void_p:
@@ -714,3 +722,88 @@ def fcos_box_loss_backward(bbox_regression: Tensor, bbox_ctrness: Tensor, anchor
                                             _ptr(grad_ctr), _stream(dev))
     _C.check(rc, "od_fcos_box_loss_backward")
     return grad_reg, grad_ctr
+
+
+# ------------------------------------------------------------------------------------------------
+# Scratch of the calls below comes from torch's allocator call by call: it is ordered with the stream the call runs on,
+# and a call recorded into a HIP graph holds memory of that graph's own pool -- two graphs never share it.
+def _norm_args(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor]):
+    """Checks of group_norm_act_*; returns (element code, parameter code)."""
+    _require_gpu(x, "x")
+    if x.dim() != 3 or not x.is_contiguous():
+        raise ValueError(f"group_norm_act: x must be contiguous [batch, pixels, channels], got {tuple(x.shape)}")
+    C = int(x.shape[2])
+    if num_groups < 1 or C < 1 or C % num_groups:
+        raise ValueError(f"group_norm_act: {C} channels cannot be divided into {num_groups} groups")
+    pcode = _C.DTYPE_F32
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if tuple(p.shape) != (C,):
+            raise ValueError(f"group_norm_act: {name} must be [{C}], got {tuple(p.shape)}")
+        if p.device != x.device:
+            raise RuntimeError(f"group_norm_act: {name} is on {p.device}, x on {x.device}")
+        pcode = _dtype_code(p, f"group_norm_act: {name}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"group_norm_act: weight is {weight.dtype}, bias {bias.dtype}")
+    return _dtype_code(x, "group_norm_act: x"), pcode
+
+
+def _norm_workspace(x: Tensor, num_groups: int) -> Tensor:
+    B, P, C = x.shape
+    key = ("norm", B, P, C, num_groups)
+    nbytes = _ws_bytes.get(key)
+    if nbytes is None:
+        nbytes = _C.lib().od_group_norm_act_workspace_bytes(B, P, C, num_groups)
+        if nbytes == 0:
+            raise _C.OdBoxesError(f"od_group_norm_act: batch {B}, {C} channels exceed the limits of "
+                                  f"{_C.OD_MAX_NORM_BATCH} images and {_C.OD_MAX_NORM_CHANNELS} channels")
+        if len(_ws_bytes) > 65536:
+            _ws_bytes.clear()
+        _ws_bytes[key] = nbytes
+    return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+
+
+def group_norm_act_forward(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                           activation: int) -> Tuple[Tensor, Tensor, Tensor]:
+    """Group norm + activation of channels-last rows x [B, P, C] fp32 / fp16 / bf16; weight / bias [C] (one type, fp32 or
+    16-bit) or None.  Returns (y [B, P, C], mean [B, G], rstd [B, G])."""
+    code, pcode = _norm_args(x, num_groups, weight, bias)
+    B, P, C = x.shape
+    ws = _norm_workspace(x, num_groups)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    y = torch.empty_like(x)
+    mean = torch.empty((B, num_groups), dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    with _on(x.device):
+        rc = _C.lib().od_group_norm_act_forward(_ptr(x), code, B, P, C, int(num_groups), _ptr(weight), _ptr(bias), pcode,
+                                                float(eps), int(activation), _ptr(y), _ptr(mean), _ptr(rstd), _ptr(ws),
+                                                ws.numel(), _stream(x.device))
+    _C.check(rc, "od_group_norm_act_forward")
+    return y, mean, rstd
+
+
+def group_norm_act_backward(x: Tensor, dy: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor],
+                            activation: int, mean: Tensor, rstd: Tensor, want_dx: bool = True, want_dweight: bool = True,
+                            want_dbias: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """Gradients of group_norm_act_forward: (dx [B, P, C], dweight [C], dbias [C]); None for what is not wanted or not
+    there."""
+    code, pcode = _norm_args(x, num_groups, weight, bias)
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device or not dy.is_contiguous():
+        raise ValueError(f"group_norm_act: dy must be contiguous {x.dtype} {tuple(x.shape)} on {x.device}, got {dy.dtype} "
+                         f"{tuple(dy.shape)} on {dy.device}")
+    B, P, C = x.shape
+    ws = _norm_workspace(x, num_groups)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    fresh = torch.zeros_like if x.numel() == 0 else torch.empty_like      # no launch fills the sums of an empty map
+    dx = torch.empty_like(x) if want_dx else None
+    dweight = fresh(weight) if want_dweight and weight is not None else None
+    dbias = fresh(bias) if want_dbias and bias is not None else None
+    with _on(x.device):
+        rc = _C.lib().od_group_norm_act_backward(_ptr(x), _ptr(dy), code, B, P, C, int(num_groups), _ptr(weight), _ptr(bias),
+                                                 pcode, int(activation), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight),
+                                                 _ptr(dbias), _ptr(ws), ws.numel(), _stream(x.device))
+    _C.check(rc, "od_group_norm_act_backward")
+    return dx, dweight, dbias

@@ -20,7 +20,7 @@ from typing import Callable, Dict, List, Optional, Tuple
 import torch
 from torch import Tensor, nn
 
-from . import _C, boxes as box_ops, det_utils, kernels
+from . import _C, boxes as box_ops, det_utils, kernels, norm
 from .anchor_utils import AnchorGenerator
 from .transform import GeneralizedRCNNTransform
 
@@ -33,7 +33,8 @@ def _conv_tower(in_channels: int, norm_layer: Optional[Callable[..., nn.Module]]
         layers: List[nn.Module] = [nn.Conv2d(in_channels, in_channels, 3, 1, 1, bias=norm_layer is None)]
         if norm_layer is not None:
             layers.append(norm_layer(in_channels))
-        layers.append(nn.ReLU(inplace=True))
+        # a norm layer that activates by itself leaves the ReLU's place empty: the keys stay the same
+        layers.append(nn.Identity() if norm.activates(layers[-1]) else nn.ReLU(inplace=True))
         blocks.append(nn.Sequential(*layers))
     tower = nn.Sequential(*blocks)
     for m in tower.modules():
@@ -48,6 +49,10 @@ def _to_anchor_major(x: Tensor, per_anchor: int) -> Tensor:
     # (B, A*K, H, W) -> (B, H*W*A, K): memory order (h, w, a, k) equals the anchor order (y, x, a)
     B, _, H, W = x.shape
     return x.view(B, -1, per_anchor, H, W).permute(0, 3, 4, 1, 2).reshape(B, -1, per_anchor)
+
+
+def _is_channels_last(x: Tensor) -> bool:
+    return not x.is_contiguous() and x.is_contiguous(memory_format=torch.channels_last)
 
 
 class RetinaNetClassificationHead(nn.Module):
@@ -386,6 +391,12 @@ def postprocess_batched(cls_levels, reg_levels, anchors, image_shapes, score_thr
     dev = cls_levels[0].device
     hw = _image_hw_tensor(image_shapes, dev)
     K = int(topk_candidates)
+    if planar_classes is not None and all(map(_is_channels_last, [*cls_levels, *reg_levels, *(ctr_levels or [])])):
+        # channels-last maps hold their anchors' rows already: read as [B, H*W*A, K] without a copy
+        cls_levels = [_to_anchor_major(m, planar_classes) for m in cls_levels]
+        reg_levels = [_to_anchor_major(m, 4) for m in reg_levels]
+        ctr_levels = None if ctr_levels is None else [_to_anchor_major(m, 1) for m in ctr_levels]
+        planar_classes = None
     if planar_classes is not None:
         cb, cs, cl, _, cc = kernels.select_candidates_planar(cls_levels, reg_levels, shared, hw, planar_classes,
                                                              score_thresh, K, coder, bbox_xform_clip, ctr_maps=ctr_levels,

@@ -15,13 +15,13 @@ from __future__ import annotations
 
 from collections import OrderedDict
 from functools import partial
-from typing import List, Optional
+from typing import Callable, List, Optional
 
 import torch
 from torch import nn
 
 from .anchor_utils import AnchorGenerator
-from .fcos import FCOS
+from .fcos import FCOS, FCOSHead
 from .retinanet import RetinaNet, RetinaNetHead
 
 
@@ -60,7 +60,10 @@ def anchor_geometry(backbone: str, layers: List[int]):
 
 def get_model(num_classes, pretrained=False, layers=[0, 2, 4, 6], arch="retinanet", backbone="poolformer_s24",
               is_torch=False, out_channels=256, baseline="fpn", num_layers=2,
-              backbone_module: Optional[nn.Module] = None, **kwargs):
+              backbone_module: Optional[nn.Module] = None, norm_layer: Optional[Callable[..., nn.Module]] = None, **kwargs):
+    """``norm_layer`` (not in the reference): the norm of the head towers, default ``partial(nn.GroupNorm, 32)`` as the
+    reference builds them; ``partial(norm.GroupNormAct, 32)`` computes the same with the ReLU fused in, on channels-last
+    maps (``model.to(memory_format=torch.channels_last)`` keeps the convolutions' weights in that order too)."""
     if pretrained:
         raise RuntimeError("pretrained weights need a network download, which this build never attempts")
     name = backbone if isinstance(backbone, str) else "custom"
@@ -82,7 +85,7 @@ def get_model(num_classes, pretrained=False, layers=[0, 2, 4, 6], arch="retinane
             backbone_module = PyramidStub(len(sizes), out_channels)
         anchor_generator = AnchorGenerator(sizes, ratios)
         head = RetinaNetHead(backbone_module.out_channels, anchor_generator.num_anchors_per_location()[0],
-                             num_classes, norm_layer=partial(nn.GroupNorm, 32))
+                             num_classes, norm_layer=norm_layer or partial(nn.GroupNorm, 32))
         head.regression_head._loss_type = "giou"
         return RetinaNet(backbone_module, num_classes=num_classes, anchor_generator=anchor_generator, head=head,
                          **kwargs)
@@ -91,5 +94,7 @@ def get_model(num_classes, pretrained=False, layers=[0, 2, 4, 6], arch="retinane
             if name != "pyramid_stub":
                 raise NotImplementedError(f"backbone '{name}' is outside this package; pass backbone_module=")
             backbone_module = PyramidStub(5, out_channels, first_stride=8)
+        if norm_layer is not None and kwargs.get("head") is None:
+            kwargs["head"] = FCOSHead(backbone_module.out_channels, 1, num_classes, norm_layer=norm_layer)
         return FCOS(backbone_module, num_classes, **kwargs)
     raise ValueError(f"unknown arch {arch!r}")

@@ -135,3 +135,31 @@ def test_no_cpu_fallback():
         boxes.nms(torch.zeros((2, 4)), torch.zeros(2), 0.5)
     with pytest.raises(RuntimeError, match="GPU tensor"):
         kernels.match_retinanet(torch.zeros((4, 4)), [torch.zeros((1, 4))], 0.6, 0.5)
+
+
+def test_argument_errors_of_group_norm_act():
+    lib = _C.lib()
+    null, p16, p256 = ctypes.c_void_p(0), ctypes.c_void_p(16), ctypes.c_void_p(256)
+    size = lib.od_group_norm_act_workspace_bytes(16, 65536, 256, 32)
+    assert size >= 16 * 256 * 8
+    assert lib.od_group_norm_act_workspace_bytes(1, 64, 256, 3) == 0            # groups do not divide the channels
+    assert lib.od_group_norm_act_workspace_bytes(1, 64, 4096, 32) == 0          # channel limit
+    assert lib.od_group_norm_act_workspace_bytes(70000, 64, 256, 32) == 0       # batch limit
+
+    def fwd(x=p256, dtype=0, batch=2, pixels=64, channels=32, groups=4, pdtype=0, act=1, y=p256, ws=p256, nbytes=1 << 20):
+        return lib.od_group_norm_act_forward(x, dtype, batch, pixels, channels, groups, null, null, pdtype, 1e-5, act, y, p256,
+                                             p256, ws, nbytes, null)
+
+    def bwd(x=p256, dtype=0, batch=2, pixels=64, channels=32, groups=4, pdtype=0, act=1, dy=p256, ws=p256, nbytes=1 << 20):
+        return lib.od_group_norm_act_backward(x, dy, dtype, batch, pixels, channels, groups, null, null, pdtype, act, p256, p256,
+                                              p256, null, null, ws, nbytes, null)
+    for call in (fwd, bwd):
+        assert call(x=null) == -1 and call(ws=null) == -1 and call(ws=p16) == -1
+        assert call(dtype=3) == -1 and call(pdtype=-1) == -1 and call(act=3) == -1
+        assert call(groups=0) == -1 and call(groups=5) == -1 and call(channels=0) == -1
+        assert call(batch=-1) == -1 and call(pixels=-1) == -1
+        assert call(channels=4096) == -2 and call(batch=65536) == -2
+        assert call(nbytes=64) == -3
+        assert call(x=ctypes.c_void_p(258)) == -1                                # not aligned to an element
+        assert call(batch=0) == 0 and call(pixels=0) == 0
+    assert fwd(y=null) == -1 and bwd(dy=null) == -1
