@@ -412,6 +412,52 @@ int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int
                                void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Losses of a classification head whose classes are a large vocabulary of embeddings (no counterpart in the reference,
+ * whose heads hold one convolution channel per class): softmax cross entropy, and distillation from a teacher's top
+ * logits, with gradients.  The logits z = (features weight^T + bias) / temperature [rows, classes] are formed in pieces
+ * and never kept.
+ *   features     : [rows, dim] of element type dtype, rows feature_pitch elements apart (>= dim)
+ *   weight       : [classes, dim] of dtype, rows weight_pitch elements apart;  bias: [classes] of dtype, may be null
+ *   top = 0      : targets int64 [rows], the class of each row; a negative one leaves the row out; temperature must be 1
+ *                  row loss = log sum exp z - z[target]
+ *   top >= 1     : targets int64 [rows, top], classes a teacher names for each row (negative: no entry), with
+ *                  teacher_logits [rows, top] of teacher_dtype; p = softmax(teacher_logits / temperature) over a row's
+ *                  entries, entries of one class added up; entries with a logit of -inf have no weight; a row without
+ *                  any entry of weight is left out
+ *                  row loss = temperature^2 * (sum p log p - sum p z[class] + log sum exp z)
+ *   A class >= classes is not followed: it makes the row's loss and its gradients NaN.  Rows left out have loss and
+ *   gradient zero whatever their features hold.
+ *   row_loss     : fp32 [rows];  loss: fp32 [1], by OD_REDUCE_*: not written, sum / max(1, rows not left out), or sum
+ *   saved        : od_vocab_loss_saved_bytes, 256-byte aligned, written by the forward call and read by the backward one
+ *                  (which takes the same weight, bias, targets and sizes)
+ *   upstream     : fp32 gradient of row_loss [rows] (OD_REDUCE_NONE) or of loss [1]
+ *   dfeatures    : [rows, dim] dense, dweight [classes, dim] dense, dbias [classes], all of dtype; any may be null
+ *   workspace    : od_vocab_loss_workspace_bytes(..., backward = 0 or 1), 256-byte aligned
+ * Sums are fp32 in a fixed order; 16-bit gradients are rounded once at the end, and the logits' gradients, an operand of
+ * the products, once before (fp16: under a power of two that keeps small ones normal).
+ */
+#define OD_REDUCE_NONE 0
+#define OD_REDUCE_MEAN 1
+#define OD_REDUCE_SUM 2
+#define OD_MAX_VOCAB_ROWS 8388608
+#define OD_MAX_VOCAB_CLASSES 16777216
+#define OD_MAX_VOCAB_DIM 16384          /* and at most 32 GiB each of features and weight */
+#define OD_MAX_TEACHER_TOP 256
+size_t od_vocab_loss_saved_bytes(int64_t rows, int64_t classes, int32_t dim, int32_t top, int32_t dtype);
+size_t od_vocab_loss_workspace_bytes(int64_t rows, int64_t classes, int32_t dim, int32_t top, int32_t dtype,
+                                     int32_t backward);
+int od_vocab_loss_forward(const void* features, int64_t feature_pitch, const void* weight, int64_t weight_pitch,
+                          const void* bias, int32_t dtype, int64_t rows, int64_t classes, int32_t dim,
+                          const int64_t* targets, int32_t top, const void* teacher_logits, int32_t teacher_dtype,
+                          float temperature, int32_t reduction, float* row_loss, float* loss, void* saved,
+                          size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);
+int od_vocab_loss_backward(const void* weight, int64_t weight_pitch, const void* bias, int32_t dtype, int64_t rows,
+                           int64_t classes, int32_t dim, const int64_t* targets, int32_t top, float temperature,
+                           int32_t reduction, const float* upstream, const void* saved, size_t saved_bytes,
+                           void* dfeatures, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/*
  * Per-kernel timing aid.  No counterpart in the reference (it has no profiling hooks); used by
  * bench.py to measure a kernel's own duration on the stream it runs on.  od_profile_select makes the
  * library launch that kernel (or all kernels) with a start and a stop event that receive the dispatch's own
@@ -447,7 +493,11 @@ int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int
 #define OD_KERNEL_NORM_APPLY 23     /* od_group_norm_act_forward: normalise + activation (small maps: all of it) */
 #define OD_KERNEL_NORM_BWD_SUMS 24  /* od_group_norm_act_backward: channel sums of large maps */
 #define OD_KERNEL_NORM_BWD_APPLY 25 /* od_group_norm_act_backward: gradient of the map (small maps: sums as well) */
-#define OD_KERNEL_COUNT 26
+#define OD_KERNEL_VOCAB_LSE 26      /* od_vocab_loss_forward: product with running maximum and sum */
+#define OD_KERNEL_VOCAB_DZ 27       /* od_vocab_loss_backward: product again, gradient of a piece of the logits */
+#define OD_KERNEL_VOCAB_GRAD_ROWS 28    /* od_vocab_loss_backward: gradient of the features */
+#define OD_KERNEL_VOCAB_GRAD_CLASSES 29 /* od_vocab_loss_backward: gradient of the weight and bias */
+#define OD_KERNEL_COUNT 30
 int od_profile_select(int32_t kernel_id);
 /* Time only every `every`-th launch of a selected kernel (default 1): a timed launch costs the host tens of
  * microseconds, which a throughput measurement should not pay on every step. */

@@ -82,6 +82,12 @@ SIGNATURES = {
                                             c_int32, _P, _P, _P, _P, c_size_t, _P]),
     "od_group_norm_act_backward": (c_int32, [_P, _P, c_int32, c_int64, c_int64, c_int32, c_int32, _P, _P, c_int32, c_int32,
                                              _P, _P, _P, _P, _P, _P, c_size_t, _P]),
+    "od_vocab_loss_saved_bytes": (c_size_t, [c_int64, c_int64, c_int32, c_int32, c_int32]),
+    "od_vocab_loss_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32]),
+    "od_vocab_loss_forward": (c_int32, [_P, c_int64, _P, c_int64, _P, c_int32, c_int64, c_int64, c_int32, _P, c_int32, _P,
+                                        c_int32, c_float, c_int32, _P, _P, _P, c_size_t, _P, c_size_t, _P]),
+    "od_vocab_loss_backward": (c_int32, [_P, c_int64, _P, c_int32, c_int64, c_int64, c_int32, _P, c_int32, c_float, c_int32,
+                                         _P, _P, c_size_t, _P, _P, _P, _P, c_size_t, _P]),
     "od_match_restore_groups": (c_int32, [c_int32]),
     "od_profile_select": (c_int32, [c_int32]),
     "od_profile_stride": (c_int32, [c_int32]),
@@ -91,9 +97,12 @@ SIGNATURES = {
 PROFILE_OFF, PROFILE_ALL = -1, -2
 KERNEL_NAMES = ["anchor", "match_assign", "match_restore", "match_fcos", "box_iou", "matcher", "decode", "filter",
                 "select", "nms", "match_heavy", "match_init", "focal_fwd", "focal_bwd", "box_loss_fwd", "box_loss_bwd", "preprocess", "sample", "filter_redo",
-                "pack", "nms_order", "predict_tail", "norm_stats", "norm_apply", "norm_bwd_sums", "norm_bwd_apply"]
+                "pack", "nms_order", "predict_tail", "norm_stats", "norm_apply", "norm_bwd_sums", "norm_bwd_apply",
+                "vocab_lse", "vocab_dz", "vocab_grad_rows", "vocab_grad_classes"]
 BOX_LOSS_L1, BOX_LOSS_SMOOTH_L1, BOX_LOSS_GIOU = 0, 1, 2
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+REDUCE_NONE, REDUCE_MEAN, REDUCE_SUM = 0, 1, 2
+OD_MAX_TEACHER_TOP = 256
 ACT_NONE, ACT_RELU, ACT_SILU = 0, 1, 2
 OD_MAX_NORM_CHANNELS = 2048
 OD_MAX_NORM_BATCH = 65535

@@ -7,10 +7,11 @@ rejected with an error that says what they take.
 from __future__ import annotations
 
 import math
-from typing import List, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _C, kernels
 
@@ -273,3 +274,83 @@ def fcos_head_losses(cls_logits: Tensor, bbox_regression: Tensor, bbox_ctrness: 
     boxes, gt_offsets, _ = kernels._pack_gt([t["boxes"] for t in targets], cls_logits.device)
     reg, ctr = _FCOSBoxLoss.apply(bbox_regression, bbox_ctrness, anchor_table, matched, boxes, gt_offsets, 1e-7)
     return {"classification": cls, "bbox_regression": reg, "bbox_ctrness": ctr}
+
+
+_REDUCTIONS = {"none": _C.REDUCE_NONE, "mean": _C.REDUCE_MEAN, "sum": _C.REDUCE_SUM}
+
+
+class _VocabularyLoss(torch.autograd.Function):
+    """Cross entropy or distillation of a head over a large vocabulary (kernels.vocab_loss_*).  Keeps the packed features
+    of the valid rows and one fp32 log-sum-exp per row; the logits are formed again, piece by piece, for the gradients."""
+
+    @staticmethod
+    def forward(ctx, features: Tensor, weight: Tensor, bias: Optional[Tensor], targets: Tensor,
+                teacher_logits: Optional[Tensor], temperature: float, reduction: int) -> Tensor:
+        rows, loss, saved = kernels.vocab_loss_forward(features, weight, bias, targets, teacher_logits, temperature,
+                                                       reduction)
+        if any(ctx.needs_input_grad[:3]):
+            ctx.save_for_backward(weight, bias, targets, saved)
+            ctx.conf = (temperature, reduction)
+        return rows if reduction == _C.REDUCE_NONE else loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out: Tensor):
+        weight, bias, targets, saved = ctx.saved_tensors
+        grads = kernels.vocab_loss_backward(weight, bias, targets, *ctx.conf, grad_out.to(torch.float32), saved,
+                                            *ctx.needs_input_grad[:3])
+        return (*grads, None, None, None, None)
+
+
+def _vocabulary_loss(features: Tensor, weight: Tensor, bias: Optional[Tensor], targets: Tensor,
+                     teacher_logits: Optional[Tensor], temperature: float, reduction: str, shape) -> Tensor:
+    kernels._require_gpu(features, "features")
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"unknown reduction {reduction!r}: one of {sorted(_REDUCTIONS)}")
+    if features.dim() < 2 or weight.dim() != 2 or features.shape[-1] != weight.shape[1] or features.shape[:-1] != shape:
+        raise ValueError(f"vocabulary loss takes features [..., D], weight [V, D] and one row of targets per row of features, "
+                         f"got {tuple(features.shape)}, {tuple(weight.shape)}, {tuple(shape)}")
+    rows = features.reshape(-1, features.shape[-1])
+    out = _VocabularyLoss.apply(rows, weight, bias, targets, teacher_logits, float(temperature), _REDUCTIONS[reduction])
+    return out.reshape(shape) if reduction == "none" else out
+
+
+def vocabulary_cross_entropy(features: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor] = None,
+                             reduction: str = "mean") -> Tensor:
+    """Softmax cross entropy of a classification head over a large vocabulary, without keeping its logits:
+    ``cross_entropy(features @ weight.T + bias, targets)``.
+
+    features [..., D] are the embeddings of anchors or locations (any strides; rows that are not contiguous are copied),
+    weight [V, D] and bias [V] (or None) those of the classes, all of one type (fp32 / fp16 / bf16) on one GPU; targets
+    int64 [...].  A negative target leaves its row out, so the indices of a matcher can be used as they are: -1 (no
+    object) and -2 (between the thresholds) take no part.  A target >= V makes the row's loss and gradients NaN.
+    reduction: "mean" over the rows that take part (0 if there are none), "sum", or "none": fp32 losses [...], zero for the
+    rows left out.  The logits are formed in pieces of the vocabulary, once forward and once backward; sums are fp32.
+    Differentiable once in features, weight and bias."""
+    if targets.dtype != torch.int64:
+        raise TypeError(f"targets must be int64, got {targets.dtype}")
+    return _vocabulary_loss(features, weight, bias, targets.reshape(-1), None, 1.0, reduction, targets.shape)
+
+
+def vocabulary_distillation(features: Tensor, weight: Tensor, teacher_logits: Tensor, teacher_classes: Tensor,
+                            bias: Optional[Tensor] = None, temperature: float = 1.0, reduction: str = "mean") -> Tensor:
+    """Distillation of a teacher's top logits into a head over a large vocabulary: T^2 * KL(p || q) per row, with
+    q = softmax((features @ weight.T + bias) / T) over all V classes and p = softmax(teacher_logits / T) over the K classes
+    that the teacher names for the row.
+
+    teacher_logits [..., K] (fp32 / fp16 / bf16), teacher_classes int64 [..., K], K <= 256.  An entry with a negative class
+    is not there, one with a logit of -inf has no weight, and entries of the same class are added up; a row without an
+    entry of weight is left out.  A class >= V makes the row's loss and gradients NaN.  The rest as in
+    ``vocabulary_cross_entropy``; the teacher gets no gradient."""
+    if teacher_classes.dtype != torch.int64:
+        raise TypeError(f"teacher_classes must be int64, got {teacher_classes.dtype}")
+    if teacher_logits.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("vocabulary_distillation: the teacher's logits take no gradient (detach them)")
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if teacher_classes.dim() < 2 or teacher_logits.shape != teacher_classes.shape or teacher_classes.shape[-1] < 1:
+        raise ValueError(f"teacher logits {tuple(teacher_logits.shape)} and classes {tuple(teacher_classes.shape)} must be "
+                         f"[..., K], K >= 1")
+    K = teacher_classes.shape[-1]
+    return _vocabulary_loss(features, weight, bias, teacher_classes.reshape(-1, K), teacher_logits.reshape(-1, K), temperature,
+                            reduction, teacher_classes.shape[:-1])

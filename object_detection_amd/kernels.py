@@ -807,3 +807,108 @@ def group_norm_act_backward(x: Tensor, dy: Tensor, num_groups: int, weight: Opti
                                                  _ptr(dbias), _ptr(ws), ws.numel(), _stream(x.device))
     _C.check(rc, "od_group_norm_act_backward")
     return dx, dweight, dbias
+
+
+def _row_pitch(t: Tensor) -> Tensor:
+    """2-D tensor whose rows are contiguous and do not overlap; anything else is copied."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        return t.contiguous()
+    return t
+
+
+def _pitch(t: Tensor) -> int:
+    return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
+
+
+def _vocab_bytes(rows: int, classes: int, dim: int, top: int, code: int, which: str) -> int:
+    key = ("vocab", rows, classes, dim, top, code, which)
+    nbytes = _ws_bytes.get(key)
+    if nbytes is None:
+        if which == "saved":
+            nbytes = _C.lib().od_vocab_loss_saved_bytes(rows, classes, dim, top, code)
+        else:
+            nbytes = _C.lib().od_vocab_loss_workspace_bytes(rows, classes, dim, top, code, int(which == "backward"))
+        if nbytes == 0:
+            raise _C.OdBoxesError(f"od_vocab_loss: {rows} rows, {classes} classes, {dim} dimensions, {top} teacher entries are "
+                                  f"beyond the limits in od_boxes.h")
+        if len(_ws_bytes) > 65536:
+            _ws_bytes.clear()
+        _ws_bytes[key] = nbytes
+    return nbytes
+
+
+def vocab_loss_forward(features: Tensor, weight: Tensor, bias: Optional[Tensor], targets: Tensor,
+                       teacher_logits: Optional[Tensor], temperature: float,
+                       reduction: int) -> Tuple[Tensor, Optional[Tensor], Tensor]:
+    """Softmax cross entropy (targets int64 [N]) or distillation (targets int64 [N, K] with teacher_logits [N, K]) of rows
+    features [N, D] against classes weight [V, D], bias [V] or None; one type, fp32 / fp16 / bf16.
+    Returns (row losses fp32 [N], loss fp32 [] or None, the buffer that vocab_loss_backward reads)."""
+    _require_gpu(features, "features")
+    dev = features.device
+    for name, t in (("weight", weight), ("bias", bias), ("targets", targets), ("teacher_logits", teacher_logits)):
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"vocab_loss: {name} is on {t.device}, features on {dev}")
+    code = _dtype_code(features, "vocab_loss: features")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.dtype != features.dtype:
+            raise TypeError(f"vocab_loss: {name} is {t.dtype}, features {features.dtype}")
+    if targets.dtype != torch.int64:
+        raise TypeError(f"vocab_loss: targets must be int64, got {targets.dtype}")
+    N, D = features.shape
+    V = int(weight.shape[0])
+    if tuple(weight.shape) != (V, D) or (bias is not None and tuple(bias.shape) != (V,)):
+        raise ValueError(f"vocab_loss: inconsistent shapes, features {tuple(features.shape)}, weight {tuple(weight.shape)}"
+                         + ("" if bias is None else f", bias {tuple(bias.shape)}"))
+    if V < 1 or D < 1:
+        raise ValueError(f"vocab_loss: needs classes and dimensions, got weight {tuple(weight.shape)}")
+    top, tcode = 0, code
+    if teacher_logits is not None:
+        top, tcode = int(targets.shape[1]) if targets.dim() == 2 else 0, _dtype_code(teacher_logits, "vocab_loss: teacher_logits")
+        if targets.dim() != 2 or top < 1 or teacher_logits.shape != targets.shape:
+            raise ValueError(f"vocab_loss: teacher classes {tuple(targets.shape)} and logits {tuple(teacher_logits.shape)} must "
+                             f"be [N, K], K >= 1")
+        if top > _C.OD_MAX_TEACHER_TOP:
+            raise _C.OdBoxesError(f"od_vocab_loss: {top} teacher entries per row exceed the limit of {_C.OD_MAX_TEACHER_TOP}")
+        teacher_logits = teacher_logits.contiguous()
+    if targets.shape[0] != N or (top == 0 and targets.dim() != 1):
+        raise ValueError(f"vocab_loss: targets {tuple(targets.shape)} for {N} rows")
+    features, weight, targets = _row_pitch(features), _row_pitch(weight), targets.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    row_loss = torch.empty((N,), dtype=torch.float32, device=dev)
+    loss = None if reduction == _C.REDUCE_NONE else torch.empty((), dtype=torch.float32, device=dev)
+    saved = torch.empty(_vocab_bytes(N, V, D, top, code, "saved"), dtype=torch.uint8, device=dev)
+    ws = torch.empty(_vocab_bytes(N, V, D, top, code, "forward"), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = _C.lib().od_vocab_loss_forward(_ptr(features), _pitch(features), _ptr(weight), _pitch(weight), _ptr(bias), code, N,
+                                            V, D, _ptr(targets), top, _ptr(teacher_logits), tcode, float(temperature),
+                                            int(reduction), _ptr(row_loss), _ptr(loss), _ptr(saved), saved.numel(), _ptr(ws), ws.numel(), _stream(dev))
+    _C.check(rc, "od_vocab_loss_forward")
+    return row_loss, loss, saved
+
+
+def vocab_loss_backward(weight: Tensor, bias: Optional[Tensor], targets: Tensor, temperature: float, reduction: int,
+                        upstream: Tensor, saved: Tensor, want_features: bool = True, want_weight: bool = True,
+                        want_bias: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """Gradients of vocab_loss_forward: (features [N, D], weight [V, D], bias [V]), None for what is not wanted or not there.
+    upstream: fp32 gradient of the row losses [N] (REDUCE_NONE) or of the loss."""
+    dev = weight.device
+    V, D = weight.shape
+    N = int(targets.shape[0])
+    top = int(targets.shape[1]) if targets.dim() == 2 else 0
+    code = _dtype_code(weight, "vocab_loss: weight")
+    if upstream.dtype != torch.float32 or upstream.numel() != (N if reduction == _C.REDUCE_NONE else 1) \
+            or upstream.device != dev:
+        raise ValueError(f"vocab_loss: upstream gradient {upstream.dtype} {tuple(upstream.shape)} on {upstream.device}")
+    weight, targets, upstream = _row_pitch(weight), targets.contiguous(), upstream.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    fresh = torch.zeros if N == 0 else torch.empty
+    dfeatures = fresh((N, D), dtype=weight.dtype, device=dev) if want_features else None
+    dweight = fresh((V, D), dtype=weight.dtype, device=dev) if want_weight else None
+    dbias = fresh((V,), dtype=weight.dtype, device=dev) if want_bias and bias is not None else None
+    ws = torch.empty(_vocab_bytes(N, V, D, top, code, "backward"), dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = _C.lib().od_vocab_loss_backward(_ptr(weight), _pitch(weight), _ptr(bias), code, N, V, D, _ptr(targets), top,
+                                             float(temperature), int(reduction), _ptr(upstream), _ptr(saved), saved.numel(),
+                                             _ptr(dfeatures), _ptr(dweight), _ptr(dbias), _ptr(ws), ws.numel(), _stream(dev))
+    _C.check(rc, "od_vocab_loss_backward")
+    return dfeatures, dweight, dbias

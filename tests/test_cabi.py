@@ -163,3 +163,36 @@ def test_argument_errors_of_group_norm_act():
         assert call(x=ctypes.c_void_p(258)) == -1                                # not aligned to an element
         assert call(batch=0) == 0 and call(pixels=0) == 0
     assert fwd(y=null) == -1 and bwd(dy=null) == -1
+
+
+def test_argument_errors_of_vocab_loss():
+    lib = _C.lib()
+    null, p16, p256 = ctypes.c_void_p(0), ctypes.c_void_p(16), ctypes.c_void_p(256)
+    assert lib.od_vocab_loss_saved_bytes(1000, 1204, 256, 0, 2) >= 1024 * 256 * 2
+    assert lib.od_vocab_loss_workspace_bytes(32768, 65536, 512, 0, 2, 1) < 32768 * 65536     # never the logits
+    assert lib.od_vocab_loss_workspace_bytes(1000, 1204, 256, 8, 2, 0) > 0
+    assert lib.od_vocab_loss_saved_bytes(10, 0, 256, 0, 2) == 0 and lib.od_vocab_loss_saved_bytes(10, 5, 0, 0, 2) == 0
+    assert lib.od_vocab_loss_saved_bytes(10, 5, 8, 257, 2) == 0 and lib.od_vocab_loss_saved_bytes(10, 5, 16385, 0, 2) == 0
+    assert lib.od_vocab_loss_saved_bytes(1 << 23, 5, 16384, 0, 0) == 0                       # 512 GiB of features
+    assert lib.od_vocab_loss_saved_bytes((1 << 23) + 1, 5, 8, 0, 0) == 0
+
+    def fwd(f=p256, fp=64, w=p256, wp=64, bias=null, dtype=2, rows=10, classes=50, dim=64, t=p256, top=0, tl=null, td=2, temp=1.0,
+            red=1, loss=p256, saved=p256, ws=p256, nbytes=1 << 30):
+        return lib.od_vocab_loss_forward(f, fp, w, wp, bias, dtype, rows, classes, dim, t, top, tl, td, temp, red, p256, loss,
+                                         saved, nbytes, ws, nbytes, null)
+
+    def bwd(w=p256, wp=64, bias=null, dtype=2, rows=10, classes=50, dim=64, t=p256, top=0, temp=1.0, red=1, up=p256, saved=p256,
+            ws=p256, nbytes=1 << 30):
+        return lib.od_vocab_loss_backward(w, wp, bias, dtype, rows, classes, dim, t, top, temp, red, up, saved, nbytes, p256,
+                                          p256, null, ws, nbytes, null)
+    for call in (fwd, bwd):
+        assert call(w=null) == -1 and call(t=null) == -1 and call(saved=null) == -1 and call(ws=p16) == -1
+        assert call(dtype=3) == -1 and call(red=3) == -1 and call(rows=-1) == -1 and call(classes=0) == -1 and call(dim=0) == -1
+        assert call(top=-1) == -1 and call(temp=2.0) == -1                        # cross entropy has no temperature
+        assert call(wp=63) == -1 and call(w=ctypes.c_void_p(257)) == -1
+        assert call(top=257, temp=2.0) == -2 and call(dim=16385, wp=16385) == -2
+        assert call(nbytes=1024) == -3
+    assert fwd(f=null) == -1 and fwd(fp=63) == -1 and fwd(loss=null) == -1 and fwd(top=4) == -1     # no teacher logits
+    assert fwd(top=4, tl=p256, temp=0.0) == -1 and fwd(top=4, tl=p256, temp=float("nan")) == -1
+    assert fwd(top=4, tl=p256, td=5) == -1
+    assert bwd(up=null) == -1 and bwd(rows=0) == 0

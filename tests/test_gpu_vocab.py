@@ -1,0 +1,515 @@
+"""The losses of a head over a large vocabulary (softmax cross entropy, distillation from a teacher's top logits) against
+their definition in float64, their gradients against the formula and against differences, and together with the head tower
+they are used behind."""
+import math
+from functools import partial
+
+import pytest
+import torch
+from torch import nn
+
+from object_detection_amd import _C, det_utils, kernels
+from object_detection_amd.norm import GroupNormAct
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 1e-38, torch.float16: 2.0 ** -25, torch.bfloat16: 1e-38}     # half the smallest subnormal
+NAN = float("nan")
+
+
+def _inputs(device, N, V, D, dtype, bias, seed):
+    gen = torch.Generator().manual_seed(seed)
+    w = (torch.randn((V, D), generator=gen) / math.sqrt(D)).to(device, dtype)
+    t = torch.randint(0, V, (N,), generator=gen).to(device)
+    f = (torch.randn((N, D), generator=gen) * 1.5).to(device)
+    f = (f + w[t].float() * 4).to(dtype)
+    b = (torch.randn((V,), generator=gen) * 0.5).to(device, dtype) if bias else None
+    return f, w, b, t
+
+
+def _teacher(device, N, V, K, seed, dtype=torch.float32):
+    gen = torch.Generator().manual_seed(seed)
+    classes = torch.stack([torch.randperm(V, generator=gen)[:K] for _ in range(N)]) if N else torch.zeros((0, K), dtype=torch.int64)
+    return classes.to(device), (torch.randn((N, K), generator=gen) * 2).to(device, dtype)
+
+
+def _definition(f, w, b, classes, p, valid, T, gr):
+    """Row losses and gradients in float64 and how far fp32 sums with dz held in f's type may be off them.
+
+    e_z: a sum of D products in fp32 is off by (D + 4) half steps of the sum of their sizes at most.  A log-sum-exp is off
+    by that and by 2^-18 for its own sum and exponentials (V <= 2^17 additions in lanes, splits and waves of at most 64
+    terms each, two exponentials of one unit), and by the rounding of its own value.  q is off by e_z twice (z and lse), and
+    2^-18 again; dz is rounded once to f's type; a product of K terms is off by K + 8 half steps of its terms' sizes; the
+    result is rounded once."""
+    dtype = f.dtype
+    F, W = f.double(), w.double()
+    N, D = F.shape
+    V = W.shape[0]
+    B = torch.zeros(V, dtype=torch.float64, device=f.device) if b is None else b.double()
+    F = torch.where(valid[:, None], F, torch.zeros_like(F))
+    z = (torch.mm(F, W.t()) + B) / T
+    size = (torch.mm(F.abs(), W.abs().t()) + B.abs()) / T
+    lse = torch.logsumexp(z, dim=1)
+    e_z = (D + 4) * U * size.max(dim=1).values
+    e_lse = e_z + 2.0 ** -18 + 4 * U * lse.abs()
+    safe = classes.clamp(min=0)
+    at = z.gather(1, safe)
+    row = T * T * (torch.xlogy(p, p).sum(1) - (p * at).sum(1) + lse)
+    row = torch.where(valid, row, torch.zeros_like(row))
+    e_row = T * T * (e_lse + e_z + 2.0 ** -18 * (1 + (p * at.abs()).sum(1) + lse.abs()))
+    q = torch.exp(z - lse[:, None])
+    dz = q.clone()
+    dz.scatter_add_(1, safe, -p)
+    gr = torch.where(valid, gr.double(), torch.zeros_like(gr.double()))[:, None] * T
+    dz = torch.where(gr == 0, torch.zeros_like(dz), dz * gr)
+    e_q = (2 * e_z + 2.0 ** -18 + 8 * U * lse.abs())[:, None]
+    e_dz = gr.abs() * q * e_q * 1.1 + HALF[dtype] * dz.abs() * 1.01
+    e_dz.scatter_add_(1, safe, gr.abs() * p * 2.0 ** -18)
+    if dtype == torch.float16:
+        e_dz = e_dz + gr.abs().max() * 2.0 ** -37 * (gr != 0)
+    tiny = TINY[dtype]
+    dF, dW, db = torch.mm(dz, W), torch.mm(dz.t(), F), dz.sum(0)
+    half = HALF[dtype] * 1.01
+    t_dF = torch.mm(e_dz + (V + 8) * U * dz.abs(), W.abs()) + half * dF.abs() + tiny
+    t_dW = torch.mm((e_dz + (N + 8) * U * dz.abs()).t(), F.abs()) + half * dW.abs() + tiny
+    t_db = (e_dz + (N + 8) * U * dz.abs()).sum(0) + half * db.abs() + tiny
+    return (row, dF, dW, db), (e_row, t_dF, t_dW, t_db)
+
+
+def _close(got, want, tol, what):
+    assert got.shape == want.shape, what
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} off, by up to {float(err[bad].max())} " \
+                                f"where {float(tol[bad].max())} is allowed"
+
+
+def _check_ce(f, w, b, t, reduction="mean", scale=1.0):
+    valid = t >= 0
+    count = max(1, int(valid.sum()))
+    N = f.shape[0]
+    if reduction == "none":
+        up = (torch.rand((N,), generator=torch.Generator().manual_seed(1)) * 2 - 0.5).to(f.device) * scale
+        gr = up
+    else:
+        up = torch.tensor(scale, device=f.device)
+        gr = up.expand(N) / (count if reduction == "mean" else 1)
+    want, tol = _definition(f, w, b, t[:, None], valid.double()[:, None], valid, 1.0, gr)
+    _check(lambda *a: det_utils.vocabulary_cross_entropy(a[0], a[1], t, bias=a[2] if b is not None else None,
+                                                         reduction=reduction), f, w, b, want, tol, up, reduction, count)
+
+
+def _check_kd(f, w, b, tl, tc, T, reduction="mean", scale=1.0):
+    on = (tc >= 0) & (tl != -math.inf)
+    valid = on.any(dim=1)
+    count = max(1, int(valid.sum()))
+    p = torch.softmax(torch.where(on, tl.double() / T, torch.full_like(tl.double(), -math.inf)), dim=1)
+    p = torch.where(valid[:, None], p, torch.zeros_like(p))
+    merged = torch.zeros_like(p)                                    # entries of one class are one class
+    for k in range(p.shape[1]):
+        same = (tc == tc[:, k:k + 1]) & (tc >= 0)
+        first = same.double().argmax(dim=1) == k
+        merged[:, k] = torch.where(first & (tc[:, k] >= 0), (p * same).sum(1), torch.zeros_like(p[:, k]))
+    N = f.shape[0]
+    up = torch.tensor(scale, device=f.device)
+    gr = up.expand(N) / (count if reduction == "mean" else 1)
+    if reduction == "none":
+        up = gr = torch.linspace(-1, 2, N, device=f.device) * scale
+    want, tol = _definition(f, w, b, tc, merged, valid, T, gr)
+    _check(lambda *a: det_utils.vocabulary_distillation(a[0], a[1], tl, tc, bias=a[2] if b is not None else None,
+                                                        temperature=T, reduction=reduction),
+           f, w, b, want, tol, up, reduction, count)
+
+
+def _check(call, f, w, b, want, tol, up, reduction, count):
+    leaves = [x.detach().requires_grad_(True) for x in (f, w, b) if x is not None]
+    out = call(*leaves)
+    assert out.dtype == torch.float32
+    if reduction == "none":
+        _close(out.detach(), want[0], tol[0], "row losses")
+    else:
+        share = count if reduction == "mean" else 1
+        _close(out.detach(), want[0].sum() / share, (tol[0].sum() + 2 * U * want[0].sum().abs()) / share, "loss")
+    grads = torch.autograd.grad(out, leaves, up)
+    for g, x, r, e, name in zip(grads, leaves, want[1:], tol[1:], ("dF", "dW", "db")):
+        assert g.dtype == x.dtype
+        _close(g, r, e, name)
+
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V,D,bias", [
+    (1, 1, 1, True),                    # one class: loss and gradients are zero
+    (1, 2, 8, False),
+    (2, 127, 64, True),
+    (3, 128, 100, True),                # packed weight rows (100 is no whole stage of K)
+    (127, 129, 64, False),
+    (128, 1204, 256, True),
+    (129, 1000, 320, True),
+    (300, 5003, 200, True),
+    (100, 20000, 64, True),             # few rows: classes split over workgroups, dF split over K
+    (5000, 300, 128, True),             # few classes: dW split over K
+])
+def test_cross_entropy_matches_definition(device, N, V, D, bias, dtype):
+    f, w, b, t = _inputs(device, N, V, D, dtype, bias, seed=N + V + D)
+    t = torch.where(torch.arange(N, device=device) % 5 == 3, torch.full_like(t, -1 - (N % 2)), t)
+    _check_ce(f, w, b, t, scale=256.0 if dtype == torch.float16 else 1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V,D,K,T,bias", [
+    (1, 3, 16, 1, 1.0, False),
+    (4, 64, 24, 64, 2.0, True),         # the teacher names every class
+    (130, 1204, 256, 8, 2.0, True),
+    (65, 5003, 100, 33, 4.0, False),
+    (9, 700, 64, 256, 1.0, True),       # the limit of K
+    (600, 300, 64, 5, 0.5, True),
+])
+def test_distillation_matches_definition(device, N, V, D, K, T, bias, dtype):
+    f, w, b, _ = _inputs(device, N, V, D, dtype, bias, seed=N + V + D + K)
+    tc, tl = _teacher(device, N, V, K, seed=K, dtype=dtype)
+    _check_kd(f, w, b, tl, tc, T, scale=256.0 if dtype == torch.float16 else 1.0)
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_other_reductions(device, reduction, dtype):
+    f, w, b, t = _inputs(device, 140, 333, 64, dtype, True, seed=2)
+    t[7:90:3] = -2
+    scale = 0.01 if reduction == "none" else 1.0                # fp16: small row gradients have to survive
+    _check_ce(f, w, b, t, reduction, scale)
+    tc, tl = _teacher(device, 140, 333, 12, seed=3)
+    _check_kd(f, w, b, tl, tc, 2.0, reduction, scale)
+
+
+def test_teacher_entries_that_are_missing_repeated_or_without_weight(device):
+    f, w, b, _ = _inputs(device, 12, 200, 64, torch.bfloat16, True, seed=4)
+    tc, tl = _teacher(device, 12, 200, 6, seed=5)
+    tc[0, 2:] = -1                       # a short list
+    tc[1] = -1                           # no list
+    tl[2] = -math.inf                    # a list without weight
+    tl[3, 1:4] = -math.inf
+    tc[4] = tc[4, 0]                     # one class six times
+    tc[5, 3] = tc[5, 1]                  # one class twice
+    tc[6, 0], tl[6, 0] = -1, NAN         # what a missing entry holds is not looked at
+    tl[7, 5] = torch.finfo(torch.float32).min
+    tl[8] = torch.finfo(torch.float32).min                          # all alike: uniform
+    for T in (1.0, 3.0, 0.25):
+        on = (tc >= 0)
+        tl_ref = torch.where(on, tl, torch.zeros_like(tl))
+        call = tl.clone()
+        want_tl = torch.where(on, tl_ref, torch.full_like(tl, -math.inf))
+        # the definition sees the missing entries as weightless ones
+        for reduction in ("mean", "none"):
+            N = 12
+            valid = (on & (want_tl != -math.inf)).any(1)
+            count = int(valid.sum())
+            p = torch.nan_to_num(torch.softmax(want_tl.double() / T, dim=1))
+            merged = torch.zeros_like(p)
+            for n in range(N):
+                for k in range(6):
+                    if on[n, k]:
+                        first = tc[n].tolist().index(int(tc[n, k]))
+                        merged[n, first] += p[n, k]
+            up = torch.ones((N,), device=device) if reduction == "none" else torch.tensor(1.0, device=device)
+            gr = torch.ones((N,), device=device) / (1 if reduction == "none" else count)
+            want, tol = _definition(f, w, b, tc, merged, valid, T, gr)
+            _check(lambda *a: det_utils.vocabulary_distillation(a[0], a[1], call, tc, bias=a[2], temperature=T,
+                                                                reduction=reduction), f, w, b, want, tol, up, reduction, count)
+
+
+def test_rows_left_out_may_hold_anything(device):
+    f, w, b, t = _inputs(device, 200, 300, 64, torch.bfloat16, True, seed=6)
+    t[::3] = -1
+    clean = f.clone()
+    clean[::3] = 0
+    f[::3] = NAN
+    f[3::6] = math.inf
+    for make in (lambda a, x: det_utils.vocabulary_cross_entropy(x[0], x[1], t, bias=x[2]),):
+        a = [x.clone().requires_grad_(True) for x in (f, w, b)]
+        c = [x.clone().requires_grad_(True) for x in (clean, w, b)]
+        la, lc = make(None, a), make(None, c)
+        assert torch.equal(la, lc) and bool(torch.isfinite(la))
+        ga, gc = torch.autograd.grad(la, a), torch.autograd.grad(lc, c)
+        assert all(torch.equal(x, y) for x, y in zip(ga, gc)) and not ga[0][::3].any()
+
+
+@pytest.mark.parametrize("rows", [0, 5])
+def test_nothing_takes_part(device, rows):
+    f, w, b, _ = _inputs(device, rows, 50, 16, torch.float32, True, seed=7)
+    t = torch.full((rows,), -1, device=device)
+    tc, tl = torch.full((rows, 3), -1, device=device), torch.zeros((rows, 3), device=device)
+    for reduction in ("mean", "sum", "none"):
+        for call in (lambda x: det_utils.vocabulary_cross_entropy(x[0], x[1], t, bias=x[2], reduction=reduction),
+                     lambda x: det_utils.vocabulary_distillation(x[0], x[1], tl, tc, bias=x[2], reduction=reduction)):
+            leaves = [x.clone().requires_grad_(True) for x in (f, w, b)]
+            out = call(leaves)
+            assert out.shape == ((rows,) if reduction == "none" else ()) and not out.any()
+            for g, x in zip(torch.autograd.grad(out.sum(), leaves), leaves):
+                assert g.shape == x.shape and not g.any()
+
+
+def test_class_outside_the_vocabulary_is_loud(device):
+    f, w, b, t = _inputs(device, 6, 50, 32, torch.float32, True, seed=8)
+    t[2] = 50
+    rows = det_utils.vocabulary_cross_entropy(f, w, t, bias=b, reduction="none")
+    assert rows.isnan().tolist() == [False, False, True, False, False, False]
+    fl = f.clone().requires_grad_(True)
+    g = torch.autograd.grad(det_utils.vocabulary_cross_entropy(fl, w, t, bias=b, reduction="none").sum(), fl)[0]
+    assert g.isnan().all(dim=1).tolist() == [False, False, True, False, False, False]
+    tc, tl = _teacher(device, 6, 50, 4, seed=9)
+    tc[4, 1] = 10 ** 12
+    rows = det_utils.vocabulary_distillation(f, w, tl, tc, bias=b, reduction="none")
+    assert rows.isnan().tolist() == [False, False, False, False, True, False]
+    tl[0, 0] = NAN
+    rows = det_utils.vocabulary_distillation(f, w, tl, tc, bias=b, reduction="none")
+    assert rows.isnan().tolist() == [True, False, False, False, True, False]
+
+
+def test_classes_without_chance(device):
+    """A bias of -inf, or of the type's lowest value, takes a class out of the softmax."""
+    f, w, b, t = _inputs(device, 40, 260, 64, torch.bfloat16, True, seed=10)
+    t = t % 100
+    b[100:200] = -math.inf
+    b[200:] = torch.finfo(torch.bfloat16).min
+    few = det_utils.vocabulary_cross_entropy(f, w[:100], t, bias=b[:100], reduction="none")
+    leaves = [x.clone().requires_grad_(True) for x in (f, w, b)]
+    out = det_utils.vocabulary_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2], reduction="none")
+    assert torch.allclose(out, few, rtol=0, atol=2.0 ** -17)        # two log-sum-exps of the same terms, 2^-18 each
+    g = torch.autograd.grad(out.sum(), leaves)
+    assert not g[1][100:].any() and not g[2][100:].any() and all(bool(x.isfinite().all()) for x in g)
+
+
+def test_large_and_confident_logits(device):
+    """Logits of several hundred: nothing overflows, and a confident row keeps the digits of 1 - q."""
+    w = torch.eye(64, device=device) * 300
+    f = torch.eye(64, device=device)[:8]
+    t = torch.arange(8, device=device)
+    t[4:] = 20                                                       # wrong by 300
+    rows = det_utils.vocabulary_cross_entropy(f, w, t, reduction="none")
+    assert torch.equal(rows, torch.tensor([0.0] * 4 + [300.0] * 4, device=device))
+    f2 = (f * 0.05).requires_grad_(True)                             # margins of 15: 1 - q = 63 e^-15 = 1.9e-5
+    g = torch.autograd.grad(det_utils.vocabulary_cross_entropy(f2, w, torch.arange(8, device=device), reduction="none").sum(), f2)[0]
+    share = math.exp(-15.0) / (1 + 63 * math.exp(-15.0))
+    diag = g.diagonal()
+    # log q is a difference of two fp32 values near 15, each off by 15 * 2^-23: 4e-6 of 2e-5 absolute; a plain q - 1 would
+    # have steps of 6e-8 * 300 in the gradient
+    assert float((diag / 300 + 63 * share).abs().max()) <= 4e-6
+    assert float((g[0, 8:] / 300 - share).abs().max()) <= 1e-4 * share
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_than_one_piece(device, dtype):
+    N, V = (20000, 9000) if dtype == torch.bfloat16 else (12000, 7001)
+    assert N * V * dtype.itemsize > 256 << 20                        # the logits' gradient does not fit one piece
+    f, w, b, t = _inputs(device, N, V, 64, dtype, True, seed=12)
+    t[::10] = -1
+    _check_ce(f, w, b, t, "sum")
+
+
+def test_strides_alignment_and_shapes(device):
+    f, w, b, t = _inputs(device, 24, 150, 64, torch.bfloat16, True, seed=13)
+    want = det_utils.vocabulary_cross_entropy(f, w, t, bias=b, reduction="none")
+    tc, tl = _teacher(device, 24, 150, 5, seed=14)
+    want_kd = det_utils.vocabulary_distillation(f, w, tl, tc, bias=b, reduction="none")
+
+    def forms(x):
+        wide = torch.zeros((x.shape[0], 200), dtype=x.dtype, device=device)
+        wide[:, 3:67] = x
+        yield wide[:, 3:67]                                          # rows off the 16-byte grid
+        wide[:, 8:72] = x
+        yield wide[:, 8:72]                                          # on it, with a pitch
+        yield x.t().contiguous().t()                                 # columns contiguous
+        flat = torch.zeros(x.numel() + 1, dtype=x.dtype, device=device)
+        flat[1:] = x.reshape(-1)
+        yield flat[1:].view(x.shape)
+    for ff in forms(f):
+        for ww in forms(w):
+            got = det_utils.vocabulary_cross_entropy(ff, ww, t, bias=b, reduction="none")
+            assert torch.equal(got, want)
+            assert torch.equal(det_utils.vocabulary_distillation(ff, ww, tl, tc, bias=b, reduction="none"), want_kd)
+    got = det_utils.vocabulary_cross_entropy(f.view(2, 3, 4, 64), w, t.view(2, 3, 4), bias=b, reduction="none")
+    assert got.shape == (2, 3, 4) and torch.equal(got.reshape(-1), want)
+    got = det_utils.vocabulary_distillation(f.view(4, 6, 64), w, tl.t().contiguous().t().view(4, 6, 5), tc.view(4, 6, 5), bias=b,
+                                            reduction="none")
+    assert torch.equal(got.reshape(-1), want_kd)
+    one = f[:1].expand(24, 64)                                       # one row shared by all: its gradient is their sum
+    leaf = f[:1].clone().requires_grad_(True)
+    g = torch.autograd.grad(det_utils.vocabulary_cross_entropy(leaf.expand(24, 64), w, t, bias=b, reduction="sum"), leaf)[0]
+    full = one.clone().requires_grad_(True)
+    g24 = torch.autograd.grad(det_utils.vocabulary_cross_entropy(full, w, t, bias=b, reduction="sum"), full)[0]
+    assert torch.equal(g, g24.sum(0, keepdim=True))
+
+
+def test_partial_gradients_and_repeated_results(device):
+    f, w, b, t = _inputs(device, 300, 700, 128, torch.bfloat16, True, seed=15)
+    def grads(which):
+        leaves = [x.clone().requires_grad_(k in which) for k, x in zip("fwb", (f, w, b))]
+        out = det_utils.vocabulary_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+        return dict(zip(which, torch.autograd.grad(out, [x for x in leaves if x.requires_grad])))
+    full = grads("fwb")
+    for which in ("f", "w", "b", "fb", "fwb"):
+        assert all(torch.equal(g, full[k]) for k, g in grads(which).items())
+    with torch.no_grad():
+        assert torch.equal(det_utils.vocabulary_cross_entropy(f, w, t, bias=b), det_utils.vocabulary_cross_entropy(f, w, t, bias=b))
+    leaf = f.clone().requires_grad_(True)
+    out = det_utils.vocabulary_cross_entropy(leaf, w, t)
+    first = torch.autograd.grad(out, leaf, retain_graph=True)[0]
+    assert torch.equal(first, torch.autograd.grad(out, leaf)[0])
+
+
+def test_gradient_against_differences(device):
+    """Central differences along the gradient (fp32, step 1e-2 of entries up to 1): the sums of 20 losses are off by
+    20 * 2^-18 = 8e-5 each, 8e-3 in the quotient; the third derivative of a log-sum-exp along v is below |z_v|^3 / 4 with
+    |z_v| <= 16 * 0.5, 20 * 128 * 1e-4 / 6 = 0.05."""
+    f, w, b, t = _inputs(device, 20, 90, 16, torch.float32, True, seed=16)
+    tc, tl = _teacher(device, 20, 90, 7, seed=17)
+    for loss in (lambda a: det_utils.vocabulary_cross_entropy(a[0], a[1], t, bias=a[2], reduction="none"),
+                 lambda a: det_utils.vocabulary_distillation(a[0], a[1], tl, tc, bias=a[2], temperature=2.0, reduction="none")):
+        leaves = [x.clone().requires_grad_(True) for x in (f, w, b)]
+        grads = torch.autograd.grad(loss(leaves).sum(), leaves)
+        for k in range(3):
+            v = grads[k] / grads[k].abs().max()
+            ends = []
+            for s in (1, -1):
+                args = [f, w, b]
+                args[k] = args[k] + s * 1e-2 * v
+                ends.append(float(loss(args).double().sum()))
+            want = float((grads[k].double() * v.double()).sum())
+            assert abs((ends[0] - ends[1]) / 2e-2 - want) <= 0.06, k
+
+
+def test_refusals(device):
+    f, w, b, t = _inputs(device, 4, 10, 8, torch.float32, True, seed=18)
+    ce, kd = det_utils.vocabulary_cross_entropy, det_utils.vocabulary_distillation
+    tc, tl = _teacher(device, 4, 10, 3, seed=1)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        ce(f.cpu(), w, t)
+    with pytest.raises(RuntimeError, match="weight is on"):
+        ce(f, w.cpu(), t)
+    with pytest.raises(RuntimeError, match="targets is on"):
+        ce(f, w, t.cpu())
+    with pytest.raises(TypeError, match="int64"):
+        ce(f, w, t.int())
+    with pytest.raises(TypeError, match="float64"):
+        ce(f.double(), w.double(), t)
+    with pytest.raises(TypeError, match="weight is"):
+        ce(f, w.half(), t)
+    with pytest.raises(TypeError, match="bias is"):
+        ce(f, w, t, bias=b.half())
+    with pytest.raises(ValueError, match="features"):
+        ce(f, w[:, :4], t)
+    with pytest.raises(ValueError, match="features"):
+        ce(f, w, t[:3])
+    with pytest.raises(ValueError, match="bias"):
+        ce(f, w, t, bias=b[:3])
+    with pytest.raises(ValueError, match="reduction"):
+        ce(f, w, t, reduction="avg")
+    with pytest.raises(ValueError, match="classes"):
+        ce(f, w[:0], t)
+    with pytest.raises(ValueError, match="temperature"):
+        kd(f, w, tl, tc, temperature=0.0)
+    with pytest.raises(ValueError, match="temperature"):
+        kd(f, w, tl, tc, temperature=NAN)
+    with pytest.raises(ValueError, match="teacher"):
+        kd(f, w, tl[:, :2], tc)
+    with pytest.raises(ValueError, match="teacher"):
+        kd(f, w, tl[:, :0], tc[:, :0])
+    with pytest.raises(TypeError, match="int64"):
+        kd(f, w, tl, tc.int())
+    with pytest.raises(RuntimeError, match="teacher"):
+        kd(f, w, tl.clone().requires_grad_(True), tc)
+    with pytest.raises(_C.OdBoxesError, match="256"):
+        kd(f, w, torch.zeros((4, 257), device=device), torch.zeros((4, 257), dtype=torch.int64, device=device))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        leaf = f.clone().requires_grad_(True)
+        g = torch.autograd.grad(ce(leaf, w, t), leaf, torch.ones((), device=device, requires_grad=True), create_graph=True)[0]
+        g.sum().backward()
+
+
+def test_another_stream_and_captured_steps(device):
+    f, w, b, t = _inputs(device, 500, 1204, 256, torch.bfloat16, True, seed=19)
+    tc, tl = _teacher(device, 500, 1204, 8, seed=20)
+
+    def step(x):
+        loss = det_utils.vocabulary_cross_entropy(x[0], x[1], t, bias=x[2]) \
+            + det_utils.vocabulary_distillation(x[0], x[1], tl, tc, bias=x[2], temperature=2.0)
+        return [loss.detach()] + list(torch.autograd.grad(loss, x))
+
+    def fresh():
+        return [x.detach().clone().requires_grad_(True) for x in (f, w, b)]
+    want = step(fresh())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(fresh())
+    side.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+    from object_detection_amd.graph_step import capture
+    leaves = fresh()
+    first, second = capture(lambda: step(leaves), device), capture(lambda: step(leaves), device)
+    for k in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(f * (1 + 0.25 * k))
+            t.copy_(torch.where(torch.arange(500, device=device) % (k + 2) == 0, -torch.ones_like(t), t.abs()))
+        outs = [x.clone() for x in first.replay()]
+        eager = step([x.detach().clone().requires_grad_(True) for x in leaves])
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(outs, eager)), k
+        # two graphs at once, each with scratch of its own
+        side.wait_stream(torch.cuda.current_stream())
+        second.replay()
+        with torch.cuda.stream(side):
+            first.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(first.outputs, eager)), k
+        assert all(torch.equal(x, y) for x, y in zip(second.outputs, eager)), k
+
+
+def test_head_over_a_vocabulary_trains_through_tower_and_losses(device):
+    """A classification head as it would be used: conv + GroupNormAct tower on a channels-last map, embeddings per anchor,
+    cross entropy on the matched anchors and distillation on some, backward to every parameter; against the same head in
+    elementary fp32 operations.  The convolutions' own rounding (four of 288 products, 2^-24 * 288 * 4 of the largest value)
+    is behind the 1e-3, as in the towers' own test."""
+    torch.manual_seed(0)
+    A, D, V = 3, 64, 500
+    from object_detection_amd.retinanet import _conv_tower, _to_anchor_major
+    fused = nn.Sequential(_conv_tower(32, partial(GroupNormAct, 8)), nn.Conv2d(32, A * D, 3, 1, 1)).to(device)
+    plain = nn.Sequential(_conv_tower(32, partial(nn.GroupNorm, 8)), nn.Conv2d(32, A * D, 3, 1, 1)).to(device)
+    plain.load_state_dict(fused.state_dict())
+    fused = fused.to(memory_format=torch.channels_last)
+    classes = (torch.randn((V, D), device=device) / 8)
+    bias = torch.zeros(V, device=device)
+    x = torch.randn((2, 32, 12, 10), device=device)
+    matched = torch.randint(-2, 4, (2, 12 * 10 * A), device=device)
+    labels = torch.tensor([5, 77, 499, 0], device=device)
+    targets = torch.where(matched >= 0, labels[matched.clamp(min=0)], matched)
+    tl, tc = torch.randn((2, 12 * 10 * A, 6), device=device), torch.randint(0, V, (2, 12 * 10 * A, 6), device=device)
+    tc[matched < 2] = -1
+
+    wa, ba = classes.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+    rows = _to_anchor_major(fused(x.contiguous(memory_format=torch.channels_last)), D)
+    assert rows.shape == (2, 360, D)
+    loss_a = det_utils.vocabulary_cross_entropy(rows, wa, targets, bias=ba) \
+        + 0.5 * det_utils.vocabulary_distillation(rows, wa, tl, tc, bias=ba, temperature=2.0)
+    ga = torch.autograd.grad(loss_a, list(fused.parameters()) + [wa, ba])
+
+    wb, bb = classes.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+    rows = _to_anchor_major(plain(x), D).reshape(-1, D)
+    z = rows @ wb.t() + bb
+    t = targets.reshape(-1)
+    ce = nn.functional.cross_entropy(z, t.clamp(min=0), reduction="none")[t >= 0].mean()
+    on = (tc.reshape(-1, 6) >= 0).all(1)
+    q = torch.log_softmax(z[on] / 2, dim=1)
+    p = torch.zeros_like(q).scatter_add_(1, tc.reshape(-1, 6)[on], torch.softmax(tl.reshape(-1, 6)[on] / 2, dim=1))
+    kd = 4 * (torch.xlogy(p, p) - p * q).sum(1).mean()
+    loss_b = ce + 0.5 * kd
+    gb = torch.autograd.grad(loss_b, list(plain.parameters()) + [wb, bb])
+    assert abs(float(loss_a.detach()) - float(loss_b.detach())) <= 1e-3 * abs(float(loss_b.detach()))
+    for p_, q_ in zip(ga, gb):
+        assert float((p_ - q_).abs().max()) <= 1e-2 * float(q_.abs().max()) + 1e-7
