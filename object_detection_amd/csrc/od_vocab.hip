@@ -29,7 +29,8 @@ namespace {
 using namespace od;
 
 constexpr int VT = 256;                 // threads per workgroup: four waves in a 2 x 2 arrangement
-constexpr int TILE = 128;               // rows and columns of a workgroup's tile (64 x 64 per wave)
+constexpr int TILE = 128;               // rows and classes of a workgroup's tile where both operands stream
+constexpr int ROW_TILE = 256;           // rows and classes are padded to this: tiles of every kernel divide it
 constexpr int STAGE = TILE * 128;       // bytes of one operand's stage in LDS
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float LN2 = 0.69314718055994531f;
@@ -66,77 +67,111 @@ template <> struct Mma<float> {
 typedef __attribute__((address_space(3))) char lds_char;
 typedef const __attribute__((address_space(1))) uint32_t* global_words;
 
+__device__ __forceinline__ long long up_to(long long v, int to) { return (v + to - 1) / to * to; }
+
 // 16 bytes per lane from global memory straight into LDS: lane l lands at base + 16 l
 __device__ __forceinline__ void stage16(const char* src, char* base) {
     __builtin_amdgcn_global_load_lds((global_words)src, (__attribute__((address_space(3))) uint32_t*)base, 16, 0, 0);
 }
 
-// ---- operand with K contiguous: 128 rows x 128 bytes of K.  The 16-byte chunks of a row are permuted by row % 8, which
-// spreads the eight rows that a quarter wave reads at once over all banks.
+// A tile of classes is the A operand, whose 32 rows reach a lane's accumulators in four groups of four; reading tile row
+// class_row(r) as row r of the operand makes them 16 neighbouring classes: acc[i] is class 16 (lane / 32) + i of the 32.
+__device__ __forceinline__ int class_row(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
+
+// LDS serves 16 lanes of a 16-byte read at a time, from 64 banks.  The 16-byte chunks of a tile row are permuted by an
+// exclusive-or with a function of the row under which those 16 lanes' chunks lie in 16 different bank groups: for the row
+// order of class_row (rows 0-3, 16-19, 4-7, 20-23, ...), and for rows in order.
+// ROW bytes a row: a multiple of 256 needs four bits; an odd multiple of 128 has one from the row's own parity.
+template <int ROW>
+__device__ __forceinline__ int class_swizzle(int r) {
+    return ROW % 256 == 0 ? ((r & 7) | (((r >> 4) & 1) << 3)) : (((r >> 1) & 3) | (((r >> 4) & 1) << 2));
+}
+__device__ __forceinline__ int line_swizzle(int r) { return (r >> 1) & 7; }     // rows of 128 bytes, in order
+
+// ---- operand with K contiguous, streamed: R rows x 128 bytes of K per stage, by THREADS threads
+template <int R, int THREADS, bool CLASSES>
 struct ChunkedOperand {
-    const char* row[4];                 // this lane's source rows (four rows of eight per wave and instruction)
-    int chunk;
-    __device__ __forceinline__ void init(const char* base, long long pitch, long long first, long long last) {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    static constexpr int PASSES = R * 8 / THREADS;
+    const char* base;                   // the tile's first row
+    uint32_t offset[PASSES];            // this lane's rows and chunks, within 31 bits
+    __device__ __forceinline__ void init(const char* from, long long pitch, long long first, long long last) {
+        first = min(first, last);                                   // a tile wholly behind the last row
+        base = from + first * pitch;
+        const int most = (int)min(last - first, (long long)R);      // rows past the last one repeat it
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            long long r = first + (wave * 4 + i) * 8 + (lane >> 3);
-            row[i] = base + (r < last ? r : last) * pitch;          // rows past the end repeat the last one
+        for (int i = 0; i < PASSES; ++i) {
+            const int r = (i * THREADS + threadIdx.x) >> 3;
+            const int swz = CLASSES ? class_swizzle<128>(r) : line_swizzle(r);
+            offset[i] = (uint32_t)min(r, most) * (uint32_t)pitch + (((threadIdx.x & 7) ^ swz) << 4);
         }
-        chunk = ((lane & 7) ^ (lane >> 3)) * 16;
     }
     __device__ __forceinline__ void stage(char* lds, long long kbytes) const {
-        const int wave = threadIdx.x >> 6;
+        const char* from = base + kbytes;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) stage16(row[i] + kbytes + chunk, lds + (wave * 4 + i) * 1024);
+        for (int i = 0; i < PASSES; ++i) stage16(from + offset[i], lds + i * THREADS * 16 + (threadIdx.x >> 6) * 1024);
     }
     // fragment of rows [r0, r0 + 32), slab j of four
-    static __device__ __forceinline__ u32x4 frag(const char* lds, int r0, int j) {
-        const int lane = threadIdx.x & 63;
-        const int r = r0 + (lane & 31);
-        return *reinterpret_cast<const u32x4*>(lds + r * 128 + (((2 * j + (lane >> 5)) ^ (r & 7)) << 4));
+    static __device__ __forceinline__ u32x4 frag(const char* lds, int r0, int j, int lane) {
+        const int r = r0 + (CLASSES ? class_row(lane & 31) : (lane & 31));
+        const int swz = CLASSES ? class_swizzle<128>(r) : line_swizzle(r);
+        return *reinterpret_cast<const u32x4*>(lds + r * 128 + (((2 * j + (lane >> 5)) ^ swz) << 4));
     }
 };
 
-// ---- operand with K strided: KE rows of K x 128 contiguous elements; read transposed.
-template <typename T>
+// ---- operand with K strided, streamed: KE rows of K x W contiguous elements per stage; read transposed.
+template <typename T, int W, int THREADS>
 struct StridedOperand {
     static constexpr int KE = 128 / sizeof(T);                      // K per stage
-    static constexpr int ROWB = TILE * sizeof(T);                   // bytes per K row
+    static constexpr int ROWB = W * sizeof(T);                      // bytes per K row
     static constexpr int CHUNKS = ROWB / 16;
-    static constexpr int RPI = 1024 / ROWB;                         // K rows per wave and instruction
+    static constexpr int PASSES = KE * CHUNKS / THREADS;
     const char* base;
     long long pitch;
-    int lane_row, first_byte, last_byte;
-    // chunk permutation of K row k: the rows that one transposing read touches at once go to different banks
+    uint32_t offset[PASSES];            // this lane's rows and columns of a stage, within 31 bits
+    // Chunk permutation of K row k.  16-bit: a transposing read takes two neighbouring 32-byte pieces of four rows at a
+    // time; they land in eight different bank groups.  fp32: two rows, four apart, 128 bytes each.
     static __device__ __forceinline__ int swizzle(int k) {
-        return sizeof(T) == 2 ? (((k & 3) | (((k >> 3) & 1) << 2)) << 1) : (((k >> 2) & 1) << 3);
+        if (sizeof(T) == 4) return ((k >> 2) & 1) << 3;
+        return ROWB % 256 == 0 ? (k & 3) << 2 : ((k >> 1) & 1) << 2;
     }
+    static __device__ __forceinline__ uint32_t column(int i, uint32_t first_byte, uint32_t last) {
+        const int at = i * THREADS + threadIdx.x;
+        const uint32_t c = first_byte + (((at % CHUNKS) ^ swizzle(at / CHUNKS)) << 4);
+        return c < last ? c : last;                                 // columns past the end repeat the last chunk
+    }
+    uint32_t first_byte, last_byte;
     __device__ __forceinline__ void init(const char* b, long long p, long long first_col, long long cols) {
         base = b;
         pitch = p;
-        lane_row = (threadIdx.x & 63) / CHUNKS;
-        first_byte = (int)(first_col * sizeof(T));
-        last_byte = (int)(cols * sizeof(T)) - 16;                   // columns past the end repeat the last chunk
+        first_byte = (uint32_t)(first_col * (long long)sizeof(T));
+        last_byte = (uint32_t)(cols * (long long)sizeof(T)) - 16;
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+            offset[i] = (uint32_t)((i * THREADS + threadIdx.x) / CHUNKS) * (uint32_t)p + column(i, first_byte, last_byte);
     }
     // K rows [k0, k0 + KE); rows past `last` repeat it
     __device__ __forceinline__ void stage(char* lds, long long k0, long long last) const {
-        const int wave = threadIdx.x >> 6, pos = (threadIdx.x & 63) % CHUNKS;
+        const char* from = base + k0 * pitch;
+        if (k0 + KE - 1 <= last) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int k = (wave * 4 + i) * RPI + lane_row;
-            const long long r = k0 + k;
-            const int byte = first_byte + ((pos ^ swizzle(k)) << 4);
-            stage16(base + (r < last ? r : last) * pitch + (byte < last_byte ? byte : last_byte), lds + (wave * 4 + i) * 1024);
+            for (int i = 0; i < PASSES; ++i) stage16(from + offset[i], lds + i * THREADS * 16 + (threadIdx.x >> 6) * 1024);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int r = min((i * THREADS + (int)threadIdx.x) / CHUNKS, (int)(last - k0));
+                stage16(from + (r * pitch + column(i, first_byte, last_byte)),
+                        lds + i * THREADS * 16 + (threadIdx.x >> 6) * 1024);
+            }
         }
     }
-    static __device__ __forceinline__ u32x4 frag(const char* lds, int m0, int j) {
-        const int lane = threadIdx.x & 63, h = lane >> 5;
+    // fragment of columns [m0, m0 + 32), slab j of four
+    static __device__ __forceinline__ u32x4 frag(const char* lds, int m0, int j, int lane) {
+        const int h = lane >> 5;
         if constexpr (sizeof(T) == 2) {
             // a transposing read hands lane i of 16 the i-th element of the four rows that lanes 4r .. 4r+3 point at
             const int r = (lane & 15) >> 2;
             const int chunk = (m0 >> 3) + (((lane >> 4) & 1) << 1) + ((lane & 3) >> 1);
-            const char* p = lds + (16 * j + 8 * h + r) * ROWB + ((chunk ^ ((r | (h << 2)) << 1)) << 4) + ((lane & 1) << 3);
+            const char* p = lds + (16 * j + 8 * h + r) * ROWB + ((chunk ^ swizzle(r)) << 4) + ((lane & 1) << 3);
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * ROWB));
             const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
@@ -158,6 +193,18 @@ struct StridedOperand {
 __device__ __forceinline__ void stage_barrier() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
+}
+
+// Order of a stage's instructions: `ahead` LDS reads first, then `steps` times `mfma` products and `reads` further reads.
+template <int AHEAD, int STEPS, int PRODUCTS, int READS>
+__device__ __forceinline__ void interleave() {
+    constexpr int READ = 0x100, MFMA = 0x008;
+    __builtin_amdgcn_sched_group_barrier(READ, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(MFMA, PRODUCTS, 0);
+        __builtin_amdgcn_sched_group_barrier(READ, READS, 0);
+    }
 }
 
 // Workgroup number -> work number such that each of the eight XCDs (hardware hands workgroups to them in turn) gets one
@@ -284,7 +331,7 @@ __global__ __launch_bounds__(VT) void teacher_kernel(const long long* __restrict
     }
 }
 
-// Features of the valid rows, dense: [rows rounded up to TILE][dim_pad], zero behind the last valid row and the last
+// Features of the valid rows, dense: [rows rounded up to ROW_TILE][dim_pad], zero behind the last valid row and the last
 // column.  A thread copies one 16-byte chunk; sources that are not aligned for it are read element by element.
 template <typename T>
 __global__ __launch_bounds__(VT) void pack_rows_kernel(const T* __restrict__ src, long long pitch, int dim, int dim_pad,
@@ -307,7 +354,7 @@ __global__ __launch_bounds__(VT) void pack_rows_kernel(const T* __restrict__ src
             for (int i = 0; i < E; ++i) v[i] = c + i < dim ? p[i] : Elem<T>::from_float(0.0f);
         }
     } else {
-        if (count && r >= (limit + TILE - 1) / TILE * TILE) return;            // no tile reads behind the last one's end
+        if (count && r >= up_to(limit, ROW_TILE)) return;                 // no tile reads behind the last one's end
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] = Elem<T>::from_float(0.0f);
     }
@@ -332,142 +379,347 @@ struct ProductArgs {
     const float* bias2;                 // at the piece's first class
     const int* count;
     int tiles, splits;                  // class tiles of the piece, workgroups per row tile
+    int row_tiles;
     float scale;                        // log2(e) / temperature
     long long rows_pad;
     // forward
     float2* part;                       // [splits][rows_pad] (maximum, sum), log2 units
     // backward
     const float* lse2;                  // [rows_pad] in log2 units
-    const float* row_grad;              // [rows_pad]
-    void* dz;                           // [rows_pad][piece]
+    void* dz;                           // rows_pad x piece, see Dz
     long long piece;
 };
 
-// Accumulators: acc[f][g] holds classes f*32 + 8*(i/4) + 4*(lane/32) + i%4 (i = 0 .. 15) of row g*32 + lane%32.
+// What the gradient products hold dz, weight and features in, and the power of two that dz is stored under.
+template <typename T> struct GradOf { typedef _Float16 type; static constexpr int LOG2_DZ = 14; };
+template <> struct GradOf<float> { typedef float type; static constexpr int LOG2_DZ = 0; };
+
+// dz lies in blocks of 256 rows x 128 bytes of classes, [rows / 256][classes / DZ_CLASSES][256][DZ_CLASSES]: a tile of the
+// product writes, and a stage of either gradient product reads, pieces of 8 KiB or more that are contiguous (rows of a
+// plain layout lie a piece apart: writing 16384 x 8192 of them took 153 us instead of 110).
+template <typename G> struct Dz {
+    static constexpr int CLASSES = 128 / sizeof(G);                 // per block
+    static constexpr long long BLOCK = 256 * CLASSES;               // elements
+    // element (row, class) of a piece
+    static __host__ __device__ __forceinline__ long long at(long long row, long long cls, long long piece) {
+        return ((row >> 8) * (piece / CLASSES) + cls / CLASSES) * BLOCK + (row & 255) * CLASSES + cls % CLASSES;
+    }
+};
+
+// Folds a tile's logits into the running maximum and sum of NF rows of this lane.  acc[f][g][i]: class 32 f + 16 h + i of
+// the tile; bias: at class 16 h.
+template <int CF, int NF>
+__device__ __forceinline__ void fold(f32x16 (&acc)[CF][NF], const float* bias, float scale, float (&m)[NF], float (&s)[NF]) {
+    float top[NF];
+#pragma unroll
+    for (int g = 0; g < NF; ++g) top[g] = m[g];
+#pragma unroll
+    for (int f = 0; f < CF; ++f)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const vec4f b = *reinterpret_cast<const vec4f*>(bias + f * 32 + 4 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int g = 0; g < NF; ++g) {
+                    const float z = fmaf(acc[f][g][4 * q + e], scale, b[e]);
+                    acc[f][g][4 * q + e] = z;
+                    top[g] = fmaxf(top[g], z);
+                }
+        }
+#pragma unroll
+    for (int g = 0; g < NF; ++g) {
+        float sum = s[g] * __builtin_amdgcn_exp2f(m[g] - top[g]);
+#pragma unroll
+        for (int f = 0; f < CF; ++f)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(acc[f][g][i] - top[g]);
+        m[g] = top[g];
+        s[g] = sum;
+    }
+}
+
+// Writes a tile of q times the power of two to dz, from class `first` (a multiple of 32) on; rows behind the last valid one
+// get zeros.  shift: lse - LOG2_DZ;  out: the row's element of the piece's class 16 h.
+template <typename G, int CF, int NF>
+__device__ __forceinline__ void store_dz(const f32x16 (&acc)[CF][NF], const float* bias, float scale, const float (&shift)[NF],
+                                         const bool (&on)[NF], G* (&out)[NF], int first) {
+    constexpr int E = 16 / sizeof(G);
+#pragma unroll
+    for (int f = 0; f < CF; ++f) {
+        const long long at = (first + f * 32) / Dz<G>::CLASSES * Dz<G>::BLOCK + (first + f * 32) % Dz<G>::CLASSES;
+#pragma unroll
+        for (int c = 0; c < 16; c += E) {
+            float b[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) b[e] = bias[f * 32 + c + e];
+#pragma unroll
+            for (int g = 0; g < NF; ++g) {
+                float v[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    v[e] = __builtin_amdgcn_exp2f(fmaf(acc[f][g][c + e], scale, b[e] - shift[g]));
+                    if (!on[g]) v[e] = 0.0f;
+                }
+                store_vec<G, E>(out[g] + at + c, v);
+            }
+        }
+    }
+}
+
+// Joins the two lanes that share a row; lane < 32 then holds it.
+__device__ __forceinline__ void join_halves(float& m, float& s) {
+    const float om = __shfl_xor(m, 32, 64), os = __shfl_xor(s, 32, 64);
+    const float top = fmaxf(m, om);
+    s = s * __builtin_amdgcn_exp2f(m - top) + os * __builtin_amdgcn_exp2f(om - top);
+    m = top;
+}
+
+// Rows of up to 1 KiB: a wave keeps the features of its 32 NF rows in registers for the whole sweep over the classes (128
+// VGPRs), and only tiles of CT classes stream through LDS, two of them in turn.  That takes 16 bytes per cycle and compute
+// unit out of L2 at full matrix rate where a 128 x 128 tile that streams both operands takes 64, all that L2 gives.  Two
+// workgroups per compute unit drift apart, so that one's exponentials run beside the other's products.
+template <typename T, int KS, bool GRAD>
+struct Resident {
+    static constexpr int ROW = KS * 32;                             // bytes of a row
+    static constexpr int NF = KS <= 16 ? 2 : 1;                     // row fragments per wave
+    static constexpr int CT = KS <= 16 ? 64 : 32;                   // classes per tile
+    static constexpr int ROWS = 4 * 32 * NF;                        // rows per workgroup
+};
+
+template <typename T, int KS, bool GRAD>
+__global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
+    typedef Resident<T, KS, GRAD> S;
+    typedef typename GradOf<T>::type G;
+    constexpr int ROW = S::ROW, NF = S::NF, CT = S::CT, CF = CT / 32, CHUNKS = ROW / 16, PASSES = CT * CHUNKS / VT;
+    __shared__ __align__(1024) char lds0[CT * ROW], lds1[CT * ROW];
+    __shared__ __align__(16) float s_bias[2][CT];
+    const int id = xcd_range(blockIdx.x, gridDim.x);
+    const int split = id / p.row_tiles;
+    const long long r0 = (long long)(id % p.row_tiles) * S::ROWS;
+    const int count = *p.count;
+    if (r0 >= count) return;
+    const int t0 = (int)((long long)p.tiles * split / p.splits), t1 = (int)((long long)p.tiles * (split + 1) / p.splits);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
+    const long long mine = r0 + wave * 32 * NF + (lane & 31);      // this lane's first row
+
+    uint32_t offset[PASSES];                                        // this lane's source bytes within a class tile
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+        const int at = i * VT + threadIdx.x, r = at / CHUNKS;
+        offset[i] = r * (uint32_t)p.weight_pitch + (((at % CHUNKS) ^ class_swizzle<ROW>(r)) << 4);
+    }
+    const long long behind = p.last_class + 1 - p.first_class;      // classes of the piece that exist
+    auto stage = [&](char* to, int t) {
+        const long long c = (long long)t * CT;
+        const char* from = p.weight + (p.first_class + c) * p.weight_pitch;
+        if (c + CT <= behind) {
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) stage16(from + offset[i], to + i * VT * 16 + wave * 1024);
+        } else {                                                    // rows behind the last class repeat it
+#pragma unroll
+            for (int i = 0; i < PASSES; ++i) {
+                const int at = i * VT + threadIdx.x, r = at / CHUNKS;
+                const long long cls = c + r < behind ? p.first_class + c + r : p.last_class;
+                stage16(p.weight + cls * p.weight_pitch + (((at % CHUNKS) ^ class_swizzle<ROW>(r)) << 4),
+                        to + i * VT * 16 + wave * 1024);
+            }
+        }
+    };
+
+    float m[NF], s[NF], shift[NF];
+    bool on[NF];
+    G* out[NF];
+#pragma unroll
+    for (int g = 0; g < NF; ++g) {
+        m[g] = LOWEST;
+        s[g] = 0.0f;
+        if (GRAD) {
+            shift[g] = p.lse2[mine + g * 32] - GradOf<T>::LOG2_DZ;
+            on[g] = mine + g * 32 < count;
+            out[g] = (G*)p.dz + Dz<G>::at(mine + g * 32, 16 * h, p.piece);
+        }
+    }
+    float tile_bias = 0.0f;
+    auto fetch_bias = [&](int t) { if (threadIdx.x < CT && t < t1) tile_bias = p.bias2[(long long)t * CT + threadIdx.x]; };
+
+    if (t0 < t1) {
+        fetch_bias(t0);
+        stage(lds0, t0);
+    }
+    u32x4 rows[NF][KS];
+#pragma unroll
+    for (int g = 0; g < NF; ++g)
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+            rows[g][k] = *reinterpret_cast<const u32x4*>(p.features + (mine + g * 32) * ROW + k * 32 + 16 * h);
+    if (threadIdx.x < CT) s_bias[t0 & 1][threadIdx.x] = tile_bias;
+    fetch_bias(t0 + 1);
+
+    const int my_class = class_row(lane & 31);
+    int first_chunk = my_class * ROW + ((h ^ class_swizzle<ROW>(my_class)) << 4);
+    auto step = [&](const char* now, char* next, int t) {
+        stage_barrier();
+        if (threadIdx.x < CT) s_bias[(t + 1) & 1][threadIdx.x] = tile_bias;
+        fetch_bias(t + 2);
+        if (t + 1 < t1) stage(next, t + 1);
+        f32x16 acc[CF][NF];
+#pragma unroll
+        for (int f = 0; f < CF; ++f)
+#pragma unroll
+            for (int g = 0; g < NF; ++g)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
+        // chunk (2 k + h) ^ swizzle is chunk h ^ swizzle with the bits of 2 k flipped (rows of an odd multiple of 128 bytes:
+        // of its low three bits); formed anew in every step, since KS addresses held over the loop would not fit
+        asm volatile("" : "+v"(first_chunk));
+        constexpr int FLIP = ROW % 256 == 0 ? 15 : 7;
+        // the wave that multiplies goes first, the one beside it fills in with its exponentials
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            u32x4 a[CF];
+            const char* from = now + ((first_chunk ^ (((2 * k) & FLIP) << 4)) + (((2 * k) & ~FLIP) << 4));
+#pragma unroll
+            for (int f = 0; f < CF; ++f) a[f] = *reinterpret_cast<const u32x4*>(from + f * 32 * ROW);
+#pragma unroll
+            for (int f = 0; f < CF; ++f)
+#pragma unroll
+                for (int g = 0; g < NF; ++g) acc[f][g] = Mma<T>::run(a[f], rows[g][k], acc[f][g]);
+        }
+        interleave<4 * CF, KS, CF * NF*(sizeof(T) == 4 ? 4 : 1), CF>();
+        __builtin_amdgcn_s_setprio(0);
+        const float* bias = s_bias[t & 1] + 16 * h;
+        if (GRAD) store_dz<G, CF, NF>(acc, bias, p.scale, shift, on, out, t * CT);
+        else fold<CF, NF>(acc, bias, p.scale, m, s);
+    };
+    int t = t0;
+    while (t < t1) {
+        step(lds0, lds1, t++);
+        if (t == t1) break;
+        step(lds1, lds0, t++);
+    }
+    if (!GRAD) {
+#pragma unroll
+        for (int g = 0; g < NF; ++g) {
+            join_halves(m[g], s[g]);
+            if (h == 0) p.part[(long long)split * p.rows_pad + mine + g * 32] = make_float2(m[g], s[g]);
+        }
+    }
+}
+
+// Wider rows: both operands stream through LDS in stages of 128 bytes of K.
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
-    __shared__ __align__(1024) char lds[4 * STAGE];                 // two stages of (classes, rows)
+    typedef typename GradOf<T>::type G;
+    __shared__ __align__(1024) char lds0[2 * STAGE], lds1[2 * STAGE];       // two stages of (classes, rows)
     __shared__ float2 joined[2][TILE];
+    __shared__ __align__(16) float s_bias[TILE];
     const int id = xcd_range(blockIdx.x, gridDim.x);
-    const int split = id % p.splits;
-    const long long r0 = (long long)(id / p.splits) * TILE;
-    if (r0 >= *p.count) return;
+    const int split = id / p.row_tiles;
+    const long long r0 = (long long)(id % p.row_tiles) * TILE;
+    const int count = *p.count;
+    if (r0 >= count) return;
     const int t0 = (int)((long long)p.tiles * split / p.splits), t1 = (int)((long long)p.tiles * (split + 1) / p.splits);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
     const int wc = (wave & 1) * 64, wr = (wave >> 1) * 64;          // this wave's classes and rows within the tile
     constexpr int KE = 128 / sizeof(T);
     const int ksteps = p.dim_pad / KE;
-
-    ChunkedOperand rows, cls;
+    typedef ChunkedOperand<TILE, VT, true> Classes;
+    typedef ChunkedOperand<TILE, VT, false> Rows;
+    Rows rows;
+    Classes cls;
     rows.init(p.features, (long long)p.dim_pad * sizeof(T), r0, r0 + TILE);
 
-    float m[2], s[2], lse2[2], grad[2];
+    float m[2], s[2], shift[2];
+    bool on[2];
+    G* out[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
         m[g] = LOWEST;
         s[g] = 0.0f;
         if (GRAD) {
-            lse2[g] = p.lse2[r0 + wr + g * 32 + (lane & 31)];
-            grad[g] = p.row_grad[r0 + wr + g * 32 + (lane & 31)];
+            const long long row = r0 + wr + g * 32 + (lane & 31);
+            shift[g] = p.lse2[row] - GradOf<T>::LOG2_DZ;
+            on[g] = row < count;
+            out[g] = (G*)p.dz + Dz<G>::at(row, 16 * h, p.piece);
         }
     }
 
     f32x16 acc[2][2];
-    int buf = 0;
-    if (t0 < t1) {
-        cls.init(p.weight, p.weight_pitch, p.first_class + (long long)t0 * TILE, p.last_class);
-        cls.stage(lds, 0);
-        rows.stage(lds + STAGE, 0);
-    }
-    for (int t = t0; t < t1; ++t) {
+    auto clear = [&] {
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int g = 0; g < 2; ++g)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
-        for (int k = 0; k < ksteps; ++k) {
-            stage_barrier();
-            const char* now = lds + buf * 2 * STAGE;
-            char* next = lds + (buf ^ 1) * 2 * STAGE;
-            if (k + 1 < ksteps) {
-                cls.stage(next, (long long)(k + 1) * 128);
-                rows.stage(next + STAGE, (long long)(k + 1) * 128);
-            } else if (t + 1 < t1) {
-                cls.init(p.weight, p.weight_pitch, p.first_class + (long long)(t + 1) * TILE, p.last_class);
-                cls.stage(next, 0);
-                rows.stage(next + STAGE, 0);
-            }
-            buf ^= 1;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 a[2], b[2];
-#pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    a[f] = ChunkedOperand::frag(now, wc + f * 32, j);
-                    b[f] = ChunkedOperand::frag(now + STAGE, wr + f * 32, j);
-                }
-#pragma unroll
-                for (int f = 0; f < 2; ++f)
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(a[f], b[g], acc[f][g]);
-            }
+    };
+    int next_t = t0, next_k = 0;                                    // what is staged next
+    float tile_bias = 0.0f;
+    auto fetch_bias = [&](int t) { if (threadIdx.x < TILE && t < t1) tile_bias = p.bias2[(long long)t * TILE + threadIdx.x]; };
+    auto stage_next = [&](char* to) {
+        if (next_t >= t1) return;
+        if (next_k == 0) cls.init(p.weight, p.weight_pitch, p.first_class + (long long)next_t * TILE, p.last_class);
+        cls.stage(to, (long long)next_k * 128);
+        rows.stage(to + STAGE, (long long)next_k * 128);
+        if (++next_k == ksteps) {
+            next_k = 0;
+            ++next_t;
         }
-        const float* bias = p.bias2 + (long long)t * TILE + wc + 4 * h;
-        if (!GRAD) {
-            float top[2] = {m[0], m[1]};
+    };
+    auto multiply = [&](const char* now) {
+        int at = lane;
+        asm volatile("" : "+v"(at));                                // addresses are formed anew in every stage, see resident_kernel
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            u32x4 a[2], b[2];
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                a[f] = Classes::frag(now, wc + f * 32, j, at);
+                b[f] = Rows::frag(now + STAGE, wr + f * 32, j, at);
+            }
 #pragma unroll
             for (int f = 0; f < 2; ++f)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const vec4f bq = *reinterpret_cast<const vec4f*>(bias + f * 32 + 8 * q);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            const float z = fmaf(acc[f][g][4 * q + e], p.scale, bq[e]);
-                            acc[f][g][4 * q + e] = z;
-                            top[g] = fmaxf(top[g], z);
-                        }
-                }
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                float sum = s[g] * __builtin_amdgcn_exp2f(m[g] - top[g]);
-#pragma unroll
-                for (int f = 0; f < 2; ++f)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(acc[f][g][i] - top[g]);
-                m[g] = top[g];
-                s[g] = sum;
-            }
-        } else {
-            T* out = (T*)p.dz + (long long)t * TILE + wc + 4 * h;
-#pragma unroll
-            for (int f = 0; f < 2; ++f)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const vec4f bq = *reinterpret_cast<const vec4f*>(bias + f * 32 + 8 * q);
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        float v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float z = fmaf(acc[f][g][4 * q + e], p.scale, bq[e] - lse2[g]);
-                            v[e] = grad[g] == 0.0f ? 0.0f : grad[g] * __builtin_amdgcn_exp2f(z);
-                        }
-                        store_vec<T, 4>(out + (r0 + wr + g * 32 + (lane & 31)) * p.piece + f * 32 + 8 * q, v);
-                    }
-                }
+                for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(a[f], b[g], acc[f][g]);
         }
+        interleave<8, 4, 4 * (sizeof(T) == 4 ? 4 : 1), 4>();
+    };
+    // The bias of a tile is fetched ahead of the tile's first stage (waiting for it later would wait for the stages behind
+    // it as well) and written to LDS in its first step.  The two stages are variables of their own, used by turns in
+    // straight code: the compiler then knows that reading one need not wait for the loads into the other.
+    auto step = [&](const char* now, char* next, int& t, int& k) {
+        stage_barrier();
+        if (k == 0 && threadIdx.x < TILE) s_bias[threadIdx.x] = tile_bias;
+        if (k + 1 == ksteps) fetch_bias(t + 1);
+        stage_next(next);
+        multiply(now);
+        if (++k == ksteps) {
+            if (ksteps == 1) __syncthreads();                       // s_bias was written in this very step
+            const float* bias = s_bias + wc + 16 * h;
+            if (GRAD) store_dz<G, 2, 2>(acc, bias, p.scale, shift, on, out, t * TILE + wc);
+            else fold<2, 2>(acc, bias, p.scale, m, s);
+            clear();
+            k = 0;
+            ++t;
+        }
+    };
+    clear();
+    fetch_bias(t0);
+    stage_next(lds0);
+    int t = t0, k = 0;
+    const int steps = (t1 - t0) * ksteps;
+    for (int i = 0; i + 1 < steps; i += 2) {
+        step(lds0, lds1, t, k);
+        step(lds1, lds0, t, k);
     }
+    if (steps & 1) step(lds0, lds1, t, k);
     if (!GRAD) {
         // a row's classes lie in two lanes and two waves
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-            const float om = __shfl_xor(m[g], 32, 64), os = __shfl_xor(s[g], 32, 64);
-            const float top = fmaxf(m[g], om);
-            s[g] = s[g] * __builtin_amdgcn_exp2f(m[g] - top) + os * __builtin_amdgcn_exp2f(om - top);
-            m[g] = top;
+            join_halves(m[g], s[g]);
             if (h == 0) joined[wave & 1][wr + g * 32 + lane] = make_float2(m[g], s[g]);
         }
         __syncthreads();
@@ -576,51 +828,122 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
-// row_grad[place] = gradient of the row's loss times the temperature, times `scale[0]`; scale[1] = 1 / scale[0].
-// fp16: scale is the power of two that brings the largest |row_grad| into [2^13, 2^14): |dz| <= |row_grad| stays finite
-// and a probability of 2^-28 is still a normal number.  The other types take 1.
-__global__ __launch_bounds__(1024) void row_grads_kernel(const float* __restrict__ upstream, int reduction, RowLists lists,
-                                                         long long rows_pad, float temperature, int scaled,
-                                                         float* __restrict__ row_grad, float* __restrict__ scale) {
+// Scalars of a backward call, on the device.
+struct Scales {
+    float common;                       // largest |upstream| times share and temperature
+    uint32_t features_max, weight_max;  // bits of the largest finite |weighted feature| and |weight|
+};
+
+// Power of two under which an operand with this largest size lies in [2^13, 2^14): what is 2^27 times smaller is still a
+// normal fp16 number, what is 2^37 times smaller vanishes.
+__device__ __forceinline__ int exponent_of(uint32_t max_bits) {
+    if (max_bits == 0) return 0;
+    int e = 0;
+    (void)frexpf(u2f(max_bits), &e);                                // max = f * 2^e, f in [0.5, 1)
+    return min(max(14 - e, -100), 100);
+}
+
+// weight[place] = upstream of the row / the largest |upstream| (1 where one gradient serves all rows), zero behind the
+// last valid row; clears the maxima.
+__global__ __launch_bounds__(1024) void row_weights_kernel(const float* __restrict__ upstream, int reduction, RowLists lists,
+                                                           long long rows_pad, float temperature, float* __restrict__ weight,
+                                                           Scales* __restrict__ scales) {
     __shared__ float red[1024];
     const int count = *lists.count;
-    const float share = temperature / (reduction == OD_REDUCE_MEAN ? (float)max(1, count) : 1.0f);
-    float top = 0.0f;
-    if (scaled)
+    float top = 1.0f;
+    if (reduction == OD_REDUCE_NONE) {
+        top = 0.0f;
         for (int i = threadIdx.x; i < count; i += 1024) {
-            const float g = fabsf(upstream[reduction == OD_REDUCE_NONE ? lists.row_of[i] : 0] * share);
-            if (g < 3.0e38f) top = fmaxf(top, g);                  // infinities and NaN go through as they are
+            const float g = fabsf(upstream[lists.row_of[i]]);
+            if (g < __builtin_inff()) top = fmaxf(top, g);         // infinities and NaN go through as they are
         }
-    red[threadIdx.x] = top;
-    __syncthreads();
-    for (int o = 512; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + o]);
+        red[threadIdx.x] = top;
         __syncthreads();
-    }
-    float s = 1.0f;
-    if (scaled && red[0] > 0.0f) {
-        int e = 0;
-        (void)frexpf(red[0], &e);                                   // red[0] = f * 2^e, f in [0.5, 1)
-        e = min(max(14 - e, -100), 100);
-        s = ldexpf(1.0f, e);
+        for (int o = 512; o > 0; o >>= 1) {
+            if ((int)threadIdx.x < o) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + o]);
+            __syncthreads();
+        }
+        top = red[0] > 0.0f ? red[0] : 1.0f;
     }
     for (long long i = threadIdx.x; i < rows_pad; i += 1024)
-        row_grad[i] = i < count ? upstream[reduction == OD_REDUCE_NONE ? lists.row_of[i] : 0] * share * s : 0.0f;
+        weight[i] = i >= count ? 0.0f : reduction == OD_REDUCE_NONE ? upstream[lists.row_of[i]] / top : 1.0f;
     if (threadIdx.x == 0) {
-        scale[0] = s;
-        scale[1] = 1.0f / s;
+        const float share = temperature / (reduction == OD_REDUCE_MEAN ? (float)max(1, count) : 1.0f);
+        scales->common = (reduction == OD_REDUCE_NONE ? top : upstream[0]) * share;
+        scales->features_max = 0;
+        scales->weight_max = 0;
     }
 }
 
-// The target entries of a piece of dz: g (q - p).  Next to p = 1 it is expm1(log q) + (1 - p), which keeps the digits of
-// 1 - q of a confident row; for small p that sum would lose those of q and p.  Each (row, class) is written once: repeated classes carry their whole p in the first entry.
+// Largest finite |x| of rows [0, rows) (or the valid ones), each times its weight.  The maximum of integers does not
+// depend on the order of the atomics.
 template <typename T>
+__global__ __launch_bounds__(VT) void max_kernel(const T* __restrict__ x, long long pitch, int dim_pad,
+                                                 const float* __restrict__ weight, const int* __restrict__ count,
+                                                 long long rows, uint32_t* __restrict__ out) {
+    constexpr int E = 16 / sizeof(T);
+    const int chunks = dim_pad / E;
+    const long long total = (count ? (long long)*count : rows) * chunks;
+    float top = 0.0f;
+    for (long long at = (long long)blockIdx.x * VT + threadIdx.x; at < total; at += (long long)gridDim.x * VT) {
+        const long long r = at / chunks;
+        float v[E];
+        load_vec<T, E>(x + r * pitch + (at % chunks) * E, v);
+        const float w = weight ? weight[r] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float a = fabsf(v[i] * w);
+            if (a < __builtin_inff()) top = fmaxf(top, a);
+        }
+    }
+    __shared__ float red[VT / 64];
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {                                         // the atomics of a launch queue up: one per workgroup
+        for (int w = 1; w < VT / 64; ++w) top = fmaxf(top, red[w]);
+        if (top > 0.0f) atomicMax(out, f2u(top));
+    }
+}
+
+// Rows in the gradient products' type: x times the row's weight times the operand's power of two; zero rows behind the
+// last valid one up to a whole tile.
+template <typename T, typename G>
+__global__ __launch_bounds__(VT) void scale_rows_kernel(const T* __restrict__ x, long long pitch, int dim_pad,
+                                                        const float* __restrict__ weight, const int* __restrict__ count,
+                                                        long long rows, const uint32_t* __restrict__ max_bits,
+                                                        G* __restrict__ dst) {
+    constexpr int E = 16 / sizeof(T);
+    const int chunks = dim_pad / E;
+    const long long at = (long long)blockIdx.x * VT + threadIdx.x;
+    const long long r = at / chunks;
+    if (r >= rows) return;
+    if (count && r >= up_to((long long)*count, ROW_TILE)) return;
+    const int c = (int)(at % chunks) * E;
+    float v[E];
+    load_vec<T, E>(x + r * pitch + c, v);
+    const float f = max_bits ? ldexpf(1.0f, exponent_of(*max_bits)) : 1.0f;
+    const float w = weight ? weight[r] : 1.0f;
+    const bool on = !count || r < *count;
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = on ? v[i] * f * w : 0.0f;
+    if constexpr (sizeof(G) == sizeof(T)) {
+        store_vec<G, E>(dst + r * dim_pad + c, v);
+    } else {
+        static_assert(sizeof(G) == sizeof(T), "operands change their type, not their size");
+    }
+}
+
+// The target entries of a piece of dz: q - p.  Next to p = 1 it is expm1(log q) + (1 - p), which keeps the digits of
+// 1 - q of a confident row; for small p that sum would lose those of q and p.  Each (row, class) is written once: repeated
+// classes carry their whole p in the first entry.
+template <typename G>
 __global__ __launch_bounds__(VT) void correct_targets_kernel(const long long* __restrict__ targets, int top,
                                                              const float* __restrict__ prob, RowLists lists,
                                                              const float* __restrict__ lse2,
-                                                             const float* __restrict__ target_logit,
-                                                             const float* __restrict__ row_grad, long long first_class,
-                                                             long long piece, long long classes, T* __restrict__ dz) {
+                                                             const float* __restrict__ target_logit, long long first_class,
+                                                             long long piece, long long classes, float scale,
+                                                             G* __restrict__ dz) {
     const int n = top > 0 ? top : 1;
     const long long at = (long long)blockIdx.x * VT + threadIdx.x;
     const long long place = at / n;
@@ -632,15 +955,38 @@ __global__ __launch_bounds__(VT) void correct_targets_kernel(const long long* __
     const float p = top > 0 ? prob[src] : 1.0f;
     if (p == 0.0f) return;                                          // what the product wrote is q already
     const float log_q = target_logit[at] - lse2[place] * LN2;
-    const float g = row_grad[place];
-    const float v = g == 0.0f ? 0.0f : g * (p > 0.5f ? expm1f(log_q) + (1.0f - p) : expf(log_q) - p);
-    dz[place * piece + (c - first_class)] = Elem<T>::from_float(v);
+    const float v = p > 0.5f ? expm1f(log_q) + (1.0f - p) : expf(log_q) - p;
+    dz[Dz<G>::at(place, c - first_class, piece)] = Elem<G>::from_float(v * scale);
 }
 
+// 256 classes of KE rows of dz as an operand with K strided: four (fp32: eight) blocks side by side.
+template <typename T, int THREADS>
+struct DzOperand {
+    typedef StridedOperand<T, ROW_TILE, THREADS> Tile;              // its place in LDS, and its fragments
+    const char* base;
+    long long row_block;                // bytes from 256 rows to the next
+    uint32_t offset[Tile::PASSES];
+    __device__ __forceinline__ void init(const char* dz, long long piece, long long first_class) {
+        base = dz + Dz<T>::at(0, first_class, piece) * (long long)sizeof(T);
+        row_block = Dz<T>::at(256, 0, piece) * (long long)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < Tile::PASSES; ++i) {
+            const int at = i * THREADS + threadIdx.x, k = at / Tile::CHUNKS;
+            const int c = (at % Tile::CHUNKS) ^ Tile::swizzle(k);
+            offset[i] = (c >> 3) * (uint32_t)(Dz<T>::BLOCK * sizeof(T)) + k * 128 + (c & 7) * 16;
+        }
+    }
+    __device__ __forceinline__ void stage(char* lds, long long k0) const {
+        const char* from = base + (k0 >> 8) * row_block + (k0 & 255) * 128;
+#pragma unroll
+        for (int i = 0; i < Tile::PASSES; ++i) stage16(from + offset[i], lds + i * THREADS * 16 + (threadIdx.x >> 6) * 1024);
+    }
+};
+
 struct GradArgs {
-    const char* a;                      // [K][a_pitch bytes], dim_pad columns: weight rows of the piece, or packed features
+    const char* a;                      // [K][a_pitch bytes], dim_pad columns: weight rows of the piece, or features
     long long a_pitch, a_last;          // last readable K row
-    const char* dz;                     // [rows_pad][piece]
+    const char* dz;                     // rows_pad x piece, see Dz
     long long piece;
     int dim_pad;
     const int* count;
@@ -649,20 +995,32 @@ struct GradArgs {
     int splits;
     float* out;                         // [splits][cols][dim_pad]
     int accumulate;
-    float* bias_out;                    // [splits][cols] sums of dz over K, or null
+    float* bias_out;                    // [splits][cols] weighted sums of dz over K, or null
+    const float* row_weight;            // [rows_pad], or null: ones
 };
 
+// c plus both fp16 halves of a word, added in fp32
+__device__ __forceinline__ float sum_pair(uint32_t w, float c) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w), one, c, false);
+}
+
 // out[col][d] = sum_k dz(k, col) * a[k][d].  ROWS: columns are rows of dz and K runs over the classes of the piece (dF);
-// otherwise columns are classes and K runs over the valid rows (dW).
-template <typename T, bool ROWS>
-__global__ __launch_bounds__(VT, 2) void grad_kernel(GradArgs p) {
-    __shared__ __align__(1024) char lds[4 * STAGE];
+// otherwise columns are classes and K runs over the valid rows (dW).  A workgroup of eight waves takes 64 AF columns d and
+// 256 columns of the result, 32 AF x 64 per wave: at AF = 4 a stage of 64 KiB feeds 2048 cycles of the matrix units, half
+// of what L2 gives per cycle.
+template <typename T, int AF, bool ROWS>
+__global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
+    constexpr int THREADS = 2 * VT, DT = 64 * AF;
+    constexpr int A_BYTES = DT * 128, B_BYTES = ROW_TILE * 128;
+    __shared__ __align__(1024) char a0[A_BYTES], b0[B_BYTES], a1[A_BYTES], b1[B_BYTES];
     constexpr int KE = 128 / sizeof(T);
-    const int dtiles = (p.dim_pad + TILE - 1) / TILE;
+    const int dtiles = (p.dim_pad + DT - 1) / DT;
     const int id = xcd_range(blockIdx.x, gridDim.x);
-    const int d0 = (id % dtiles) * TILE;
-    const long long ctiles = p.cols / TILE;
-    const long long c0 = (id / dtiles) % ctiles * TILE;
+    const int d0 = (id % dtiles) * DT;
+    const long long ctiles = p.cols / ROW_TILE;
+    const long long c0 = (id / dtiles) % ctiles * ROW_TILE;
     const int split = (int)(id / dtiles / ctiles);
     const int count = *p.count;
     if (ROWS && c0 >= count) return;
@@ -670,94 +1028,143 @@ __global__ __launch_bounds__(VT, 2) void grad_kernel(GradArgs p) {
     if (!ROWS) ksteps = min(ksteps, (long long)(count + KE - 1) / KE);
     const long long k_first = ksteps * split / p.splits, k_end = ksteps * (split + 1) / p.splits;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
-    const int wd = (wave & 1) * 64, wcol = (wave >> 1) * 64;
+    const int wd = (wave & 1) * 32 * AF, wcol = (wave >> 1) * 64;
 
-    StridedOperand<T> a, bs;
-    ChunkedOperand bc;
+    typedef StridedOperand<T, DT, THREADS> A;
+    typedef DzOperand<T, THREADS> BS;
+    typedef ChunkedOperand<ROW_TILE, THREADS, false> BC;
+    A a;
+    BS bs;
+    BC bc;
     a.init(p.a, p.a_pitch, d0, p.dim_pad);
-    if (ROWS) bc.init(p.dz, p.piece * (long long)sizeof(T), c0, p.cols - 1);
-    else bs.init(p.dz, p.piece * (long long)sizeof(T), c0, p.piece);
+    // 256 rows of dz times the classes of a stage are one block
+    if (ROWS) bc.init(p.dz + Dz<T>::at(c0, 0, p.piece) * (long long)sizeof(T), 128, 0, ROW_TILE - 1);
+    else bs.init(p.dz, p.piece, c0);
 
-    f32x16 acc[2][2];
+    f32x16 acc[AF][2];
 #pragma unroll
-    for (int f = 0; f < 2; ++f)
+    for (int f = 0; f < AF; ++f)
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
-    float bias[2] = {0.0f, 0.0f};
-    const bool want_bias = !ROWS && p.bias_out && d0 == 0 && wd == 0;
+    float bias = 0.0f;
+    const bool want_bias = !ROWS && p.bias_out && d0 == 0;
 
-    auto stage = [&](char* to, long long k) {
-        a.stage(to, k * KE, p.a_last);
-        if (ROWS) bc.stage(to + STAGE, k * 128);
-        else bs.stage(to + STAGE, k * KE, k * KE + KE);
+    auto stage = [&](char* to_a, char* to_b, long long k) {
+        a.stage(to_a, k * KE, p.a_last);
+        if (ROWS) bc.stage(to_b, k * Dz<T>::BLOCK * (long long)sizeof(T));
+        else bs.stage(to_b, k * KE);
     };
-    int buf = 0;
-    if (k_first < k_end) stage(lds, k_first);
-    for (long long k = k_first; k < k_end; ++k) {
-        stage_barrier();
-        const char* now = lds + buf * 2 * STAGE;
-        if (k + 1 < k_end) stage(lds + (buf ^ 1) * 2 * STAGE, k + 1);
-        buf ^= 1;
+    auto multiply = [&](const char* ta, const char* tb, long long k) {
+        int at = lane;
+        asm volatile("" : "+v"(at));                                // addresses are formed anew in every stage, see resident_kernel
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            u32x4 x[2], y[2];
+            u32x4 x[AF], y[2];
 #pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                x[f] = StridedOperand<T>::frag(now, wd + f * 32, j);
-                y[f] = ROWS ? ChunkedOperand::frag(now + STAGE, wcol + f * 32, j)
-                            : StridedOperand<T>::frag(now + STAGE, wcol + f * 32, j);
-            }
+            for (int g = 0; g < 2; ++g) y[g] = ROWS ? BC::frag(tb, wcol + g * 32, j, at) : BS::Tile::frag(tb, wcol + g * 32, j, at);
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
+            for (int f = 0; f < AF; ++f) x[f] = A::frag(ta, wd + f * 32, j, at);
+#pragma unroll
+            for (int f = 0; f < AF; ++f)
 #pragma unroll
                 for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(x[f], y[g], acc[f][g]);
             if (want_bias) {
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
+                constexpr int E = 16 / sizeof(T);                   // a lane's K of slab j: E from (2 j + h) E on
+                const u32x4 mine = (wave & 1) ? y[1] : y[0];        // the two waves of these columns take one fragment each
+                if (p.row_weight) {
+                    const float* weight = p.row_weight + k * KE + (2 * j + h) * E;
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         if constexpr (sizeof(T) == 2) {
                             float lo, hi;
-                            unpack2(y[g][w], lo, hi, (const T*)nullptr);
-                            bias[g] += lo + hi;
+                            unpack2(mine[w], lo, hi, (const T*)nullptr);
+                            bias += lo * weight[2 * w] + hi * weight[2 * w + 1];
                         } else {
-                            bias[g] += u2f(y[g][w]);
+                            bias += u2f(mine[w]) * weight[w];
                         }
                     }
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        if constexpr (sizeof(T) == 2) bias = sum_pair(mine[w], bias);
+                        else bias += u2f(mine[w]);
+                    }
+                }
             }
         }
+    };
+    auto order = [&] {
+        constexpr int PER = sizeof(T) == 4 ? 4 : 2;                 // LDS reads of a transposed fragment
+        constexpr int READS = AF * PER + 2 * (ROWS ? 1 : PER);
+        interleave<(sizeof(T) == 4 ? 1 : 2) * READS, 4, 2 * AF * (sizeof(T) == 4 ? 4 : 1), READS>();
+    };
+    if (k_first < k_end) stage(a0, b0, k_first);
+    long long k = k_first;
+    for (; k + 1 < k_end; k += 2) {
+        stage_barrier();
+        stage(a1, b1, k + 1);
+        multiply(a0, b0, k);
+        order();
+        stage_barrier();
+        if (k + 2 < k_end) stage(a0, b0, k + 2);
+        multiply(a1, b1, k + 1);
+        order();
     }
-    float* out = p.out + ((long long)split * p.cols + c0) * p.dim_pad + d0;
+    if (k < k_end) {
+        stage_barrier();
+        multiply(a0, b0, k);
+        order();
+    }
+    // The result leaves through LDS, 32 columns of the wave at a time, so that a store covers whole lines: a lane holds 4
+    // neighbouring d of one column, and stores of those reach memory in pieces of 32 bytes (25 us of 108 for dW of
+    // 4096 x 32000 x 256).
+    constexpr int WIDTH = 32 * AF, REGION = 32 * WIDTH * 4, ROW_CHUNKS = WIDTH / 4;
+    static_assert(2 * REGION <= A_BYTES && 2 * REGION <= B_BYTES, "two waves' regions per stage");
+    stage_barrier();
+    char* region = (wave < 2 ? a0 : wave < 4 ? b0 : wave < 6 ? a1 : b1) + (wave & 1) * REGION;
+    float* out = p.out + ((long long)split * p.cols + c0 + wcol) * p.dim_pad + d0 + wd;
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-        float* line = out + (long long)(wcol + g * 32 + (lane & 31)) * p.dim_pad;
+        const int col = lane & 31;
 #pragma unroll
-        for (int f = 0; f < 2; ++f)
+        for (int f = 0; f < AF; ++f)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int d = wd + f * 32 + 8 * q + 4 * h;
-                if (d0 + d >= p.dim_pad) continue;                  // dim_pad is a multiple of four
                 vec4f v;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v[e] = acc[f][g][4 * q + e];
-                vec4f* at = reinterpret_cast<vec4f*>(line + d);
-                if (p.accumulate) v += *at;
-                *at = v;
+                const int chunk = f * 8 + 2 * q + h;                // of 4 d; permuted against bank conflicts
+                *reinterpret_cast<vec4f*>(region + (col * ROW_CHUNKS + (chunk ^ (col & 7))) * 16) = v;
             }
-        if (want_bias) {
-            const float sum = bias[g] + __shfl_xor(bias[g], 32, 64);
-            if (h == 0) p.bias_out[(long long)split * p.cols + c0 + wcol + g * 32 + lane] = sum;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the region is this wave's own
+#pragma unroll
+        for (int i = 0; i < 32 * ROW_CHUNKS / 64; ++i) {
+            const int at = i * 64 + lane, c = at / ROW_CHUNKS, chunk = at % ROW_CHUNKS;
+            vec4f v = *reinterpret_cast<const vec4f*>(region + (c * ROW_CHUNKS + (chunk ^ (c & 7))) * 16);
+            if (d0 + wd + chunk * 4 < p.dim_pad) {                  // dim_pad is a multiple of four
+                vec4f* to = reinterpret_cast<vec4f*>(out + (long long)(g * 32 + c) * p.dim_pad + chunk * 4);
+                if (p.accumulate) v += *to;
+                *to = v;
+            }
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+    if (want_bias) {
+        const float sum = bias + __shfl_xor(bias, 32, 64);
+        if (h == 0) p.bias_out[(long long)split * p.cols + c0 + wcol + (wave & 1) * 32 + lane] = sum;
     }
 }
 
-// out[row][0 .. dim) = the splits' sum over line place[row] (or row itself), times scale[1]; zero where place < 0
+// What the sums of the products still lack: 2^-LOG2_DZ, the other operand's power of two, the common factor, and (dF) the
+// row's weight.  The powers of two are applied apart, so that no intermediate factor leaves the range.
+// out[row][0 .. dim) = the splits' sum over line place[row] (or row itself); zero where place < 0
 template <typename T>
 __global__ __launch_bounds__(VT) void finish_kernel(const float* __restrict__ part, long long cols, int splits, int dim,
                                                     int dim_pad, const int* __restrict__ place,
-                                                    const float* __restrict__ scale, long long rows, T* __restrict__ out) {
+                                                    const float* __restrict__ weight, const Scales* __restrict__ scales,
+                                                    int rows_of_dz, int scaled, long long rows, T* __restrict__ out) {
     const int groups = (dim + 3) / 4;
     const long long at = (long long)blockIdx.x * VT + threadIdx.x;
     const long long row = at / groups;
@@ -768,7 +1175,9 @@ __global__ __launch_bounds__(VT) void finish_kernel(const float* __restrict__ pa
     if (line >= 0) {
         for (int s = 0; s < splits; ++s)
             v += *reinterpret_cast<const vec4f*>(part + ((long long)s * cols + line) * dim_pad + d);
-        v *= scale[1];
+        const int e = scaled ? exponent_of(rows_of_dz ? scales->weight_max : scales->features_max) : 0;
+        v *= ldexpf(1.0f, -e - GradOf<T>::LOG2_DZ);
+        v *= scales->common * (weight ? weight[line] : 1.0f);
     }
     T* to = out + row * dim + d;
     if (dim % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0) {
@@ -783,37 +1192,55 @@ __global__ __launch_bounds__(VT) void finish_kernel(const float* __restrict__ pa
 
 template <typename T>
 __global__ __launch_bounds__(VT) void finish_bias_kernel(const float* __restrict__ part, long long cols, int splits,
-                                                         const float* __restrict__ scale, long long classes,
+                                                         const Scales* __restrict__ scales, long long classes,
                                                          T* __restrict__ out) {
     const long long v = (long long)blockIdx.x * VT + threadIdx.x;
     if (v >= classes) return;
     float sum = 0.0f;
     for (int s = 0; s < splits; ++s) sum += part[(long long)s * cols + v];
-    out[v] = Elem<T>::from_float(sum * scale[1]);
+    out[v] = Elem<T>::from_float(sum * ldexpf(1.0f, -GradOf<T>::LOG2_DZ) * scales->common);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 constexpr long long DZ_BYTES = 256ll << 20;     // size aimed at for a piece of dz
-constexpr int FILL = 512;                       // workgroups that fill the chip: two per compute unit
+constexpr int SLOTS = 512;                      // workgroups of the products that run at once: two per compute unit
+constexpr int GRAD_SLOTS = 256;                 // of the gradient products: one
 
 long long up(long long v, long long to) { return (v + to - 1) / to * to; }
 long long least(long long a, long long b) { return a < b ? a : b; }
 long long most(long long a, long long b) { return a > b ? a : b; }
 int elem_size(int dtype) { return dtype == OD_DTYPE_F32 ? 4 : 2; }
 
+// Splits of `steps` steps of work, for each of `tiles` workgroups: the number with which the last workgroup ends first when
+// `slots` run at once and each costs `fixed` steps beside its share.
+int splits_for(long long tiles, long long steps, int slots, int fixed, int limit) {
+    long long best = 1, best_cost = -1;
+    for (long long s = 1; s <= least(steps, limit); ++s) {
+        const long long cost = (tiles * s + slots - 1) / slots * ((steps + s - 1) / s + fixed);
+        if (best_cost < 0 || cost < best_cost) {
+            best = s;
+            best_cost = cost;
+        }
+        if (tiles * s > 4 * slots) break;
+    }
+    return (int)best;
+}
+
 // Everything that follows from the sizes.
 struct Plan {
     long long rows, rows_pad, classes, classes_pad;
     int dim, dim_pad, size, n;                  // n: targets per row
-    int tiles, splits;                          // forward
+    int slabs;                                  // 32-byte slabs of a row where the rows are resident, 0 where they stream
+    int row_tile, class_tile, row_tiles;        // of the product
+    int splits, splits_z;                       // of the classes: forward, a piece of dz
     long long piece;                            // classes per piece
-    int pieces, splits_f, splits_w;             // backward
+    int pieces, grad_tile, splits_f, splits_w;  // backward; grad_tile: columns of dim per workgroup
     // saved buffer
     size_t o_count, o_row_of, o_place, o_lse, o_logit, o_prob, o_packed, saved;
     // forward's scratch
     size_t f_weight, f_bias, f_part, f_entropy, f_flags, forward;
     // backward's scratch
-    size_t b_weight, b_bias, b_grad, b_scale, b_dz, b_part_f, b_part_w, b_part_b, backward;
+    size_t b_weight, b_bias, b_row_weight, b_scales, b_scaled_f, b_scaled_w, b_dz, b_part_f, b_part_w, b_part_b, backward;
 };
 
 size_t take(size_t& at, long long bytes) {
@@ -825,29 +1252,36 @@ size_t take(size_t& at, long long bytes) {
 bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Plan& p) {
     p.size = elem_size(dtype);
     p.rows = rows;
-    p.rows_pad = up(most(rows, 1), TILE);
+    p.rows_pad = up(most(rows, 1), ROW_TILE);
     p.classes = classes;
-    p.classes_pad = up(classes, TILE);
+    p.classes_pad = up(classes, ROW_TILE);
     p.dim = dim;
-    p.dim_pad = (int)up(dim, 128 / p.size);
+    // resident rows of 128, 256, 384, 512, 768 or 1024 bytes; wider ones stream in stages of 128
+    long long bytes = up((long long)dim * p.size, 128);
+    if (bytes > 512 && bytes <= 1024) bytes = up(bytes, 256);
+    p.dim_pad = (int)(bytes / p.size);
+    p.slabs = bytes <= 1024 ? (int)(bytes / 32) : 0;
+    p.row_tile = p.slabs > 0 && p.slabs <= 16 ? 256 : 128;
+    p.class_tile = p.slabs == 0 ? TILE : p.slabs <= 16 ? 64 : 32;
     // one thread per 16 bytes of the packed operands, fewer than 2^32 threads in a launch
     if (most(p.rows_pad, p.classes_pad) * p.dim_pad * p.size / 16 > (1ll << 31)) return false;
     p.n = top > 0 ? top : 1;
-    p.tiles = (int)(p.classes_pad / TILE);
-    const long long row_tiles = p.rows_pad / TILE;
-    // splits of the classes: enough workgroups to fill the chip twice, in eights (one range per XCD) where there are tiles
-    long long s = (2 * FILL + row_tiles - 1) / row_tiles;
-    if (s > 1) s = up(s, 8);
-    p.splits = (int)least(s, p.tiles);
-    long long piece = most(TILE, DZ_BYTES / (p.rows_pad * p.size) / TILE * TILE);
+    p.row_tiles = (int)((most(rows, 1) + p.row_tile - 1) / p.row_tile);
+    p.splits = splits_for(p.row_tiles, p.classes_pad / p.class_tile, SLOTS, 2, SLOTS);
+    long long piece = most(ROW_TILE, DZ_BYTES / (p.rows_pad * p.size) / ROW_TILE * ROW_TILE);
     p.pieces = (int)((p.classes_pad + piece - 1) / piece);
-    p.piece = up((p.classes_pad + p.pieces - 1) / p.pieces, TILE);
+    p.piece = up((p.classes_pad + p.pieces - 1) / p.pieces, ROW_TILE);
     p.pieces = (int)((p.classes_pad + p.piece - 1) / p.piece);
-    const long long dtiles = (p.dim_pad + TILE - 1) / TILE;
+    p.splits_z = splits_for(p.row_tiles, p.piece / p.class_tile, SLOTS, 2, SLOTS);
+    // columns of dim per workgroup of the gradient products: what leaves least unused, the widest of those
+    p.grad_tile = 256;
+    for (int t = 128; t >= 64; t /= 2)
+        if (up(p.dim_pad, t) < up(p.dim_pad, p.grad_tile)) p.grad_tile = t;
+    const long long dtiles = (p.dim_pad + p.grad_tile - 1) / p.grad_tile;
     const long long ke = 128 / p.size;
-    // splits of K where the result has too few tiles; at least eight steps each
-    p.splits_f = (int)most(1, least((FILL + row_tiles * dtiles - 1) / (row_tiles * dtiles), p.piece / ke / 8));
-    p.splits_w = (int)most(1, least((FILL + p.piece / TILE * dtiles - 1) / (p.piece / TILE * dtiles), p.rows_pad / ke / 8));
+    // each split writes its own partial result, which costs about as much as eight steps
+    p.splits_f = splits_for(p.rows_pad / ROW_TILE * dtiles, p.piece / ke, GRAD_SLOTS, 8, 64);
+    p.splits_w = splits_for(p.piece / ROW_TILE * dtiles, p.rows_pad / ke, GRAD_SLOTS, 8, 64);
 
     size_t at = 0;
     p.o_count = take(at, 4);
@@ -870,8 +1304,10 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     at = 0;
     p.b_weight = take(at, p.classes * p.dim_pad * p.size);
     p.b_bias = take(at, 4 * p.classes_pad + 4 * p.piece);
-    p.b_grad = take(at, 4 * p.rows_pad);
-    p.b_scale = take(at, 8);
+    p.b_row_weight = take(at, 4 * p.rows_pad);
+    p.b_scales = take(at, sizeof(Scales));
+    p.b_scaled_f = take(at, p.rows_pad * p.dim_pad * p.size);
+    p.b_scaled_w = take(at, dtype == OD_DTYPE_BF16 ? p.classes * p.dim_pad * p.size : 0);
     p.b_dz = take(at, p.rows_pad * p.piece * p.size);
     p.b_part_f = take(at, 4 * p.rows_pad * p.dim_pad * p.splits_f);
     p.b_part_w = take(at, 4 * p.piece * p.dim_pad * p.splits_w);
@@ -894,9 +1330,9 @@ int check_call(int64_t rows, int64_t classes, int32_t dim, int32_t top, int32_t 
 
 unsigned blocks_of(long long n, int per) { return (unsigned)((n + per - 1) / per); }
 
-// Whether tiles can be read from the caller's weight rows: whole stages of K and 16-byte chunks.
+// Whether tiles can be read from the caller's weight rows: whole stages of K, 16-byte chunks, and 64 rows within 31 bits.
 bool weight_in_place(const Plan& p, const void* weight, long long pitch) {
-    return p.dim == p.dim_pad && (pitch * p.size) % 16 == 0 && ((uintptr_t)weight & 15) == 0;
+    return p.dim == p.dim_pad && (pitch * p.size) % 16 == 0 && pitch * p.size <= (1 << 24) && ((uintptr_t)weight & 15) == 0;
 }
 
 struct Call {
@@ -929,6 +1365,36 @@ int weight_rows(const Call& c, size_t scratch, const char** rows, long long* pit
     OD_LAUNCH_CHECK();
     *rows = c.ws + scratch;
     *pitch = (long long)p.dim_pad * p.size;
+    return OD_OK;
+}
+
+// The product by the kernel for its row width.
+template <typename T, bool GRAD>
+int launch_product(const Call& c, int kernel, const ProductArgs& a) {
+    const dim3 grid((unsigned)((long long)a.row_tiles * a.splits));
+    switch (c.p.slabs) {
+#define OD_PRODUCT(KS) \
+    case KS: OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, KS, GRAD>), grid, dim3(VT), 0, c.stream, a); break
+        OD_PRODUCT(4);
+        OD_PRODUCT(8);
+        OD_PRODUCT(12);
+        OD_PRODUCT(16);
+        OD_PRODUCT(24);
+        OD_PRODUCT(32);
+#undef OD_PRODUCT
+        default: OD_LAUNCH_KERNEL(kernel, (product_kernel<T, GRAD>), grid, dim3(VT), 0, c.stream, a); break;
+    }
+    return OD_OK;
+}
+
+template <typename G, bool ROWS>
+int launch_grad(const Call& c, int kernel, const GradArgs& g) {
+    const Plan& p = c.p;
+    const long long dtiles = (p.dim_pad + p.grad_tile - 1) / p.grad_tile;
+    const dim3 grid((unsigned)(dtiles * (g.cols / ROW_TILE) * g.splits)), block(2 * VT);
+    if (p.grad_tile == 256) OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 4, ROWS>), grid, block, 0, c.stream, g);
+    else if (p.grad_tile == 128) OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 2, ROWS>), grid, block, 0, c.stream, g);
+    else OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 1, ROWS>), grid, block, 0, c.stream, g);
     return OD_OK;
 }
 
@@ -971,7 +1437,7 @@ int forward_typed(const Call& c) {
                        (int)p.classes, (int)p.classes_pad, scale, (float*)(c.ws + p.f_bias));
     OD_LAUNCH_CHECK();
     ProductArgs a = {};
-    const int rc = weight_rows<T>(c, p.f_weight, &a.weight, &a.weight_pitch);
+    int rc = weight_rows<T>(c, p.f_weight, &a.weight, &a.weight_pitch);
     if (rc != OD_OK) return rc;
     a.features = c.saved + p.o_packed;
     a.dim_pad = p.dim_pad;
@@ -979,13 +1445,14 @@ int forward_typed(const Call& c) {
     a.last_class = p.classes - 1;
     a.bias2 = (const float*)(c.ws + p.f_bias);
     a.count = lists.count;
-    a.tiles = p.tiles;
+    a.tiles = (int)(p.classes_pad / p.class_tile);
     a.splits = p.splits;
+    a.row_tiles = p.row_tiles;
     a.scale = scale;
     a.rows_pad = p.rows_pad;
     a.part = (float2*)(c.ws + p.f_part);
-    OD_LAUNCH_KERNEL(OD_KERNEL_VOCAB_LSE, (product_kernel<T, false>), dim3((unsigned)(p.rows_pad / TILE * p.splits)), dim3(VT),
-                     0, c.stream, a);
+    rc = launch_product<T, false>(c, OD_KERNEL_VOCAB_LSE, a);
+    if (rc != OD_OK) return rc;
     TargetArgs t = {};
     t.features = a.features;
     t.dim = p.dim;
@@ -1018,12 +1485,15 @@ int forward_typed(const Call& c) {
 
 template <typename T>
 int backward_typed(const Call& c) {
+    typedef typename GradOf<T>::type G;
+    constexpr bool BF16 = std::is_same<T, bf16_t>::value, WIDE = sizeof(T) == 4;
     const Plan& p = c.p;
     const RowLists lists = lists_of(c);
-    float* row_grad = (float*)(c.ws + p.b_grad);
-    float* scale = (float*)(c.ws + p.b_scale);
-    hipLaunchKernelGGL(row_grads_kernel, dim3(1), dim3(1024), 0, c.stream, c.upstream, c.reduction, lists, p.rows_pad,
-                       c.temperature, (int)std::is_same<T, _Float16>::value, row_grad, scale);
+    const bool weighted = c.reduction == OD_REDUCE_NONE;
+    float* row_weight = (float*)(c.ws + p.b_row_weight);
+    Scales* scales = (Scales*)(c.ws + p.b_scales);
+    hipLaunchKernelGGL(row_weights_kernel, dim3(1), dim3(1024), 0, c.stream, c.upstream, c.reduction, lists, p.rows_pad,
+                       c.temperature, row_weight, scales);
     OD_LAUNCH_CHECK();
     const float log2_scale = LOG2E / c.temperature;
     const long long bias_len = p.classes_pad + p.piece;             // the last piece may reach past the last tile
@@ -1031,34 +1501,64 @@ int backward_typed(const Call& c) {
                        (int)p.classes, (int)bias_len, log2_scale, (float*)(c.ws + p.b_bias));
     OD_LAUNCH_CHECK();
     ProductArgs a = {};
-    const int rc = weight_rows<T>(c, p.b_weight, &a.weight, &a.weight_pitch);
+    int rc = weight_rows<T>(c, p.b_weight, &a.weight, &a.weight_pitch);
     if (rc != OD_OK) return rc;
     a.features = c.saved + p.o_packed;
+
+    // operands of the gradient products: bf16 values and weighted rows change their form, the others stay what they are
+    const char *grad_features = a.features, *grad_weight = a.weight;
+    long long grad_weight_pitch = a.weight_pitch;
+    const bool scale_f = !WIDE && (BF16 || weighted), scale_w = BF16;
+    if (scale_f || weighted) {
+        const float* rw = weighted ? row_weight : nullptr;
+        uint32_t* max_bits = scale_f ? &scales->features_max : nullptr;
+        if (scale_f) {
+            const long long work = blocks_of(p.rows_pad * (p.dim_pad * p.size / 16), VT);
+            hipLaunchKernelGGL(max_kernel<T>, dim3((unsigned)least(work, 512)), dim3(VT), 0, c.stream, (const T*)a.features,
+                               (long long)p.dim_pad, p.dim_pad, rw, (const int*)lists.count, p.rows, max_bits);
+            OD_LAUNCH_CHECK();
+        }
+        hipLaunchKernelGGL((scale_rows_kernel<T, G>), dim3(blocks_of(p.rows_pad * (p.dim_pad * p.size / 16), VT)), dim3(VT), 0,
+                           c.stream, (const T*)a.features, (long long)p.dim_pad, p.dim_pad, rw, (const int*)lists.count,
+                           p.rows_pad, (const uint32_t*)max_bits, (G*)(c.ws + p.b_scaled_f));
+        OD_LAUNCH_CHECK();
+        grad_features = c.ws + p.b_scaled_f;
+    }
+    if (scale_w && c.dfeatures) {
+        const long long chunks = p.classes * (p.dim_pad * p.size / 16);
+        hipLaunchKernelGGL(max_kernel<T>, dim3((unsigned)least(blocks_of(chunks, VT), 512)), dim3(VT), 0, c.stream,
+                           (const T*)a.weight, a.weight_pitch / p.size, p.dim_pad, (const float*)nullptr, (const int*)nullptr,
+                           p.classes, &scales->weight_max);
+        OD_LAUNCH_CHECK();
+        hipLaunchKernelGGL((scale_rows_kernel<T, G>), dim3(blocks_of(chunks, VT)), dim3(VT), 0, c.stream, (const T*)a.weight,
+                           a.weight_pitch / p.size, p.dim_pad, (const float*)nullptr, (const int*)nullptr, p.classes,
+                           (const uint32_t*)&scales->weight_max, (G*)(c.ws + p.b_scaled_w));
+        OD_LAUNCH_CHECK();
+        grad_weight = c.ws + p.b_scaled_w;
+        grad_weight_pitch = (long long)p.dim_pad * p.size;
+    }
+
     a.dim_pad = p.dim_pad;
     a.last_class = p.classes - 1;
     a.count = lists.count;
-    a.tiles = (int)(p.piece / TILE);
-    const long long row_tiles = p.rows_pad / TILE;
-    long long s = (4 * FILL + row_tiles - 1) / row_tiles;
-    a.splits = (int)most(1, least(s, a.tiles));
+    a.tiles = (int)(p.piece / p.class_tile);
+    a.row_tiles = p.row_tiles;
+    a.splits = p.splits_z;
     a.scale = log2_scale;
     a.rows_pad = p.rows_pad;
     a.lse2 = (const float*)(c.saved + p.o_lse);
-    a.row_grad = row_grad;
     a.dz = c.ws + p.b_dz;
     a.piece = p.piece;
-    const int dtiles = (p.dim_pad + TILE - 1) / TILE;
     const int ke = 128 / p.size;
     for (int k = 0; k < p.pieces; ++k) {
         const long long first = k * p.piece;
         a.first_class = first;
         a.bias2 = (const float*)(c.ws + p.b_bias) + first;
-        OD_LAUNCH_KERNEL(OD_KERNEL_VOCAB_DZ, (product_kernel<T, true>), dim3((unsigned)(row_tiles * a.splits)), dim3(VT), 0,
-                         c.stream, a);
-        hipLaunchKernelGGL(correct_targets_kernel<T>, dim3(blocks_of(p.rows * p.n, VT)), dim3(VT), 0, c.stream, c.targets,
-                           c.top, (const float*)(c.saved + p.o_prob), lists, a.lse2,
-                           (const float*)(c.saved + p.o_logit), (const float*)row_grad, first, p.piece, p.classes,
-                           (T*)(c.ws + p.b_dz));
+        rc = launch_product<T, true>(c, OD_KERNEL_VOCAB_DZ, a);
+        if (rc != OD_OK) return rc;
+        hipLaunchKernelGGL(correct_targets_kernel<G>, dim3(blocks_of(p.rows * p.n, VT)), dim3(VT), 0, c.stream, c.targets,
+                           c.top, (const float*)(c.saved + p.o_prob), lists, a.lse2, (const float*)(c.saved + p.o_logit),
+                           first, p.piece, p.classes, (float)(1 << GradOf<T>::LOG2_DZ), (G*)(c.ws + p.b_dz));
         OD_LAUNCH_CHECK();
         GradArgs g = {};
         g.dz = c.ws + p.b_dz;
@@ -1066,19 +1566,19 @@ int backward_typed(const Call& c) {
         g.dim_pad = p.dim_pad;
         g.count = lists.count;
         if (c.dfeatures) {
-            g.a = a.weight + first * a.weight_pitch;
-            g.a_pitch = a.weight_pitch;
+            g.a = grad_weight + first * grad_weight_pitch;
+            g.a_pitch = grad_weight_pitch;
             g.a_last = p.classes - 1 - first;
             g.cols = p.rows_pad;
             g.ksteps = p.piece / ke;
             g.splits = p.splits_f;
             g.out = (float*)(c.ws + p.b_part_f);
             g.accumulate = k > 0;
-            OD_LAUNCH_KERNEL(OD_KERNEL_VOCAB_GRAD_ROWS, (grad_kernel<T, true>),
-                             dim3((unsigned)(dtiles * row_tiles * g.splits)), dim3(VT), 0, c.stream, g);
+            rc = launch_grad<G, true>(c, OD_KERNEL_VOCAB_GRAD_ROWS, g);
+            if (rc != OD_OK) return rc;
         }
         if (c.dweight || c.dbias) {
-            g.a = a.features;
+            g.a = grad_features;
             g.a_pitch = (long long)p.dim_pad * p.size;
             g.a_last = p.rows_pad - 1;
             g.cols = p.piece;
@@ -1087,18 +1587,20 @@ int backward_typed(const Call& c) {
             g.out = (float*)(c.ws + p.b_part_w);
             g.accumulate = 0;
             g.bias_out = c.dbias ? (float*)(c.ws + p.b_part_b) : nullptr;
-            OD_LAUNCH_KERNEL(OD_KERNEL_VOCAB_GRAD_CLASSES, (grad_kernel<T, false>),
-                             dim3((unsigned)(dtiles * (p.piece / TILE) * g.splits)), dim3(VT), 0, c.stream, g);
+            g.row_weight = weighted ? row_weight : nullptr;
+            rc = launch_grad<G, false>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g);
+            if (rc != OD_OK) return rc;
             const long long here = least(p.piece, p.classes - first);
             if (c.dweight) {
                 hipLaunchKernelGGL(finish_kernel<T>, dim3(blocks_of(here * ((p.dim + 3) / 4), VT)), dim3(VT), 0, c.stream,
                                    (const float*)g.out, p.piece, p.splits_w, p.dim, p.dim_pad, (const int*)nullptr,
-                                   (const float*)scale, here, (T*)c.dweight + first * p.dim);
+                                   (const float*)nullptr, (const Scales*)scales, 0, (int)scale_f, here,
+                                   (T*)c.dweight + first * p.dim);
                 OD_LAUNCH_CHECK();
             }
             if (c.dbias) {
                 hipLaunchKernelGGL(finish_bias_kernel<T>, dim3(blocks_of(here, VT)), dim3(VT), 0, c.stream,
-                                   (const float*)g.bias_out, p.piece, p.splits_w, (const float*)scale, here,
+                                   (const float*)g.bias_out, p.piece, p.splits_w, (const Scales*)scales, here,
                                    (T*)c.dbias + first);
                 OD_LAUNCH_CHECK();
             }
@@ -1107,7 +1609,8 @@ int backward_typed(const Call& c) {
     if (c.dfeatures) {
         hipLaunchKernelGGL(finish_kernel<T>, dim3(blocks_of(p.rows * ((p.dim + 3) / 4), VT)), dim3(VT), 0, c.stream,
                            (const float*)(c.ws + p.b_part_f), p.rows_pad, p.splits_f, p.dim, p.dim_pad,
-                           (const int*)lists.place, (const float*)scale, p.rows, (T*)c.dfeatures);
+                           (const int*)lists.place, weighted ? (const float*)row_weight : nullptr, (const Scales*)scales, 1,
+                           (int)scale_w, p.rows, (T*)c.dfeatures);
         OD_LAUNCH_CHECK();
     }
     return OD_OK;

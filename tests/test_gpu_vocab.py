@@ -153,6 +153,10 @@ DTYPES = [torch.float32, torch.float16, torch.bfloat16]
     (300, 5003, 200, True),
     (100, 20000, 64, True),             # few rows: classes split over workgroups, dF split over K
     (5000, 300, 128, True),             # few classes: dW split over K
+    (300, 900, 384, False),
+    (260, 513, 512, True),              # the widest rows of 16-bit types that stay in registers
+    (200, 700, 640, True),              # wider ones stream
+    (70, 1000, 1030, True),
 ])
 def test_cross_entropy_matches_definition(device, N, V, D, bias, dtype):
     f, w, b, t = _inputs(device, N, V, D, dtype, bias, seed=N + V + D)
