@@ -389,9 +389,11 @@ int od_preprocess_images(const float* const* images, const int32_t* image_h, con
  *                  overlap it, nor dx overlap x or dy
  *   weight, bias : [channels] of element type param_dtype, either may be null (one, zero); groups divides channels
  *   activation   : OD_ACT_*: identity, max(u, 0), u * sigmoid(u)
- *   forward  -> y, and mean / rstd fp32 [batch, groups] for the backward pass
+ *   stats        : double [batch, groups, 2], mean and 1/std, 16-byte aligned: written by the forward pass, read by the
+ *                  backward one, whose rectifier decides by them where fp32 cannot tell the side of its corner
+ *   forward  -> y, stats
  *   backward -> dx (may be null), dweight / dbias [channels] of param_dtype (either may be null)
- * Arithmetic is fp32 with sums merged in a fixed order; 16-bit results are rounded once, to nearest even.
+ * Arithmetic is fp32, statistics are merged in 64 bits, in a fixed order; 16-bit results are rounded once, to nearest even.
  * Nothing is done for batch = 0 or pixels = 0 (dweight / dbias are then left as they are).
  *   workspace: od_group_norm_act_workspace_bytes (0: shape outside the limits), 256-byte aligned, for both directions
  */
@@ -404,12 +406,12 @@ int od_preprocess_images(const float* const* images, const int32_t* image_h, con
 size_t od_group_norm_act_workspace_bytes(int64_t batch, int64_t pixels, int32_t channels, int32_t groups);
 int od_group_norm_act_forward(const void* x, int32_t dtype, int64_t batch, int64_t pixels, int32_t channels,
                               int32_t groups, const void* weight, const void* bias, int32_t param_dtype, float eps,
-                              int32_t activation, void* y, float* mean, float* rstd, void* workspace,
-                              size_t workspace_bytes, void* stream);
+                              int32_t activation, void* y, double* stats, void* workspace, size_t workspace_bytes,
+                              void* stream);
 int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int64_t batch, int64_t pixels,
                                int32_t channels, int32_t groups, const void* weight, const void* bias,
-                               int32_t param_dtype, int32_t activation, const float* mean, const float* rstd, void* dx,
-                               void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+                               int32_t param_dtype, int32_t activation, const double* stats, void* dx, void* dweight,
+                               void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Losses of a classification head whose classes are a large vocabulary of embeddings (no counterpart in the reference,

@@ -79,9 +79,9 @@ SIGNATURES = {
     "od_preprocess_images": (c_int32, [_P, _P, _P, _P, _P, c_int32, c_int32, _P, _P, _P, c_int32, c_int32, _P]),
     "od_group_norm_act_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32, c_int32]),
     "od_group_norm_act_forward": (c_int32, [_P, c_int32, c_int64, c_int64, c_int32, c_int32, _P, _P, c_int32, c_float,
-                                            c_int32, _P, _P, _P, _P, c_size_t, _P]),
+                                            c_int32, _P, _P, _P, c_size_t, _P]),
     "od_group_norm_act_backward": (c_int32, [_P, _P, c_int32, c_int64, c_int64, c_int32, c_int32, _P, _P, c_int32, c_int32,
-                                             _P, _P, _P, _P, _P, _P, c_size_t, _P]),
+                                             _P, _P, _P, _P, _P, c_size_t, _P]),
     "od_vocab_loss_saved_bytes": (c_size_t, [c_int64, c_int64, c_int32, c_int32, c_int32]),
     "od_vocab_loss_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32]),
     "od_vocab_loss_forward": (c_int32, [_P, c_int64, _P, c_int64, _P, c_int32, c_int64, c_int64, c_int32, _P, c_int32, _P,

@@ -14,7 +14,9 @@
 //
 // Statistics: a thread sums x - k and (x - k)^2 with k its own first value of the channel, which bounds what the
 // subtraction of the two sums can lose by the number of its pixels whatever the mean of the map is; everything above a
-// thread is merged as (count, mean, M2) in two passes, M2 = sum M2_i + n_i (mean_i - mean)^2.  Fixed order, no atomics.
+// thread is merged in 64 bits as (count, mean, M2) in two passes, M2 = sum M2_i + n_i (mean_i - mean)^2.  Fixed order, no
+// atomics.  Mean and 1/std stay 64-bit: a rectifier's gradient is all or nothing, and since a 16-bit map holds few different
+// values, hundreds of pixels of a channel lie on its corner together; where fp32 cannot tell the side, 64 bits decide.
 #include "od_common.h"
 #include "../../include/od_boxes.h"
 #include "od_elem.h"
@@ -87,9 +89,9 @@ __device__ __forceinline__ int taken(long long n, int ty, int rows) {
 }
 
 // Statistics of channels [c0, c0 + nc) over `n` pixels at src (row stride `channels`), by the whole workgroup.
-// Leaves (mean, M2) of each channel in ch[0 .. nc).  red: 2 * NT * VEC floats.
+// Leaves (mean, M2) of each channel in ch[0 .. nc).  red: 3 * NT * VEC floats.
 template <typename T, int VEC>
-__device__ __forceinline__ void channel_stats(const T* src, int channels, int c0, int nc, long long n, float2* ch,
+__device__ __forceinline__ void channel_stats(const T* src, int channels, int c0, int nc, long long n, double2* ch,
                                               float* red) {
     const int cols = nc / VEC;
     const Lay lay(cols);
@@ -133,28 +135,30 @@ __device__ __forceinline__ void channel_stats(const T* src, int channels, int c0
         }
         __syncthreads();                                // red may still be read for the previous columns
         if (on) {
-            const float inv = mine > 0 ? 1.0f / (float)mine : 0.0f;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float m = s1[i] * inv;
-                red[(lay.ty * lay.width + lay.tx) * VEC + i] = k[i] + m;
-                red[NT * VEC + (lay.ty * lay.width + lay.tx) * VEC + i] = s2[i] - s1[i] * m;
+                red[(lay.ty * lay.width + lay.tx) * VEC + i] = k[i];
+                red[NT * VEC + (lay.ty * lay.width + lay.tx) * VEC + i] = s1[i];
+                red[2 * NT * VEC + (lay.ty * lay.width + lay.tx) * VEC + i] = s2[i];
             }
         }
         __syncthreads();
         const int here = min(lay.width, cols - base) * VEC;              // channels of this window
         for (int c = threadIdx.x; c < here; c += NT) {
-            float mean = 0.0f;
-            for (int r = 0; r < lay.rows; ++r)
-                mean += (float)taken(n, r, lay.rows) * red[r * lay.width * VEC + c];
-            mean /= (float)n;
-            float m2 = 0.0f;
+            double mean = 0.0;
             for (int r = 0; r < lay.rows; ++r) {
-                const float cnt = (float)taken(n, r, lay.rows);
-                const float d = cnt > 0.0f ? red[r * lay.width * VEC + c] - mean : 0.0f;
-                m2 += red[NT * VEC + r * lay.width * VEC + c] + cnt * d * d;
+                const int at = r * lay.width * VEC + c;
+                mean += (double)taken(n, r, lay.rows) * (double)red[at] + (double)red[NT * VEC + at];
             }
-            ch[base * VEC + c] = make_float2(mean, m2);
+            mean /= (double)n;
+            double m2 = 0.0;                                            // sum (x - mean)^2, k - mean apart from the sums
+            for (int r = 0; r < lay.rows; ++r) {
+                const int at = r * lay.width * VEC + c;
+                const double d = (double)red[at] - mean;
+                m2 += (double)red[2 * NT * VEC + at] + d * (2.0 * (double)red[NT * VEC + at] + (double)taken(n, r, lay.rows) * d);
+            }
+            m2 = m2 < 0.0 ? 0.0 : m2;                                   // NaN stays NaN
+            ch[base * VEC + c] = make_double2(mean, m2);
         }
     }
     __syncthreads();
@@ -166,26 +170,27 @@ __device__ __forceinline__ int lanes_of(int per) {
     while (l < per && l < 64) l <<= 1;
     return l;
 }
-__device__ __forceinline__ float lane_sum(float v, int lanes) {
+template <typename F>
+__device__ __forceinline__ F lane_sum(F v, int lanes) {
     for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
 
 // (mean, M2) of group g over n pixels out of its channels' values ch[g * per ..); f(g, mean, M2) once per group
 template <typename F>
-__device__ __forceinline__ void merge_groups(const float2* ch, int groups, int per, long long n, F f) {
+__device__ __forceinline__ void merge_groups(const double2* ch, int groups, int per, long long n, F f) {
     const int lanes = lanes_of(per);
     const int at = threadIdx.x % lanes;
     for (int g0 = 0; g0 < groups; g0 += NT / lanes) {
         const int g = g0 + threadIdx.x / lanes;
-        float mean = 0.0f, m2 = 0.0f;
+        double mean = 0.0, m2 = 0.0;
         if (g < groups)
             for (int c = at; c < per; c += lanes) mean += ch[g * per + c].x;
-        mean = lane_sum(mean, lanes) / (float)per;
+        mean = lane_sum(mean, lanes) / (double)per;
         if (g < groups)
             for (int c = at; c < per; c += lanes) {
-                const float d = ch[g * per + c].x - mean;
-                m2 += ch[g * per + c].y + (float)n * d * d;
+                const double d = ch[g * per + c].x - mean;
+                m2 += ch[g * per + c].y + (double)n * d * d;
             }
         m2 = lane_sum(m2, lanes);
         if (g < groups && at == 0) f(g, mean, m2);
@@ -195,24 +200,23 @@ __device__ __forceinline__ void merge_groups(const float2* ch, int groups, int p
 // ---- two-pass form ------------------------------------------------------------------------------------------
 // part[(image * chunks + chunk) * groups + g] = (mean, M2) of the chunk
 template <typename T, int VEC>
-__global__ __launch_bounds__(NT) void norm_stats_kernel(NormShape s, const T* __restrict__ x, float2* __restrict__ part) {
-    extern __shared__ float smem[];
-    float* red = smem;
-    float2* ch = reinterpret_cast<float2*>(smem + 2 * NT * VEC);
+__global__ __launch_bounds__(NT) void norm_stats_kernel(NormShape s, const T* __restrict__ x, double2* __restrict__ part) {
+    extern __shared__ double smem[];
+    double2* ch = reinterpret_cast<double2*>(smem);
+    float* red = reinterpret_cast<float*>(ch + s.channels);
     const long long b = blockIdx.x / s.chunks;
     const int chunk = blockIdx.x % s.chunks;
     const long long p0 = chunk * s.chunk_pixels;
     const long long n = min(s.chunk_pixels, s.pixels - p0);
     channel_stats<T, VEC>(x + (b * s.pixels + p0) * s.channels, s.channels, 0, s.channels, n, ch, red);
-    float2* out = part + (long long)blockIdx.x * s.groups;
-    merge_groups(ch, s.groups, s.per_group, n, [&](int g, float mean, float m2) { out[g] = make_float2(mean, m2); });
+    double2* out = part + (long long)blockIdx.x * s.groups;
+    merge_groups(ch, s.groups, s.per_group, n, [&](int g, double mean, double m2) { out[g] = make_double2(mean, m2); });
 }
 
-// y of one window of channels and pixels; s_mean / s_rstd: per group, g counted from the window's first channel
+// y of one window of channels and pixels; stats: (mean, 1/std) per group, counted from the window's first channel
 template <typename T, int VEC, int ACT>
 __device__ __forceinline__ void apply_window(const NormShape& s, const T* src, T* dst, int c0, int nc, long long n,
-                                             const float* s_mean, const float* s_rstd, const void* weight,
-                                             const void* bias, int pdtype) {
+                                             const double2* stats, const void* weight, const void* bias, int pdtype) {
     const int cols = nc / VEC;
     const Lay lay(cols);
     for (int base = 0; base < cols; base += lay.width) {
@@ -222,8 +226,8 @@ __device__ __forceinline__ void apply_window(const NormShape& s, const T* src, T
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const int c = col * VEC + i, g = c / s.per_group;
-            mean[i] = s_mean[g];
-            a[i] = s_rstd[g] * param(weight, pdtype, c0 + c, 1.0f);
+            mean[i] = (float)stats[g].x;
+            a[i] = (float)(stats[g].y * (double)param(weight, pdtype, c0 + c, 1.0f));
             beta[i] = param(bias, pdtype, c0 + c, 0.0f);
         }
         const int mine = taken(n, lay.ty, lay.rows);
@@ -255,61 +259,48 @@ __device__ __forceinline__ void apply_window(const NormShape& s, const T* src, T
     }
 }
 
-// Every workgroup merges the chunks of its image again (at most 256 x groups pairs out of L2) instead of waiting for a
-// launch of its own that would do it once.
+// The chunks of one image joined: a workgroup takes 8 groups, 32 slices of the chunks each.
+__global__ __launch_bounds__(NT) void norm_join_kernel(NormShape s, const double2* __restrict__ part,
+                                                       double2* __restrict__ stats) {
+    __shared__ double red[NT];
+    const int blocks = (s.groups + 7) / 8;
+    const long long b = blockIdx.x / blocks;
+    const int g = (int)(blockIdx.x % blocks) * 8 + (threadIdx.x & 7);
+    const bool on = g < s.groups;
+    const double2* mine = part + b * s.chunks * s.groups;
+    auto count = [&](int k) { return (double)min(s.chunk_pixels, s.pixels - k * s.chunk_pixels); };
+    auto joined = [&](double v) {
+        __syncthreads();
+        red[threadIdx.x] = v;
+        __syncthreads();
+        v = 0.0;
+        for (int r = 0; r < NT / 8; ++r) v += red[r * 8 + (threadIdx.x & 7)];
+        return v;
+    };
+    double mean = 0.0;
+    if (on)
+        for (int k = threadIdx.x >> 3; k < s.chunks; k += NT / 8) mean += count(k) * mine[(long long)k * s.groups + g].x;
+    mean = joined(mean) / (double)s.pixels;
+    double m2 = 0.0;
+    if (on)
+        for (int k = threadIdx.x >> 3; k < s.chunks; k += NT / 8) {
+            const double2 v = mine[(long long)k * s.groups + g];
+            const double d = v.x - mean;
+            m2 += v.y + count(k) * s.per_group * d * d;
+        }
+    m2 = joined(m2);
+    if (on && threadIdx.x < 8)
+        stats[b * s.groups + g] = make_double2(mean, 1.0 / sqrt(m2 / ((double)s.pixels * s.per_group) + (double)s.eps));
+}
+
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(NT) void norm_apply_kernel(NormShape s, const T* __restrict__ x, T* __restrict__ y,
-                                                        const float2* __restrict__ part, const void* __restrict__ weight,
-                                                        const void* __restrict__ bias, int pdtype,
-                                                        float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-    extern __shared__ float smem[];
-    float* s_mean = smem;
-    float* s_rstd = smem + s.groups;
-    float* red = smem + 2 * s.groups;                   // NT floats
+                                                        const void* __restrict__ weight, const void* __restrict__ bias,
+                                                        int pdtype, const double2* __restrict__ stats) {
     const long long b = blockIdx.x / s.chunks;
-    const int chunk = blockIdx.x % s.chunks;
-    const float2* mine = part + b * s.chunks * s.groups;
-    const int slices = s.groups < NT ? NT / s.groups : 1;
-    const int slice = s.groups < NT ? threadIdx.x / s.groups : 0;
-    for (int g0 = 0; g0 < s.groups; g0 += NT) {         // one turn unless there are more groups than threads
-        const int g = s.groups < NT ? threadIdx.x % s.groups : g0 + threadIdx.x;
-        const bool on = slice < slices && g < s.groups;
-        float mean = 0.0f, m2 = 0.0f;
-        if (on)
-            for (int k = slice; k < s.chunks; k += slices)
-                mean += (float)min(s.chunk_pixels, s.pixels - k * s.chunk_pixels) * mine[k * s.groups + g].x;
-        __syncthreads();
-        red[threadIdx.x] = mean;
-        __syncthreads();
-        if (on) {
-            mean = 0.0f;
-            for (int r = 0; r < slices; ++r) mean += red[slices > 1 ? r * s.groups + g : threadIdx.x];
-            mean /= (float)s.pixels;
-            for (int k = slice; k < s.chunks; k += slices) {
-                const float2 v = mine[k * s.groups + g];
-                const float d = v.x - mean;
-                m2 += v.y + (float)(min(s.chunk_pixels, s.pixels - k * s.chunk_pixels) * s.per_group) * d * d;
-            }
-        }
-        __syncthreads();
-        red[threadIdx.x] = m2;
-        __syncthreads();
-        if (on && slice == 0) {
-            m2 = 0.0f;
-            for (int r = 0; r < slices; ++r) m2 += red[slices > 1 ? r * s.groups + g : threadIdx.x];
-            const float rstd = 1.0f / sqrtf(m2 / ((float)s.pixels * (float)s.per_group) + s.eps);
-            s_mean[g] = mean;
-            s_rstd[g] = rstd;
-            if (chunk == 0) {
-                mean_out[b * s.groups + g] = mean;
-                rstd_out[b * s.groups + g] = rstd;
-            }
-        }
-    }
-    __syncthreads();
-    const long long p0 = chunk * s.chunk_pixels;
+    const long long p0 = (long long)(blockIdx.x % s.chunks) * s.chunk_pixels;
     const long long first = (b * s.pixels + p0) * s.channels;
-    apply_window<T, VEC, ACT>(s, x + first, y + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0), s_mean, s_rstd,
+    apply_window<T, VEC, ACT>(s, x + first, y + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0), stats + b * s.groups,
                               weight, bias, pdtype);
 }
 
@@ -317,13 +308,11 @@ __global__ __launch_bounds__(NT) void norm_apply_kernel(NormShape s, const T* __
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(NT) void norm_small_kernel(NormShape s, int slab, const T* __restrict__ x, T* __restrict__ y,
                                                         const void* __restrict__ weight, const void* __restrict__ bias,
-                                                        int pdtype, float* __restrict__ mean_out,
-                                                        float* __restrict__ rstd_out) {
-    extern __shared__ float smem[];
-    float* red = smem;
-    float2* ch = reinterpret_cast<float2*>(smem + 2 * NT * VEC);
-    float* s_mean = smem + 2 * NT * VEC + 2 * slab;
-    float* s_rstd = s_mean + slab;                      // at most one group per channel
+                                                        int pdtype, double2* __restrict__ stats_out) {
+    extern __shared__ double smem[];
+    double2* ch = reinterpret_cast<double2*>(smem);
+    double2* stats = ch + slab;
+    float* red = reinterpret_cast<float*>(stats + slab / s.per_group);
     const int slabs = (s.channels + slab - 1) / slab;
     const long long b = blockIdx.x / slabs;
     const int c0 = (int)(blockIdx.x % slabs) * slab;
@@ -331,23 +320,63 @@ __global__ __launch_bounds__(NT) void norm_small_kernel(NormShape s, int slab, c
     const long long first = b * s.pixels * s.channels;
     channel_stats<T, VEC>(x + first, s.channels, c0, nc, s.pixels, ch, red);
     const long long g0 = b * s.groups + c0 / s.per_group;
-    merge_groups(ch, nc / s.per_group, s.per_group, s.pixels, [&](int g, float mean, float m2) {
-        const float rstd = 1.0f / sqrtf(m2 / ((float)s.pixels * (float)s.per_group) + s.eps);
-        s_mean[g] = mean;
-        s_rstd[g] = rstd;
-        mean_out[g0 + g] = mean;
-        rstd_out[g0 + g] = rstd;
+    merge_groups(ch, nc / s.per_group, s.per_group, s.pixels, [&](int g, double mean, double m2) {
+        const double2 v = make_double2(mean, 1.0 / sqrt(m2 / ((double)s.pixels * s.per_group) + (double)s.eps));
+        stats[g] = v;
+        stats_out[g0 + g] = v;
     });
     __syncthreads();
-    apply_window<T, VEC, ACT>(s, x + first, y + first, c0, nc, s.pixels, s_mean, s_rstd, weight, bias, pdtype);
+    apply_window<T, VEC, ACT>(s, x + first, y + first, c0, nc, s.pixels, stats, weight, bias, pdtype);
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------
+// What a thread holds of its VEC channels, and du = dy act'(u) of a vector of them.
+template <int VEC, int ACT>
+struct Channels {
+    float mean[VEC], rstd[VEC], a[VEC], beta[VEC], corner[VEC];     // a = gamma / std
+    const double2* stats;
+    const void *weight, *bias;
+    int pdtype, per_group, c0;
+    __device__ __forceinline__ void init(const double2* st, const void* w, const void* b, int dtype, int per, int first) {
+        stats = st; weight = w; bias = b; pdtype = dtype; per_group = per; c0 = first;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const double2 v = stats[(c0 + i) / per_group];
+            mean[i] = (float)v.x;
+            rstd[i] = (float)v.y;
+            a[i] = (float)(v.y * (double)param(weight, pdtype, c0 + i, 1.0f));
+            beta[i] = param(bias, pdtype, c0 + i, 0.0f);
+            // u is off by a few half steps of its terms, |x - mean| |a| = |beta| where it is zero, and of mean * a
+            corner[i] = 5.0e-7f * (fabsf(beta[i]) + fabsf(mean[i] * a[i]));
+        }
+    }
+    __device__ __forceinline__ float gamma(int i) const { return param(weight, pdtype, c0 + i, 1.0f); }
+    // d = x - mean and du, from x and dy
+    __device__ __forceinline__ void run(const float* x, const float* dy, float* d, float* du) const {
+        bool near = false;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            d[i] = x[i] - mean[i];
+            const float u = fmaf(d[i], a[i], beta[i]);
+            du[i] = act_grad<ACT>(u, dy[i]);
+            if (ACT == OD_ACT_RELU) near = near || fabsf(u) <= corner[i];
+        }
+        if (ACT == OD_ACT_RELU && near) {                           // about one vector in ten thousand
+            for (int i = 0; i < VEC; ++i) {
+                const double2 v = stats[(c0 + i) / per_group];
+                const double u = ((double)x[i] - v.x) * v.y * (double)param(weight, pdtype, c0 + i, 1.0f)
+                                 + (double)param(bias, pdtype, c0 + i, 0.0f);
+                du[i] = u <= 0.0 ? 0.0f : dy[i];
+            }
+        }
+    }
+};
+
 // Per-channel sums (du, du * xhat) of `n` pixels of channels [c0, c0 + nc); into out[0 .. nc).  red: 2 * NT * VEC floats.
 template <typename T, int VEC, int ACT>
 __device__ __forceinline__ void channel_sums(const NormShape& s, const T* x, const T* dy, int c0, int nc, long long n,
-                                             const float* mean_b, const float* rstd_b, const void* weight,
-                                             const void* bias, int pdtype, float2* out, float* red) {
+                                             const double2* stats_b, const void* weight, const void* bias, int pdtype,
+                                             float2* out, float* red) {
     const int cols = nc / VEC;
     const Lay lay(cols);
     for (int base = 0; base < cols; base += lay.width) {
@@ -357,26 +386,18 @@ __device__ __forceinline__ void channel_sums(const NormShape& s, const T* x, con
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = 0.0f;
         if (on) {
-            float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int c = c0 + col * VEC + i, g = c / s.per_group;
-                mean[i] = mean_b[g];
-                rstd[i] = rstd_b[g];
-                gamma[i] = param(weight, pdtype, c, 1.0f);
-                beta[i] = param(bias, pdtype, c, 0.0f);
-            }
+            Channels<VEC, ACT> ch;
+            ch.init(stats_b, weight, bias, pdtype, s.per_group, c0 + col * VEC);
             const int mine = taken(n, lay.ty, lay.rows);
             const long long step = (long long)lay.rows * s.channels;
             long long off = (long long)lay.ty * s.channels + c0 + col * VEC;
             auto add = [&](const float* v, const float* g) {
+                float d[VEC], du[VEC];
+                ch.run(v, g, d, du);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float d = v[i] - mean[i];
-                    // the forward's own expression, so that the mask of a rectified value is the forward's
-                    const float du = act_grad<ACT>(fmaf(d, rstd[i] * gamma[i], beta[i]), g[i]);
-                    s1[i] += du;
-                    s2[i] = fmaf(du, d * rstd[i], s2[i]);
+                    s1[i] += du[i];
+                    s2[i] = fmaf(du[i], d[i], s2[i]);               // times 1/std at the end
                 }
             };
             int j = 0;
@@ -395,6 +416,8 @@ __device__ __forceinline__ void channel_sums(const NormShape& s, const T* x, con
                 load_vec<T, VEC>(dy + off, g0);
                 add(v0, g0);
             }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s2[i] *= ch.rstd[i];
         }
         __syncthreads();
         if (on)
@@ -418,34 +441,30 @@ __device__ __forceinline__ void channel_sums(const NormShape& s, const T* x, con
 
 template <typename T, int VEC, int ACT>
 __device__ __forceinline__ void grad_window(const NormShape& s, const T* x, const T* dy, T* dx, int c0, int nc, long long n,
-                                            const float* mean_b, const float* rstd_b, const float2* s_avg, int g_first,
-                                            const void* weight, const void* bias, int pdtype) {
+                                            const double2* stats_b, const float2* s_avg, int g_first, const void* weight,
+                                            const void* bias, int pdtype) {
     const int cols = nc / VEC;
     const Lay lay(cols);
     for (int base = 0; base < cols; base += lay.width) {
         const int col = base + lay.tx;
         if (!lay.active || col >= cols) continue;
-        float mean[VEC], rstd[VEC], gamma[VEC], beta[VEC], avg1[VEC], avg2[VEC];
+        Channels<VEC, ACT> ch;
+        ch.init(stats_b, weight, bias, pdtype, s.per_group, c0 + col * VEC);
+        float shift[VEC], slope[VEC];                   // dx = a du - shift - d slope
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const int c = c0 + col * VEC + i, g = c / s.per_group;
-            mean[i] = mean_b[g];
-            rstd[i] = rstd_b[g];
-            gamma[i] = param(weight, pdtype, c, 1.0f);
-            beta[i] = param(bias, pdtype, c, 0.0f);
-            avg1[i] = s_avg[g - g_first].x;
-            avg2[i] = s_avg[g - g_first].y;
+            const float2 avg = s_avg[(c0 + col * VEC + i) / s.per_group - g_first];
+            shift[i] = ch.rstd[i] * avg.x;
+            slope[i] = ch.rstd[i] * ch.rstd[i] * avg.y;
         }
         const int mine = taken(n, lay.ty, lay.rows);
         const long long step = (long long)lay.rows * s.channels;
         long long off = (long long)lay.ty * s.channels + c0 + col * VEC;
         auto grad = [&](float* v, const float* g) {
+            float d[VEC], du[VEC];
+            ch.run(v, g, d, du);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float d = v[i] - mean[i];
-                const float du = act_grad<ACT>(fmaf(d, rstd[i] * gamma[i], beta[i]), g[i]);
-                v[i] = rstd[i] * (fmaf(gamma[i], du, -avg1[i]) - d * rstd[i] * avg2[i]);
-            }
+            for (int i = 0; i < VEC; ++i) v[i] = fmaf(ch.a[i], du[i], -shift[i]) - d[i] * slope[i];
         };
         int j = 0;
         for (; j + 2 <= mine; j += 2, off += 2 * step) {
@@ -494,17 +513,16 @@ __device__ __forceinline__ void group_averages(const float2* ch, int groups, int
 // part[(image * chunks + chunk) * channels + c] = channel sums of the chunk
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(NT) void norm_bwd_sums_kernel(NormShape s, const T* __restrict__ x, const T* __restrict__ dy,
-                                                           const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                           const double2* __restrict__ stats,
                                                            const void* __restrict__ weight, const void* __restrict__ bias,
                                                            int pdtype, float2* __restrict__ part) {
-    extern __shared__ float smem[];
+    extern __shared__ double smem[];
     const long long b = blockIdx.x / s.chunks;
     const int chunk = blockIdx.x % s.chunks;
     const long long p0 = chunk * s.chunk_pixels;
     const long long first = (b * s.pixels + p0) * s.channels;
     channel_sums<T, VEC, ACT>(s, x + first, dy + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0),
-                              mean + b * s.groups, rstd + b * s.groups, weight, bias, pdtype,
-                              part + (long long)blockIdx.x * s.channels, smem);
+                              stats + b * s.groups, weight, bias, pdtype, part + (long long)blockIdx.x * s.channels, reinterpret_cast<float*>(smem));
 }
 
 // sums[image * channels + c] = the chunks of one image joined.  A workgroup: 64 channels x 4 slices of the chunks.
@@ -534,11 +552,11 @@ __global__ __launch_bounds__(NT) void norm_bwd_join_kernel(NormShape s, const fl
 
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(NT) void norm_bwd_apply_kernel(NormShape s, const T* __restrict__ x, const T* __restrict__ dy,
-                                                            T* __restrict__ dx, const float* __restrict__ mean,
-                                                            const float* __restrict__ rstd, const void* __restrict__ weight,
+                                                            T* __restrict__ dx, const double2* __restrict__ stats,
+                                                            const void* __restrict__ weight,
                                                             const void* __restrict__ bias, int pdtype,
                                                             const float2* __restrict__ sums) {
-    extern __shared__ float smem[];
+    extern __shared__ double smem[];
     float2* avg = reinterpret_cast<float2*>(smem);
     const long long b = blockIdx.x / s.chunks;
     const int chunk = blockIdx.x % s.chunks;
@@ -548,34 +566,33 @@ __global__ __launch_bounds__(NT) void norm_bwd_apply_kernel(NormShape s, const T
     const long long p0 = chunk * s.chunk_pixels;
     const long long first = (b * s.pixels + p0) * s.channels;
     grad_window<T, VEC, ACT>(s, x + first, dy + first, dx + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0),
-                             mean + b * s.groups, rstd + b * s.groups, avg, 0, weight, bias, pdtype);
+                             stats + b * s.groups, avg, 0, weight, bias, pdtype);
 }
 
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(NT) void norm_bwd_small_kernel(NormShape s, int slab, const T* __restrict__ x,
                                                             const T* __restrict__ dy, T* __restrict__ dx,
-                                                            const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                            const double2* __restrict__ stats,
                                                             const void* __restrict__ weight, const void* __restrict__ bias,
                                                             int pdtype, float2* __restrict__ sums) {
-    extern __shared__ float smem[];
-    float* red = smem;
-    float2* ch = reinterpret_cast<float2*>(smem + 2 * NT * VEC);
+    extern __shared__ double smem[];
+    float* red = reinterpret_cast<float*>(smem);
+    float2* ch = reinterpret_cast<float2*>(red + 2 * NT * VEC);
     float2* avg = ch + slab;
     const int slabs = (s.channels + slab - 1) / slab;
     const long long b = blockIdx.x / slabs;
     const int c0 = (int)(blockIdx.x % slabs) * slab;
     const int nc = min(slab, s.channels - c0);
     const long long first = b * s.pixels * s.channels;
-    channel_sums<T, VEC, ACT>(s, x + first, dy + first, c0, nc, s.pixels, mean + b * s.groups, rstd + b * s.groups, weight,
-                              bias, pdtype, ch, red);
+    channel_sums<T, VEC, ACT>(s, x + first, dy + first, c0, nc, s.pixels, stats + b * s.groups, weight, bias, pdtype, ch, red);
     __syncthreads();
     for (int c = threadIdx.x; c < nc; c += NT) sums[b * s.channels + c0 + c] = ch[c];
     if (dx) {
         group_averages(ch, nc / s.per_group, s.per_group, c0, (double)s.pixels * s.per_group, weight, pdtype,
                        [&](int g, float a, float q) { avg[g] = make_float2(a, q); });
         __syncthreads();
-        grad_window<T, VEC, ACT>(s, x + first, dy + first, dx + first, c0, nc, s.pixels, mean + b * s.groups,
-                                 rstd + b * s.groups, avg, c0 / s.per_group, weight, bias, pdtype);
+        grad_window<T, VEC, ACT>(s, x + first, dy + first, dx + first, c0, nc, s.pixels, stats + b * s.groups, avg,
+                                 c0 / s.per_group, weight, bias, pdtype);
     }
 }
 
@@ -621,7 +638,7 @@ bool small_form(const NormShape& s, int slab, int size) {
     return s.pixels * slab * size <= (64 << 10);
 }
 
-NormShape shape_of(long long batch, long long pixels, int channels, int groups, float eps) {
+NormShape shape_of(long long batch, long long pixels, int channels, int groups, float eps, int size) {
     NormShape s;
     s.batch = batch;
     s.pixels = pixels;
@@ -629,8 +646,11 @@ NormShape shape_of(long long batch, long long pixels, int channels, int groups, 
     s.groups = groups;
     s.per_group = channels / groups;
     s.eps = eps;
-    // enough workgroups for 256 compute units several times over, at most MAX_CHUNKS per image, at least 16 pixels each
-    long long chunks = batch > 0 ? (2048 + batch - 1) / batch : 1;
+    // workgroups of at least 64 KiB (a smaller one is mostly its own start: 39 us instead of 15 to normalise 16 x 64 x 64 x 256 bf16 by 2048 of 16 KiB),
+    // two to eight per compute unit, at most MAX_CHUNKS per image, at least 16 pixels each
+    long long blocks = (long long)((double)batch * pixels * channels * size / 65536.0);
+    blocks = blocks < 512 ? 512 : blocks > 2048 ? 2048 : blocks;
+    long long chunks = batch > 0 ? (blocks + batch - 1) / batch : 1;
     if (chunks > MAX_CHUNKS) chunks = MAX_CHUNKS;
     if (chunks > (pixels + 15) / 16) chunks = (pixels + 15) / 16;
     if (chunks < 1) chunks = 1;
@@ -656,7 +676,7 @@ struct FwdCall {
     const void *x, *weight, *bias;
     void* y;
     int pdtype;
-    float *mean, *rstd;
+    double2* stats;
     void* ws;
     hipStream_t stream;
 };
@@ -668,18 +688,20 @@ int forward_typed(const FwdCall& c) {
     T* y = (T*)c.y;
     if (small_form(c.s, slab, sizeof(T))) {
         const long long grid = c.s.batch * ((c.s.channels + slab - 1) / slab);
-        const size_t lds = (2 * NT * VEC + 4 * (size_t)slab) * sizeof(float);
+        const size_t lds = (size_t)(slab + slab / c.s.per_group) * sizeof(double2) + 3 * NT * VEC * sizeof(float);
         OD_LAUNCH_KERNEL(OD_KERNEL_NORM_APPLY, (norm_small_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT), lds, c.stream,
-                         c.s, slab, x, y, c.weight, c.bias, c.pdtype, c.mean, c.rstd);
+                         c.s, slab, x, y, c.weight, c.bias, c.pdtype, c.stats);
         return OD_OK;
     }
-    float2* part = (float2*)c.ws;
+    double2* part = (double2*)c.ws;
     const long long grid = c.s.batch * c.s.chunks;
     OD_LAUNCH_KERNEL(OD_KERNEL_NORM_STATS, (norm_stats_kernel<T, VEC>), dim3((unsigned)grid), dim3(NT),
-                     (2 * NT * VEC + 2 * (size_t)c.s.channels) * sizeof(float), c.stream, c.s, x, part);
-    OD_LAUNCH_KERNEL(OD_KERNEL_NORM_APPLY, (norm_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
-                     (2 * (size_t)c.s.groups + NT) * sizeof(float), c.stream, c.s, x, y, (const float2*)part, c.weight, c.bias,
-                     c.pdtype, c.mean, c.rstd);
+                     c.s.channels * sizeof(double2) + 3 * NT * VEC * sizeof(float), c.stream, c.s, x, part);
+    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(c.s.batch * ((c.s.groups + 7) / 8))), dim3(NT), 0, c.stream, c.s,
+                       (const double2*)part, c.stats);
+    OD_LAUNCH_CHECK();
+    OD_LAUNCH_KERNEL(OD_KERNEL_NORM_APPLY, (norm_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT), 0, c.stream, c.s, x,
+                     y, c.weight, c.bias, c.pdtype, (const double2*)c.stats);
     return OD_OK;
 }
 
@@ -688,7 +710,7 @@ struct BwdCall {
     const void *x, *dy, *weight, *bias;
     void *dx, *dweight, *dbias;
     int pdtype;
-    const float *mean, *rstd;
+    const double2* stats;
     void* ws;
     hipStream_t stream;
 };
@@ -703,19 +725,19 @@ int backward_typed(const BwdCall& c) {
         const long long grid = c.s.batch * ((c.s.channels + slab - 1) / slab);
         const size_t lds = (2 * NT * VEC + 4 * (size_t)slab) * sizeof(float);
         OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_APPLY, (norm_bwd_small_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT), lds,
-                         c.stream, c.s, slab, x, dy, dx, c.mean, c.rstd, c.weight, c.bias, c.pdtype, sums);
+                         c.stream, c.s, slab, x, dy, dx, c.stats, c.weight, c.bias, c.pdtype, sums);
     } else {
         float2* part = sums + c.s.batch * c.s.channels;
         const long long grid = c.s.batch * c.s.chunks;
         OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_SUMS, (norm_bwd_sums_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
-                         2 * NT * VEC * sizeof(float), c.stream, c.s, x, dy, c.mean, c.rstd, c.weight, c.bias, c.pdtype, part);
-        hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(c.s.batch * ((c.s.channels + 63) / 64))), dim3(NT), 0,
-                           c.stream, c.s, (const float2*)part, sums);
+                         2 * NT * VEC * sizeof(float), c.stream, c.s, x, dy, c.stats, c.weight, c.bias, c.pdtype, part);
+        hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(c.s.batch * ((c.s.channels + 63) / 64))), dim3(NT), 0, c.stream,
+                           c.s, (const float2*)part, sums);
         OD_LAUNCH_CHECK();
         if (dx) {
             OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_APPLY, (norm_bwd_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
-                             2 * (size_t)c.s.groups * sizeof(float), c.stream, c.s, x, dy, dx, c.mean, c.rstd, c.weight,
-                             c.bias, c.pdtype, (const float2*)sums);
+                             2 * (size_t)c.s.groups * sizeof(float), c.stream, c.s, x, dy, dx, c.stats, c.weight, c.bias,
+                             c.pdtype, (const float2*)sums);
         }
     }
     if (c.dweight || c.dbias) {
@@ -760,37 +782,38 @@ int vector_width(int dtype, int channels, uintptr_t addresses) {
 
 extern "C" size_t od_group_norm_act_workspace_bytes(int64_t batch, int64_t pixels, int32_t channels, int32_t groups) {
     if (check_shape(OD_DTYPE_F32, batch, pixels, channels, groups, OD_DTYPE_F32, OD_ACT_NONE) != OD_OK) return 0;
-    const NormShape s = shape_of(batch, pixels, channels, groups, 0.0f);
-    return (size_t)(batch * (s.chunks + 1)) * channels * sizeof(float2) + 256;
+    // part: at most 2048 + batch chunks in a launch, of a float2 per channel or a double2 per group; sums: one per image
+    const long long chunks = 2048 + batch, each = (long long)channels * sizeof(float2) > groups * (long long)sizeof(double2)
+                                                      ? (long long)channels * sizeof(float2) : groups * (long long)sizeof(double2);
+    return (size_t)(chunks * each + batch * channels * (long long)sizeof(float2)) + 256;
 }
 
 extern "C" int od_group_norm_act_forward(const void* x, int32_t dtype, int64_t batch, int64_t pixels, int32_t channels,
                                          int32_t groups, const void* weight, const void* bias, int32_t param_dtype,
-                                         float eps, int32_t activation, void* y, float* mean, float* rstd,
-                                         void* workspace, size_t workspace_bytes, void* stream) {
+                                         float eps, int32_t activation, void* y, double* stats, void* workspace,
+                                         size_t workspace_bytes, void* stream) {
     const int rc = check_shape(dtype, batch, pixels, channels, groups, param_dtype, activation);
     if (rc != OD_OK) return rc;
     if (batch == 0 || pixels == 0) return OD_OK;
-    if (!x || !y || !mean || !rstd || !workspace || ((uintptr_t)workspace & 255)) return OD_ERR_ARG;
+    if (!x || !y || !stats || ((uintptr_t)stats & 15) || !workspace || ((uintptr_t)workspace & 255)) return OD_ERR_ARG;
     if (((uintptr_t)x | (uintptr_t)y) % elem_size(dtype)) return OD_ERR_ARG;
     if (workspace_bytes < od_group_norm_act_workspace_bytes(batch, pixels, channels, groups)) return OD_ERR_WORKSPACE;
-    const FwdCall call = {shape_of(batch, pixels, channels, groups, eps), x, weight, bias, y, param_dtype, mean, rstd,
+    const FwdCall call = {shape_of(batch, pixels, channels, groups, eps, elem_size(dtype)), x, weight, bias, y, param_dtype, (double2*)stats,
                           workspace, (hipStream_t)stream};
     OD_NORM_DISPATCH(forward_typed, call, vector_width(dtype, channels, (uintptr_t)x | (uintptr_t)y));
 }
 
 extern "C" int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int64_t batch, int64_t pixels,
                                           int32_t channels, int32_t groups, const void* weight, const void* bias,
-                                          int32_t param_dtype, int32_t activation, const float* mean, const float* rstd,
-                                          void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                                          int32_t param_dtype, int32_t activation, const double* stats, void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
                                           void* stream) {
     const int rc = check_shape(dtype, batch, pixels, channels, groups, param_dtype, activation);
     if (rc != OD_OK) return rc;
     if (batch == 0 || pixels == 0) return OD_OK;
-    if (!x || !dy || !mean || !rstd || !workspace || ((uintptr_t)workspace & 255)) return OD_ERR_ARG;
+    if (!x || !dy || !stats || ((uintptr_t)stats & 15) || !workspace || ((uintptr_t)workspace & 255)) return OD_ERR_ARG;
     if (((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx) % elem_size(dtype)) return OD_ERR_ARG;
     if (workspace_bytes < od_group_norm_act_workspace_bytes(batch, pixels, channels, groups)) return OD_ERR_WORKSPACE;
-    const BwdCall call = {shape_of(batch, pixels, channels, groups, 0.0f), x, dy, weight, bias, dx, dweight, dbias,
-                          param_dtype, mean, rstd, workspace, (hipStream_t)stream};
+    const BwdCall call = {shape_of(batch, pixels, channels, groups, 0.0f, elem_size(dtype)), x, dy, weight, bias, dx, dweight, dbias,
+                          param_dtype, (const double2*)stats, workspace, (hipStream_t)stream};
     OD_NORM_DISPATCH(backward_typed, call, vector_width(dtype, channels, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx));
 }

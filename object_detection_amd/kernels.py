@@ -727,19 +727,23 @@ def fcos_box_loss_backward(bbox_regression: Tensor, bbox_ctrness: Tensor, anchor
 # ------------------------------------------------------------------------------------------------
 # Scratch of the calls below comes from torch's allocator call by call: it is ordered with the stream the call runs on,
 # and a call recorded into a HIP graph holds memory of that graph's own pool -- two graphs never share it.
-def _norm_args(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor]):
+def _addr(t: Optional[Tensor]) -> Optional[int]:
+    """Address of a tensor for a pointer argument, without a ctypes object per call."""
+    return None if t is None else t.data_ptr()
+
+
+def _norm_args(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor]) -> Tuple[int, int]:
     """Checks of group_norm_act_*; returns (element code, parameter code)."""
-    _require_gpu(x, "x")
     if x.dim() != 3 or not x.is_contiguous():
         raise ValueError(f"group_norm_act: x must be contiguous [batch, pixels, channels], got {tuple(x.shape)}")
-    C = int(x.shape[2])
+    C = x.shape[2]
     if num_groups < 1 or C < 1 or C % num_groups:
         raise ValueError(f"group_norm_act: {C} channels cannot be divided into {num_groups} groups")
     pcode = _C.DTYPE_F32
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
-        if tuple(p.shape) != (C,):
+        if p.dim() != 1 or p.shape[0] != C:
             raise ValueError(f"group_norm_act: {name} must be [{C}], got {tuple(p.shape)}")
         if p.device != x.device:
             raise RuntimeError(f"group_norm_act: {name} is on {p.device}, x on {x.device}")
@@ -765,35 +769,38 @@ def _norm_workspace(x: Tensor, num_groups: int) -> Tensor:
 
 
 def group_norm_act_forward(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
-                           activation: int) -> Tuple[Tensor, Tensor, Tensor]:
+                           activation: int) -> Tuple[Tensor, Tensor]:
     """Group norm + activation of channels-last rows x [B, P, C] fp32 / fp16 / bf16; weight / bias [C] (one type, fp32 or
-    16-bit) or None.  Returns (y [B, P, C], mean [B, G], rstd [B, G])."""
+    16-bit) or None.  Returns (y [B, P, C], stats float64 [B, G, 2]: mean and 1/std)."""
+    _require_gpu(x, "x")
     code, pcode = _norm_args(x, num_groups, weight, bias)
     B, P, C = x.shape
+    dev = x.device
     ws = _norm_workspace(x, num_groups)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     y = torch.empty_like(x)
-    mean = torch.empty((B, num_groups), dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    with _on(x.device):
-        rc = _C.lib().od_group_norm_act_forward(_ptr(x), code, B, P, C, int(num_groups), _ptr(weight), _ptr(bias), pcode,
-                                                float(eps), int(activation), _ptr(y), _ptr(mean), _ptr(rstd), _ptr(ws),
-                                                ws.numel(), _stream(x.device))
+    stats = torch.empty((B, num_groups, 2), dtype=torch.float64, device=dev)
+    with _on(dev):
+        rc = _C.lib().od_group_norm_act_forward(x.data_ptr(), code, B, P, C, num_groups, _addr(weight), _addr(bias), pcode, eps,
+                                                activation, y.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(),
+                                                _raw_stream(dev))
     _C.check(rc, "od_group_norm_act_forward")
-    return y, mean, rstd
+    return y, stats
 
 
 def group_norm_act_backward(x: Tensor, dy: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor],
-                            activation: int, mean: Tensor, rstd: Tensor, want_dx: bool = True, want_dweight: bool = True,
+                            activation: int, stats: Tensor, want_dx: bool = True, want_dweight: bool = True,
                             want_dbias: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
     """Gradients of group_norm_act_forward: (dx [B, P, C], dweight [C], dbias [C]); None for what is not wanted or not
     there."""
+    _require_gpu(x, "x")
     code, pcode = _norm_args(x, num_groups, weight, bias)
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device or not dy.is_contiguous():
-        raise ValueError(f"group_norm_act: dy must be contiguous {x.dtype} {tuple(x.shape)} on {x.device}, got {dy.dtype} "
-                         f"{tuple(dy.shape)} on {dy.device}")
     B, P, C = x.shape
+    dev = x.device
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != dev or not dy.is_contiguous():
+        raise ValueError(f"group_norm_act: dy must be contiguous {x.dtype} {tuple(x.shape)} on {dev}, got {dy.dtype} "
+                         f"{tuple(dy.shape)} on {dy.device}")
     ws = _norm_workspace(x, num_groups)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
@@ -801,10 +808,10 @@ def group_norm_act_backward(x: Tensor, dy: Tensor, num_groups: int, weight: Opti
     dx = torch.empty_like(x) if want_dx else None
     dweight = fresh(weight) if want_dweight and weight is not None else None
     dbias = fresh(bias) if want_dbias and bias is not None else None
-    with _on(x.device):
-        rc = _C.lib().od_group_norm_act_backward(_ptr(x), _ptr(dy), code, B, P, C, int(num_groups), _ptr(weight), _ptr(bias),
-                                                 pcode, int(activation), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(dweight),
-                                                 _ptr(dbias), _ptr(ws), ws.numel(), _stream(x.device))
+    with _on(dev):
+        rc = _C.lib().od_group_norm_act_backward(x.data_ptr(), dy.data_ptr(), code, B, P, C, num_groups, _addr(weight),
+                                                 _addr(bias), pcode, activation, stats.data_ptr(), _addr(dx), _addr(dweight),
+                                                 _addr(dbias), ws.data_ptr(), ws.numel(), _raw_stream(dev))
     _C.check(rc, "od_group_norm_act_backward")
     return dx, dweight, dbias
 
@@ -845,18 +852,19 @@ def vocab_loss_forward(features: Tensor, weight: Tensor, bias: Optional[Tensor],
     Returns (row losses fp32 [N], loss fp32 [] or None, the buffer that vocab_loss_backward reads)."""
     _require_gpu(features, "features")
     dev = features.device
-    for name, t in (("weight", weight), ("bias", bias), ("targets", targets), ("teacher_logits", teacher_logits)):
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"vocab_loss: {name} is on {t.device}, features on {dev}")
     code = _dtype_code(features, "vocab_loss: features")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and t.dtype != features.dtype:
+    for name, t in (("weight", weight), ("bias", bias), ("targets", targets), ("teacher_logits", teacher_logits)):
+        if t is None:
+            continue
+        if t.device != dev:
+            raise RuntimeError(f"vocab_loss: {name} is on {t.device}, features on {dev}")
+        if t.dtype != features.dtype and (t is weight or t is bias):
             raise TypeError(f"vocab_loss: {name} is {t.dtype}, features {features.dtype}")
     if targets.dtype != torch.int64:
         raise TypeError(f"vocab_loss: targets must be int64, got {targets.dtype}")
     N, D = features.shape
     V = int(weight.shape[0])
-    if tuple(weight.shape) != (V, D) or (bias is not None and tuple(bias.shape) != (V,)):
+    if weight.shape[1] != D or (bias is not None and tuple(bias.shape) != (V,)):
         raise ValueError(f"vocab_loss: inconsistent shapes, features {tuple(features.shape)}, weight {tuple(weight.shape)}"
                          + ("" if bias is None else f", bias {tuple(bias.shape)}"))
     if V < 1 or D < 1:
@@ -879,9 +887,10 @@ def vocab_loss_forward(features: Tensor, weight: Tensor, bias: Optional[Tensor],
     saved = torch.empty(_vocab_bytes(N, V, D, top, code, "saved"), dtype=torch.uint8, device=dev)
     ws = torch.empty(_vocab_bytes(N, V, D, top, code, "forward"), dtype=torch.uint8, device=dev)
     with _on(dev):
-        rc = _C.lib().od_vocab_loss_forward(_ptr(features), _pitch(features), _ptr(weight), _pitch(weight), _ptr(bias), code, N,
-                                            V, D, _ptr(targets), top, _ptr(teacher_logits), tcode, float(temperature),
-                                            int(reduction), _ptr(row_loss), _ptr(loss), _ptr(saved), saved.numel(), _ptr(ws), ws.numel(), _stream(dev))
+        rc = _C.lib().od_vocab_loss_forward(features.data_ptr(), _pitch(features), weight.data_ptr(), _pitch(weight), _addr(bias),
+                                            code, N, V, D, targets.data_ptr(), top, _addr(teacher_logits), tcode, temperature,
+                                            reduction, row_loss.data_ptr(), _addr(loss), saved.data_ptr(), saved.numel(),
+                                            ws.data_ptr(), ws.numel(), _raw_stream(dev))
     _C.check(rc, "od_vocab_loss_forward")
     return row_loss, loss, saved
 
@@ -907,8 +916,9 @@ def vocab_loss_backward(weight: Tensor, bias: Optional[Tensor], targets: Tensor,
     dbias = fresh((V,), dtype=weight.dtype, device=dev) if want_bias and bias is not None else None
     ws = torch.empty(_vocab_bytes(N, V, D, top, code, "backward"), dtype=torch.uint8, device=dev)
     with _on(dev):
-        rc = _C.lib().od_vocab_loss_backward(_ptr(weight), _pitch(weight), _ptr(bias), code, N, V, D, _ptr(targets), top,
-                                             float(temperature), int(reduction), _ptr(upstream), _ptr(saved), saved.numel(),
-                                             _ptr(dfeatures), _ptr(dweight), _ptr(dbias), _ptr(ws), ws.numel(), _stream(dev))
+        rc = _C.lib().od_vocab_loss_backward(weight.data_ptr(), _pitch(weight), _addr(bias), code, N, V, D, targets.data_ptr(),
+                                             top, temperature, reduction, upstream.data_ptr(), saved.data_ptr(), saved.numel(),
+                                             _addr(dfeatures), _addr(dweight), _addr(dbias), ws.data_ptr(), ws.numel(),
+                                             _raw_stream(dev))
     _C.check(rc, "od_vocab_loss_backward")
     return dfeatures, dweight, dbias

@@ -38,19 +38,19 @@ class _GroupNormAct(torch.autograd.Function):
     def forward(ctx, x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
                 activation: int) -> Tensor:
         rows = _rows(x)
-        y, mean, rstd = kernels.group_norm_act_forward(rows, num_groups, weight, bias, eps, activation)
-        ctx.save_for_backward(rows, weight, bias, mean, rstd)
+        y, stats = kernels.group_norm_act_forward(rows, num_groups, weight, bias, eps, activation)
+        ctx.save_for_backward(rows, weight, bias, stats)
         ctx.conf = (num_groups, activation, x.shape)
         return _map(y, x.shape)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out: Tensor):
-        rows, weight, bias, mean, rstd = ctx.saved_tensors
+        rows, weight, bias, stats = ctx.saved_tensors
         num_groups, activation, shape = ctx.conf
         need = ctx.needs_input_grad
         dx, dweight, dbias = kernels.group_norm_act_backward(rows, _rows(grad_out), num_groups, weight, bias, activation,
-                                                             mean, rstd, need[0], need[2], need[3])
+                                                             stats, need[0], need[2], need[3])
         return (None if dx is None else _map(dx, shape)), None, dweight, dbias, None, None
 
 

@@ -148,11 +148,11 @@ def test_argument_errors_of_group_norm_act():
 
     def fwd(x=p256, dtype=0, batch=2, pixels=64, channels=32, groups=4, pdtype=0, act=1, y=p256, ws=p256, nbytes=1 << 20):
         return lib.od_group_norm_act_forward(x, dtype, batch, pixels, channels, groups, null, null, pdtype, 1e-5, act, y, p256,
-                                             p256, ws, nbytes, null)
+                                             ws, nbytes, null)
 
     def bwd(x=p256, dtype=0, batch=2, pixels=64, channels=32, groups=4, pdtype=0, act=1, dy=p256, ws=p256, nbytes=1 << 20):
         return lib.od_group_norm_act_backward(x, dy, dtype, batch, pixels, channels, groups, null, null, pdtype, act, p256, p256,
-                                              p256, null, null, ws, nbytes, null)
+                                              null, null, ws, nbytes, null)
     for call in (fwd, bwd):
         assert call(x=null) == -1 and call(ws=null) == -1 and call(ws=p16) == -1
         assert call(dtype=3) == -1 and call(pdtype=-1) == -1 and call(act=3) == -1

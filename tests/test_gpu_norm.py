@@ -126,13 +126,36 @@ def test_offset_far_above_the_spread(device, dtype):
     gen = torch.Generator().manual_seed(9)
     x = (300.0 + torch.randn((2, 64, 50, 50), generator=gen)).to(device, dtype).contiguous(memory_format=torch.channels_last)
     x[0, 0, 0, 0] = -5000.0                                                          # an outlier in a shift's place
-    y, mean, rstd = kernels.group_norm_act_forward(x.permute(0, 2, 3, 1).reshape(2, 2500, 64), 8, None, None, 1e-5, 0)
+    y, stats = kernels.group_norm_act_forward(x.permute(0, 2, 3, 1).reshape(2, 2500, 64), 8, None, None, 1e-5, 0)
     v = x.double().reshape(2, 8, -1)
     spread = v.std(dim=2, unbiased=False)
-    # means are held in fp32: 300 * 2^-24 each, plus CHAIN of the spread; see CHAIN
-    assert float((mean.double() - v.mean(dim=2)).abs().sub(CHAIN * spread + 302 * 4 * U32).max()) <= 0
+    assert float((stats[..., 0] - v.mean(dim=2)).abs().sub(CHAIN * spread).max()) <= 0
     # the outlier's own thread: the mean of its pixels is 5300 / 64 off its shift, a factor n = 64 on its half steps
-    assert float((rstd.double() * (spread ** 2 + 1e-5).sqrt() - 1).abs().max()) <= 64 * CHAIN
+    assert float((stats[..., 1] * (spread ** 2 + 1e-5).sqrt() - 1).abs().max()) <= 64 * CHAIN
+
+
+def test_rectifier_decides_as_64_bits_do(device):
+    """A bf16 map holds few different values: at mean 0, 1/std 1 and a bias that is a value of the map, hundreds of pixels of
+    a channel lie next to the corner, on the side that the statistics' last digits decide."""
+    gen = torch.Generator().manual_seed(4)
+    x = torch.randn((4, 32, 64, 64), generator=gen).to(device, torch.bfloat16).contiguous(memory_format=torch.channels_last)
+    dy = torch.ones_like(x)
+    gamma = torch.ones(32, device=device)
+    for trial in range(4):
+        v = x.double().reshape(4, 8, -1)
+        mean, std = v.mean(2), (v.var(2, unbiased=False) + 1e-5).sqrt()
+        at = x[trial, ::4, trial, trial].double()                                # a value of each group of image `trial`
+        beta = -((at - mean[trial]) / std[trial]).repeat_interleave(4).float()   # u of that value: a rounding of zero
+        xl, bl = x.clone(memory_format=torch.preserve_format).requires_grad_(True), beta.clone().requires_grad_(True)
+        y = group_norm_act(xl, 8, gamma, bl)
+        db = torch.autograd.grad(y, bl, dy)[0]
+        u = (x.double() - mean.repeat_interleave(4, 1)[..., None, None]) / std.repeat_interleave(4, 1)[..., None, None] \
+            + beta.double()[None, :, None, None]
+        # the side of a value is certain where u is further from zero than the sums' own error, 64 additions of 2^-24
+        # averaged over the 16384 * 4 values of a group: 1e-8
+        low, high = (u > 1e-8).sum(dim=(0, 2, 3)), (u > -1e-8).sum(dim=(0, 2, 3))
+        assert bool(((db >= low) & (db <= high)).all())
+        assert int((u.abs() < 1e-6).sum()) > 100                                # and the case is there
 
 
 def test_nan_and_inf_stay_in_their_group(device):
