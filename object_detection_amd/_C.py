@@ -133,6 +133,24 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_binding = None
+
+
+def torch_binding():
+    """The torch binding of the differentiable operators (``_od_torch.so``, built beside the library)."""
+    global _binding
+    if _binding is None:
+        lib()
+        try:
+            from . import _od_torch
+        except ImportError as e:
+            raise ImportError(f"{os.path.join(_HERE, '_od_torch.so')} is missing or does not load ({e}). Run "
+                              f"`make -C {os.path.join(_HERE, 'csrc')}` or "
+                              f"`python -c 'import __graft_entry__ as g; g.build()'` from the repository root.") from e
+        _binding = _od_torch
+    return _binding
+
+
 def check(code: int, what: str) -> None:
     if code == 0:
         return

@@ -1212,16 +1212,19 @@ long long most(long long a, long long b) { return a > b ? a : b; }
 int elem_size(int dtype) { return dtype == OD_DTYPE_F32 ? 4 : 2; }
 
 // Splits of `steps` steps of work, for each of `tiles` workgroups: the number with which the last workgroup ends first when
-// `slots` run at once and each costs `fixed` steps beside its share.
+// `slots` run at once and each costs `fixed` steps beside its share.  Only numbers that fill the slots a whole number of
+// times are worth a look.
 int splits_for(long long tiles, long long steps, int slots, int fixed, int limit) {
     long long best = 1, best_cost = -1;
-    for (long long s = 1; s <= least(steps, limit); ++s) {
-        const long long cost = (tiles * s + slots - 1) / slots * ((steps + s - 1) / s + fixed);
+    for (int turns = 1; turns <= 4; ++turns) {
+        long long s = most(1, least(turns * (long long)slots / tiles, least(steps, limit)));
+        const long long share = (steps + s - 1) / s;
+        s = (steps + share - 1) / share;                            // the fewest with this share
+        const long long cost = (tiles * s + slots - 1) / slots * (share + fixed);
         if (best_cost < 0 || cost < best_cost) {
             best = s;
             best_cost = cost;
         }
-        if (tiles * s > 4 * slots) break;
     }
     return (int)best;
 }

@@ -11,7 +11,6 @@ from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _C, kernels
 
@@ -279,29 +278,6 @@ def fcos_head_losses(cls_logits: Tensor, bbox_regression: Tensor, bbox_ctrness: 
 _REDUCTIONS = {"none": _C.REDUCE_NONE, "mean": _C.REDUCE_MEAN, "sum": _C.REDUCE_SUM}
 
 
-class _VocabularyLoss(torch.autograd.Function):
-    """Cross entropy or distillation of a head over a large vocabulary (kernels.vocab_loss_*).  Keeps the packed features
-    of the valid rows and one fp32 log-sum-exp per row; the logits are formed again, piece by piece, for the gradients."""
-
-    @staticmethod
-    def forward(ctx, features: Tensor, weight: Tensor, bias: Optional[Tensor], targets: Tensor,
-                teacher_logits: Optional[Tensor], temperature: float, reduction: int) -> Tensor:
-        rows, loss, saved = kernels.vocab_loss_forward(features, weight, bias, targets, teacher_logits, temperature,
-                                                       reduction)
-        if any(ctx.needs_input_grad[:3]):
-            ctx.save_for_backward(weight, bias, targets, saved)
-            ctx.conf = (temperature, reduction)
-        return rows if reduction == _C.REDUCE_NONE else loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out: Tensor):
-        weight, bias, targets, saved = ctx.saved_tensors
-        grads = kernels.vocab_loss_backward(weight, bias, targets, *ctx.conf, grad_out.to(torch.float32), saved,
-                                            *ctx.needs_input_grad[:3])
-        return (*grads, None, None, None, None)
-
-
 def _vocabulary_loss(features: Tensor, weight: Tensor, bias: Optional[Tensor], targets: Tensor,
                      teacher_logits: Optional[Tensor], temperature: float, reduction: str, shape) -> Tensor:
     kernels._require_gpu(features, "features")
@@ -310,9 +286,9 @@ def _vocabulary_loss(features: Tensor, weight: Tensor, bias: Optional[Tensor], t
     if features.dim() < 2 or weight.dim() != 2 or features.shape[-1] != weight.shape[1] or features.shape[:-1] != shape:
         raise ValueError(f"vocabulary loss takes features [..., D], weight [V, D] and one row of targets per row of features, "
                          f"got {tuple(features.shape)}, {tuple(weight.shape)}, {tuple(shape)}")
-    rows = features.reshape(-1, features.shape[-1])
-    out = _VocabularyLoss.apply(rows, weight, bias, targets, teacher_logits, float(temperature), _REDUCTIONS[reduction])
-    return out.reshape(shape) if reduction == "none" else out
+    rows = features if features.dim() == 2 else features.reshape(-1, features.shape[-1])
+    out = kernels.vocab_loss(rows, weight, bias, targets, teacher_logits, temperature, _REDUCTIONS[reduction])
+    return out.reshape(shape) if reduction == "none" and len(shape) != 1 else out
 
 
 def vocabulary_cross_entropy(features: Tensor, weight: Tensor, targets: Tensor, bias: Optional[Tensor] = None,
@@ -329,7 +305,8 @@ def vocabulary_cross_entropy(features: Tensor, weight: Tensor, targets: Tensor, 
     Differentiable once in features, weight and bias."""
     if targets.dtype != torch.int64:
         raise TypeError(f"targets must be int64, got {targets.dtype}")
-    return _vocabulary_loss(features, weight, bias, targets.reshape(-1), None, 1.0, reduction, targets.shape)
+    flat = targets if targets.dim() == 1 else targets.reshape(-1)
+    return _vocabulary_loss(features, weight, bias, flat, None, 1.0, reduction, targets.shape)
 
 
 def vocabulary_distillation(features: Tensor, weight: Tensor, teacher_logits: Tensor, teacher_classes: Tensor,

@@ -6,9 +6,8 @@ a GPU; none of them has a CPU implementation.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
-from typing import Dict, Optional, Sequence, Tuple
+from typing import Callable, Dict, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
@@ -46,13 +45,6 @@ def _raw_stream(device: torch.device) -> int:
 
 def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(_raw_stream(device))
-
-
-def _on(device: torch.device):
-    """Makes ``device`` the current one for a launch (a stream belongs to its device); free where it already is."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
 
 
 def _ptr(t: Optional[Tensor]) -> ctypes.c_void_p:
@@ -725,21 +717,36 @@ def fcos_box_loss_backward(bbox_regression: Tensor, bbox_ctrness: Tensor, anchor
 
 
 # ------------------------------------------------------------------------------------------------
-# Scratch of the calls below comes from torch's allocator call by call: it is ordered with the stream the call runs on,
-# and a call recorded into a HIP graph holds memory of that graph's own pool -- two graphs never share it.
-def _addr(t: Optional[Tensor]) -> Optional[int]:
-    """Address of a tensor for a pointer argument, without a ctypes object per call."""
-    return None if t is None else t.data_ptr()
+# The operators below are differentiable: their launches and their autograd nodes are in the torch binding
+# (csrc/od_torch.cpp).  Their scratch comes from torch's allocator call by call: it is ordered with the stream the call runs
+# on, and a call recorded into a HIP graph holds memory of that graph's own pool -- two graphs never share it.
+def _bytes(key: tuple, what: str, query: Callable[..., int], *sizes: int) -> int:
+    """Answer of a ``*_bytes`` query, which depends on its sizes alone; zero means sizes beyond the library's limits."""
+    nbytes = _ws_bytes.get(key)
+    if nbytes is None:
+        nbytes = query(*sizes)
+        if nbytes == 0:
+            raise _C.OdBoxesError(f"{what} beyond the limits in od_boxes.h ({key[1:]})")
+        if len(_ws_bytes) > 65536:
+            _ws_bytes.clear()
+        _ws_bytes[key] = nbytes
+    return nbytes
 
 
-def _norm_args(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor]) -> Tuple[int, int]:
-    """Checks of group_norm_act_*; returns (element code, parameter code)."""
-    if x.dim() != 3 or not x.is_contiguous():
-        raise ValueError(f"group_norm_act: x must be contiguous [batch, pixels, channels], got {tuple(x.shape)}")
-    C = x.shape[2]
+def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
+                   activation: int) -> Tensor:
+    """Group norm + activation of a map x [B, C, H, W] fp32 / fp16 / bf16, in channels-last memory; weight / bias [C] (one
+    type, fp32 or 16-bit) or None.  Differentiable once in x, weight and bias."""
+    _require_gpu(x, "x")
+    if x.dim() != 4:
+        raise ValueError(f"group_norm_act takes a map [B, C, H, W], got {tuple(x.shape)}")
+    B, C, H, W = x.shape
     if num_groups < 1 or C < 1 or C % num_groups:
         raise ValueError(f"group_norm_act: {C} channels cannot be divided into {num_groups} groups")
-    pcode = _C.DTYPE_F32
+    if C > _C.OD_MAX_NORM_CHANNELS or B > _C.OD_MAX_NORM_BATCH:
+        raise _C.OdBoxesError(f"group_norm_act: {B} images of {C} channels exceed the limits of {_C.OD_MAX_NORM_BATCH} images "
+                              f"and {_C.OD_MAX_NORM_CHANNELS} channels")
+    _dtype_code(x, "group_norm_act: x")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
@@ -747,109 +754,19 @@ def _norm_args(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optio
             raise ValueError(f"group_norm_act: {name} must be [{C}], got {tuple(p.shape)}")
         if p.device != x.device:
             raise RuntimeError(f"group_norm_act: {name} is on {p.device}, x on {x.device}")
-        pcode = _dtype_code(p, f"group_norm_act: {name}")
+        _dtype_code(p, f"group_norm_act: {name}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"group_norm_act: weight is {weight.dtype}, bias {bias.dtype}")
-    return _dtype_code(x, "group_norm_act: x"), pcode
+    nbytes = _bytes(("norm", B, H * W, C, num_groups), "group_norm_act: sizes",
+                    _C.lib().od_group_norm_act_workspace_bytes, B, H * W, C, num_groups)
+    return _C.torch_binding().group_norm_act(x, num_groups, weight, bias, eps, activation, nbytes)
 
 
-def _norm_workspace(x: Tensor, num_groups: int) -> Tensor:
-    B, P, C = x.shape
-    key = ("norm", B, P, C, num_groups)
-    nbytes = _ws_bytes.get(key)
-    if nbytes is None:
-        nbytes = _C.lib().od_group_norm_act_workspace_bytes(B, P, C, num_groups)
-        if nbytes == 0:
-            raise _C.OdBoxesError(f"od_group_norm_act: batch {B}, {C} channels exceed the limits of "
-                                  f"{_C.OD_MAX_NORM_BATCH} images and {_C.OD_MAX_NORM_CHANNELS} channels")
-        if len(_ws_bytes) > 65536:
-            _ws_bytes.clear()
-        _ws_bytes[key] = nbytes
-    return torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-
-
-def group_norm_act_forward(x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
-                           activation: int) -> Tuple[Tensor, Tensor]:
-    """Group norm + activation of channels-last rows x [B, P, C] fp32 / fp16 / bf16; weight / bias [C] (one type, fp32 or
-    16-bit) or None.  Returns (y [B, P, C], stats float64 [B, G, 2]: mean and 1/std)."""
-    _require_gpu(x, "x")
-    code, pcode = _norm_args(x, num_groups, weight, bias)
-    B, P, C = x.shape
-    dev = x.device
-    ws = _norm_workspace(x, num_groups)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    y = torch.empty_like(x)
-    stats = torch.empty((B, num_groups, 2), dtype=torch.float64, device=dev)
-    with _on(dev):
-        rc = _C.lib().od_group_norm_act_forward(x.data_ptr(), code, B, P, C, num_groups, _addr(weight), _addr(bias), pcode, eps,
-                                                activation, y.data_ptr(), stats.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                _raw_stream(dev))
-    _C.check(rc, "od_group_norm_act_forward")
-    return y, stats
-
-
-def group_norm_act_backward(x: Tensor, dy: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor],
-                            activation: int, stats: Tensor, want_dx: bool = True, want_dweight: bool = True,
-                            want_dbias: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
-    """Gradients of group_norm_act_forward: (dx [B, P, C], dweight [C], dbias [C]); None for what is not wanted or not
-    there."""
-    _require_gpu(x, "x")
-    code, pcode = _norm_args(x, num_groups, weight, bias)
-    B, P, C = x.shape
-    dev = x.device
-    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != dev or not dy.is_contiguous():
-        raise ValueError(f"group_norm_act: dy must be contiguous {x.dtype} {tuple(x.shape)} on {dev}, got {dy.dtype} "
-                         f"{tuple(dy.shape)} on {dy.device}")
-    ws = _norm_workspace(x, num_groups)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    fresh = torch.zeros_like if x.numel() == 0 else torch.empty_like      # no launch fills the sums of an empty map
-    dx = torch.empty_like(x) if want_dx else None
-    dweight = fresh(weight) if want_dweight and weight is not None else None
-    dbias = fresh(bias) if want_dbias and bias is not None else None
-    with _on(dev):
-        rc = _C.lib().od_group_norm_act_backward(x.data_ptr(), dy.data_ptr(), code, B, P, C, num_groups, _addr(weight),
-                                                 _addr(bias), pcode, activation, stats.data_ptr(), _addr(dx), _addr(dweight),
-                                                 _addr(dbias), ws.data_ptr(), ws.numel(), _raw_stream(dev))
-    _C.check(rc, "od_group_norm_act_backward")
-    return dx, dweight, dbias
-
-
-def _row_pitch(t: Tensor) -> Tensor:
-    """2-D tensor whose rows are contiguous and do not overlap; anything else is copied."""
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        return t.contiguous()
-    return t
-
-
-def _pitch(t: Tensor) -> int:
-    return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1])
-
-
-def _vocab_bytes(rows: int, classes: int, dim: int, top: int, code: int, which: str) -> int:
-    key = ("vocab", rows, classes, dim, top, code, which)
-    nbytes = _ws_bytes.get(key)
-    if nbytes is None:
-        if which == "saved":
-            nbytes = _C.lib().od_vocab_loss_saved_bytes(rows, classes, dim, top, code)
-        else:
-            nbytes = _C.lib().od_vocab_loss_workspace_bytes(rows, classes, dim, top, code, int(which == "backward"))
-        if nbytes == 0:
-            raise _C.OdBoxesError(f"od_vocab_loss: {rows} rows, {classes} classes, {dim} dimensions, {top} teacher entries are "
-                                  f"beyond the limits in od_boxes.h")
-        if len(_ws_bytes) > 65536:
-            _ws_bytes.clear()
-        _ws_bytes[key] = nbytes
-    return nbytes
-
-
-def vocab_loss_forward(features: Tensor, weight: Tensor, bias: Optional[Tensor], targets: Tensor,
-                       teacher_logits: Optional[Tensor], temperature: float,
-                       reduction: int) -> Tuple[Tensor, Optional[Tensor], Tensor]:
+def vocab_loss(features: Tensor, weight: Tensor, bias: Optional[Tensor], targets: Tensor, teacher_logits: Optional[Tensor],
+               temperature: float, reduction: int) -> Tensor:
     """Softmax cross entropy (targets int64 [N]) or distillation (targets int64 [N, K] with teacher_logits [N, K]) of rows
     features [N, D] against classes weight [V, D], bias [V] or None; one type, fp32 / fp16 / bf16.
-    Returns (row losses fp32 [N], loss fp32 [] or None, the buffer that vocab_loss_backward reads)."""
+    Returns the row losses fp32 [N] (REDUCE_NONE) or the loss fp32 []; differentiable once in features, weight and bias."""
     _require_gpu(features, "features")
     dev = features.device
     code = _dtype_code(features, "vocab_loss: features")
@@ -863,62 +780,34 @@ def vocab_loss_forward(features: Tensor, weight: Tensor, bias: Optional[Tensor],
     if targets.dtype != torch.int64:
         raise TypeError(f"vocab_loss: targets must be int64, got {targets.dtype}")
     N, D = features.shape
-    V = int(weight.shape[0])
+    V = weight.shape[0]
     if weight.shape[1] != D or (bias is not None and tuple(bias.shape) != (V,)):
         raise ValueError(f"vocab_loss: inconsistent shapes, features {tuple(features.shape)}, weight {tuple(weight.shape)}"
                          + ("" if bias is None else f", bias {tuple(bias.shape)}"))
     if V < 1 or D < 1:
         raise ValueError(f"vocab_loss: needs classes and dimensions, got weight {tuple(weight.shape)}")
-    top, tcode = 0, code
+    top = 0
     if teacher_logits is not None:
-        top, tcode = int(targets.shape[1]) if targets.dim() == 2 else 0, _dtype_code(teacher_logits, "vocab_loss: teacher_logits")
+        top = targets.shape[1] if targets.dim() == 2 else 0
+        _dtype_code(teacher_logits, "vocab_loss: teacher_logits")
         if targets.dim() != 2 or top < 1 or teacher_logits.shape != targets.shape:
             raise ValueError(f"vocab_loss: teacher classes {tuple(targets.shape)} and logits {tuple(teacher_logits.shape)} must "
                              f"be [N, K], K >= 1")
         if top > _C.OD_MAX_TEACHER_TOP:
-            raise _C.OdBoxesError(f"od_vocab_loss: {top} teacher entries per row exceed the limit of {_C.OD_MAX_TEACHER_TOP}")
-        teacher_logits = teacher_logits.contiguous()
+            raise _C.OdBoxesError(f"vocab_loss: {top} teacher entries per row exceed the limit of {_C.OD_MAX_TEACHER_TOP}")
     if targets.shape[0] != N or (top == 0 and targets.dim() != 1):
         raise ValueError(f"vocab_loss: targets {tuple(targets.shape)} for {N} rows")
-    features, weight, targets = _row_pitch(features), _row_pitch(weight), targets.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    row_loss = torch.empty((N,), dtype=torch.float32, device=dev)
-    loss = None if reduction == _C.REDUCE_NONE else torch.empty((), dtype=torch.float32, device=dev)
-    saved = torch.empty(_vocab_bytes(N, V, D, top, code, "saved"), dtype=torch.uint8, device=dev)
-    ws = torch.empty(_vocab_bytes(N, V, D, top, code, "forward"), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = _C.lib().od_vocab_loss_forward(features.data_ptr(), _pitch(features), weight.data_ptr(), _pitch(weight), _addr(bias),
-                                            code, N, V, D, targets.data_ptr(), top, _addr(teacher_logits), tcode, temperature,
-                                            reduction, row_loss.data_ptr(), _addr(loss), saved.data_ptr(), saved.numel(),
-                                            ws.data_ptr(), ws.numel(), _raw_stream(dev))
-    _C.check(rc, "od_vocab_loss_forward")
-    return row_loss, loss, saved
+    key = ("vocab", N, V, D, top, code)
+    sizes = _vocab_sizes.get(key)
+    if sizes is None:
+        lib = _C.lib()
+        sizes = (_bytes(key + ("saved",), "vocab_loss: sizes", lib.od_vocab_loss_saved_bytes, N, V, D, top, code),
+                 _bytes(key + ("forward",), "vocab_loss: sizes", lib.od_vocab_loss_workspace_bytes, N, V, D, top, code, 0),
+                 _bytes(key + ("backward",), "vocab_loss: sizes", lib.od_vocab_loss_workspace_bytes, N, V, D, top, code, 1))
+        if len(_vocab_sizes) > 4096:
+            _vocab_sizes.clear()
+        _vocab_sizes[key] = sizes
+    return _C.torch_binding().vocab_loss(features, weight, bias, targets, teacher_logits, temperature, reduction, *sizes)
 
 
-def vocab_loss_backward(weight: Tensor, bias: Optional[Tensor], targets: Tensor, temperature: float, reduction: int,
-                        upstream: Tensor, saved: Tensor, want_features: bool = True, want_weight: bool = True,
-                        want_bias: bool = True) -> Tuple[Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
-    """Gradients of vocab_loss_forward: (features [N, D], weight [V, D], bias [V]), None for what is not wanted or not there.
-    upstream: fp32 gradient of the row losses [N] (REDUCE_NONE) or of the loss."""
-    dev = weight.device
-    V, D = weight.shape
-    N = int(targets.shape[0])
-    top = int(targets.shape[1]) if targets.dim() == 2 else 0
-    code = _dtype_code(weight, "vocab_loss: weight")
-    if upstream.dtype != torch.float32 or upstream.numel() != (N if reduction == _C.REDUCE_NONE else 1) \
-            or upstream.device != dev:
-        raise ValueError(f"vocab_loss: upstream gradient {upstream.dtype} {tuple(upstream.shape)} on {upstream.device}")
-    weight, targets, upstream = _row_pitch(weight), targets.contiguous(), upstream.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    fresh = torch.zeros if N == 0 else torch.empty
-    dfeatures = fresh((N, D), dtype=weight.dtype, device=dev) if want_features else None
-    dweight = fresh((V, D), dtype=weight.dtype, device=dev) if want_weight else None
-    dbias = fresh((V,), dtype=weight.dtype, device=dev) if want_bias and bias is not None else None
-    ws = torch.empty(_vocab_bytes(N, V, D, top, code, "backward"), dtype=torch.uint8, device=dev)
-    with _on(dev):
-        rc = _C.lib().od_vocab_loss_backward(weight.data_ptr(), _pitch(weight), _addr(bias), code, N, V, D, targets.data_ptr(),
-                                             top, temperature, reduction, upstream.data_ptr(), saved.data_ptr(), saved.numel(),
-                                             _addr(dfeatures), _addr(dweight), _addr(dbias), ws.data_ptr(), ws.numel(),
-                                             _raw_stream(dev))
-    _C.check(rc, "od_vocab_loss_backward")
-    return dfeatures, dweight, dbias
+_vocab_sizes: Dict[tuple, Tuple[int, int, int]] = {}

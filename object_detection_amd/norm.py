@@ -10,48 +10,11 @@ from __future__ import annotations
 
 from typing import Optional
 
-import torch
 from torch import Tensor, nn
-from torch.autograd.function import once_differentiable
 
 from . import _C, kernels
 
 _ACTIVATIONS = {"none": _C.ACT_NONE, "relu": _C.ACT_RELU, "silu": _C.ACT_SILU}
-
-
-def _rows(t: Tensor) -> Tensor:
-    """[B, C, H, W] in any memory order -> dense [B, H*W, C] rows (a view of a channels-last map)."""
-    B, C, H, W = t.shape
-    return t.permute(0, 2, 3, 1).contiguous().view(B, H * W, C)
-
-
-def _map(rows: Tensor, shape) -> Tensor:
-    B, C, H, W = shape
-    if H * W == 1:
-        # one pixel is both orders at once; under channels-last strides torch's convolution to one output channel refuses it
-        return rows.view(B, C, 1, 1)
-    return rows.view(B, H, W, C).permute(0, 3, 1, 2)
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x: Tensor, num_groups: int, weight: Optional[Tensor], bias: Optional[Tensor], eps: float,
-                activation: int) -> Tensor:
-        rows = _rows(x)
-        y, stats = kernels.group_norm_act_forward(rows, num_groups, weight, bias, eps, activation)
-        ctx.save_for_backward(rows, weight, bias, stats)
-        ctx.conf = (num_groups, activation, x.shape)
-        return _map(y, x.shape)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out: Tensor):
-        rows, weight, bias, stats = ctx.saved_tensors
-        num_groups, activation, shape = ctx.conf
-        need = ctx.needs_input_grad
-        dx, dweight, dbias = kernels.group_norm_act_backward(rows, _rows(grad_out), num_groups, weight, bias, activation,
-                                                             stats, need[0], need[2], need[3])
-        return (None if dx is None else _map(dx, shape)), None, dweight, dbias, None, None
 
 
 def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
@@ -62,14 +25,11 @@ def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, 
     "relu" or "silu".  weight / bias [C] share one type, which may differ from x's (fp32 parameters of a tower that runs
     under autocast).  Statistics, normalisation and the sums of the gradients are fp32 for every type; the result is
     rounded once.  Differentiable once in x, weight and bias.  Limits: 2048 channels, 65535 images."""
-    kernels._require_gpu(x, "x")
-    if x.dim() != 4:
-        raise ValueError(f"group_norm_act takes a map [B, C, H, W], got {tuple(x.shape)}")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(_ACTIVATIONS)}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    return _GroupNormAct.apply(x, int(num_groups), weight, bias, float(eps), _ACTIVATIONS[activation])
+    return kernels.group_norm_act(x, num_groups, weight, bias, eps, _ACTIVATIONS[activation])
 
 
 class GroupNormAct(nn.GroupNorm):

@@ -8,7 +8,7 @@ import pytest
 import torch
 from torch import nn
 
-from object_detection_amd import _C, det_utils, kernels
+from object_detection_amd import _C, det_utils
 from object_detection_amd.norm import GroupNormAct
 
 pytestmark = pytest.mark.gpu
