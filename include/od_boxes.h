@@ -443,7 +443,7 @@ int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int
 #define OD_REDUCE_SUM 2
 #define OD_MAX_VOCAB_ROWS 8388608
 #define OD_MAX_VOCAB_CLASSES 16777216
-#define OD_MAX_VOCAB_DIM 16384          /* and at most 32 GiB each of features and weight */
+#define OD_MAX_VOCAB_DIM 16384          /* and at most 16 GiB each of features and weight */
 #define OD_MAX_TEACHER_TOP 256
 size_t od_vocab_loss_saved_bytes(int64_t rows, int64_t classes, int32_t dim, int32_t top, int32_t dtype);
 size_t od_vocab_loss_workspace_bytes(int64_t rows, int64_t classes, int32_t dim, int32_t top, int32_t dtype,

@@ -230,6 +230,7 @@ __global__ __launch_bounds__(1024) void list_rows_kernel(const long long* __rest
     const int per = (rows + 1023) / 1024;
     const int a = min(rows, (int)threadIdx.x * per), b = min(rows, a + per);
     int n = 0;
+#pragma unroll 8
     for (int r = a; r < b; ++r) n += flags ? flags[r] : (targets[r] >= 0);
     sums[threadIdx.x] = n;
     __syncthreads();
@@ -240,6 +241,7 @@ __global__ __launch_bounds__(1024) void list_rows_kernel(const long long* __rest
         __syncthreads();
     }
     int at = sums[threadIdx.x] - n;
+#pragma unroll 8
     for (int r = a; r < b; ++r) {
         const bool on = flags ? flags[r] != 0 : targets[r] >= 0;
         lists.place[r] = on ? at : -1;
@@ -331,42 +333,133 @@ __global__ __launch_bounds__(VT) void teacher_kernel(const long long* __restrict
     }
 }
 
-// Features of the valid rows, dense: [rows rounded up to ROW_TILE][dim_pad], zero behind the last valid row and the last
-// column.  A thread copies one 16-byte chunk; sources that are not aligned for it are read element by element.
+// Scalars of a backward call, on the device.
+struct Scales {
+    float common;                       // largest |upstream| times share and temperature
+    uint32_t features_max, weight_max;  // bits of the largest finite |weighted feature| and |weight|
+};
+
+// What the product reads, by one launch: features of the valid rows, weight rows where the caller's cannot be read in
+// place, and the bias.
+struct PrepareArgs {
+    // features: dense, [rows rounded up to ROW_TILE][dim_pad], zero behind the last valid row and the last column
+    const void* features;
+    long long feature_pitch;
+    void* packed;
+    long long rows_pad;
+    RowLists lists;
+    // weight: [classes][dim_pad], zero behind the last column
+    const void* weight;
+    long long weight_pitch, classes;
+    void* packed_weight;
+    // bias in units of log2, -inf behind the last class: the tiles' tail then drops out of maxima and sums by itself
+    const void* bias;
+    int bias_len;
+    float scale;
+    float* bias2;
+    int dim, dim_pad;
+    unsigned feature_blocks, weight_blocks;
+    // few rows: the lists are made here, by every workgroup for itself, instead of by a launch of their own
+    const long long* targets;
+    const unsigned char* flags;
+    int rows;
+    float* row_loss;
+    // backward: the scalars of a call whose rows share one gradient
+    Scales* scales;
+    const float* upstream;
+    int reduction;
+    float temperature;
+};
+
+// 16 bytes of a packed row; a source that is not aligned for it is read element by element
 template <typename T>
-__global__ __launch_bounds__(VT) void pack_rows_kernel(const T* __restrict__ src, long long pitch, int dim, int dim_pad,
-                                                       const int* __restrict__ row_of, const int* __restrict__ count,
-                                                       long long rows_out, T* __restrict__ dst) {
+__device__ __forceinline__ void pack_chunk(const T* row, int c, int dim, T* dst) {
     constexpr int E = 16 / sizeof(T);
-    const int chunks = dim_pad / E;
-    const long long at = (long long)blockIdx.x * VT + threadIdx.x;
-    const long long r = at / chunks;
-    if (r >= rows_out) return;
-    const int c = (int)(at % chunks) * E;
-    const long long limit = count ? *count : rows_out;
     alignas(16) T v[E];
-    if (r < limit) {
-        const T* p = src + (row_of ? (long long)row_of[r] : r) * pitch + c;
-        if (c + E <= dim && ((uintptr_t)p & 15) == 0) {
-            *reinterpret_cast<u32x4*>(v) = *reinterpret_cast<const u32x4*>(p);
-        } else {
-#pragma unroll
-            for (int i = 0; i < E; ++i) v[i] = c + i < dim ? p[i] : Elem<T>::from_float(0.0f);
-        }
+    const T* p = row + c;
+    if (row && c + E <= dim && ((uintptr_t)p & 15) == 0) {
+        *reinterpret_cast<u32x4*>(v) = *reinterpret_cast<const u32x4*>(p);
     } else {
-        if (count && r >= up_to(limit, ROW_TILE)) return;                 // no tile reads behind the last one's end
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = Elem<T>::from_float(0.0f);
+        for (int i = 0; i < E; ++i) v[i] = row && c + i < dim ? p[i] : Elem<T>::from_float(0.0f);
     }
-    *reinterpret_cast<u32x4*>(dst + r * dim_pad + c) = *reinterpret_cast<const u32x4*>(v);
+    *reinterpret_cast<u32x4*>(dst) = *reinterpret_cast<const u32x4*>(v);
 }
 
-// bias in units of log2, -inf behind the last class: the tiles' tail then drops out of maxima and sums by itself
-template <typename T>
-__global__ __launch_bounds__(VT) void bias_kernel(const T* __restrict__ bias, int classes, int classes_pad, float scale,
-                                                  float* __restrict__ out) {
-    const int v = blockIdx.x * VT + threadIdx.x;
-    if (v < classes_pad) out[v] = v >= classes ? -__builtin_inff() : bias ? Elem<T>::to_float(bias[v]) * scale : 0.0f;
+// SCAN: rows per thread that a workgroup lists for itself; 0: they are listed already
+template <typename T, int SCAN>
+__global__ __launch_bounds__(VT) void prepare_kernel(PrepareArgs p) {
+    constexpr int E = 16 / sizeof(T);
+    const unsigned chunks = p.dim_pad / E;
+    unsigned block = blockIdx.x;
+    if (block < p.feature_blocks) {
+        __shared__ int s_row_of[SCAN ? SCAN * VT : 1];
+        __shared__ int s_sum[VT / 64];
+        int count = 0;
+        if (SCAN) {
+            bool on[SCAN ? SCAN : 1];
+            int mine = 0;
+#pragma unroll
+            for (int i = 0; i < SCAN; ++i) {
+                const int r = threadIdx.x * SCAN + i;
+                on[i] = r < p.rows && (p.flags ? p.flags[r] != 0 : p.targets[r] >= 0);
+                mine += on[i] ? 1 : 0;
+            }
+            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+            int upto = (int)wave_scan_incl((uint32_t)mine);
+            if (lane == 63) s_sum[wave] = upto;
+            __syncthreads();
+            int before = 0;
+            for (int w = 0; w < VT / 64; ++w) {
+                if (w < wave) before += s_sum[w];
+                count += s_sum[w];
+            }
+            int at = before + upto - mine;
+#pragma unroll
+            for (int i = 0; i < SCAN; ++i) {
+                const int r = threadIdx.x * SCAN + i;
+                if (block == 0 && r < p.rows) {
+                    p.lists.place[r] = on[i] ? at : -1;
+                    p.row_loss[r] = 0.0f;
+                }
+                if (on[i]) {
+                    s_row_of[at] = r;
+                    if (block == 0) p.lists.row_of[at] = r;
+                    ++at;
+                }
+            }
+            if (block == 0 && threadIdx.x == 0) *p.lists.count = count;
+            __syncthreads();
+        } else {
+            count = *p.lists.count;
+        }
+        const unsigned at = block * VT + threadIdx.x;
+        const long long r = at / chunks;
+        if (r >= p.rows_pad || r >= up_to(count, ROW_TILE)) return;     // no tile reads behind the last one's end
+        const int c = (int)(at % chunks) * E;
+        const T* row = r < count ? (const T*)p.features + (long long)(SCAN ? s_row_of[r] : p.lists.row_of[r]) * p.feature_pitch
+                                 : nullptr;
+        pack_chunk<T>(row, c, p.dim, (T*)p.packed + r * p.dim_pad + c);
+        return;
+    }
+    block -= p.feature_blocks;
+    if (block < p.weight_blocks) {
+        const unsigned at = block * VT + threadIdx.x;
+        const long long r = at / chunks;
+        if (r >= p.classes) return;
+        const int c = (int)(at % chunks) * E;
+        pack_chunk<T>((const T*)p.weight + r * p.weight_pitch, c, p.dim, (T*)p.packed_weight + r * p.dim_pad + c);
+        return;
+    }
+    block -= p.weight_blocks;
+    const int v = (int)block * VT + threadIdx.x;
+    if (v < p.bias_len)
+        p.bias2[v] = v >= p.classes ? -__builtin_inff() : p.bias ? Elem<T>::to_float(((const T*)p.bias)[v]) * p.scale : 0.0f;
+    if (p.scales && v == 0) {
+        p.scales->common = p.upstream[0] * (p.temperature / (p.reduction == OD_REDUCE_MEAN ? (float)max(1, *p.lists.count) : 1.0f));
+        p.scales->features_max = 0;
+        p.scales->weight_max = 0;
+    }
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------
@@ -735,9 +828,9 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
 // ---- forward's end -----------------------------------------------------------------------------------------------------
 struct TargetArgs {
     const char* features;               // packed
-    int dim, dim_pad;
-    const void* weight;                 // the caller's rows
-    long long weight_pitch;             // elements
+    int dim_pad;
+    const char* weight;                 // rows as the product reads them
+    long long weight_pitch;             // bytes
     const void* bias;
     long long classes;
     const long long* targets;           // [rows] or [rows, top]
@@ -788,8 +881,16 @@ __global__ __launch_bounds__(VT) void targets_kernel(TargetArgs p) {
         float z = 0.0f;
         if (c >= p.classes) outside = true;
         if (c >= 0 && c < p.classes) {
-            const T* w = (const T*)p.weight + c * p.weight_pitch;
-            for (int d = lane & 15; d < p.dim; d += 16) z = fmaf(Elem<T>::to_float(f[d]), Elem<T>::to_float(w[d]), z);
+            const T* w = (const T*)(p.weight + c * p.weight_pitch);
+            constexpr int E = 16 / sizeof(T);
+#pragma unroll 2
+            for (int d = (lane & 15) * E; d < p.dim_pad; d += 16 * E) {
+                float x[E], y[E];
+                load_vec<T, E>(f + d, x);
+                load_vec<T, E>(w + d, y);
+#pragma unroll
+                for (int i = 0; i < E; ++i) z = fmaf(x[i], y[i], z);
+            }
         }
         for (int o = 8; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
         if (c >= 0 && c < p.classes) {
@@ -828,12 +929,6 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
 }
 
 // ---- backward ------------------------------------------------------------------------------------------------------
-// Scalars of a backward call, on the device.
-struct Scales {
-    float common;                       // largest |upstream| times share and temperature
-    uint32_t features_max, weight_max;  // bits of the largest finite |weighted feature| and |weight|
-};
-
 // Power of two under which an operand with this largest size lies in [2^13, 2^14): what is 2^27 times smaller is still a
 // normal fp16 number, what is 2^37 times smaller vanishes.
 __device__ __forceinline__ int exponent_of(uint32_t max_bits) {
@@ -843,95 +938,110 @@ __device__ __forceinline__ int exponent_of(uint32_t max_bits) {
     return min(max(14 - e, -100), 100);
 }
 
-// weight[place] = upstream of the row / the largest |upstream| (1 where one gradient serves all rows), zero behind the
-// last valid row; clears the maxima.
-__global__ __launch_bounds__(1024) void row_weights_kernel(const float* __restrict__ upstream, int reduction, RowLists lists,
+// A gradient per row: weight[place] = upstream of the row / the largest |upstream|, zero behind the last valid row; and the
+// scalars.
+__global__ __launch_bounds__(1024) void row_weights_kernel(const float* __restrict__ upstream, RowLists lists,
                                                            long long rows_pad, float temperature, float* __restrict__ weight,
                                                            Scales* __restrict__ scales) {
     __shared__ float red[1024];
     const int count = *lists.count;
-    float top = 1.0f;
-    if (reduction == OD_REDUCE_NONE) {
-        top = 0.0f;
-        for (int i = threadIdx.x; i < count; i += 1024) {
-            const float g = fabsf(upstream[lists.row_of[i]]);
-            if (g < __builtin_inff()) top = fmaxf(top, g);         // infinities and NaN go through as they are
-        }
-        red[threadIdx.x] = top;
-        __syncthreads();
-        for (int o = 512; o > 0; o >>= 1) {
-            if ((int)threadIdx.x < o) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + o]);
-            __syncthreads();
-        }
-        top = red[0] > 0.0f ? red[0] : 1.0f;
+    float top = 0.0f;
+    for (int i = threadIdx.x; i < count; i += 1024) {
+        const float g = fabsf(upstream[lists.row_of[i]]);
+        if (g < __builtin_inff()) top = fmaxf(top, g);             // infinities and NaN go through as they are
     }
+    red[threadIdx.x] = top;
+    __syncthreads();
+    for (int o = 512; o > 0; o >>= 1) {
+        if ((int)threadIdx.x < o) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + o]);
+        __syncthreads();
+    }
+    top = red[0] > 0.0f ? red[0] : 1.0f;
     for (long long i = threadIdx.x; i < rows_pad; i += 1024)
-        weight[i] = i >= count ? 0.0f : reduction == OD_REDUCE_NONE ? upstream[lists.row_of[i]] / top : 1.0f;
+        weight[i] = i < count ? upstream[lists.row_of[i]] / top : 0.0f;
     if (threadIdx.x == 0) {
-        const float share = temperature / (reduction == OD_REDUCE_MEAN ? (float)max(1, count) : 1.0f);
-        scales->common = (reduction == OD_REDUCE_NONE ? top : upstream[0]) * share;
+        scales->common = top * temperature;
         scales->features_max = 0;
         scales->weight_max = 0;
     }
 }
 
-// Largest finite |x| of rows [0, rows) (or the valid ones), each times its weight.  The maximum of integers does not
-// depend on the order of the atomics.
+// An operand of the gradient products: rows of features (those valid, each times its weight) or of weight.
+struct Operand {
+    const void* x;
+    long long pitch, rows;              // elements
+    const float* weight;                // of the rows, or null: ones
+    const int* count;                   // valid rows, or null: all
+    uint32_t* max_bits;                 // null: no power of two
+    void* out;                          // [rows][dim_pad]; null: not wanted
+    unsigned blocks;
+};
+struct Operands {
+    Operand part[2];
+    int dim_pad;
+};
+
+// Largest finite |x| of an operand.  The maximum of integers does not depend on the order of the atomics.
 template <typename T>
-__global__ __launch_bounds__(VT) void max_kernel(const T* __restrict__ x, long long pitch, int dim_pad,
-                                                 const float* __restrict__ weight, const int* __restrict__ count,
-                                                 long long rows, uint32_t* __restrict__ out) {
+__global__ __launch_bounds__(VT) void max_kernel(Operands ops) {
     constexpr int E = 16 / sizeof(T);
-    const int chunks = dim_pad / E;
-    const long long total = (count ? (long long)*count : rows) * chunks;
+    const bool second = blockIdx.x >= ops.part[0].blocks;
+    const Operand& o = ops.part[second ? 1 : 0];
+    const unsigned block = blockIdx.x - (second ? ops.part[0].blocks : 0);
+    const unsigned chunks = ops.dim_pad / E;
+    const unsigned total = (unsigned)(o.count ? *o.count : (int)o.rows) * chunks;
+    constexpr int AHEAD = 4;                                        // loads in flight; behind the end the last chunk again
     float top = 0.0f;
-    for (long long at = (long long)blockIdx.x * VT + threadIdx.x; at < total; at += (long long)gridDim.x * VT) {
-        const long long r = at / chunks;
-        float v[E];
-        load_vec<T, E>(x + r * pitch + (at % chunks) * E, v);
-        const float w = weight ? weight[r] : 1.0f;
+    for (unsigned at = block * VT + threadIdx.x; at < total; at += AHEAD * o.blocks * VT) {
+        float v[AHEAD][E], w[AHEAD];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float a = fabsf(v[i] * w);
-            if (a < __builtin_inff()) top = fmaxf(top, a);
+        for (int k = 0; k < AHEAD; ++k) {
+            const unsigned i = min(at + k * o.blocks * VT, total - 1), r = i / chunks;
+            load_vec<T, E>((const T*)o.x + r * o.pitch + (i - r * chunks) * E, v[k]);
+            w[k] = o.weight ? o.weight[r] : 1.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const float a = fabsf(v[k][i] * w[k]);
+                if (a < __builtin_inff()) top = fmaxf(top, a);
+            }
         }
     }
     __shared__ float red[VT / 64];
     top = wave_max(top);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) {                                         // the atomics of a launch queue up: one per workgroup
+    if (threadIdx.x == 0) {                                         // atomics on one address queue up: few workgroups
         for (int w = 1; w < VT / 64; ++w) top = fmaxf(top, red[w]);
-        if (top > 0.0f) atomicMax(out, f2u(top));
+        if (top > 0.0f) atomicMax(o.max_bits, f2u(top));
     }
 }
 
 // Rows in the gradient products' type: x times the row's weight times the operand's power of two; zero rows behind the
 // last valid one up to a whole tile.
-template <typename T, typename G>
-__global__ __launch_bounds__(VT) void scale_rows_kernel(const T* __restrict__ x, long long pitch, int dim_pad,
-                                                        const float* __restrict__ weight, const int* __restrict__ count,
-                                                        long long rows, const uint32_t* __restrict__ max_bits,
-                                                        G* __restrict__ dst) {
+template <typename T>
+__global__ __launch_bounds__(VT) void scale_kernel(Operands ops) {
+    typedef typename GradOf<T>::type G;
+    static_assert(sizeof(G) == sizeof(T), "operands change their type, not their size");
     constexpr int E = 16 / sizeof(T);
-    const int chunks = dim_pad / E;
-    const long long at = (long long)blockIdx.x * VT + threadIdx.x;
+    const bool second = blockIdx.x >= ops.part[0].blocks;
+    const Operand& o = ops.part[second ? 1 : 0];
+    const unsigned chunks = ops.dim_pad / E;
+    const unsigned at = (blockIdx.x - (second ? ops.part[0].blocks : 0)) * VT + threadIdx.x;
     const long long r = at / chunks;
-    if (r >= rows) return;
-    if (count && r >= up_to((long long)*count, ROW_TILE)) return;
+    if (r >= o.rows) return;
+    if (o.count && r >= up_to((long long)*o.count, ROW_TILE)) return;
     const int c = (int)(at % chunks) * E;
     float v[E];
-    load_vec<T, E>(x + r * pitch + c, v);
-    const float f = max_bits ? ldexpf(1.0f, exponent_of(*max_bits)) : 1.0f;
-    const float w = weight ? weight[r] : 1.0f;
-    const bool on = !count || r < *count;
+    load_vec<T, E>((const T*)o.x + r * o.pitch + c, v);
+    const float f = o.max_bits ? ldexpf(1.0f, exponent_of(*o.max_bits)) : 1.0f;
+    const float w = o.weight ? o.weight[r] : 1.0f;
+    const bool on = !o.count || r < *o.count;
 #pragma unroll
     for (int i = 0; i < E; ++i) v[i] = on ? v[i] * f * w : 0.0f;
-    if constexpr (sizeof(G) == sizeof(T)) {
-        store_vec<G, E>(dst + r * dim_pad + c, v);
-    } else {
-        static_assert(sizeof(G) == sizeof(T), "operands change their type, not their size");
-    }
+    store_vec<G, E>((G*)o.out + r * ops.dim_pad + c, v);
 }
 
 // The target entries of a piece of dz: q - p.  Next to p = 1 it is expm1(log q) + (1 - p), which keeps the digits of
@@ -1159,27 +1269,36 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
 
 // What the sums of the products still lack: 2^-LOG2_DZ, the other operand's power of two, the common factor, and (dF) the
 // row's weight.  The powers of two are applied apart, so that no intermediate factor leaves the range.
-// out[row][0 .. dim) = the splits' sum over line place[row] (or row itself); zero where place < 0
+struct FinishArgs {
+    const Scales* scales;
+    int dim, dim_pad;
+    // classes of a piece: out[class][0 .. dim) and bias[class], the splits' sums over the piece's columns
+    const float *part_w, *part_b;
+    long long piece, classes;
+    int splits_w, scaled_f;
+    void *dweight, *dbias;
+    unsigned weight_blocks, bias_blocks;
+    // rows, behind the last piece: out[row][0 .. dim) of line place[row], zero where there is none
+    const float* part_f;
+    long long rows_pad, rows;
+    int splits_f, scaled_w;
+    const int* place;
+    const float* row_weight;
+    void* dfeatures;
+};
+
+// four elements of a result line
 template <typename T>
-__global__ __launch_bounds__(VT) void finish_kernel(const float* __restrict__ part, long long cols, int splits, int dim,
-                                                    int dim_pad, const int* __restrict__ place,
-                                                    const float* __restrict__ weight, const Scales* __restrict__ scales,
-                                                    int rows_of_dz, int scaled, long long rows, T* __restrict__ out) {
-    const int groups = (dim + 3) / 4;
-    const long long at = (long long)blockIdx.x * VT + threadIdx.x;
-    const long long row = at / groups;
-    if (row >= rows) return;
-    const int d = (int)(at % groups) * 4;
-    const long long line = place ? place[row] : row;
+__device__ __forceinline__ void finish_line(const float* part, long long step, int splits, int exponent, float factor, int dim,
+                                            int d, T* out, T* line) {
     vec4f v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (line >= 0) {
-        for (int s = 0; s < splits; ++s)
-            v += *reinterpret_cast<const vec4f*>(part + ((long long)s * cols + line) * dim_pad + d);
-        const int e = scaled ? exponent_of(rows_of_dz ? scales->weight_max : scales->features_max) : 0;
-        v *= ldexpf(1.0f, -e - GradOf<T>::LOG2_DZ);
-        v *= scales->common * (weight ? weight[line] : 1.0f);
+    if (part) {
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const vec4f*>(part + s * step + d);
+        v *= ldexpf(1.0f, -exponent - GradOf<T>::LOG2_DZ);
+        v *= factor;
     }
-    T* to = out + row * dim + d;
+    T* to = line + d;
     if (dim % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0) {
         const float f[4] = {v.x, v.y, v.z, v.w};
         store_vec<T, 4>(to, f);
@@ -1191,14 +1310,36 @@ __global__ __launch_bounds__(VT) void finish_kernel(const float* __restrict__ pa
 }
 
 template <typename T>
-__global__ __launch_bounds__(VT) void finish_bias_kernel(const float* __restrict__ part, long long cols, int splits,
-                                                         const Scales* __restrict__ scales, long long classes,
-                                                         T* __restrict__ out) {
-    const long long v = (long long)blockIdx.x * VT + threadIdx.x;
-    if (v >= classes) return;
-    float sum = 0.0f;
-    for (int s = 0; s < splits; ++s) sum += part[(long long)s * cols + v];
-    out[v] = Elem<T>::from_float(sum * ldexpf(1.0f, -GradOf<T>::LOG2_DZ) * scales->common);
+__global__ __launch_bounds__(VT) void finish_kernel(FinishArgs p) {
+    const unsigned groups = (p.dim + 3) / 4;
+    unsigned block = blockIdx.x;
+    if (block < p.weight_blocks) {
+        const unsigned at = block * VT + threadIdx.x;
+        const long long c = at / groups;
+        if (c >= p.classes) return;
+        finish_line<T>(p.part_w + c * p.dim_pad, p.piece * p.dim_pad, p.splits_w,
+                       p.scaled_f ? exponent_of(p.scales->features_max) : 0, p.scales->common, p.dim, (int)(at % groups) * 4,
+                       (T*)p.dweight, (T*)p.dweight + c * p.dim);
+        return;
+    }
+    block -= p.weight_blocks;
+    if (block < p.bias_blocks) {
+        const long long c = (long long)block * VT + threadIdx.x;
+        if (c >= p.classes) return;
+        float sum = 0.0f;
+        for (int s = 0; s < p.splits_w; ++s) sum += p.part_b[s * p.piece + c];
+        ((T*)p.dbias)[c] = Elem<T>::from_float(sum * ldexpf(1.0f, -GradOf<T>::LOG2_DZ) * p.scales->common);
+        return;
+    }
+    block -= p.bias_blocks;
+    const unsigned at = block * VT + threadIdx.x;
+    const long long row = at / groups;
+    if (row >= p.rows) return;
+    const int line = p.place[row];
+    finish_line<T>(line < 0 ? nullptr : p.part_f + (long long)line * p.dim_pad, p.rows_pad * p.dim_pad, p.splits_f,
+                   p.scaled_w ? exponent_of(p.scales->weight_max) : 0,
+                   p.scales->common * (p.row_weight && line >= 0 ? p.row_weight[line] : 1.0f), p.dim, (int)(at % groups) * 4,
+                   (T*)p.dfeatures, (T*)p.dfeatures + row * p.dim);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
@@ -1266,8 +1407,8 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.slabs = bytes <= 1024 ? (int)(bytes / 32) : 0;
     p.row_tile = p.slabs > 0 && p.slabs <= 16 ? 256 : 128;
     p.class_tile = p.slabs == 0 ? TILE : p.slabs <= 16 ? 64 : 32;
-    // one thread per 16 bytes of the packed operands, fewer than 2^32 threads in a launch
-    if (most(p.rows_pad, p.classes_pad) * p.dim_pad * p.size / 16 > (1ll << 31)) return false;
+    // one thread per 16 bytes of both packed operands, fewer than 2^32 threads in a launch
+    if (most(p.rows_pad, p.classes_pad) * p.dim_pad * p.size / 16 > (1ll << 30)) return false;
     p.n = top > 0 ? top : 1;
     p.row_tiles = (int)((most(rows, 1) + p.row_tile - 1) / p.row_tile);
     p.splits = splits_for(p.row_tiles, p.classes_pad / p.class_tile, SLOTS, 2, SLOTS);
@@ -1352,22 +1493,62 @@ struct Call {
     hipStream_t stream;
 };
 
-// weight rows as the product reads them: in place, or packed into the scratch
+RowLists lists_of(const Call& c) {
+    return {(int*)(c.saved + c.p.o_count), (int*)(c.saved + c.p.o_row_of), (int*)(c.saved + c.p.o_place)};
+}
+
+// Packs what has to be packed and says where the product finds its weight rows.  `with_features`: forward.
 template <typename T>
-int weight_rows(const Call& c, size_t scratch, const char** rows, long long* pitch) {
+int prepare(const Call& c, bool with_features, const unsigned char* flags, size_t weight_at, size_t bias_at, long long bias_len,
+            Scales* scales, const char** rows, long long* pitch) {
     const Plan& p = c.p;
-    if (weight_in_place(p, c.weight, c.weight_pitch)) {
-        *rows = (const char*)c.weight;
-        *pitch = c.weight_pitch * p.size;
-        return OD_OK;
+    PrepareArgs a = {};
+    const long long row_chunks = p.dim_pad * p.size / 16;
+    a.lists = lists_of(c);
+    a.dim = p.dim;
+    a.dim_pad = p.dim_pad;
+    int scan = 0;
+    if (with_features) {
+        a.features = c.features;
+        a.feature_pitch = c.feature_pitch;
+        a.packed = c.saved + p.o_packed;
+        a.rows_pad = p.rows_pad;
+        a.feature_blocks = blocks_of(p.rows_pad * row_chunks, VT);
+        a.targets = c.targets;
+        a.flags = flags;
+        a.rows = (int)p.rows;
+        a.row_loss = c.row_loss;
+        scan = p.rows <= 4 * VT ? 4 : p.rows <= 16 * VT ? 16 : 0;
+        if (scan == 0) {
+            hipLaunchKernelGGL(list_rows_kernel, dim3(1), dim3(1024), 0, c.stream, c.targets, flags, (int)p.rows, a.lists,
+                               c.row_loss);
+            OD_LAUNCH_CHECK();
+        }
     }
-    const long long chunks = p.classes * (p.dim_pad * p.size / 16);
-    hipLaunchKernelGGL(pack_rows_kernel<T>, dim3(blocks_of(chunks, VT)), dim3(VT), 0, c.stream, (const T*)c.weight,
-                       c.weight_pitch, p.dim, p.dim_pad, (const int*)nullptr, (const int*)nullptr, p.classes,
-                       (T*)(c.ws + scratch));
+    *rows = (const char*)c.weight;
+    *pitch = c.weight_pitch * p.size;
+    if (!weight_in_place(p, c.weight, c.weight_pitch)) {
+        a.weight = c.weight;
+        a.weight_pitch = c.weight_pitch;
+        a.packed_weight = c.ws + weight_at;
+        a.weight_blocks = blocks_of(p.classes * row_chunks, VT);
+        *rows = c.ws + weight_at;
+        *pitch = (long long)p.dim_pad * p.size;
+    }
+    a.classes = p.classes;
+    a.bias = c.bias;
+    a.bias_len = (int)bias_len;
+    a.scale = LOG2E / c.temperature;
+    a.bias2 = (float*)(c.ws + bias_at);
+    a.scales = scales;
+    a.upstream = c.upstream;
+    a.reduction = c.reduction;
+    a.temperature = c.temperature;
+    const dim3 grid(a.feature_blocks + a.weight_blocks + blocks_of(bias_len, VT));
+    if (scan == 4) hipLaunchKernelGGL((prepare_kernel<T, 4>), grid, dim3(VT), 0, c.stream, a);
+    else if (scan == 16) hipLaunchKernelGGL((prepare_kernel<T, 16>), grid, dim3(VT), 0, c.stream, a);
+    else hipLaunchKernelGGL((prepare_kernel<T, 0>), grid, dim3(VT), 0, c.stream, a);
     OD_LAUNCH_CHECK();
-    *rows = c.ws + scratch;
-    *pitch = (long long)p.dim_pad * p.size;
     return OD_OK;
 }
 
@@ -1401,10 +1582,6 @@ int launch_grad(const Call& c, int kernel, const GradArgs& g) {
     return OD_OK;
 }
 
-RowLists lists_of(const Call& c) {
-    return {(int*)(c.saved + c.p.o_count), (int*)(c.saved + c.p.o_row_of), (int*)(c.saved + c.p.o_place)};
-}
-
 template <typename T>
 int forward_typed(const Call& c) {
     const Plan& p = c.p;
@@ -1427,20 +1604,8 @@ int forward_typed(const Call& c) {
                                (const bf16_t*)c.teacher_logits, (int)p.rows, c.top, inv, prob, entropy, flags);
         OD_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL(list_rows_kernel, dim3(1), dim3(1024), 0, c.stream, c.targets, (const unsigned char*)flags, (int)p.rows,
-                       lists, c.row_loss);
-    OD_LAUNCH_CHECK();
-    const long long chunks = p.rows_pad * (p.dim_pad * p.size / 16);
-    hipLaunchKernelGGL(pack_rows_kernel<T>, dim3(blocks_of(chunks, VT)), dim3(VT), 0, c.stream, (const T*)c.features,
-                       c.feature_pitch, p.dim, p.dim_pad, (const int*)lists.row_of, (const int*)lists.count, p.rows_pad,
-                       (T*)(c.saved + p.o_packed));
-    OD_LAUNCH_CHECK();
-    const float scale = LOG2E / c.temperature;
-    hipLaunchKernelGGL(bias_kernel<T>, dim3(blocks_of(p.classes_pad, VT)), dim3(VT), 0, c.stream, (const T*)c.bias,
-                       (int)p.classes, (int)p.classes_pad, scale, (float*)(c.ws + p.f_bias));
-    OD_LAUNCH_CHECK();
     ProductArgs a = {};
-    int rc = weight_rows<T>(c, p.f_weight, &a.weight, &a.weight_pitch);
+    int rc = prepare<T>(c, true, flags, p.f_weight, p.f_bias, p.classes_pad, nullptr, &a.weight, &a.weight_pitch);
     if (rc != OD_OK) return rc;
     a.features = c.saved + p.o_packed;
     a.dim_pad = p.dim_pad;
@@ -1451,17 +1616,16 @@ int forward_typed(const Call& c) {
     a.tiles = (int)(p.classes_pad / p.class_tile);
     a.splits = p.splits;
     a.row_tiles = p.row_tiles;
-    a.scale = scale;
+    a.scale = LOG2E / c.temperature;
     a.rows_pad = p.rows_pad;
     a.part = (float2*)(c.ws + p.f_part);
     rc = launch_product<T, false>(c, OD_KERNEL_VOCAB_LSE, a);
     if (rc != OD_OK) return rc;
     TargetArgs t = {};
     t.features = a.features;
-    t.dim = p.dim;
     t.dim_pad = p.dim_pad;
-    t.weight = c.weight;
-    t.weight_pitch = c.weight_pitch;
+    t.weight = a.weight;
+    t.weight_pitch = a.weight_pitch;
     t.bias = c.bias;
     t.classes = p.classes;
     t.targets = c.targets;
@@ -1495,16 +1659,15 @@ int backward_typed(const Call& c) {
     const bool weighted = c.reduction == OD_REDUCE_NONE;
     float* row_weight = (float*)(c.ws + p.b_row_weight);
     Scales* scales = (Scales*)(c.ws + p.b_scales);
-    hipLaunchKernelGGL(row_weights_kernel, dim3(1), dim3(1024), 0, c.stream, c.upstream, c.reduction, lists, p.rows_pad,
-                       c.temperature, row_weight, scales);
-    OD_LAUNCH_CHECK();
-    const float log2_scale = LOG2E / c.temperature;
-    const long long bias_len = p.classes_pad + p.piece;             // the last piece may reach past the last tile
-    hipLaunchKernelGGL(bias_kernel<T>, dim3(blocks_of(bias_len, VT)), dim3(VT), 0, c.stream, (const T*)c.bias,
-                       (int)p.classes, (int)bias_len, log2_scale, (float*)(c.ws + p.b_bias));
-    OD_LAUNCH_CHECK();
+    if (weighted) {
+        hipLaunchKernelGGL(row_weights_kernel, dim3(1), dim3(1024), 0, c.stream, c.upstream, lists, p.rows_pad, c.temperature,
+                           row_weight, scales);
+        OD_LAUNCH_CHECK();
+    }
     ProductArgs a = {};
-    int rc = weight_rows<T>(c, p.b_weight, &a.weight, &a.weight_pitch);
+    // the bias table: the last piece may reach past the last tile
+    int rc = prepare<T>(c, false, nullptr, p.b_weight, p.b_bias, p.classes_pad + p.piece, weighted ? nullptr : scales, &a.weight,
+                        &a.weight_pitch);
     if (rc != OD_OK) return rc;
     a.features = c.saved + p.o_packed;
 
@@ -1512,33 +1675,31 @@ int backward_typed(const Call& c) {
     const char *grad_features = a.features, *grad_weight = a.weight;
     long long grad_weight_pitch = a.weight_pitch;
     const bool scale_f = !WIDE && (BF16 || weighted), scale_w = BF16;
-    if (scale_f || weighted) {
-        const float* rw = weighted ? row_weight : nullptr;
-        uint32_t* max_bits = scale_f ? &scales->features_max : nullptr;
-        if (scale_f) {
-            const long long work = blocks_of(p.rows_pad * (p.dim_pad * p.size / 16), VT);
-            hipLaunchKernelGGL(max_kernel<T>, dim3((unsigned)least(work, 512)), dim3(VT), 0, c.stream, (const T*)a.features,
-                               (long long)p.dim_pad, p.dim_pad, rw, (const int*)lists.count, p.rows, max_bits);
-            OD_LAUNCH_CHECK();
-        }
-        hipLaunchKernelGGL((scale_rows_kernel<T, G>), dim3(blocks_of(p.rows_pad * (p.dim_pad * p.size / 16), VT)), dim3(VT), 0,
-                           c.stream, (const T*)a.features, (long long)p.dim_pad, p.dim_pad, rw, (const int*)lists.count,
-                           p.rows_pad, (const uint32_t*)max_bits, (G*)(c.ws + p.b_scaled_f));
-        OD_LAUNCH_CHECK();
+    const long long row_chunks = p.dim_pad * p.size / 16;
+    Operands ops = {};
+    ops.dim_pad = p.dim_pad;
+    if ((scale_f || weighted) && (c.dweight || c.dbias)) {
+        ops.part[0] = {a.features, p.dim_pad, p.rows_pad, weighted ? row_weight : nullptr, lists.count,
+                       scale_f ? &scales->features_max : nullptr, c.ws + p.b_scaled_f, 0};
         grad_features = c.ws + p.b_scaled_f;
     }
     if (scale_w && c.dfeatures) {
-        const long long chunks = p.classes * (p.dim_pad * p.size / 16);
-        hipLaunchKernelGGL(max_kernel<T>, dim3((unsigned)least(blocks_of(chunks, VT), 512)), dim3(VT), 0, c.stream,
-                           (const T*)a.weight, a.weight_pitch / p.size, p.dim_pad, (const float*)nullptr, (const int*)nullptr,
-                           p.classes, &scales->weight_max);
-        OD_LAUNCH_CHECK();
-        hipLaunchKernelGGL((scale_rows_kernel<T, G>), dim3(blocks_of(chunks, VT)), dim3(VT), 0, c.stream, (const T*)a.weight,
-                           a.weight_pitch / p.size, p.dim_pad, (const float*)nullptr, (const int*)nullptr, p.classes,
-                           (const uint32_t*)&scales->weight_max, (G*)(c.ws + p.b_scaled_w));
-        OD_LAUNCH_CHECK();
+        ops.part[1] = {a.weight, a.weight_pitch / p.size, p.classes, nullptr, nullptr, &scales->weight_max, c.ws + p.b_scaled_w,
+                       0};
         grad_weight = c.ws + p.b_scaled_w;
         grad_weight_pitch = (long long)p.dim_pad * p.size;
+    }
+    unsigned blocks = 0;
+    for (Operand& o : ops.part) blocks += o.blocks = o.max_bits ? (unsigned)least(blocks_of(o.rows * row_chunks, VT), 256) : 0;
+    if (blocks > 0) {
+        hipLaunchKernelGGL(max_kernel<T>, dim3(blocks), dim3(VT), 0, c.stream, ops);
+        OD_LAUNCH_CHECK();
+    }
+    blocks = 0;
+    for (Operand& o : ops.part) blocks += o.blocks = o.out ? blocks_of(o.rows * row_chunks, VT) : 0;
+    if (blocks > 0) {
+        hipLaunchKernelGGL(scale_kernel<T>, dim3(blocks), dim3(VT), 0, c.stream, ops);
+        OD_LAUNCH_CHECK();
     }
 
     a.dim_pad = p.dim_pad;
@@ -1547,7 +1708,7 @@ int backward_typed(const Call& c) {
     a.tiles = (int)(p.piece / p.class_tile);
     a.row_tiles = p.row_tiles;
     a.splits = p.splits_z;
-    a.scale = log2_scale;
+    a.scale = LOG2E / c.temperature;
     a.rows_pad = p.rows_pad;
     a.lse2 = (const float*)(c.saved + p.o_lse);
     a.dz = c.ws + p.b_dz;
@@ -1593,28 +1754,42 @@ int backward_typed(const Call& c) {
             g.row_weight = weighted ? row_weight : nullptr;
             rc = launch_grad<G, false>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g);
             if (rc != OD_OK) return rc;
-            const long long here = least(p.piece, p.classes - first);
-            if (c.dweight) {
-                hipLaunchKernelGGL(finish_kernel<T>, dim3(blocks_of(here * ((p.dim + 3) / 4), VT)), dim3(VT), 0, c.stream,
-                                   (const float*)g.out, p.piece, p.splits_w, p.dim, p.dim_pad, (const int*)nullptr,
-                                   (const float*)nullptr, (const Scales*)scales, 0, (int)scale_f, here,
-                                   (T*)c.dweight + first * p.dim);
-                OD_LAUNCH_CHECK();
-            }
-            if (c.dbias) {
-                hipLaunchKernelGGL(finish_bias_kernel<T>, dim3(blocks_of(here, VT)), dim3(VT), 0, c.stream,
-                                   (const float*)g.bias_out, p.piece, p.splits_w, (const Scales*)scales, here,
-                                   (T*)c.dbias + first);
-                OD_LAUNCH_CHECK();
-            }
         }
-    }
-    if (c.dfeatures) {
-        hipLaunchKernelGGL(finish_kernel<T>, dim3(blocks_of(p.rows * ((p.dim + 3) / 4), VT)), dim3(VT), 0, c.stream,
-                           (const float*)(c.ws + p.b_part_f), p.rows_pad, p.splits_f, p.dim, p.dim_pad,
-                           (const int*)lists.place, weighted ? (const float*)row_weight : nullptr, (const Scales*)scales, 1,
-                           (int)scale_w, p.rows, (T*)c.dfeatures);
-        OD_LAUNCH_CHECK();
+        FinishArgs f = {};
+        f.scales = scales;
+        f.dim = p.dim;
+        f.dim_pad = p.dim_pad;
+        f.piece = p.piece;
+        f.classes = least(p.piece, p.classes - first);
+        const int groups = (p.dim + 3) / 4;
+        unsigned finish_blocks = 0;
+        if (c.dweight) {
+            f.part_w = (const float*)(c.ws + p.b_part_w);
+            f.dweight = (T*)c.dweight + first * p.dim;
+            finish_blocks += f.weight_blocks = blocks_of(f.classes * groups, VT);
+        }
+        if (c.dbias) {
+            f.part_b = (const float*)(c.ws + p.b_part_b);
+            f.dbias = (T*)c.dbias + first;
+            finish_blocks += f.bias_blocks = blocks_of(f.classes, VT);
+        }
+        f.splits_w = p.splits_w;
+        f.scaled_f = scale_f;
+        if (c.dfeatures && k == p.pieces - 1) {
+            f.part_f = (const float*)(c.ws + p.b_part_f);
+            f.rows_pad = p.rows_pad;
+            f.rows = p.rows;
+            f.splits_f = p.splits_f;
+            f.scaled_w = scale_w;
+            f.place = lists.place;
+            f.row_weight = weighted ? row_weight : nullptr;
+            f.dfeatures = c.dfeatures;
+            finish_blocks += blocks_of(f.rows * groups, VT);
+        }
+        if (finish_blocks > 0) {
+            hipLaunchKernelGGL(finish_kernel<T>, dim3(finish_blocks), dim3(VT), 0, c.stream, f);
+            OD_LAUNCH_CHECK();
+        }
     }
     return OD_OK;
 }
