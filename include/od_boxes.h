@@ -435,8 +435,9 @@ int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int
  *   upstream     : fp32 gradient of row_loss [rows] (OD_REDUCE_NONE) or of loss [1]
  *   dfeatures    : [rows, dim] dense, dweight [classes, dim] dense, dbias [classes], all of dtype; any may be null
  *   workspace    : od_vocab_loss_workspace_bytes(..., backward = 0 or 1), 256-byte aligned
- * Sums are fp32 in a fixed order; 16-bit gradients are rounded once at the end, and the logits' gradients, an operand of
- * the products, once before (fp16: under a power of two that keeps small ones normal).
+ * Sums are fp32 in a fixed order.  16-bit gradients are rounded once at the end, and the logits' gradients, an operand of
+ * the products, once before, to fp16 under a power of two.  bf16 features and weights enter those products as fp16 under one
+ * power of two for all of them: what is 2^27 times smaller than the largest loses bits, 2^38 times smaller it counts as zero.
  */
 #define OD_REDUCE_NONE 0
 #define OD_REDUCE_MEAN 1

@@ -6,9 +6,11 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/od_boxes.h"
@@ -55,6 +57,23 @@ variable_list once(variable_list grads) {
         out[i] = (*stop)({part})[0];
     }
     return out;
+}
+
+// A step recorded into a graph must not share leaves with an earlier step whose results still live: its backward pass would
+// have to wait for the stream on which the leaves' accumulators came to be, which a recording cannot, and the process would
+// end there.  Such a call is refused before it records anything.
+void check_recording(const Tensor& on, std::initializer_list<const Tensor*> inputs) {
+    if (!at::GradMode::is_enabled() || !on.is_cuda()) return;
+    const c10::Stream stream = c10::impl::VirtualGuardImpl(on.device().type()).getStream(on.device());
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing((hipStream_t)stream_of(on), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    for (const Tensor* t : inputs) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (accumulator && accumulator->stream() && *accumulator->stream() != stream)
+            TORCH_CHECK(false, "a training step cannot be recorded while results of an earlier one with the same parameters, on "
+                               "another stream, are alive: drop them first");
+    }
 }
 
 // ---- group norm with an activation -----------------------------------------------------------------------------
@@ -191,12 +210,18 @@ struct VocabLoss : torch::autograd::Function<VocabLoss> {
 PYBIND11_MODULE(_od_torch, m) {
     m.def("group_norm_act",
           [](const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps, int64_t activation,
-             int64_t workspace) { return GroupNormAct::apply(x, weight, bias, groups, eps, activation, workspace); },
+             int64_t workspace) {
+              const Tensor none;
+              check_recording(x, {&x, weight ? &*weight : &none, bias ? &*bias : &none});
+              return GroupNormAct::apply(x, weight, bias, groups, eps, activation, workspace);
+          },
           pybind11::call_guard<pybind11::gil_scoped_release>());
     m.def("vocab_loss",
           [](const Tensor& features, const Tensor& weight, const OptTensor& bias, const Tensor& targets,
              const OptTensor& teacher_logits, double temperature, int64_t reduction, int64_t saved_bytes,
              int64_t forward_bytes, int64_t backward_bytes) {
+              const Tensor none;
+              check_recording(features, {&features, &weight, bias ? &*bias : &none});
               return VocabLoss::apply(features, weight, bias, targets, teacher_logits, temperature, reduction, saved_bytes,
                                       forward_bytes, backward_bytes);
           },

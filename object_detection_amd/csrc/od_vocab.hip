@@ -7,17 +7,21 @@
 //   loss_n = T^2 (sum p log p - sum p z_class + lse)
 //   dz = g T (q - p), g the gradient of the row's loss;   dF = dz W,  dW = dz^T F,  db = sum_n dz
 //
-// Forward: one product over tiles of 128 rows x 128 classes whose epilogue folds a tile into a running maximum and sum
-// per row (in the lane that owns the row: no traffic between lanes before the end); the classes are split over
-// workgroups and joined by a second kernel, which also forms the few logits of the targets by dot products.
-// Backward: the classes are taken in pieces; a piece's dz is recomputed from the saved lse into a buffer of bounded size
-// (in the type of the inputs: it is an operand of the two products that follow), the target entries are corrected, and
-// dF and dW accumulate in fp32.  16-bit dz: bf16 keeps the exponents of fp32; fp16 rows are scaled by one power of two,
-// taken from the largest row gradient, so that small probabilities do not underflow; the scale leaves in the fp32 results.
+// Forward: one product whose epilogue folds each tile of logits into a running maximum and sum per row, in the lane that
+// owns the row: nothing passes between lanes before the end.  The classes are split over workgroups; a second kernel joins
+// the splits and forms the few logits of the targets by dot products.
+// Backward: the classes are taken in pieces.  A piece's dz is recomputed from the saved lse into a buffer of 256 MB at most,
+// its target entries are corrected, and the two products that read it, dF and dW, accumulate in fp32.
+// Operands of those two products, for 16-bit inputs: dz, features and weight in fp16, dz times 2^14 and the others (bf16, or
+// weighted by a gradient per row) under one power of two each, which brings the largest value to [2^13, 2^14).  fp16 keeps
+// three bits of dz more than bf16 (gradients 1.05 instead of 1.5 final roundings from the exact ones), and bf16 values no
+// more than 2^27 times smaller than the largest come through unchanged; the powers of two leave in the fp32 results.
 //
 // Rows without a target (negative class; no finite teacher entry) are left out at the start: the valid rows are listed in
 // order and their features packed densely, so that masked rows cost nothing and whatever they hold (infinities, NaN)
-// reaches no product.  All sums run in a fixed order; there are no atomics.
+// reaches no product.  All sums run in a fixed order; the only atomics are integer maxima, whose order changes nothing.
+//
+// A product of n rows, V classes and dim D costs 2 n V D operations, four times a training step (forward, dz again, dF, dW).
 #include "od_common.h"
 #include "../../include/od_boxes.h"
 #include "od_elem.h"
@@ -28,7 +32,7 @@ namespace {
 
 using namespace od;
 
-constexpr int VT = 256;                 // threads per workgroup: four waves in a 2 x 2 arrangement
+constexpr int VT = 256;                 // threads per workgroup (twice that in the gradient products)
 constexpr int TILE = 128;               // rows and classes of a workgroup's tile where both operands stream
 constexpr int ROW_TILE = 256;           // rows and classes are padded to this: tiles of every kernel divide it
 constexpr int STAGE = TILE * 128;       // bytes of one operand's stage in LDS
@@ -216,7 +220,7 @@ __device__ __forceinline__ int xcd_range(int id, int total) {
 
 // ---- preparation --------------------------------------------------------------------------------------------------
 // Number of valid rows, their list and each row's place in it, in row order, by one workgroup; clears row_loss.
-// A row is valid if valid_of(targets, flags) says so.
+// A row is valid if its flag is set (distillation) or its target is not negative.
 struct RowLists {
     int* count;
     int* row_of;                        // [rows] valid rows in order
@@ -251,9 +255,6 @@ __global__ __launch_bounds__(1024) void list_rows_kernel(const long long* __rest
     if (threadIdx.x == 1023) *lists.count = sums[1023];
 }
 
-// Teacher's distribution of a row over its listed classes, one wave per row: p = softmax(t / T) over the entries with a
-// class >= 0 and a logit above -inf.  Entries that name the same class are one class: the first of them gets the sum, the
-// others 0, and the entropy term sum p log p is the merged distribution's.
 __device__ __forceinline__ float wave_max(float v) {
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
@@ -263,6 +264,9 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
+// Teacher's distribution of a row over its listed classes, one wave per row: p = softmax(t / T) over the entries with a
+// class >= 0 and a logit above -inf.  Entries that name the same class are one class: the first of them gets the sum, the
+// others 0, and the entropy term sum p log p is the merged distribution's.
 template <typename T>
 __global__ __launch_bounds__(VT) void teacher_kernel(const long long* __restrict__ classes, const T* __restrict__ logits,
                                                      int rows, int top, float inv_temp, float* __restrict__ prob,

@@ -23,7 +23,7 @@ def group_norm_act(x: Tensor, num_groups: int, weight: Optional[Tensor] = None, 
 
     The result has x's type and channels-last memory; x in another memory order is copied once.  ``activation``: "none",
     "relu" or "silu".  weight / bias [C] share one type, which may differ from x's (fp32 parameters of a tower that runs
-    under autocast).  Statistics, normalisation and the sums of the gradients are fp32 for every type; the result is
+    under autocast).  Statistics are merged and kept in 64 bits, everything else is fp32 for every type; the result is
     rounded once.  Differentiable once in x, weight and bias.  Limits: 2048 channels, 65535 images."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(_ACTIVATIONS)}")

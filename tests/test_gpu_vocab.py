@@ -475,6 +475,36 @@ def test_another_stream_and_captured_steps(device):
         assert all(torch.equal(x, y) for x, y in zip(second.outputs, eager)), k
 
 
+def test_a_recorded_step_shares_no_leaves_with_a_live_eager_one(device):
+    """Refused while the results of an eager step over the same leaves live on another stream; recorded once they are gone."""
+    from object_detection_amd.graph_step import capture
+    from object_detection_amd.norm import group_norm_act
+    f, w, b, t = _inputs(device, 300, 513, 64, torch.bfloat16, True, seed=23)
+    leaves = [x.detach().clone().requires_grad_(True) for x in (f, w, b)]
+    maps = [torch.randn((2, 32, 8, 8), device=device).contiguous(memory_format=torch.channels_last).requires_grad_(True)]
+    up = torch.randn_like(maps[0])
+
+    def loss_of():
+        return det_utils.vocabulary_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+
+    def map_of():
+        return group_norm_act(maps[0], 8, None, None, 1e-5, "relu")
+    for forward, inputs, grad in ((loss_of, leaves, None), (map_of, maps, up)):
+        def step():
+            y = forward()
+            return [y.detach()] + list(torch.autograd.grad(y, inputs, grad))
+        alive = forward()
+        with pytest.raises(RuntimeError, match="recorded while results of an earlier one"):
+            capture(step, device)
+        want = [alive.detach().clone()] + list(torch.autograd.grad(alive, inputs, grad))
+        del alive
+        recorded = capture(step, device)
+        for _ in range(2):
+            got = [x.clone() for x in recorded.replay()]
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_head_over_a_vocabulary_trains_through_tower_and_losses(device):
     """A classification head as it would be used: conv + GroupNormAct tower on a channels-last map, embeddings per anchor,
     cross entropy on the matched anchors and distillation on some, backward to every parameter; against the same head in
