@@ -475,16 +475,54 @@ struct ProductArgs {
     long long first_class, last_class;  // of the piece; last class of all
     const float* bias2;                 // at the piece's first class
     const int* count;
-    int tiles, splits;                  // class tiles of the piece, workgroups per row tile
-    int row_tiles;
+    int tiles, groups;                  // class tiles of the piece, groups of workgroups that share them out
+    int row_tiles;                      // of all rows
     float scale;                        // log2(e) / temperature
-    long long rows_pad;
     // forward
-    float2* part;                       // [splits][rows_pad] (maximum, sum), log2 units
+    float2* part;                       // (maximum, sum) in log2 units, see Share
     // backward
     const float* lse2;                  // [rows_pad] in log2 units
     void* dz;                           // rows_pad x piece, see Dz
     long long piece;
+};
+
+// A value that every lane holds, in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long long uniform(long long v) {
+    return (long long)(((unsigned long long)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
+}
+
+// How the tiles of a product are shared out.  Only the device knows the number of valid rows, so the division is made
+// there: the class tiles fall to `groups` groups of workgroups (8: one per XCD, whose L2 then sees an eighth of the weight;
+// 1 where that would be uneven), and the `units` of a group, its class tiles of one row tile after the other, are cut into
+// equal runs, one for each of its workgroups.  A run is one or more segments of neighbouring class tiles of one row tile.
+// Against equal numbers of class tiles for every row tile, valid or not: 777 x 5003 x 200 fp32, a fifth of the rows left
+// out, 34 -> NN us; 32768 x 65536 x 512 bf16, a tenth left out, 2050 -> NN.
+// A segment of a row is (maximum, sum) number segment(group, workgroup, row tile): along a group's runs either the
+// workgroup or the row tile or both advance, so that the sum of the two numbers names the segment.
+struct Share {
+    long long units, workers;           // of the group; every worker has a unit at least
+    int tiles, first_tile;              // of the group
+    // rows: valid ones; per_group: workgroups launched
+    __device__ __forceinline__ Share(int all_tiles, int groups, int group, long long row_tiles, int per_group) {
+        first_tile = (int)((long long)all_tiles * group / groups);
+        tiles = (int)((long long)all_tiles * (group + 1) / groups) - first_tile;
+        units = row_tiles * tiles;
+        workers = min(units, (long long)per_group);
+    }
+    // worker w has the units [start(w), start(w + 1))
+    __device__ __forceinline__ long long start(long long w) const { return workers == units ? w : quotient(w * units, workers); }
+    // the worker that has a unit
+    __device__ __forceinline__ int worker(long long unit) const {
+        return workers == units ? (int)unit : (int)quotient((unit + 1) * workers + units - 1, units) - 1;
+    }
+    static __device__ __forceinline__ long long segment(int group, int per_group, int row_tiles, long long w, long long row_tile) {
+        return (long long)group * (per_group + row_tiles) + w + row_tile;
+    }
+    static __device__ __forceinline__ long long quotient(long long a, long long b) {
+        if (a < b) return 0;                                        // divisions are software: small calls do without
+        return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+    }
 };
 
 // What the gradient products hold dz, weight and features in, and the power of two that dz is stored under.
@@ -537,14 +575,15 @@ __device__ __forceinline__ void fold(f32x16 (&acc)[CF][NF], const float* bias, f
 }
 
 // Writes a tile of q times the power of two to dz, from class `first` (a multiple of 32) on; rows behind the last valid one
-// get zeros.  shift: lse - LOG2_DZ;  out: the row's element of the piece's class 16 h.
+// get zeros.  shift: lse - LOG2_DZ;  out + lane_at: the first row's element of the piece's class 16 h,
+// out the same in every lane.
 template <typename G, int CF, int NF>
 __device__ __forceinline__ void store_dz(const f32x16 (&acc)[CF][NF], const float* bias, float scale, const float (&shift)[NF],
-                                         const bool (&on)[NF], G* (&out)[NF], int first) {
+                                         const bool (&on)[NF], G* out, uint32_t lane_at, int first) {
     constexpr int E = 16 / sizeof(G);
 #pragma unroll
     for (int f = 0; f < CF; ++f) {
-        const long long at = (first + f * 32) / Dz<G>::CLASSES * Dz<G>::BLOCK + (first + f * 32) % Dz<G>::CLASSES;
+        G* const to = out + ((first + f * 32) / Dz<G>::CLASSES * Dz<G>::BLOCK + (first + f * 32) % Dz<G>::CLASSES);
 #pragma unroll
         for (int c = 0; c < 16; c += E) {
             float b[E];
@@ -558,7 +597,7 @@ __device__ __forceinline__ void store_dz(const f32x16 (&acc)[CF][NF], const floa
                     v[e] = __builtin_amdgcn_exp2f(fmaf(acc[f][g][c + e], scale, b[e] - shift[g]));
                     if (!on[g]) v[e] = 0.0f;
                 }
-                store_vec<G, E>(out[g] + at + c, v);
+                store_vec<G, E>(to + (lane_at + (uint32_t)(g * 32 * Dz<G>::CLASSES + c)), v);
             }
         }
     }
@@ -591,28 +630,48 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
     constexpr int ROW = S::ROW, NF = S::NF, CT = S::CT, CF = CT / 32, CHUNKS = ROW / 16, PASSES = CT * CHUNKS / VT;
     __shared__ __align__(1024) char lds0[CT * ROW], lds1[CT * ROW];
     __shared__ __align__(16) float s_bias[2][CT];
-    const int id = xcd_range(blockIdx.x, gridDim.x);
-    const int split = id / p.row_tiles;
-    const long long r0 = (long long)(id % p.row_tiles) * S::ROWS;
     const int count = *p.count;
-    if (r0 >= count) return;
-    const int t0 = (int)((long long)p.tiles * split / p.splits), t1 = (int)((long long)p.tiles * (split + 1) / p.splits);
+    if (count == 0) return;
+    const int per_group = gridDim.x / p.groups;
+    const int group = p.groups == 1 ? 0 : blockIdx.x % p.groups;    // hardware hands workgroups to the XCDs in turn
+    const int worker = p.groups == 1 ? xcd_range(blockIdx.x, gridDim.x) : blockIdx.x / p.groups;
+    const Share share(p.tiles, p.groups, group, (count + S::ROWS - 1) / S::ROWS, per_group);
+    if (worker >= share.workers) return;
+    long long unit = uniform(share.start(worker));
+    const long long end = uniform(share.start(worker + 1));
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
-    const long long mine = r0 + wave * 32 * NF + (lane & 31);      // this lane's first row
 
-    uint32_t offset[PASSES];                                        // this lane's source bytes within a class tile
+    // This lane's source bytes within a class tile: chunk at % CHUNKS of row at / CHUNKS, at = i VT + thread.  Where a pass
+    // covers a power of two of rows, the row's bits and so the permutation's come apart into the pass's and the thread's, and
+    // one register serves all passes.
+    constexpr bool APART = VT % CHUNKS == 0;
+    constexpr int PASS_ROWS = VT / CHUNKS;
+    const int my_row = threadIdx.x / CHUNKS;
+    int my_chunk = ((threadIdx.x % CHUNKS) ^ class_swizzle<ROW>(my_row)) << 4;
+    uint32_t offset[APART ? 1 : PASSES];
+    if constexpr (APART) {
+        offset[0] = my_row * (uint32_t)p.weight_pitch;
+    } else {
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-        const int at = i * VT + threadIdx.x, r = at / CHUNKS;
-        offset[i] = r * (uint32_t)p.weight_pitch + (((at % CHUNKS) ^ class_swizzle<ROW>(r)) << 4);
+        for (int i = 0; i < PASSES; ++i) {
+            const int at = i * VT + threadIdx.x, r = at / CHUNKS;
+            offset[i] = r * (uint32_t)p.weight_pitch + (((at % CHUNKS) ^ class_swizzle<ROW>(r)) << 4);
+        }
     }
     const long long behind = p.last_class + 1 - p.first_class;      // classes of the piece that exist
     auto stage = [&](char* to, int t) {
         const long long c = (long long)t * CT;
         const char* from = p.weight + (p.first_class + c) * p.weight_pitch;
         if (c + CT <= behind) {
+            asm volatile("" : "+v"(my_chunk));                      // formed anew in every step, as first_chunk below
 #pragma unroll
-            for (int i = 0; i < PASSES; ++i) stage16(from + offset[i], to + i * VT * 16 + wave * 1024);
+            for (int i = 0; i < PASSES; ++i) {
+                if constexpr (APART)
+                    stage16(from + i * PASS_ROWS * p.weight_pitch +
+                                (offset[0] + (uint32_t)(my_chunk ^ (class_swizzle<ROW>(i * PASS_ROWS) << 4))),
+                            to + i * VT * 16 + wave * 1024);
+                else stage16(from + offset[i], to + i * VT * 16 + wave * 1024);
+            }
         } else {                                                    // rows behind the last class repeat it
 #pragma unroll
             for (int i = 0; i < PASSES; ++i) {
@@ -624,84 +683,90 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
         }
     };
 
-    float m[NF], s[NF], shift[NF];
-    bool on[NF];
-    G* out[NF];
-#pragma unroll
-    for (int g = 0; g < NF; ++g) {
-        m[g] = LOWEST;
-        s[g] = 0.0f;
-        if (GRAD) {
-            shift[g] = p.lse2[mine + g * 32] - GradOf<T>::LOG2_DZ;
-            on[g] = mine + g * 32 < count;
-            out[g] = (G*)p.dz + Dz<G>::at(mine + g * 32, 16 * h, p.piece);
-        }
-    }
-    float tile_bias = 0.0f;
-    auto fetch_bias = [&](int t) { if (threadIdx.x < CT && t < t1) tile_bias = p.bias2[(long long)t * CT + threadIdx.x]; };
-
-    if (t0 < t1) {
-        fetch_bias(t0);
-        stage(lds0, t0);
-    }
-    u32x4 rows[NF][KS];
-#pragma unroll
-    for (int g = 0; g < NF; ++g)
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-            rows[g][k] = *reinterpret_cast<const u32x4*>(p.features + (mine + g * 32) * ROW + k * 32 + 16 * h);
-    if (threadIdx.x < CT) s_bias[t0 & 1][threadIdx.x] = tile_bias;
-    fetch_bias(t0 + 1);
-
     const int my_class = class_row(lane & 31);
     int first_chunk = my_class * ROW + ((h ^ class_swizzle<ROW>(my_class)) << 4);
-    auto step = [&](const char* now, char* next, int t) {
-        stage_barrier();
-        if (threadIdx.x < CT) s_bias[(t + 1) & 1][threadIdx.x] = tile_bias;
-        fetch_bias(t + 2);
-        if (t + 1 < t1) stage(next, t + 1);
-        f32x16 acc[CF][NF];
+    while (unit < end) {
+        const long long row_tile = uniform(Share::quotient(unit, share.tiles));
+        const int t0 = share.first_tile + (int)(unit - row_tile * share.tiles);
+        const int t1 = min(share.first_tile + share.tiles, t0 + (int)min(end - unit, (long long)share.tiles));
+        unit += t1 - t0;
+        const long long mine = row_tile * S::ROWS + wave * 32 * NF + (lane & 31);       // this lane's first row
+        float m[NF], s[NF], shift[NF];
+        bool on[NF];
 #pragma unroll
-        for (int f = 0; f < CF; ++f)
+        for (int g = 0; g < NF; ++g) {
+            m[g] = LOWEST;
+            s[g] = 0.0f;
+            if (GRAD) {
+                shift[g] = p.lse2[mine + g * 32] - GradOf<T>::LOG2_DZ;
+                on[g] = mine + g * 32 < count;
+            }
+        }
+        G* const out = (G*)p.dz + Dz<G>::at(row_tile * S::ROWS, 0, p.piece);
+        const uint32_t lane_at = (wave * 32 * NF + (lane & 31)) * Dz<G>::CLASSES + 16 * h;
+        float tile_bias = 0.0f;
+        auto fetch_bias = [&](int t) { if (threadIdx.x < CT && t < t1) tile_bias = p.bias2[(long long)t * CT + threadIdx.x]; };
+        fetch_bias(t0);
+        stage(lds0, t0);
+        u32x4 rows[NF][KS];
 #pragma unroll
-            for (int g = 0; g < NF; ++g)
+        for (int g = 0; g < NF; ++g)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
-        // chunk (2 k + h) ^ swizzle is chunk h ^ swizzle with the bits of 2 k flipped (rows of an odd multiple of 128 bytes:
-        // of its low three bits); formed anew in every step, since KS addresses held over the loop would not fit
-        asm volatile("" : "+v"(first_chunk));
-        constexpr int FLIP = ROW % 256 == 0 ? 15 : 7;
-        // the wave that multiplies goes first, the one beside it fills in with its exponentials
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            u32x4 a[CF];
-            const char* from = now + ((first_chunk ^ (((2 * k) & FLIP) << 4)) + (((2 * k) & ~FLIP) << 4));
-#pragma unroll
-            for (int f = 0; f < CF; ++f) a[f] = *reinterpret_cast<const u32x4*>(from + f * 32 * ROW);
+            for (int k = 0; k < KS; ++k)
+                rows[g][k] = *reinterpret_cast<const u32x4*>(p.features + (mine + g * 32) * ROW + k * 32 + 16 * h);
+        if (threadIdx.x < CT) s_bias[t0 & 1][threadIdx.x] = tile_bias;
+        fetch_bias(t0 + 1);
+
+        auto step = [&](const char* now, char* next, int t) {
+            stage_barrier();
+            if (threadIdx.x < CT) s_bias[(t + 1) & 1][threadIdx.x] = tile_bias;
+            fetch_bias(t + 2);
+            if (t + 1 < t1) stage(next, t + 1);
+            f32x16 acc[CF][NF];
 #pragma unroll
             for (int f = 0; f < CF; ++f)
 #pragma unroll
-                for (int g = 0; g < NF; ++g) acc[f][g] = Mma<T>::run(a[f], rows[g][k], acc[f][g]);
-        }
-        interleave<4 * CF, KS, CF * NF*(sizeof(T) == 4 ? 4 : 1), CF>();
-        __builtin_amdgcn_s_setprio(0);
-        const float* bias = s_bias[t & 1] + 16 * h;
-        if (GRAD) store_dz<G, CF, NF>(acc, bias, p.scale, shift, on, out, t * CT);
-        else fold<CF, NF>(acc, bias, p.scale, m, s);
-    };
-    int t = t0;
-    while (t < t1) {
-        step(lds0, lds1, t++);
-        if (t == t1) break;
-        step(lds1, lds0, t++);
-    }
-    if (!GRAD) {
+                for (int g = 0; g < NF; ++g)
 #pragma unroll
-        for (int g = 0; g < NF; ++g) {
-            join_halves(m[g], s[g]);
-            if (h == 0) p.part[(long long)split * p.rows_pad + mine + g * 32] = make_float2(m[g], s[g]);
+                    for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
+            // chunk (2 k + h) ^ swizzle is chunk h ^ swizzle with the bits of 2 k flipped (rows of an odd multiple of 128
+            // bytes: of its low three bits); formed anew in every step, since KS addresses held over the loop would not fit
+            asm volatile("" : "+v"(first_chunk));
+            constexpr int FLIP = ROW % 256 == 0 ? 15 : 7;
+            // the wave that multiplies goes first, the one beside it fills in with its exponentials
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                u32x4 a[CF];
+                const char* from = now + ((first_chunk ^ (((2 * k) & FLIP) << 4)) + (((2 * k) & ~FLIP) << 4));
+#pragma unroll
+                for (int f = 0; f < CF; ++f) a[f] = *reinterpret_cast<const u32x4*>(from + f * 32 * ROW);
+#pragma unroll
+                for (int f = 0; f < CF; ++f)
+#pragma unroll
+                    for (int g = 0; g < NF; ++g) acc[f][g] = Mma<T>::run(a[f], rows[g][k], acc[f][g]);
+            }
+            interleave<4 * CF, KS, CF * NF*(sizeof(T) == 4 ? 4 : 1), CF>();
+            __builtin_amdgcn_s_setprio(0);
+            const float* bias = s_bias[t & 1] + 16 * h;
+            if (GRAD) store_dz<G, CF, NF>(acc, bias, p.scale, shift, on, out, lane_at, t * CT);
+            else fold<CF, NF>(acc, bias, p.scale, m, s);
+        };
+        int t = t0;
+        while (t < t1) {
+            step(lds0, lds1, t++);
+            if (t == t1) break;
+            step(lds1, lds0, t++);
         }
+        if (!GRAD) {
+            float2* part = p.part + Share::segment(group, per_group, p.row_tiles, worker, row_tile) * S::ROWS;
+#pragma unroll
+            for (int g = 0; g < NF; ++g) {
+                join_halves(m[g], s[g]);
+                if (h == 0) part[wave * 32 * NF + g * 32 + lane] = make_float2(m[g], s[g]);
+            }
+        }
+        __syncthreads();                                            // the next segment writes to LDS what others still read
     }
 }
 
@@ -712,120 +777,129 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
     __shared__ __align__(1024) char lds0[2 * STAGE], lds1[2 * STAGE];       // two stages of (classes, rows)
     __shared__ float2 joined[2][TILE];
     __shared__ __align__(16) float s_bias[TILE];
-    const int id = xcd_range(blockIdx.x, gridDim.x);
-    const int split = id / p.row_tiles;
-    const long long r0 = (long long)(id % p.row_tiles) * TILE;
     const int count = *p.count;
-    if (r0 >= count) return;
-    const int t0 = (int)((long long)p.tiles * split / p.splits), t1 = (int)((long long)p.tiles * (split + 1) / p.splits);
+    if (count == 0) return;
+    const int per_group = gridDim.x / p.groups;
+    const int group = p.groups == 1 ? 0 : blockIdx.x % p.groups;
+    const int worker = p.groups == 1 ? xcd_range(blockIdx.x, gridDim.x) : blockIdx.x / p.groups;
+    const Share share(p.tiles, p.groups, group, (count + TILE - 1) / TILE, per_group);
+    if (worker >= share.workers) return;
+    long long unit = uniform(share.start(worker));
+    const long long end = uniform(share.start(worker + 1));
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
     const int wc = (wave & 1) * 64, wr = (wave >> 1) * 64;          // this wave's classes and rows within the tile
     constexpr int KE = 128 / sizeof(T);
     const int ksteps = p.dim_pad / KE;
     typedef ChunkedOperand<TILE, VT, true> Classes;
     typedef ChunkedOperand<TILE, VT, false> Rows;
-    Rows rows;
-    Classes cls;
-    rows.init(p.features, (long long)p.dim_pad * sizeof(T), r0, r0 + TILE);
+    while (unit < end) {
+        const long long row_tile = uniform(Share::quotient(unit, share.tiles)), r0 = row_tile * TILE;
+        const int t0 = share.first_tile + (int)(unit - row_tile * share.tiles);
+        const int t1 = min(share.first_tile + share.tiles, t0 + (int)min(end - unit, (long long)share.tiles));
+        unit += t1 - t0;
+        Rows rows;
+        Classes cls;
+        rows.init(p.features, (long long)p.dim_pad * sizeof(T), r0, r0 + TILE);
 
-    float m[2], s[2], shift[2];
-    bool on[2];
-    G* out[2];
+        float m[2], s[2], shift[2];
+        bool on[2];
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-        m[g] = LOWEST;
-        s[g] = 0.0f;
-        if (GRAD) {
-            const long long row = r0 + wr + g * 32 + (lane & 31);
-            shift[g] = p.lse2[row] - GradOf<T>::LOG2_DZ;
-            on[g] = row < count;
-            out[g] = (G*)p.dz + Dz<G>::at(row, 16 * h, p.piece);
-        }
-    }
-
-    f32x16 acc[2][2];
-    auto clear = [&] {
-#pragma unroll
-        for (int f = 0; f < 2; ++f)
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
-    };
-    int next_t = t0, next_k = 0;                                    // what is staged next
-    float tile_bias = 0.0f;
-    auto fetch_bias = [&](int t) { if (threadIdx.x < TILE && t < t1) tile_bias = p.bias2[(long long)t * TILE + threadIdx.x]; };
-    auto stage_next = [&](char* to) {
-        if (next_t >= t1) return;
-        if (next_k == 0) cls.init(p.weight, p.weight_pitch, p.first_class + (long long)next_t * TILE, p.last_class);
-        cls.stage(to, (long long)next_k * 128);
-        rows.stage(to + STAGE, (long long)next_k * 128);
-        if (++next_k == ksteps) {
-            next_k = 0;
-            ++next_t;
-        }
-    };
-    auto multiply = [&](const char* now) {
-        int at = lane;
-        asm volatile("" : "+v"(at));                                // addresses are formed anew in every stage, see resident_kernel
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            u32x4 a[2], b[2];
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                a[f] = Classes::frag(now, wc + f * 32, j, at);
-                b[f] = Rows::frag(now + STAGE, wr + f * 32, j, at);
+        for (int g = 0; g < 2; ++g) {
+            m[g] = LOWEST;
+            s[g] = 0.0f;
+            if (GRAD) {
+                const long long row = r0 + wr + g * 32 + (lane & 31);
+                shift[g] = p.lse2[row] - GradOf<T>::LOG2_DZ;
+                on[g] = row < count;
             }
+        }
+        G* const out = (G*)p.dz + Dz<G>::at(r0, 0, p.piece);
+        const uint32_t lane_at = (wr + (lane & 31)) * Dz<G>::CLASSES + 16 * h;
+
+        f32x16 acc[2][2];
+        auto clear = [&] {
 #pragma unroll
             for (int f = 0; f < 2; ++f)
 #pragma unroll
-                for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(a[f], b[g], acc[f][g]);
-        }
-        interleave<8, 4, 4 * (sizeof(T) == 4 ? 4 : 1), 4>();
-    };
-    // The bias of a tile is fetched ahead of the tile's first stage (waiting for it later would wait for the stages behind
-    // it as well) and written to LDS in its first step.  The two stages are variables of their own, used by turns in
-    // straight code: the compiler then knows that reading one need not wait for the loads into the other.
-    auto step = [&](const char* now, char* next, int& t, int& k) {
-        stage_barrier();
-        if (k == 0 && threadIdx.x < TILE) s_bias[threadIdx.x] = tile_bias;
-        if (k + 1 == ksteps) fetch_bias(t + 1);
-        stage_next(next);
-        multiply(now);
-        if (++k == ksteps) {
-            if (ksteps == 1) __syncthreads();                       // s_bias was written in this very step
-            const float* bias = s_bias + wc + 16 * h;
-            if (GRAD) store_dz<G, 2, 2>(acc, bias, p.scale, shift, on, out, t * TILE + wc);
-            else fold<2, 2>(acc, bias, p.scale, m, s);
-            clear();
-            k = 0;
-            ++t;
-        }
-    };
-    clear();
-    fetch_bias(t0);
-    stage_next(lds0);
-    int t = t0, k = 0;
-    const int steps = (t1 - t0) * ksteps;
-    for (int i = 0; i + 1 < steps; i += 2) {
-        step(lds0, lds1, t, k);
-        step(lds1, lds0, t, k);
-    }
-    if (steps & 1) step(lds0, lds1, t, k);
-    if (!GRAD) {
-        // a row's classes lie in two lanes and two waves
+                for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            join_halves(m[g], s[g]);
-            if (h == 0) joined[wave & 1][wr + g * 32 + lane] = make_float2(m[g], s[g]);
+                    for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
+        };
+        int next_t = t0, next_k = 0;                                    // what is staged next
+        float tile_bias = 0.0f;
+        auto fetch_bias = [&](int t) { if (threadIdx.x < TILE && t < t1) tile_bias = p.bias2[(long long)t * TILE + threadIdx.x]; };
+        auto stage_next = [&](char* to) {
+            if (next_t >= t1) return;
+            if (next_k == 0) cls.init(p.weight, p.weight_pitch, p.first_class + (long long)next_t * TILE, p.last_class);
+            cls.stage(to, (long long)next_k * 128);
+            rows.stage(to + STAGE, (long long)next_k * 128);
+            if (++next_k == ksteps) {
+                next_k = 0;
+                ++next_t;
+            }
+        };
+        auto multiply = [&](const char* now) {
+            int at = lane;
+            asm volatile("" : "+v"(at));                                // addresses are formed anew in every stage, see resident_kernel
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u32x4 a[2], b[2];
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    a[f] = Classes::frag(now, wc + f * 32, j, at);
+                    b[f] = Rows::frag(now + STAGE, wr + f * 32, j, at);
+                }
+#pragma unroll
+                for (int f = 0; f < 2; ++f)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(a[f], b[g], acc[f][g]);
+            }
+            interleave<8, 4, 4 * (sizeof(T) == 4 ? 4 : 1), 4>();
+        };
+        // The bias of a tile is fetched ahead of the tile's first stage (waiting for it later would wait for the stages behind
+        // it as well) and written to LDS in its first step.  The two stages are variables of their own, used by turns in
+        // straight code: the compiler then knows that reading one need not wait for the loads into the other.
+        auto step = [&](const char* now, char* next, int& t, int& k) {
+            stage_barrier();
+            if (k == 0 && threadIdx.x < TILE) s_bias[threadIdx.x] = tile_bias;
+            if (k + 1 == ksteps) fetch_bias(t + 1);
+            stage_next(next);
+            multiply(now);
+            if (++k == ksteps) {
+                if (ksteps == 1) __syncthreads();                       // s_bias was written in this very step
+                const float* bias = s_bias + wc + 16 * h;
+                if (GRAD) store_dz<G, 2, 2>(acc, bias, p.scale, shift, on, out, lane_at, t * TILE + wc);
+                else fold<2, 2>(acc, bias, p.scale, m, s);
+                clear();
+                k = 0;
+                ++t;
+            }
+        };
+        clear();
+        fetch_bias(t0);
+        stage_next(lds0);
+        int t = t0, k = 0;
+        const int steps = (t1 - t0) * ksteps;
+        for (int i = 0; i + 1 < steps; i += 2) {
+            step(lds0, lds1, t, k);
+            step(lds1, lds0, t, k);
         }
-        __syncthreads();
-        if (threadIdx.x < TILE) {
-            const float2 a = joined[0][threadIdx.x], b = joined[1][threadIdx.x];
-            const float top = fmaxf(a.x, b.x);
-            p.part[(long long)split * p.rows_pad + r0 + threadIdx.x] =
-                make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top));
-        }
+        if (steps & 1) step(lds0, lds1, t, k);
+        if (!GRAD) {
+            // a row's classes lie in two lanes and two waves
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                join_halves(m[g], s[g]);
+                if (h == 0) joined[wave & 1][wr + g * 32 + lane] = make_float2(m[g], s[g]);
+            }
+            __syncthreads();
+            if (threadIdx.x < TILE) {
+                const float2 a = joined[0][threadIdx.x], b = joined[1][threadIdx.x];
+                const float top = fmaxf(a.x, b.x);
+                p.part[Share::segment(group, per_group, p.row_tiles, worker, row_tile) * TILE + threadIdx.x] =
+                    make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top));
+            }
+        }    __syncthreads();                                                // the next segment writes to LDS what others still read
     }
 }
 
@@ -843,7 +917,7 @@ struct TargetArgs {
     const float* entropy;               // [rows]
     RowLists lists;
     const float2* part;
-    int splits;
+    int tiles, groups, row_tile, row_tiles, workgroups;             // of the product, see Share
     long long rows_pad;
     float temperature;
     float* lse2;                        // [rows_pad]
@@ -864,8 +938,12 @@ __global__ __launch_bounds__(VT) void targets_kernel(TargetArgs p) {
     }
     const long long row = p.lists.row_of[place];
     float m = LOWEST, s = 0.0f;
-    for (int k = lane; k < p.splits; k += 64) {
-        const float2 v = p.part[(long long)k * p.rows_pad + place];
+    const int lanes = 64 / p.groups, group = lane / lanes, per_group = p.workgroups / p.groups;
+    const Share share(p.tiles, p.groups, group, (count + p.row_tile - 1) / p.row_tile, per_group);
+    const long long row_tile = place / p.row_tile;
+    const int first = share.worker(row_tile * share.tiles), last = share.worker((row_tile + 1) * share.tiles - 1);
+    for (int w = first + lane % lanes; w <= last; w += lanes) {
+        const float2 v = p.part[Share::segment(group, per_group, p.row_tiles, w, row_tile) * p.row_tile + place % p.row_tile];
         const float top = fmaxf(m, v.x);
         s = s * __builtin_amdgcn_exp2f(m - top) + v.y * __builtin_amdgcn_exp2f(v.x - top);
         m = top;
@@ -1374,13 +1452,20 @@ int splits_for(long long tiles, long long steps, int slots, int fixed, int limit
     return (int)best;
 }
 
+// Groups that share out the class tiles of a product: one per XCD, unless one would get an eighth more than another, or a
+// run would pass from row tile to row tile (and load its rows again) after fewer than 64 class tiles: a piece of 4096
+// classes for 32768 rows 150 us instead of 171.
+int groups_of(long long tiles, long long row_tiles) {
+    return tiles >= 64 && (row_tiles <= SLOTS / 8 || tiles >= 512) ? 8 : 1;
+}
+
 // Everything that follows from the sizes.
 struct Plan {
     long long rows, rows_pad, classes, classes_pad;
     int dim, dim_pad, size, n;                  // n: targets per row
     int slabs;                                  // 32-byte slabs of a row where the rows are resident, 0 where they stream
     int row_tile, class_tile, row_tiles;        // of the product
-    int splits, splits_z;                       // of the classes: forward, a piece of dz
+    int workgroups;                             // of the product
     long long piece;                            // classes per piece
     int pieces, grad_tile, splits_f, splits_w;  // backward; grad_tile: columns of dim per workgroup
     // saved buffer
@@ -1415,12 +1500,11 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     if (most(p.rows_pad, p.classes_pad) * p.dim_pad * p.size / 16 > (1ll << 30)) return false;
     p.n = top > 0 ? top : 1;
     p.row_tiles = (int)((most(rows, 1) + p.row_tile - 1) / p.row_tile);
-    p.splits = splits_for(p.row_tiles, p.classes_pad / p.class_tile, SLOTS, 2, SLOTS);
+    p.workgroups = (int)least(SLOTS, up(p.row_tiles * (p.classes_pad / p.class_tile), 8));
     long long piece = most(ROW_TILE, DZ_BYTES / (p.rows_pad * p.size) / ROW_TILE * ROW_TILE);
     p.pieces = (int)((p.classes_pad + piece - 1) / piece);
     p.piece = up((p.classes_pad + p.pieces - 1) / p.pieces, ROW_TILE);
     p.pieces = (int)((p.classes_pad + p.piece - 1) / p.piece);
-    p.splits_z = splits_for(p.row_tiles, p.piece / p.class_tile, SLOTS, 2, SLOTS);
     // columns of dim per workgroup of the gradient products: what leaves least unused, the widest of those
     p.grad_tile = 256;
     for (int t = 128; t >= 64; t /= 2)
@@ -1444,7 +1528,8 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     at = 0;
     p.f_weight = take(at, p.classes * p.dim_pad * p.size);
     p.f_bias = take(at, 4 * p.classes_pad);
-    p.f_part = take(at, 8 * p.rows_pad * p.splits);
+    p.f_part = take(at, 8ll * p.row_tile * groups_of(p.classes_pad / p.class_tile, p.row_tiles) *
+                            (p.workgroups / groups_of(p.classes_pad / p.class_tile, p.row_tiles) + p.row_tiles));
     p.f_entropy = take(at, 4 * p.rows_pad);
     p.f_flags = take(at, p.rows_pad);
     p.forward = at;
@@ -1559,7 +1644,7 @@ int prepare(const Call& c, bool with_features, const unsigned char* flags, size_
 // The product by the kernel for its row width.
 template <typename T, bool GRAD>
 int launch_product(const Call& c, int kernel, const ProductArgs& a) {
-    const dim3 grid((unsigned)((long long)a.row_tiles * a.splits));
+    const dim3 grid((unsigned)c.p.workgroups);
     switch (c.p.slabs) {
 #define OD_PRODUCT(KS) \
     case KS: OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, KS, GRAD>), grid, dim3(VT), 0, c.stream, a); break
@@ -1618,10 +1703,9 @@ int forward_typed(const Call& c) {
     a.bias2 = (const float*)(c.ws + p.f_bias);
     a.count = lists.count;
     a.tiles = (int)(p.classes_pad / p.class_tile);
-    a.splits = p.splits;
+    a.groups = groups_of(a.tiles, p.row_tiles);
     a.row_tiles = p.row_tiles;
     a.scale = LOG2E / c.temperature;
-    a.rows_pad = p.rows_pad;
     a.part = (float2*)(c.ws + p.f_part);
     rc = launch_product<T, false>(c, OD_KERNEL_VOCAB_LSE, a);
     if (rc != OD_OK) return rc;
@@ -1638,7 +1722,11 @@ int forward_typed(const Call& c) {
     t.entropy = entropy;
     t.lists = lists;
     t.part = a.part;
-    t.splits = p.splits;
+    t.tiles = a.tiles;
+    t.groups = a.groups;
+    t.row_tile = p.row_tile;
+    t.row_tiles = p.row_tiles;
+    t.workgroups = p.workgroups;
     t.rows_pad = p.rows_pad;
     t.temperature = c.temperature;
     t.lse2 = (float*)(c.saved + p.o_lse);
@@ -1710,10 +1798,9 @@ int backward_typed(const Call& c) {
     a.last_class = p.classes - 1;
     a.count = lists.count;
     a.tiles = (int)(p.piece / p.class_tile);
+    a.groups = groups_of(a.tiles, p.row_tiles);
     a.row_tiles = p.row_tiles;
-    a.splits = p.splits_z;
     a.scale = LOG2E / c.temperature;
-    a.rows_pad = p.rows_pad;
     a.lse2 = (const float*)(c.saved + p.o_lse);
     a.dz = c.ws + p.b_dz;
     a.piece = p.piece;
