@@ -479,7 +479,8 @@ struct ProductArgs {
     int row_tiles;                      // of all rows
     float scale;                        // log2(e) / temperature
     // forward
-    float2* part;                       // (maximum, sum) in log2 units, see Share
+    float2* part;                       // [segment][rows of a tile] (maximum, sum) in log2 units, see Share
+    int2* ends;                         // [groups][row_tiles]
     // backward
     const float* lse2;                  // [rows_pad] in log2 units
     void* dz;                           // rows_pad x piece, see Dz
@@ -492,32 +493,42 @@ __device__ __forceinline__ long long uniform(long long v) {
     return (long long)(((unsigned long long)(uint32_t)uniform((int)(v >> 32)) << 32) | (uint32_t)uniform((int)v));
 }
 
+constexpr int FIXED_TILES = 8;          // a segment of a product costs about so many of its tiles besides
+
 // How the tiles of a product are shared out.  Only the device knows the number of valid rows, so the division is made
-// there: the class tiles fall to `groups` groups of workgroups (8: one per XCD, whose L2 then sees an eighth of the weight;
-// 1 where that would be uneven), and the `units` of a group, its class tiles of one row tile after the other, are cut into
-// equal runs, one for each of its workgroups.  A run is one or more segments of neighbouring class tiles of one row tile.
-// Against equal numbers of class tiles for every row tile, valid or not: 777 x 5003 x 200 fp32, a fifth of the rows left
-// out, 34 -> NN us; 32768 x 65536 x 512 bf16, a tenth left out, 2050 -> NN.
-// A segment of a row is (maximum, sum) number segment(group, workgroup, row tile): along a group's runs either the
-// workgroup or the row tile or both advance, so that the sum of the two numbers names the segment.
+// there.  The class tiles fall to `groups` groups of workgroups (at most 8: one per XCD, whose L2 then sees an eighth of the
+// weight).  The `units` of a group, its class tiles of one row tile after the other, are cut into equal runs, one for each
+// of its workgroups (for nearly all of them, where runs then end with their row tile).  A run is one or more segments of
+// neighbouring class tiles of one row tile.
+// Against equal numbers of class tiles for every row tile, valid or not, with dF shared out alike, a training step of
+// 16384 x 32000 x 256 bf16 takes 1050 us instead of 1204 with half the rows left out, 480 instead of 825 with nine tenths,
+// 4096 x 5003 x 200 fp32 with 30 % kept 215 instead of 342; with no row left out the two differ by 2 % either way.
+// Results of segments lie under number segment(group, worker, row tile): along a group's runs either the worker or the row
+// tile or both advance, so that the sum of the two numbers names the segment.  The workers with a row tile's first and last
+// tile write their segments' numbers to `ends`, for whoever joins them.
 struct Share {
     long long units, workers;           // of the group; every worker has a unit at least
     int tiles, first_tile;              // of the group
-    // rows: valid ones; per_group: workgroups launched
-    __device__ __forceinline__ Share(int all_tiles, int groups, int group, long long row_tiles, int per_group) {
+    // row_tiles: with valid rows; most: workers at hand; fixed: what a segment costs beside its units, in units
+    __device__ __forceinline__ Share(int all_tiles, int groups, int group, long long row_tiles, long long most, int fixed) {
         first_tile = (int)((long long)all_tiles * group / groups);
         tiles = (int)((long long)all_tiles * (group + 1) / groups) - first_tile;
         units = row_tiles * tiles;
-        workers = min(units, (long long)per_group);
+        workers = min(units, most);
+        if (workers < units && row_tiles <= workers) {              // the same number for every row tile: one segment each
+            const int each = (int)quotient(workers, row_tiles);
+            if (quotient(tiles, each) <= quotient(units, workers) + fixed) workers = each * row_tiles;
+        }
     }
     // worker w has the units [start(w), start(w + 1))
     __device__ __forceinline__ long long start(long long w) const { return workers == units ? w : quotient(w * units, workers); }
-    // the worker that has a unit
-    __device__ __forceinline__ int worker(long long unit) const {
-        return workers == units ? (int)unit : (int)quotient((unit + 1) * workers + units - 1, units) - 1;
-    }
     static __device__ __forceinline__ long long segment(int group, int per_group, int row_tiles, long long w, long long row_tile) {
         return (long long)group * (per_group + row_tiles) + w + row_tile;
+    }
+    // segment of the tiles [t0, t1) of a row tile
+    __device__ __forceinline__ void mark(int2* ends, long long segment, long long t0, long long t1) const {
+        if (t0 == first_tile) ends->x = (int)segment;
+        if (t1 == first_tile + tiles) ends->y = (int)segment;
     }
     static __device__ __forceinline__ long long quotient(long long a, long long b) {
         if (a < b) return 0;                                        // divisions are software: small calls do without
@@ -633,9 +644,9 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
     const int count = *p.count;
     if (count == 0) return;
     const int per_group = gridDim.x / p.groups;
-    const int group = p.groups == 1 ? 0 : blockIdx.x % p.groups;    // hardware hands workgroups to the XCDs in turn
-    const int worker = p.groups == 1 ? xcd_range(blockIdx.x, gridDim.x) : blockIdx.x / p.groups;
-    const Share share(p.tiles, p.groups, group, (count + S::ROWS - 1) / S::ROWS, per_group);
+    // hardware hands workgroups to the XCDs in turn; an XCD's workers are neighbours
+    const int group = blockIdx.x % p.groups, worker = blockIdx.x % 8 / p.groups * (gridDim.x / 8) + blockIdx.x / 8;
+    const Share share(p.tiles, p.groups, group, (count + S::ROWS - 1) / S::ROWS, per_group, FIXED_TILES);
     if (worker >= share.workers) return;
     long long unit = uniform(share.start(worker));
     const long long end = uniform(share.start(worker + 1));
@@ -759,7 +770,9 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
             step(lds1, lds0, t++);
         }
         if (!GRAD) {
-            float2* part = p.part + Share::segment(group, per_group, p.row_tiles, worker, row_tile) * S::ROWS;
+            const long long segment = Share::segment(group, per_group, p.row_tiles, worker, row_tile);
+            float2* part = p.part + segment * S::ROWS;
+            if (threadIdx.x == 0) share.mark(p.ends + (long long)group * p.row_tiles + row_tile, segment, t0, t1);
 #pragma unroll
             for (int g = 0; g < NF; ++g) {
                 join_halves(m[g], s[g]);
@@ -780,9 +793,9 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
     const int count = *p.count;
     if (count == 0) return;
     const int per_group = gridDim.x / p.groups;
-    const int group = p.groups == 1 ? 0 : blockIdx.x % p.groups;
-    const int worker = p.groups == 1 ? xcd_range(blockIdx.x, gridDim.x) : blockIdx.x / p.groups;
-    const Share share(p.tiles, p.groups, group, (count + TILE - 1) / TILE, per_group);
+    // hardware hands workgroups to the XCDs in turn; an XCD's workers are neighbours
+    const int group = blockIdx.x % p.groups, worker = blockIdx.x % 8 / p.groups * (gridDim.x / 8) + blockIdx.x / 8;
+    const Share share(p.tiles, p.groups, group, (count + TILE - 1) / TILE, per_group, FIXED_TILES);
     if (worker >= share.workers) return;
     long long unit = uniform(share.start(worker));
     const long long end = uniform(share.start(worker + 1));
@@ -840,7 +853,7 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
         };
         auto multiply = [&](const char* now) {
             int at = lane;
-            asm volatile("" : "+v"(at));                                // addresses are formed anew in every stage, see resident_kernel
+            asm volatile("" : "+v"(at));                            // addresses are formed anew in every stage, see resident_kernel
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 u32x4 a[2], b[2];
@@ -893,10 +906,12 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
                 if (h == 0) joined[wave & 1][wr + g * 32 + lane] = make_float2(m[g], s[g]);
             }
             __syncthreads();
+            const long long segment = Share::segment(group, per_group, p.row_tiles, worker, row_tile);
+            if (threadIdx.x == 0) share.mark(p.ends + (long long)group * p.row_tiles + row_tile, segment, t0, t1);
             if (threadIdx.x < TILE) {
                 const float2 a = joined[0][threadIdx.x], b = joined[1][threadIdx.x];
                 const float top = fmaxf(a.x, b.x);
-                p.part[Share::segment(group, per_group, p.row_tiles, worker, row_tile) * TILE + threadIdx.x] =
+                p.part[segment * TILE + threadIdx.x] =
                     make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top));
             }
         }    __syncthreads();                                                // the next segment writes to LDS what others still read
@@ -917,7 +932,8 @@ struct TargetArgs {
     const float* entropy;               // [rows]
     RowLists lists;
     const float2* part;
-    int tiles, groups, row_tile, row_tiles, workgroups;             // of the product, see Share
+    const int2* ends;
+    int groups, row_tile, row_tiles;    // of the product, see Share
     long long rows_pad;
     float temperature;
     float* lse2;                        // [rows_pad]
@@ -938,12 +954,10 @@ __global__ __launch_bounds__(VT) void targets_kernel(TargetArgs p) {
     }
     const long long row = p.lists.row_of[place];
     float m = LOWEST, s = 0.0f;
-    const int lanes = 64 / p.groups, group = lane / lanes, per_group = p.workgroups / p.groups;
-    const Share share(p.tiles, p.groups, group, (count + p.row_tile - 1) / p.row_tile, per_group);
-    const long long row_tile = place / p.row_tile;
-    const int first = share.worker(row_tile * share.tiles), last = share.worker((row_tile + 1) * share.tiles - 1);
-    for (int w = first + lane % lanes; w <= last; w += lanes) {
-        const float2 v = p.part[Share::segment(group, per_group, p.row_tiles, w, row_tile) * p.row_tile + place % p.row_tile];
+    const int lanes = 64 / p.groups, row_tile = (int)(place / p.row_tile);
+    const int2 ends = p.ends[(long long)(lane / lanes) * p.row_tiles + row_tile];
+    for (int k = ends.x + lane % lanes; k <= ends.y; k += lanes) {
+        const float2 v = p.part[(long long)k * p.row_tile + place % p.row_tile];
         const float top = fmaxf(m, v.x);
         s = s * __builtin_amdgcn_exp2f(m - top) + v.y * __builtin_amdgcn_exp2f(v.x - top);
         m = top;
@@ -1183,12 +1197,24 @@ struct GradArgs {
     int dim_pad;
     const int* count;
     long long cols;                     // columns of the result: rows_pad, or piece
-    long long ksteps;                   // K steps of all splits (of rows: at most, see count)
-    int splits;
-    float* out;                         // [splits][cols][dim_pad]
+    long long ksteps;                   // K steps of the piece (dF), or at most, see count (dW)
+    int splits;                         // dW: of K;  dF: workgroups per tile of d, see RowShare
+    float* out;                         // dW: [splits][cols][dim_pad];  dF: [segment][ROW_TILE][dim_pad]
+    int2* ends;                         // dF: [rows_pad / ROW_TILE]
     int accumulate;
     float* bias_out;                    // [splits][cols] weighted sums of dz over K, or null
     const float* row_weight;            // [rows_pad], or null: ones
+};
+
+// dF: the K steps of the valid rows' tiles, shared out as in Share.  A segment's sums are a partial result of their own,
+// which costs as much as eight steps (fp32: as two): no worker gets fewer, and no tile more than 64 workers.
+template <typename T> struct RowShare : Share {
+    static constexpr int FIXED = sizeof(T) == 4 ? 2 : 8;
+    __device__ __forceinline__ RowShare(int count, long long ksteps, int workgroups)
+        : RowShare((long long)((count + ROW_TILE - 1) / ROW_TILE), ksteps, workgroups) {}
+    __device__ __forceinline__ RowShare(long long row_tiles, long long ksteps, int workgroups)
+        : Share((int)ksteps, 1, 0, row_tiles,
+                min((long long)workgroups, min(64 * row_tiles, max(row_tiles, row_tiles * ksteps / FIXED))), FIXED) {}
 };
 
 // c plus both fp16 halves of a word, added in fp32
@@ -1210,15 +1236,16 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
     constexpr int KE = 128 / sizeof(T);
     const int dtiles = (p.dim_pad + DT - 1) / DT;
     const int id = xcd_range(blockIdx.x, gridDim.x);
-    const int d0 = (id % dtiles) * DT;
-    const long long ctiles = p.cols / ROW_TILE;
-    const long long c0 = (id / dtiles) % ctiles * ROW_TILE;
-    const int split = (int)(id / dtiles / ctiles);
+    const int d0 = (id % dtiles) * DT, member = id / dtiles;
     const int count = *p.count;
-    if (ROWS && c0 >= count) return;
-    long long ksteps = p.ksteps;
-    if (!ROWS) ksteps = min(ksteps, (long long)(count + KE - 1) / KE);
-    const long long k_first = ksteps * split / p.splits, k_end = ksteps * (split + 1) / p.splits;
+    if (count == 0 && ROWS) return;
+    long long unit = 0, end = 1;                                    // dW: one tile and split
+    const RowShare<T> share(ROWS ? count : 1, ROWS ? p.ksteps : 1, ROWS ? p.splits : 1);
+    if (ROWS) {
+        if (member >= share.workers) return;
+        unit = uniform(share.start(member));
+        end = uniform(share.start(member + 1));
+    }
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
     const int wd = (wave & 1) * 32 * AF, wcol = (wave >> 1) * 64;
 
@@ -1226,127 +1253,150 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
     typedef DzOperand<T, THREADS> BS;
     typedef ChunkedOperand<ROW_TILE, THREADS, false> BC;
     A a;
-    BS bs;
-    BC bc;
     a.init(p.a, p.a_pitch, d0, p.dim_pad);
-    // 256 rows of dz times the classes of a stage are one block
-    if (ROWS) bc.init(p.dz + Dz<T>::at(c0, 0, p.piece) * (long long)sizeof(T), 128, 0, ROW_TILE - 1);
-    else bs.init(p.dz, p.piece, c0);
-
-    f32x16 acc[AF][2];
-#pragma unroll
-    for (int f = 0; f < AF; ++f)
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
-    float bias = 0.0f;
-    const bool want_bias = !ROWS && p.bias_out && d0 == 0;
-
-    auto stage = [&](char* to_a, char* to_b, long long k) {
-        a.stage(to_a, k * KE, p.a_last);
-        if (ROWS) bc.stage(to_b, k * Dz<T>::BLOCK * (long long)sizeof(T));
-        else bs.stage(to_b, k * KE);
-    };
-    auto multiply = [&](const char* ta, const char* tb, long long k) {
-        int at = lane;
-        asm volatile("" : "+v"(at));                                // addresses are formed anew in every stage, see resident_kernel
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            u32x4 x[AF], y[2];
-#pragma unroll
-            for (int g = 0; g < 2; ++g) y[g] = ROWS ? BC::frag(tb, wcol + g * 32, j, at) : BS::Tile::frag(tb, wcol + g * 32, j, at);
-#pragma unroll
-            for (int f = 0; f < AF; ++f) x[f] = A::frag(ta, wd + f * 32, j, at);
-#pragma unroll
-            for (int f = 0; f < AF; ++f)
-#pragma unroll
-                for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(x[f], y[g], acc[f][g]);
-            if (want_bias) {
-                constexpr int E = 16 / sizeof(T);                   // a lane's K of slab j: E from (2 j + h) E on
-                const u32x4 mine = (wave & 1) ? y[1] : y[0];        // the two waves of these columns take one fragment each
-                if (p.row_weight) {
-                    const float* weight = p.row_weight + k * KE + (2 * j + h) * E;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        if constexpr (sizeof(T) == 2) {
-                            float lo, hi;
-                            unpack2(mine[w], lo, hi, (const T*)nullptr);
-                            bias += lo * weight[2 * w] + hi * weight[2 * w + 1];
-                        } else {
-                            bias += u2f(mine[w]) * weight[w];
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        if constexpr (sizeof(T) == 2) bias = sum_pair(mine[w], bias);
-                        else bias += u2f(mine[w]);
-                    }
-                }
-            }
+    do {
+        long long c0, k_first, k_end, line;                             // columns, K steps, and where the result goes
+        if (ROWS) {
+            const long long tile = uniform(Share::quotient(unit, share.tiles));
+            k_first = unit - tile * share.tiles;
+            k_end = min((long long)share.tiles, k_first + (end - unit));
+            unit += k_end - k_first;
+            c0 = tile * ROW_TILE;
+            const long long segment = Share::segment(0, 0, 0, member, tile);
+            line = segment * ROW_TILE;
+            if (threadIdx.x == 0 && d0 == 0) share.mark(p.ends + tile, segment, k_first, k_end);
+        } else {
+            const long long ctiles = p.cols / ROW_TILE, ksteps = min(p.ksteps, (long long)(count + KE - 1) / KE);
+            const int split = (int)(member / ctiles);
+            c0 = member % ctiles * ROW_TILE;
+            k_first = ksteps * split / p.splits;
+            k_end = ksteps * (split + 1) / p.splits;
+            line = split * p.cols + c0;
         }
-    };
-    auto order = [&] {
-        constexpr int PER = sizeof(T) == 4 ? 4 : 2;                 // LDS reads of a transposed fragment
-        constexpr int READS = AF * PER + 2 * (ROWS ? 1 : PER);
-        interleave<(sizeof(T) == 4 ? 1 : 2) * READS, 4, 2 * AF * (sizeof(T) == 4 ? 4 : 1), READS>();
-    };
-    if (k_first < k_end) stage(a0, b0, k_first);
-    long long k = k_first;
-    for (; k + 1 < k_end; k += 2) {
-        stage_barrier();
-        stage(a1, b1, k + 1);
-        multiply(a0, b0, k);
-        order();
-        stage_barrier();
-        if (k + 2 < k_end) stage(a0, b0, k + 2);
-        multiply(a1, b1, k + 1);
-        order();
-    }
-    if (k < k_end) {
-        stage_barrier();
-        multiply(a0, b0, k);
-        order();
-    }
-    // The result leaves through LDS, 32 columns of the wave at a time, so that a store covers whole lines: a lane holds 4
-    // neighbouring d of one column, and stores of those reach memory in pieces of 32 bytes (25 us of 108 for dW of
-    // 4096 x 32000 x 256).
-    constexpr int WIDTH = 32 * AF, REGION = 32 * WIDTH * 4, ROW_CHUNKS = WIDTH / 4;
-    static_assert(2 * REGION <= A_BYTES && 2 * REGION <= B_BYTES, "two waves' regions per stage");
-    stage_barrier();
-    char* region = (wave < 2 ? a0 : wave < 4 ? b0 : wave < 6 ? a1 : b1) + (wave & 1) * REGION;
-    float* out = p.out + ((long long)split * p.cols + c0 + wcol) * p.dim_pad + d0 + wd;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) {
-        const int col = lane & 31;
+        BS bs;
+        BC bc;
+        // 256 rows of dz times the classes of a stage are one block
+        if (ROWS) bc.init(p.dz + Dz<T>::at(c0, 0, p.piece) * (long long)sizeof(T), 128, 0, ROW_TILE - 1);
+        else bs.init(p.dz, p.piece, c0);
+
+        f32x16 acc[AF][2];
 #pragma unroll
         for (int f = 0; f < AF; ++f)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                vec4f v;
+            for (int g = 0; g < 2; ++g)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = acc[f][g][4 * q + e];
-                const int chunk = f * 8 + 2 * q + h;                // of 4 d; permuted against bank conflicts
-                *reinterpret_cast<vec4f*>(region + (col * ROW_CHUNKS + (chunk ^ (col & 7))) * 16) = v;
-            }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the region is this wave's own
+                for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
+        float bias = 0.0f;
+        const bool want_bias = !ROWS && p.bias_out && d0 == 0;
+
+        auto stage = [&](char* to_a, char* to_b, long long k) {
+            a.stage(to_a, k * KE, p.a_last);
+            if (ROWS) bc.stage(to_b, k * Dz<T>::BLOCK * (long long)sizeof(T));
+            else bs.stage(to_b, k * KE);
+        };
+        auto multiply = [&](const char* ta, const char* tb, long long k) {
+            int at = lane;
+            asm volatile("" : "+v"(at));                            // addresses are formed anew in every stage, see resident_kernel
 #pragma unroll
-        for (int i = 0; i < 32 * ROW_CHUNKS / 64; ++i) {
-            const int at = i * 64 + lane, c = at / ROW_CHUNKS, chunk = at % ROW_CHUNKS;
-            vec4f v = *reinterpret_cast<const vec4f*>(region + (c * ROW_CHUNKS + (chunk ^ (c & 7))) * 16);
-            if (d0 + wd + chunk * 4 < p.dim_pad) {                  // dim_pad is a multiple of four
-                vec4f* to = reinterpret_cast<vec4f*>(out + (long long)(g * 32 + c) * p.dim_pad + chunk * 4);
-                if (p.accumulate) v += *to;
-                *to = v;
+            for (int j = 0; j < 4; ++j) {
+                u32x4 x[AF], y[2];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) y[g] = ROWS ? BC::frag(tb, wcol + g * 32, j, at) : BS::Tile::frag(tb, wcol + g * 32, j, at);
+#pragma unroll
+                for (int f = 0; f < AF; ++f) x[f] = A::frag(ta, wd + f * 32, j, at);
+#pragma unroll
+                for (int f = 0; f < AF; ++f)
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(x[f], y[g], acc[f][g]);
+                if (want_bias) {
+                    constexpr int E = 16 / sizeof(T);                   // a lane's K of slab j: E from (2 j + h) E on
+                    const u32x4 mine = (wave & 1) ? y[1] : y[0];        // the two waves of these columns take one fragment each
+                    if (p.row_weight) {
+                        const float* weight = p.row_weight + k * KE + (2 * j + h) * E;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            if constexpr (sizeof(T) == 2) {
+                                float lo, hi;
+                                unpack2(mine[w], lo, hi, (const T*)nullptr);
+                                bias += lo * weight[2 * w] + hi * weight[2 * w + 1];
+                            } else {
+                                bias += u2f(mine[w]) * weight[w];
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            if constexpr (sizeof(T) == 2) bias = sum_pair(mine[w], bias);
+                            else bias += u2f(mine[w]);
+                        }
+                    }
+                }
             }
+        };
+        auto order = [&] {
+            constexpr int PER = sizeof(T) == 4 ? 4 : 2;                 // LDS reads of a transposed fragment
+            constexpr int READS = AF * PER + 2 * (ROWS ? 1 : PER);
+            interleave<(sizeof(T) == 4 ? 1 : 2) * READS, 4, 2 * AF * (sizeof(T) == 4 ? 4 : 1), READS>();
+        };
+        if (k_first < k_end) stage(a0, b0, k_first);
+        long long k = k_first;
+        for (; k + 1 < k_end; k += 2) {
+            stage_barrier();
+            stage(a1, b1, k + 1);
+            multiply(a0, b0, k);
+            order();
+            stage_barrier();
+            if (k + 2 < k_end) stage(a0, b0, k + 2);
+            multiply(a1, b1, k + 1);
+            order();
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    if (want_bias) {
-        const float sum = bias + __shfl_xor(bias, 32, 64);
-        if (h == 0) p.bias_out[(long long)split * p.cols + c0 + wcol + (wave & 1) * 32 + lane] = sum;
-    }
+        if (k < k_end) {
+            stage_barrier();
+            multiply(a0, b0, k);
+            order();
+        }
+        // The result leaves through LDS, 32 columns of the wave at a time, so that a store covers whole lines: a lane holds 4
+        // neighbouring d of one column, and stores of those reach memory in pieces of 32 bytes (25 us of 108 for dW of
+        // 4096 x 32000 x 256).
+        constexpr int WIDTH = 32 * AF, REGION = 32 * WIDTH * 4, ROW_CHUNKS = WIDTH / 4;
+        static_assert(2 * REGION <= A_BYTES && 2 * REGION <= B_BYTES, "two waves' regions per stage");
+        stage_barrier();
+        int at_lane = lane;
+        asm volatile("" : "+v"(at_lane));                           // formed here, not held over the loops
+        char* region = (wave < 2 ? a0 : wave < 4 ? b0 : wave < 6 ? a1 : b1) + (wave & 1) * REGION;
+        float* out = p.out + (line + wcol) * p.dim_pad + d0 + wd;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int col = at_lane & 31;
+#pragma unroll
+            for (int f = 0; f < AF; ++f)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    vec4f v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[f][g][4 * q + e];
+                    const int chunk = f * 8 + 2 * q + (at_lane >> 5);                // of 4 d; permuted against bank conflicts
+                    *reinterpret_cast<vec4f*>(region + (col * ROW_CHUNKS + (chunk ^ (col & 7))) * 16) = v;
+                }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");          // the region is this wave's own
+#pragma unroll
+            for (int i = 0; i < 32 * ROW_CHUNKS / 64; ++i) {
+                const int at = i * 64 + at_lane, c = at / ROW_CHUNKS, chunk = at % ROW_CHUNKS;
+                vec4f v = *reinterpret_cast<const vec4f*>(region + (c * ROW_CHUNKS + (chunk ^ (c & 7))) * 16);
+                if (d0 + wd + chunk * 4 < p.dim_pad) {                  // dim_pad is a multiple of four
+                    vec4f* to = reinterpret_cast<vec4f*>(out + (long long)(g * 32 + c) * p.dim_pad + chunk * 4);
+                    if (p.accumulate) v += *to;
+                    *to = v;
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        if (want_bias) {
+            const float sum = bias + __shfl_xor(bias, 32, 64);
+            if (h == 0) p.bias_out[line + wcol + (wave & 1) * 32 + lane] = sum;
+        }
+        if (ROWS) __syncthreads();                                      // the next segment writes to LDS what others still read
+    } while (ROWS && unit < end);
 }
 
 // What the sums of the products still lack: 2^-LOG2_DZ, the other operand's power of two, the common factor, and (dF) the
@@ -1362,8 +1412,9 @@ struct FinishArgs {
     unsigned weight_blocks, bias_blocks;
     // rows, behind the last piece: out[row][0 .. dim) of line place[row], zero where there is none
     const float* part_f;
-    long long rows_pad, rows;
-    int splits_f, scaled_w;
+    long long rows;
+    const int2* ends;                   // segments of part_f
+    int scaled_w;
     const int* place;
     const float* row_weight;
     void* dfeatures;
@@ -1418,7 +1469,14 @@ __global__ __launch_bounds__(VT) void finish_kernel(FinishArgs p) {
     const long long row = at / groups;
     if (row >= p.rows) return;
     const int line = p.place[row];
-    finish_line<T>(line < 0 ? nullptr : p.part_f + (long long)line * p.dim_pad, p.rows_pad * p.dim_pad, p.splits_f,
+    const float* part = nullptr;
+    int segments = 0;
+    if (line >= 0) {
+        const int2 ends = p.ends[line / ROW_TILE];
+        segments = ends.y - ends.x + 1;
+        part = p.part_f + ((long long)ends.x * ROW_TILE + line % ROW_TILE) * p.dim_pad;
+    }
+    finish_line<T>(part, (long long)ROW_TILE * p.dim_pad, segments,
                    p.scaled_w ? exponent_of(p.scales->weight_max) : 0,
                    p.scales->common * (p.row_weight && line >= 0 ? p.row_weight[line] : 1.0f), p.dim, (int)(at % groups) * 4,
                    (T*)p.dfeatures, (T*)p.dfeatures + row * p.dim);
@@ -1452,11 +1510,13 @@ int splits_for(long long tiles, long long steps, int slots, int fixed, int limit
     return (int)best;
 }
 
-// Groups that share out the class tiles of a product: one per XCD, unless one would get an eighth more than another, or a
-// run would pass from row tile to row tile (and load its rows again) after fewer than 64 class tiles: a piece of 4096
-// classes for 32768 rows 150 us instead of 171.
+// Groups that share out the class tiles of a product, in each one or more XCDs: as many as there may be with enough tiles
+// for an even division, and with a worker for every row tile unless runs are long (a run that passes from row tile to row
+// tile loads its rows again: a piece of 4096 classes for 32768 rows of 512, 149 us in two groups, 157 in one, 171 in eight).
 int groups_of(long long tiles, long long row_tiles) {
-    return tiles >= 64 && (row_tiles <= SLOTS / 8 || tiles >= 512) ? 8 : 1;
+    int groups = 8;
+    while (groups > 1 && (tiles < 8 * groups || (row_tiles * groups > SLOTS && tiles < 512))) groups /= 2;
+    return groups;
 }
 
 // Everything that follows from the sizes.
@@ -1467,13 +1527,13 @@ struct Plan {
     int row_tile, class_tile, row_tiles;        // of the product
     int workgroups;                             // of the product
     long long piece;                            // classes per piece
-    int pieces, grad_tile, splits_f, splits_w;  // backward; grad_tile: columns of dim per workgroup
+    int pieces, grad_tile, workers_f, splits_w; // backward; grad_tile: columns of dim per workgroup, workers_f: for each
     // saved buffer
     size_t o_count, o_row_of, o_place, o_lse, o_logit, o_prob, o_packed, saved;
     // forward's scratch
-    size_t f_weight, f_bias, f_part, f_entropy, f_flags, forward;
+    size_t f_weight, f_bias, f_part, f_ends, f_entropy, f_flags, forward;
     // backward's scratch
-    size_t b_weight, b_bias, b_row_weight, b_scales, b_scaled_f, b_scaled_w, b_dz, b_part_f, b_part_w, b_part_b, backward;
+    size_t b_weight, b_bias, b_row_weight, b_scales, b_scaled_f, b_scaled_w, b_dz, b_part_f, b_ends, b_part_w, b_part_b, backward;
 };
 
 size_t take(size_t& at, long long bytes) {
@@ -1511,9 +1571,9 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
         if (up(p.dim_pad, t) < up(p.dim_pad, p.grad_tile)) p.grad_tile = t;
     const long long dtiles = (p.dim_pad + p.grad_tile - 1) / p.grad_tile;
     const long long ke = 128 / p.size;
-    // each split writes its own partial result, which costs about as much as eight steps
-    p.splits_f = splits_for(p.rows_pad / ROW_TILE * dtiles, p.piece / ke, GRAD_SLOTS, 8, 64);
-    p.splits_w = splits_for(p.piece / ROW_TILE * dtiles, p.rows_pad / ke, GRAD_SLOTS, 8, 64);
+    p.workers_f = (int)most(1, GRAD_SLOTS / dtiles);
+    // each split writes its own partial result, which costs about as much as eight steps (fp32: as two)
+    p.splits_w = splits_for(p.piece / ROW_TILE * dtiles, p.rows_pad / ke, GRAD_SLOTS, p.size == 4 ? 2 : 8, 64);
 
     size_t at = 0;
     p.o_count = take(at, 4);
@@ -1530,6 +1590,7 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.f_bias = take(at, 4 * p.classes_pad);
     p.f_part = take(at, 8ll * p.row_tile * groups_of(p.classes_pad / p.class_tile, p.row_tiles) *
                             (p.workgroups / groups_of(p.classes_pad / p.class_tile, p.row_tiles) + p.row_tiles));
+    p.f_ends = take(at, 8ll * groups_of(p.classes_pad / p.class_tile, p.row_tiles) * p.row_tiles);
     p.f_entropy = take(at, 4 * p.rows_pad);
     p.f_flags = take(at, p.rows_pad);
     p.forward = at;
@@ -1542,7 +1603,8 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.b_scaled_f = take(at, p.rows_pad * p.dim_pad * p.size);
     p.b_scaled_w = take(at, dtype == OD_DTYPE_BF16 ? p.classes * p.dim_pad * p.size : 0);
     p.b_dz = take(at, p.rows_pad * p.piece * p.size);
-    p.b_part_f = take(at, 4 * p.rows_pad * p.dim_pad * p.splits_f);
+    p.b_part_f = take(at, 4 * (p.workers_f * (long long)ROW_TILE + p.rows_pad) * p.dim_pad);
+    p.b_ends = take(at, 8 * (p.rows_pad / ROW_TILE));
     p.b_part_w = take(at, 4 * p.piece * p.dim_pad * p.splits_w);
     p.b_part_b = take(at, 4 * p.piece * p.splits_w);
     p.backward = at;
@@ -1664,7 +1726,7 @@ template <typename G, bool ROWS>
 int launch_grad(const Call& c, int kernel, const GradArgs& g) {
     const Plan& p = c.p;
     const long long dtiles = (p.dim_pad + p.grad_tile - 1) / p.grad_tile;
-    const dim3 grid((unsigned)(dtiles * (g.cols / ROW_TILE) * g.splits)), block(2 * VT);
+    const dim3 grid((unsigned)(dtiles * (ROWS ? g.splits : g.cols / ROW_TILE * g.splits))), block(2 * VT);
     if (p.grad_tile == 256) OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 4, ROWS>), grid, block, 0, c.stream, g);
     else if (p.grad_tile == 128) OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 2, ROWS>), grid, block, 0, c.stream, g);
     else OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 1, ROWS>), grid, block, 0, c.stream, g);
@@ -1707,6 +1769,7 @@ int forward_typed(const Call& c) {
     a.row_tiles = p.row_tiles;
     a.scale = LOG2E / c.temperature;
     a.part = (float2*)(c.ws + p.f_part);
+    a.ends = (int2*)(c.ws + p.f_ends);
     rc = launch_product<T, false>(c, OD_KERNEL_VOCAB_LSE, a);
     if (rc != OD_OK) return rc;
     TargetArgs t = {};
@@ -1722,11 +1785,10 @@ int forward_typed(const Call& c) {
     t.entropy = entropy;
     t.lists = lists;
     t.part = a.part;
-    t.tiles = a.tiles;
+    t.ends = a.ends;
     t.groups = a.groups;
     t.row_tile = p.row_tile;
     t.row_tiles = p.row_tiles;
-    t.workgroups = p.workgroups;
     t.rows_pad = p.rows_pad;
     t.temperature = c.temperature;
     t.lse2 = (float*)(c.saved + p.o_lse);
@@ -1826,8 +1888,9 @@ int backward_typed(const Call& c) {
             g.a_last = p.classes - 1 - first;
             g.cols = p.rows_pad;
             g.ksteps = p.piece / ke;
-            g.splits = p.splits_f;
+            g.splits = p.workers_f;
             g.out = (float*)(c.ws + p.b_part_f);
+            g.ends = (int2*)(c.ws + p.b_ends);
             g.accumulate = k > 0;
             rc = launch_grad<G, true>(c, OD_KERNEL_VOCAB_GRAD_ROWS, g);
             if (rc != OD_OK) return rc;
@@ -1868,9 +1931,8 @@ int backward_typed(const Call& c) {
         f.scaled_f = scale_f;
         if (c.dfeatures && k == p.pieces - 1) {
             f.part_f = (const float*)(c.ws + p.b_part_f);
-            f.rows_pad = p.rows_pad;
             f.rows = p.rows;
-            f.splits_f = p.splits_f;
+            f.ends = (const int2*)(c.ws + p.b_ends);
             f.scaled_w = scale_w;
             f.place = lists.place;
             f.row_weight = weighted ? row_weight : nullptr;
