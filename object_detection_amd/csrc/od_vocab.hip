@@ -460,7 +460,8 @@ __global__ __launch_bounds__(VT) void prepare_kernel(PrepareArgs p) {
     if (v < p.bias_len)
         p.bias2[v] = v >= p.classes ? -__builtin_inff() : p.bias ? Elem<T>::to_float(((const T*)p.bias)[v]) * p.scale : 0.0f;
     if (p.scales && v == 0) {
-        p.scales->common = p.upstream[0] * (p.temperature / (p.reduction == OD_REDUCE_MEAN ? (float)max(1, *p.lists.count) : 1.0f));
+        const float share = p.reduction == OD_REDUCE_MEAN ? (float)max(1, *p.lists.count) : 1.0f;
+        p.scales->common = p.upstream[0] * (p.temperature / share);
         p.scales->features_max = 0;
         p.scales->weight_max = 0;
     }
@@ -521,8 +522,11 @@ struct Share {
         }
     }
     // worker w has the units [start(w), start(w + 1))
-    __device__ __forceinline__ long long start(long long w) const { return workers == units ? w : quotient(w * units, workers); }
-    static __device__ __forceinline__ long long segment(int group, int per_group, int row_tiles, long long w, long long row_tile) {
+    __device__ __forceinline__ long long start(long long w) const {
+        return workers == units ? w : quotient(w * units, workers);
+    }
+    static __device__ __forceinline__ long long segment(int group, int per_group, int row_tiles, long long w,
+                                                        long long row_tile) {
         return (long long)group * (per_group + row_tiles) + w + row_tile;
     }
     // segment of the tiles [t0, t1) of a row tile
@@ -840,7 +844,9 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
         };
         int next_t = t0, next_k = 0;                                    // what is staged next
         float tile_bias = 0.0f;
-        auto fetch_bias = [&](int t) { if (threadIdx.x < TILE && t < t1) tile_bias = p.bias2[(long long)t * TILE + threadIdx.x]; };
+        auto fetch_bias = [&](int t) {
+            if (threadIdx.x < TILE && t < t1) tile_bias = p.bias2[(long long)t * TILE + threadIdx.x];
+        };
         auto stage_next = [&](char* to) {
             if (next_t >= t1) return;
             if (next_k == 0) cls.init(p.weight, p.weight_pitch, p.first_class + (long long)next_t * TILE, p.last_class);
@@ -853,7 +859,7 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
         };
         auto multiply = [&](const char* now) {
             int at = lane;
-            asm volatile("" : "+v"(at));                            // addresses are formed anew in every stage, see resident_kernel
+            asm volatile("" : "+v"(at));                            // addresses are formed anew, see resident_kernel
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 u32x4 a[2], b[2];
@@ -879,7 +885,7 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
             stage_next(next);
             multiply(now);
             if (++k == ksteps) {
-                if (ksteps == 1) __syncthreads();                       // s_bias was written in this very step
+                if (ksteps == 1) __syncthreads();                   // s_bias was written in this very step
                 const float* bias = s_bias + wc + 16 * h;
                 if (GRAD) store_dz<G, 2, 2>(acc, bias, p.scale, shift, on, out, lane_at, t * TILE + wc);
                 else fold<2, 2>(acc, bias, p.scale, m, s);
@@ -914,7 +920,8 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
                 p.part[segment * TILE + threadIdx.x] =
                     make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top));
             }
-        }    __syncthreads();                                                // the next segment writes to LDS what others still read
+        }
+        __syncthreads();                                            // the next segment writes to LDS what others still read
     }
 }
 
@@ -1296,12 +1303,13 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
         };
         auto multiply = [&](const char* ta, const char* tb, long long k) {
             int at = lane;
-            asm volatile("" : "+v"(at));                            // addresses are formed anew in every stage, see resident_kernel
+            asm volatile("" : "+v"(at));                            // addresses are formed anew, see resident_kernel
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 u32x4 x[AF], y[2];
 #pragma unroll
-                for (int g = 0; g < 2; ++g) y[g] = ROWS ? BC::frag(tb, wcol + g * 32, j, at) : BS::Tile::frag(tb, wcol + g * 32, j, at);
+                for (int g = 0; g < 2; ++g)
+                    y[g] = ROWS ? BC::frag(tb, wcol + g * 32, j, at) : BS::Tile::frag(tb, wcol + g * 32, j, at);
 #pragma unroll
                 for (int f = 0; f < AF; ++f) x[f] = A::frag(ta, wd + f * 32, j, at);
 #pragma unroll
@@ -1395,7 +1403,7 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
             const float sum = bias + __shfl_xor(bias, 32, 64);
             if (h == 0) p.bias_out[line + wcol + (wave & 1) * 32 + lane] = sum;
         }
-        if (ROWS) __syncthreads();                                      // the next segment writes to LDS what others still read
+        if (ROWS) __syncthreads();                                  // the next segment writes to LDS what others still read
     } while (ROWS && unit < end);
 }
 
@@ -1533,7 +1541,8 @@ struct Plan {
     // forward's scratch
     size_t f_weight, f_bias, f_part, f_ends, f_entropy, f_flags, forward;
     // backward's scratch
-    size_t b_weight, b_bias, b_row_weight, b_scales, b_scaled_f, b_scaled_w, b_dz, b_part_f, b_ends, b_part_w, b_part_b, backward;
+    size_t b_weight, b_bias, b_row_weight, b_scales, b_scaled_f, b_scaled_w, b_dz, b_part_f, b_ends, b_part_w, b_part_b;
+    size_t backward;
 };
 
 size_t take(size_t& at, long long bytes) {
@@ -1820,8 +1829,8 @@ int backward_typed(const Call& c) {
     }
     ProductArgs a = {};
     // the bias table: the last piece may reach past the last tile
-    int rc = prepare<T>(c, false, nullptr, p.b_weight, p.b_bias, p.classes_pad + p.piece, weighted ? nullptr : scales, &a.weight,
-                        &a.weight_pitch);
+    int rc = prepare<T>(c, false, nullptr, p.b_weight, p.b_bias, p.classes_pad + p.piece, weighted ? nullptr : scales,
+                        &a.weight, &a.weight_pitch);
     if (rc != OD_OK) return rc;
     a.features = c.saved + p.o_packed;
 

@@ -315,6 +315,22 @@ def test_more_than_one_piece(device, dtype):
     _check_ce(f, w, b, t, "sum")
 
 
+@pytest.mark.parametrize("N,V,D,keep,dtype", [
+    (3000, 700, 64, 0.02, torch.bfloat16),          # one row tile of twelve is left
+    (2600, 2100, 256, 0.4, torch.float16),
+    (2600, 5003, 200, 0.3, torch.float32),
+    (1500, 300, 520, 0.1, torch.bfloat16),          # rows that stream
+    (3000, 4000, 512, 0.5, torch.bfloat16),
+    (140000, 100, 24, 0.97, torch.bfloat16),        # more row tiles than workgroups: runs pass from one to the next
+    (140000, 70, 530, 0.95, torch.float16),
+    (66000, 4100, 16, 0.9, torch.bfloat16),         # the same, in more than one piece
+])
+def test_rows_left_out_in_any_number(device, N, V, D, keep, dtype):
+    f, w, b, t = _inputs(device, N, V, D, dtype, True, seed=31)
+    t[torch.rand((N,), generator=torch.Generator().manual_seed(32)).to(device) >= keep] = -1
+    _check_ce(f, w, b, t)
+
+
 def test_strides_alignment_and_shapes(device):
     f, w, b, t = _inputs(device, 24, 150, 64, torch.bfloat16, True, seed=13)
     want = det_utils.vocabulary_cross_entropy(f, w, t, bias=b, reduction="none")
