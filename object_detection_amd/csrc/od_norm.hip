@@ -351,15 +351,42 @@ __global__ __launch_bounds__(NT) void norm_join_kernel(NormShape s, const double
         stats[b * s.groups + g] = make_double2(mean, 1.0 / sqrt(m2 / ((double)s.pixels * s.per_group) + (double)s.eps));
 }
 
+// part: chunks to be joined here (by every workgroup of the image for itself), or null: stats are there
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(NT) void norm_apply_kernel(NormShape s, const T* __restrict__ x, T* __restrict__ y,
                                                         const void* __restrict__ weight, const void* __restrict__ bias,
-                                                        int pdtype, const double2* __restrict__ stats) {
+                                                        int pdtype, const double2* __restrict__ part, double2* stats) {
+    extern __shared__ double smem[];
     const long long b = blockIdx.x / s.chunks;
-    const long long p0 = (long long)(blockIdx.x % s.chunks) * s.chunk_pixels;
+    const int chunk = blockIdx.x % s.chunks;
+    const long long p0 = chunk * s.chunk_pixels;
     const long long first = (b * s.pixels + p0) * s.channels;
-    apply_window<T, VEC, ACT>(s, x + first, y + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0), stats + b * s.groups,
-                              weight, bias, pdtype);
+    stats += b * s.groups;
+    const double2* mine = stats;
+    if (part) {
+        double2* joined = reinterpret_cast<double2*>(smem + NT);
+        part += b * s.chunks * s.groups;
+        auto count = [&](int k) { return (double)min(s.chunk_pixels, s.pixels - k * s.chunk_pixels); };
+        for (int g0 = 0; g0 < s.groups; g0 += NT) {
+            const Gather all(min(NT, s.groups - g0), s.chunks);
+            const int g = g0 + all.c;
+            const double mean = all.sum(smem, [&](int k) { return count(k) * part[(long long)k * s.groups + g].x; }) /
+                                (double)s.pixels;
+            const double m2 = all.sum(smem, [&](int k) {
+                const double2 v = part[(long long)k * s.groups + g];
+                return v.y + count(k) * s.per_group * (v.x - mean) * (v.x - mean);
+            });
+            if (all.slice == 0 && all.c < all.here) {
+                const double2 v = make_double2(mean, 1.0 / sqrt(m2 / ((double)s.pixels * s.per_group) + (double)s.eps));
+                joined[g] = v;
+                if (chunk == 0) stats[g] = v;
+            }
+        }
+        __syncthreads();
+        mine = joined;
+    }
+    apply_window<T, VEC, ACT>(s, x + first, y + first, 0, s.channels, min(s.chunk_pixels, s.pixels - p0), mine, weight, bias,
+                              pdtype);
 }
 
 // ---- one-launch form: a workgroup takes `slab` channels (whole groups) of one image over all its pixels -----------
@@ -672,16 +699,37 @@ __global__ __launch_bounds__(NT) void norm_bwd_join_kernel(NormShape s, const fl
     if (threadIdx.x < 16 && c < s.channels) sums[b * s.channels + c] = v;
 }
 
+// dgamma, dbeta: the images' channel sums joined, 16 channels per workgroup
+struct ParamGrads {
+    void *dweight, *dbias;
+    int dtype;
+    __device__ __forceinline__ void run(int block, long long batch, int channels, const float2* sums, float2* red) const {
+        const int c = block * 16 + (threadIdx.x & 15);
+        const float2 v = join_rows(sums, batch, channels, c, red);
+        if (threadIdx.x < 16 && c < channels) {
+            if (dbias) store_param(dbias, dtype, c, v.x);
+            if (dweight) store_param(dweight, dtype, c, v.y);
+        }
+    }
+};
+
+// The first `grad_blocks` workgroups form the parameters' gradients, which need the same sums.
 template <typename T, int VEC, int ACT>
 __global__ __launch_bounds__(NT) void norm_bwd_apply_kernel(NormShape s, const T* __restrict__ x, const T* __restrict__ dy,
                                                             T* __restrict__ dx, const double2* __restrict__ stats,
                                                             const void* __restrict__ weight,
                                                             const void* __restrict__ bias, int pdtype,
-                                                            const float2* __restrict__ sums) {
+                                                            const float2* __restrict__ sums, ParamGrads grads,
+                                                            unsigned grad_blocks) {
     extern __shared__ double smem[];
     float2* avg = reinterpret_cast<float2*>(smem);
-    const long long b = blockIdx.x / s.chunks;
-    const int chunk = blockIdx.x % s.chunks;
+    if (blockIdx.x < grad_blocks) {
+        grads.run(blockIdx.x, s.batch, s.channels, sums, avg);
+        return;
+    }
+    const unsigned block = blockIdx.x - grad_blocks;
+    const long long b = block / s.chunks;
+    const int chunk = block % s.chunks;
     group_averages(sums + b * s.channels, s.groups, s.per_group, 0, (double)s.pixels * s.per_group, weight, pdtype,
                    [&](int g, float a, float q) { avg[g] = make_float2(a, q); });
     __syncthreads();
@@ -719,17 +767,10 @@ __global__ __launch_bounds__(NT) void norm_bwd_small_kernel(NormShape s, int sla
     }
 }
 
-// dgamma, dbeta: the images' channel sums joined
 __global__ __launch_bounds__(NT) void norm_param_grads_kernel(long long batch, int channels, const float2* __restrict__ sums,
-                                                              void* __restrict__ dweight, void* __restrict__ dbias,
-                                                              int pdtype) {
+                                                              ParamGrads grads) {
     __shared__ float2 red[NT];
-    const int c = blockIdx.x * 16 + (threadIdx.x & 15);
-    const float2 v = join_rows(sums, batch, channels, c, red);
-    if (threadIdx.x < 16 && c < channels) {
-        if (dbias) store_param(dbias, pdtype, c, v.x);
-        if (dweight) store_param(dweight, pdtype, c, v.y);
-    }
+    grads.run(blockIdx.x, batch, channels, sums, red);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------
@@ -749,6 +790,12 @@ int slab_channels(int channels, int per_group, int vec, int size) {
 // up to 32 (22 us against 25 at 64).
 bool small_form(const NormShape& s, int slab, int size, int limit) { return s.pixels * slab * size <= limit; }
 
+// Statistics of an image's chunks, 16 bytes each, up to which the workgroups that normalise join them themselves: a launch
+// less for the host, which bounds a training step on such maps (77 -> 72 us with the parameters' gradients in the launch of
+// dx).  On the device the two are even at 1024 of them (16 x 64 x 64 x 256 in 32 groups, forward 23.8 us against 23.9), near
+// it at 2160 (14.6 against 14.1), not at 4096 (17.8 against 15.1).
+constexpr int APPLY_JOINS = 2304;
+
 NormShape shape_of(long long batch, long long pixels, int channels, int groups, float eps, int size) {
     NormShape s;
     s.batch = batch;
@@ -757,8 +804,8 @@ NormShape shape_of(long long batch, long long pixels, int channels, int groups, 
     s.groups = groups;
     s.per_group = channels / groups;
     s.eps = eps;
-    // workgroups of at least 64 KiB (a smaller one is mostly its own start: 39 us instead of 15 to normalise 16 x 64 x 64 x 256 bf16 by 2048 of 16 KiB),
-    // two to eight per compute unit, at most MAX_CHUNKS per image, at least 16 pixels each
+    // workgroups of at least 64 KiB (a smaller one is mostly its own start: 39 us instead of 15 to normalise
+    // 16 x 64 x 64 x 256 bf16 by 2048 of 16 KiB), two to eight per compute unit, at most MAX_CHUNKS per image, at least 16 pixels each
     long long blocks = (long long)((double)batch * pixels * channels * size / 65536.0);
     blocks = blocks < 512 ? 512 : blocks > 2048 ? 2048 : blocks;
     long long chunks = batch > 0 ? (blocks + batch - 1) / batch : 1;
@@ -799,7 +846,8 @@ int forward_typed(const FwdCall& c) {
     T* y = (T*)c.y;
     if (small_form(c.s, slab, sizeof(T), 64 << 10)) {
         const long long grid = c.s.batch * ((c.s.channels + slab - 1) / slab);
-        const size_t lds = (size_t)(slab + slab / c.s.per_group) * sizeof(double2) + NT * sizeof(double) + 3 * NT * VEC * sizeof(float);
+        const size_t lds = (size_t)(slab + slab / c.s.per_group) * sizeof(double2) + NT * sizeof(double) +
+                           3 * NT * VEC * sizeof(float);
         OD_LAUNCH_KERNEL(OD_KERNEL_NORM_APPLY, (norm_small_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT), lds, c.stream,
                          c.s, slab, x, y, c.weight, c.bias, c.pdtype, c.stats);
         return OD_OK;
@@ -808,11 +856,15 @@ int forward_typed(const FwdCall& c) {
     const long long grid = c.s.batch * c.s.chunks;
     OD_LAUNCH_KERNEL(OD_KERNEL_NORM_STATS, (norm_stats_kernel<T, VEC>), dim3((unsigned)grid), dim3(NT),
                      c.s.channels * sizeof(double2) + NT * sizeof(double) + 3 * NT * VEC * sizeof(float), c.stream, c.s, x, part);
-    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(c.s.batch * ((c.s.groups + 7) / 8))), dim3(NT), 0, c.stream, c.s,
-                       (const double2*)part, c.stats);
-    OD_LAUNCH_CHECK();
-    OD_LAUNCH_KERNEL(OD_KERNEL_NORM_APPLY, (norm_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT), 0, c.stream, c.s, x,
-                     y, c.weight, c.bias, c.pdtype, (const double2*)c.stats);
+    const bool joined = c.s.chunks * c.s.groups > APPLY_JOINS;
+    if (joined) {
+        hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(c.s.batch * ((c.s.groups + 7) / 8))), dim3(NT), 0, c.stream, c.s,
+                           (const double2*)part, c.stats);
+        OD_LAUNCH_CHECK();
+    }
+    OD_LAUNCH_KERNEL(OD_KERNEL_NORM_APPLY, (norm_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
+                     joined ? 0 : NT * sizeof(double) + c.s.groups * sizeof(double2), c.stream, c.s, x, y, c.weight, c.bias,
+                     c.pdtype, joined ? (const double2*)nullptr : (const double2*)part, c.stats);
     return OD_OK;
 }
 
@@ -832,6 +884,8 @@ int backward_typed(const BwdCall& c) {
     const T *x = (const T*)c.x, *dy = (const T*)c.dy;
     T* dx = (T*)c.dx;
     float2* sums = (float2*)c.ws;
+    const ParamGrads grads = {c.dweight, c.dbias, c.pdtype};
+    const unsigned grad_blocks = c.dweight || c.dbias ? (c.s.channels + 15) / 16 : 0;
     if (small_form(c.s, slab, sizeof(T), 32 << 10)) {
         const long long grid = c.s.batch * ((c.s.channels + slab - 1) / slab);
         const size_t lds = NT * sizeof(double) + (2 * NT * VEC + 4 * (size_t)slab) * sizeof(float);
@@ -841,19 +895,22 @@ int backward_typed(const BwdCall& c) {
         float2* part = sums + c.s.batch * c.s.channels;
         const long long grid = c.s.batch * c.s.chunks;
         OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_SUMS, (norm_bwd_sums_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
-                         NT * sizeof(double) + 2 * NT * VEC * sizeof(float), c.stream, c.s, x, dy, c.stats, c.weight, c.bias, c.pdtype, part);
+                         NT * sizeof(double) + 2 * NT * VEC * sizeof(float), c.stream, c.s, x, dy, c.stats, c.weight, c.bias,
+                         c.pdtype, part);
         hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(c.s.batch * ((c.s.channels + 15) / 16))), dim3(NT), 0, c.stream,
                            c.s, (const float2*)part, sums);
         OD_LAUNCH_CHECK();
         if (dx) {
-            OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_APPLY, (norm_bwd_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid), dim3(NT),
-                             2 * (size_t)c.s.groups * sizeof(float), c.stream, c.s, x, dy, dx, c.stats, c.weight, c.bias,
-                             c.pdtype, (const float2*)sums);
+            const size_t lds = 2 * sizeof(float) * (size_t)(c.s.groups > NT ? c.s.groups : NT);
+            OD_LAUNCH_KERNEL(OD_KERNEL_NORM_BWD_APPLY, (norm_bwd_apply_kernel<T, VEC, ACT>), dim3((unsigned)grid + grad_blocks),
+                             dim3(NT), lds, c.stream, c.s, x, dy, dx, c.stats, c.weight, c.bias, c.pdtype, (const float2*)sums,
+                             grads, grad_blocks);
+            return OD_OK;
         }
     }
-    if (c.dweight || c.dbias) {
-        hipLaunchKernelGGL(norm_param_grads_kernel, dim3((c.s.channels + 15) / 16), dim3(NT), 0, c.stream, c.s.batch,
-                           c.s.channels, (const float2*)sums, c.dweight, c.dbias, c.pdtype);
+    if (grad_blocks > 0) {
+        hipLaunchKernelGGL(norm_param_grads_kernel, dim3(grad_blocks), dim3(NT), 0, c.stream, c.s.batch, c.s.channels,
+                           (const float2*)sums, grads);
         OD_LAUNCH_CHECK();
     }
     return OD_OK;
@@ -909,22 +966,22 @@ extern "C" int od_group_norm_act_forward(const void* x, int32_t dtype, int64_t b
     if (!x || !y || !stats || ((uintptr_t)stats & 15) || !workspace || ((uintptr_t)workspace & 255)) return OD_ERR_ARG;
     if (((uintptr_t)x | (uintptr_t)y) % elem_size(dtype)) return OD_ERR_ARG;
     if (workspace_bytes < od_group_norm_act_workspace_bytes(batch, pixels, channels, groups)) return OD_ERR_WORKSPACE;
-    const FwdCall call = {shape_of(batch, pixels, channels, groups, eps, elem_size(dtype)), x, weight, bias, y, param_dtype, (double2*)stats,
-                          workspace, (hipStream_t)stream};
+    const FwdCall call = {shape_of(batch, pixels, channels, groups, eps, elem_size(dtype)), x, weight, bias, y, param_dtype,
+                          (double2*)stats, workspace, (hipStream_t)stream};
     OD_NORM_DISPATCH(forward_typed, call, vector_width(dtype, channels, (uintptr_t)x | (uintptr_t)y));
 }
 
 extern "C" int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int64_t batch, int64_t pixels,
                                           int32_t channels, int32_t groups, const void* weight, const void* bias,
-                                          int32_t param_dtype, int32_t activation, const double* stats, void* dx, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
-                                          void* stream) {
+                                          int32_t param_dtype, int32_t activation, const double* stats, void* dx,
+                                          void* dweight, void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
     const int rc = check_shape(dtype, batch, pixels, channels, groups, param_dtype, activation);
     if (rc != OD_OK) return rc;
     if (batch == 0 || pixels == 0) return OD_OK;
     if (!x || !dy || !stats || ((uintptr_t)stats & 15) || !workspace || ((uintptr_t)workspace & 255)) return OD_ERR_ARG;
     if (((uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx) % elem_size(dtype)) return OD_ERR_ARG;
     if (workspace_bytes < od_group_norm_act_workspace_bytes(batch, pixels, channels, groups)) return OD_ERR_WORKSPACE;
-    const BwdCall call = {shape_of(batch, pixels, channels, groups, 0.0f, elem_size(dtype)), x, dy, weight, bias, dx, dweight, dbias,
-                          param_dtype, (const double2*)stats, workspace, (hipStream_t)stream};
+    const BwdCall call = {shape_of(batch, pixels, channels, groups, 0.0f, elem_size(dtype)), x, dy, weight, bias, dx, dweight,
+                          dbias, param_dtype, (const double2*)stats, workspace, (hipStream_t)stream};
     OD_NORM_DISPATCH(backward_typed, call, vector_width(dtype, channels, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx));
 }
