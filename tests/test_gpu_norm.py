@@ -106,6 +106,13 @@ def test_group_norm_act_matches_definition(device, B, C, H, W, groups, act, affi
            beta, act)
 
 
+def test_many_images_of_many_groups(device):
+    """More groups than threads, whose few chunks an image's own workgroups join."""
+    x, dy, gamma, beta = _case(device, 300, 288, 33, 33, 288, "silu", torch.bfloat16, True, seed=17)
+    _check(x.contiguous(memory_format=torch.channels_last), dy.contiguous(memory_format=torch.channels_last), 288, gamma, beta,
+           "silu")
+
+
 @pytest.mark.parametrize("pdtype", [torch.float16, torch.bfloat16])
 def test_parameter_types_and_memory_orders(device, pdtype):
     x, dy, gamma, beta = _case(device, 2, 64, 12, 10, 8, "relu", torch.bfloat16, True, seed=5, pdtype=pdtype)
