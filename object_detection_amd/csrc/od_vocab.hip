@@ -787,13 +787,16 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
     }
 }
 
-// Wider rows: both operands stream through LDS in stages of 128 bytes of K.
-template <typename T, bool GRAD>
+// Wider rows: both operands stream through LDS in stages of 128 bytes of K.  Four waves take 64 x 64 each of tiles of 128
+// classes, or 32 x 32 of tiles of 32 where the wide ones would leave half the compute units without work (108 x 5992 x 736
+// fp32: 54 us by 48 workgroups of wide tiles).
+template <typename T, bool GRAD, int CT>
 __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
     typedef typename GradOf<T>::type G;
-    __shared__ __align__(1024) char lds0[2 * STAGE], lds1[2 * STAGE];       // two stages of (classes, rows)
-    __shared__ float2 joined[2][TILE];
-    __shared__ __align__(16) float s_bias[TILE];
+    constexpr int F = CT == TILE ? 2 : 1, CLASS_STAGE = CT * 128;           // F x F fragments of 32 x 32 per wave
+    __shared__ __align__(1024) char lds0[CLASS_STAGE + STAGE], lds1[CLASS_STAGE + STAGE];   // two stages of (classes, rows)
+    __shared__ float2 joined[F][TILE];
+    __shared__ __align__(16) float s_bias[CT];
     const int count = *p.count;
     if (count == 0) return;
     const int per_group = gridDim.x / p.groups;
@@ -804,10 +807,10 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
     long long unit = uniform(share.start(worker));
     const long long end = uniform(share.start(worker + 1));
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
-    const int wc = (wave & 1) * 64, wr = (wave >> 1) * 64;          // this wave's classes and rows within the tile
+    const int wc = F == 2 ? (wave & 1) * 64 : 0, wr = F == 2 ? (wave >> 1) * 64 : wave * 32;   // its classes and rows of a tile
     constexpr int KE = 128 / sizeof(T);
     const int ksteps = p.dim_pad / KE;
-    typedef ChunkedOperand<TILE, VT, true> Classes;
+    typedef ChunkedOperand<CT, VT, true> Classes;
     typedef ChunkedOperand<TILE, VT, false> Rows;
     while (unit < end) {
         const long long row_tile = uniform(Share::quotient(unit, share.tiles)), r0 = row_tile * TILE;
@@ -818,10 +821,10 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
         Classes cls;
         rows.init(p.features, (long long)p.dim_pad * sizeof(T), r0, r0 + TILE);
 
-        float m[2], s[2], shift[2];
-        bool on[2];
+        float m[F], s[F], shift[F];
+        bool on[F];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < F; ++g) {
             m[g] = LOWEST;
             s[g] = 0.0f;
             if (GRAD) {
@@ -833,25 +836,25 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
         G* const out = (G*)p.dz + Dz<G>::at(r0, 0, p.piece);
         const uint32_t lane_at = (wr + (lane & 31)) * Dz<G>::CLASSES + 16 * h;
 
-        f32x16 acc[2][2];
+        f32x16 acc[F][F];
         auto clear = [&] {
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
+            for (int f = 0; f < F; ++f)
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
+                for (int g = 0; g < F; ++g)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
         };
         int next_t = t0, next_k = 0;                                    // what is staged next
         float tile_bias = 0.0f;
         auto fetch_bias = [&](int t) {
-            if (threadIdx.x < TILE && t < t1) tile_bias = p.bias2[(long long)t * TILE + threadIdx.x];
+            if (threadIdx.x < CT && t < t1) tile_bias = p.bias2[(long long)t * CT + threadIdx.x];
         };
         auto stage_next = [&](char* to) {
             if (next_t >= t1) return;
-            if (next_k == 0) cls.init(p.weight, p.weight_pitch, p.first_class + (long long)next_t * TILE, p.last_class);
+            if (next_k == 0) cls.init(p.weight, p.weight_pitch, p.first_class + (long long)next_t * CT, p.last_class);
             cls.stage(to, (long long)next_k * 128);
-            rows.stage(to + STAGE, (long long)next_k * 128);
+            rows.stage(to + CLASS_STAGE, (long long)next_k * 128);
             if (++next_k == ksteps) {
                 next_k = 0;
                 ++next_t;
@@ -862,33 +865,33 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
             asm volatile("" : "+v"(at));                            // addresses are formed anew, see resident_kernel
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                u32x4 a[2], b[2];
+                u32x4 a[F], b[F];
 #pragma unroll
-                for (int f = 0; f < 2; ++f) {
+                for (int f = 0; f < F; ++f) {
                     a[f] = Classes::frag(now, wc + f * 32, j, at);
-                    b[f] = Rows::frag(now + STAGE, wr + f * 32, j, at);
+                    b[f] = Rows::frag(now + CLASS_STAGE, wr + f * 32, j, at);
                 }
 #pragma unroll
-                for (int f = 0; f < 2; ++f)
+                for (int f = 0; f < F; ++f)
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(a[f], b[g], acc[f][g]);
+                    for (int g = 0; g < F; ++g) acc[f][g] = Mma<T>::run(a[f], b[g], acc[f][g]);
             }
-            interleave<8, 4, 4 * (sizeof(T) == 4 ? 4 : 1), 4>();
+            interleave<4 * F, 4, F * F * (sizeof(T) == 4 ? 4 : 1), 2 * F>();
         };
         // The bias of a tile is fetched ahead of the tile's first stage (waiting for it later would wait for the stages behind
         // it as well) and written to LDS in its first step.  The two stages are variables of their own, used by turns in
         // straight code: the compiler then knows that reading one need not wait for the loads into the other.
         auto step = [&](const char* now, char* next, int& t, int& k) {
             stage_barrier();
-            if (k == 0 && threadIdx.x < TILE) s_bias[threadIdx.x] = tile_bias;
+            if (k == 0 && threadIdx.x < CT) s_bias[threadIdx.x] = tile_bias;
             if (k + 1 == ksteps) fetch_bias(t + 1);
             stage_next(next);
             multiply(now);
             if (++k == ksteps) {
                 if (ksteps == 1) __syncthreads();                   // s_bias was written in this very step
                 const float* bias = s_bias + wc + 16 * h;
-                if (GRAD) store_dz<G, 2, 2>(acc, bias, p.scale, shift, on, out, lane_at, t * TILE + wc);
-                else fold<2, 2>(acc, bias, p.scale, m, s);
+                if (GRAD) store_dz<G, F, F>(acc, bias, p.scale, shift, on, out, lane_at, t * CT + wc);
+                else fold<F, F>(acc, bias, p.scale, m, s);
                 clear();
                 k = 0;
                 ++t;
@@ -905,20 +908,20 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
         }
         if (steps & 1) step(lds0, lds1, t, k);
         if (!GRAD) {
-            // a row's classes lie in two lanes and two waves
+            // a row's classes lie in two lanes and, of a wide tile, two waves
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
+            for (int g = 0; g < F; ++g) {
                 join_halves(m[g], s[g]);
-                if (h == 0) joined[wave & 1][wr + g * 32 + lane] = make_float2(m[g], s[g]);
+                if (h == 0) joined[F == 2 ? wave & 1 : 0][wr + g * 32 + lane] = make_float2(m[g], s[g]);
             }
             __syncthreads();
             const long long segment = Share::segment(group, per_group, p.row_tiles, worker, row_tile);
             if (threadIdx.x == 0) share.mark(p.ends + (long long)group * p.row_tiles + row_tile, segment, t0, t1);
             if (threadIdx.x < TILE) {
-                const float2 a = joined[0][threadIdx.x], b = joined[1][threadIdx.x];
+                const float2 a = joined[0][threadIdx.x], b = joined[F - 1][threadIdx.x];
                 const float top = fmaxf(a.x, b.x);
                 p.part[segment * TILE + threadIdx.x] =
-                    make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top));
+                    F == 1 ? a : make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top));
             }
         }
         __syncthreads();                                            // the next segment writes to LDS what others still read
@@ -1196,6 +1199,29 @@ struct DzOperand {
     }
 };
 
+// Four elements of a result line: the sums of n partial results, and what they still lack: 2^-LOG2_DZ, the other operand's
+// power of two, the common factor.  The powers of two are applied apart, so that no intermediate factor leaves the range.
+__device__ __forceinline__ vec4f sum_parts(const float* part, long long step, int n) {
+    vec4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) v += *reinterpret_cast<const vec4f*>(part + s * step);
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void finish_line(vec4f v, int exponent, float factor, int dim, int d, T* out, T* line) {
+    v *= ldexpf(1.0f, -exponent - GradOf<T>::LOG2_DZ);
+    v *= factor;
+    T* to = line + d;
+    if (dim % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0) {
+        const float f[4] = {v.x, v.y, v.z, v.w};
+        store_vec<T, 4>(to, f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (d + i < dim) to[i] = Elem<T>::from_float(v[i]);
+    }
+}
+
 struct GradArgs {
     const char* a;                      // [K][a_pitch bytes], dim_pad columns: weight rows of the piece, or features
     long long a_pitch, a_last;          // last readable K row
@@ -1211,6 +1237,11 @@ struct GradArgs {
     int accumulate;
     float* bias_out;                    // [splits][cols] weighted sums of dz over K, or null
     const float* row_weight;            // [rows_pad], or null: ones
+    // DIRECT: [classes][dim], instead of `out`
+    void* result;
+    int bf16_result, dim, scaled;
+    long long classes;
+    const Scales* scales;
 };
 
 // dF: the K steps of the valid rows' tiles, shared out as in Share.  A segment's sums are a partial result of their own,
@@ -1235,7 +1266,8 @@ __device__ __forceinline__ float sum_pair(uint32_t w, float c) {
 // otherwise columns are classes and K runs over the valid rows (dW).  A workgroup of eight waves takes 64 AF columns d and
 // 256 columns of the result, 32 AF x 64 per wave: at AF = 4 a stage of 64 KiB feeds 2048 cycles of the matrix units, half
 // of what L2 gives per cycle.
-template <typename T, int AF, bool ROWS>
+// DIRECT: dW of one split, written as it leaves.
+template <typename T, int AF, bool ROWS, bool DIRECT>
 __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
     constexpr int THREADS = 2 * VT, DT = 64 * AF;
     constexpr int A_BYTES = DT * 128, B_BYTES = ROW_TILE * 128;
@@ -1347,22 +1379,30 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
             interleave<(sizeof(T) == 4 ? 1 : 2) * READS, 4, 2 * AF * (sizeof(T) == 4 ? 4 : 1), READS>();
         };
         if (k_first < k_end) stage(a0, b0, k_first);
-        long long k = k_first;
-        for (; k + 1 < k_end; k += 2) {
-            stage_barrier();
-            stage(a1, b1, k + 1);
-            multiply(a0, b0, k);
-            order();
-            stage_barrier();
-            if (k + 2 < k_end) stage(a0, b0, k + 2);
-            multiply(a1, b1, k + 1);
-            order();
-        }
-        if (k < k_end) {
-            stage_barrier();
-            multiply(a0, b0, k);
-            order();
-        }
+        auto sweep = [&](auto works) {
+            auto work = [&](const char* ta, const char* tb, long long k) {
+                if constexpr (decltype(works)::value) {
+                    multiply(ta, tb, k);
+                    order();
+                }
+            };
+            long long k = k_first;
+            for (; k + 1 < k_end; k += 2) {
+                stage_barrier();
+                stage(a1, b1, k + 1);
+                work(a0, b0, k);
+                stage_barrier();
+                if (k + 2 < k_end) stage(a0, b0, k + 2);
+                work(a1, b1, k + 1);
+            }
+            if (k < k_end) {
+                stage_barrier();
+                work(a0, b0, k);
+            }
+        };
+        // a wave without a valid row only takes part in the staging
+        if (!ROWS || c0 + wcol < count) sweep(std::true_type());
+        else sweep(std::false_type());
         // The result leaves through LDS, 32 columns of the wave at a time, so that a store covers whole lines: a lane holds 4
         // neighbouring d of one column, and stores of those reach memory in pieces of 32 bytes (25 us of 108 for dW of
         // 4096 x 32000 x 256).
@@ -1373,6 +1413,8 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
         asm volatile("" : "+v"(at_lane));                           // formed here, not held over the loops
         char* region = (wave < 2 ? a0 : wave < 4 ? b0 : wave < 6 ? a1 : b1) + (wave & 1) * REGION;
         float* out = p.out + (line + wcol) * p.dim_pad + d0 + wd;
+        const int exponent = DIRECT && p.scaled ? exponent_of(p.scales->features_max) : 0;
+        const float common = DIRECT ? p.scales->common : 0.0f;
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             const int col = at_lane & 31;
@@ -1391,7 +1433,15 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
             for (int i = 0; i < 32 * ROW_CHUNKS / 64; ++i) {
                 const int at = i * 64 + at_lane, c = at / ROW_CHUNKS, chunk = at % ROW_CHUNKS;
                 vec4f v = *reinterpret_cast<const vec4f*>(region + (c * ROW_CHUNKS + (chunk ^ (c & 7))) * 16);
-                if (d0 + wd + chunk * 4 < p.dim_pad) {                  // dim_pad is a multiple of four
+                if constexpr (DIRECT) {
+                    const long long cls = c0 + wcol + g * 32 + c;
+                    const int d = d0 + wd + chunk * 4;
+                    if (cls < p.classes && d < p.dim) {
+                        if (sizeof(T) == 2 && p.bf16_result)
+                            finish_line<bf16_t>(v, exponent, common, p.dim, d, (bf16_t*)p.result, (bf16_t*)p.result + cls * p.dim);
+                        else finish_line<T>(v, exponent, common, p.dim, d, (T*)p.result, (T*)p.result + cls * p.dim);
+                    }
+                } else if (d0 + wd + chunk * 4 < p.dim_pad) {           // dim_pad is a multiple of four
                     vec4f* to = reinterpret_cast<vec4f*>(out + (long long)(g * 32 + c) * p.dim_pad + chunk * 4);
                     if (p.accumulate) v += *to;
                     *to = v;
@@ -1407,8 +1457,7 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
     } while (ROWS && unit < end);
 }
 
-// What the sums of the products still lack: 2^-LOG2_DZ, the other operand's power of two, the common factor, and (dF) the
-// row's weight.  The powers of two are applied apart, so that no intermediate factor leaves the range.
+// The partial results of the gradients, joined.
 struct FinishArgs {
     const Scales* scales;
     int dim, dim_pad;
@@ -1428,28 +1477,6 @@ struct FinishArgs {
     void* dfeatures;
 };
 
-// four elements of a result line
-template <typename T>
-__device__ __forceinline__ void finish_line(const float* part, long long step, int splits, int exponent, float factor, int dim,
-                                            int d, T* out, T* line) {
-    vec4f v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (part) {
-#pragma unroll 4
-        for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const vec4f*>(part + s * step + d);
-        v *= ldexpf(1.0f, -exponent - GradOf<T>::LOG2_DZ);
-        v *= factor;
-    }
-    T* to = line + d;
-    if (dim % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0) {
-        const float f[4] = {v.x, v.y, v.z, v.w};
-        store_vec<T, 4>(to, f);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (d + i < dim) to[i] = Elem<T>::from_float(v[i]);
-    }
-}
-
 template <typename T>
 __global__ __launch_bounds__(VT) void finish_kernel(FinishArgs p) {
     const unsigned groups = (p.dim + 3) / 4;
@@ -1458,9 +1485,10 @@ __global__ __launch_bounds__(VT) void finish_kernel(FinishArgs p) {
         const unsigned at = block * VT + threadIdx.x;
         const long long c = at / groups;
         if (c >= p.classes) return;
-        finish_line<T>(p.part_w + c * p.dim_pad, p.piece * p.dim_pad, p.splits_w,
-                       p.scaled_f ? exponent_of(p.scales->features_max) : 0, p.scales->common, p.dim, (int)(at % groups) * 4,
-                       (T*)p.dweight, (T*)p.dweight + c * p.dim);
+        const int d = (int)(at % groups) * 4;
+        finish_line<T>(sum_parts(p.part_w + c * p.dim_pad + d, p.piece * p.dim_pad, p.splits_w),
+                       p.scaled_f ? exponent_of(p.scales->features_max) : 0, p.scales->common, p.dim, d, (T*)p.dweight,
+                       (T*)p.dweight + c * p.dim);
         return;
     }
     block -= p.weight_blocks;
@@ -1476,18 +1504,16 @@ __global__ __launch_bounds__(VT) void finish_kernel(FinishArgs p) {
     const unsigned at = block * VT + threadIdx.x;
     const long long row = at / groups;
     if (row >= p.rows) return;
-    const int line = p.place[row];
-    const float* part = nullptr;
-    int segments = 0;
+    const int line = p.place[row], d = (int)(at % groups) * 4;
+    vec4f v = {0.0f, 0.0f, 0.0f, 0.0f};
     if (line >= 0) {
         const int2 ends = p.ends[line / ROW_TILE];
-        segments = ends.y - ends.x + 1;
-        part = p.part_f + ((long long)ends.x * ROW_TILE + line % ROW_TILE) * p.dim_pad;
+        v = sum_parts(p.part_f + ((long long)ends.x * ROW_TILE + line % ROW_TILE) * p.dim_pad + d,
+                      (long long)ROW_TILE * p.dim_pad, ends.y - ends.x + 1);
     }
-    finish_line<T>(part, (long long)ROW_TILE * p.dim_pad, segments,
-                   p.scaled_w ? exponent_of(p.scales->weight_max) : 0,
-                   p.scales->common * (p.row_weight && line >= 0 ? p.row_weight[line] : 1.0f), p.dim, (int)(at % groups) * 4,
-                   (T*)p.dfeatures, (T*)p.dfeatures + row * p.dim);
+    finish_line<T>(v, p.scaled_w ? exponent_of(p.scales->weight_max) : 0,
+                   line < 0 ? 0.0f : p.scales->common * (p.row_weight ? p.row_weight[line] : 1.0f), p.dim, d, (T*)p.dfeatures,
+                   (T*)p.dfeatures + row * p.dim);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------
@@ -1537,7 +1563,7 @@ struct Plan {
     long long piece;                            // classes per piece
     int pieces, grad_tile, workers_f, splits_w; // backward; grad_tile: columns of dim per workgroup, workers_f: for each
     // saved buffer
-    size_t o_count, o_row_of, o_place, o_lse, o_logit, o_prob, o_packed, saved;
+    size_t o_count, o_row_of, o_place, o_lse, o_logit, o_prob, o_packed, o_weight, saved;
     // forward's scratch
     size_t f_weight, f_bias, f_part, f_ends, f_entropy, f_flags, forward;
     // backward's scratch
@@ -1564,11 +1590,11 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.dim_pad = (int)(bytes / p.size);
     p.slabs = bytes <= 1024 ? (int)(bytes / 32) : 0;
     p.row_tile = p.slabs > 0 && p.slabs <= 16 ? 256 : 128;
-    p.class_tile = p.slabs == 0 ? TILE : p.slabs <= 16 ? 64 : 32;
+    p.row_tiles = (int)((most(rows, 1) + p.row_tile - 1) / p.row_tile);
+    p.class_tile = p.slabs == 0 ? (p.row_tiles * (p.classes_pad / TILE) < SLOTS / 4 ? 32 : TILE) : p.slabs <= 16 ? 64 : 32;
     // one thread per 16 bytes of both packed operands, fewer than 2^32 threads in a launch
     if (most(p.rows_pad, p.classes_pad) * p.dim_pad * p.size / 16 > (1ll << 30)) return false;
     p.n = top > 0 ? top : 1;
-    p.row_tiles = (int)((most(rows, 1) + p.row_tile - 1) / p.row_tile);
     p.workgroups = (int)least(SLOTS, up(p.row_tiles * (p.classes_pad / p.class_tile), 8));
     long long piece = most(ROW_TILE, DZ_BYTES / (p.rows_pad * p.size) / ROW_TILE * ROW_TILE);
     p.pieces = (int)((p.classes_pad + piece - 1) / piece);
@@ -1592,10 +1618,11 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.o_logit = take(at, 4 * p.rows_pad * p.n);
     p.o_prob = take(at, top > 0 ? 4 * p.rows_pad * p.n : 0);
     p.o_packed = take(at, p.rows_pad * p.dim_pad * p.size);
+    p.o_weight = take(at, dim != p.dim_pad ? p.classes * p.dim_pad * p.size : 0);
     p.saved = at;
 
     at = 0;
-    p.f_weight = take(at, p.classes * p.dim_pad * p.size);
+    p.f_weight = take(at, dim == p.dim_pad ? p.classes * p.dim_pad * p.size : 0);
     p.f_bias = take(at, 4 * p.classes_pad);
     p.f_part = take(at, 8ll * p.row_tile * groups_of(p.classes_pad / p.class_tile, p.row_tiles) *
                             (p.workgroups / groups_of(p.classes_pad / p.class_tile, p.row_tiles) + p.row_tiles));
@@ -1605,7 +1632,7 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.forward = at;
 
     at = 0;
-    p.b_weight = take(at, p.classes * p.dim_pad * p.size);
+    p.b_weight = take(at, dim == p.dim_pad ? p.classes * p.dim_pad * p.size : 0);
     p.b_bias = take(at, 4 * p.classes_pad + 4 * p.piece);
     p.b_row_weight = take(at, 4 * p.rows_pad);
     p.b_scales = take(at, sizeof(Scales));
@@ -1688,11 +1715,15 @@ int prepare(const Call& c, bool with_features, const unsigned char* flags, size_
     *rows = (const char*)c.weight;
     *pitch = c.weight_pitch * p.size;
     if (!weight_in_place(p, c.weight, c.weight_pitch)) {
-        a.weight = c.weight;
-        a.weight_pitch = c.weight_pitch;
-        a.packed_weight = c.ws + weight_at;
-        a.weight_blocks = blocks_of(p.classes * row_chunks, VT);
-        *rows = c.ws + weight_at;
+        const bool keep = p.dim != p.dim_pad;                       // for the backward pass, which then need not pack again
+        char* packed = keep ? c.saved + p.o_weight : c.ws + weight_at;
+        if (with_features || !keep) {
+            a.weight = c.weight;
+            a.weight_pitch = c.weight_pitch;
+            a.packed_weight = packed;
+            a.weight_blocks = blocks_of(p.classes * row_chunks, VT);
+        }
+        *rows = packed;
         *pitch = (long long)p.dim_pad * p.size;
     }
     a.classes = p.classes;
@@ -1726,19 +1757,22 @@ int launch_product(const Call& c, int kernel, const ProductArgs& a) {
         OD_PRODUCT(24);
         OD_PRODUCT(32);
 #undef OD_PRODUCT
-        default: OD_LAUNCH_KERNEL(kernel, (product_kernel<T, GRAD>), grid, dim3(VT), 0, c.stream, a); break;
+        default:
+            if (c.p.class_tile == TILE) OD_LAUNCH_KERNEL(kernel, (product_kernel<T, GRAD, TILE>), grid, dim3(VT), 0, c.stream, a);
+            else OD_LAUNCH_KERNEL(kernel, (product_kernel<T, GRAD, 32>), grid, dim3(VT), 0, c.stream, a);
+            break;
     }
     return OD_OK;
 }
 
-template <typename G, bool ROWS>
+template <typename G, bool ROWS, bool DIRECT = false>
 int launch_grad(const Call& c, int kernel, const GradArgs& g) {
     const Plan& p = c.p;
     const long long dtiles = (p.dim_pad + p.grad_tile - 1) / p.grad_tile;
     const dim3 grid((unsigned)(dtiles * (ROWS ? g.splits : g.cols / ROW_TILE * g.splits))), block(2 * VT);
-    if (p.grad_tile == 256) OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 4, ROWS>), grid, block, 0, c.stream, g);
-    else if (p.grad_tile == 128) OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 2, ROWS>), grid, block, 0, c.stream, g);
-    else OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 1, ROWS>), grid, block, 0, c.stream, g);
+    if (p.grad_tile == 256) OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 4, ROWS, DIRECT>), grid, block, 0, c.stream, g);
+    else if (p.grad_tile == 128) OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 2, ROWS, DIRECT>), grid, block, 0, c.stream, g);
+    else OD_LAUNCH_KERNEL(kernel, (grad_kernel<G, 1, ROWS, DIRECT>), grid, block, 0, c.stream, g);
     return OD_OK;
 }
 
@@ -1915,7 +1949,16 @@ int backward_typed(const Call& c) {
             g.accumulate = 0;
             g.bias_out = c.dbias ? (float*)(c.ws + p.b_part_b) : nullptr;
             g.row_weight = weighted ? row_weight : nullptr;
-            rc = launch_grad<G, false>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g);
+            if (p.splits_w == 1 && c.dweight) {
+                g.result = (T*)c.dweight + first * p.dim;
+                g.bf16_result = BF16;
+                g.dim = p.dim;
+                g.scaled = scale_f;
+                g.classes = least(p.piece, p.classes - first);
+                g.scales = scales;
+            }
+            rc = g.result ? launch_grad<G, false, true>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g)
+                          : launch_grad<G, false>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g);
             if (rc != OD_OK) return rc;
         }
         FinishArgs f = {};
@@ -1926,7 +1969,7 @@ int backward_typed(const Call& c) {
         f.classes = least(p.piece, p.classes - first);
         const int groups = (p.dim + 3) / 4;
         unsigned finish_blocks = 0;
-        if (c.dweight) {
+        if (c.dweight && p.splits_w > 1) {
             f.part_w = (const float*)(c.ws + p.b_part_w);
             f.dweight = (T*)c.dweight + first * p.dim;
             finish_blocks += f.weight_blocks = blocks_of(f.classes * groups, VT);
