@@ -45,28 +45,57 @@ typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// A fragment is 16 bytes per lane: 32 rows (lane % 32) x one 32-byte slab of K (halves lane / 32).  Any assignment of K
-// to the slots of a slab gives the same product as long as both operands use it.
-template <typename T> struct Mma;
-template <> struct Mma<bf16_t> {
-    static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+// An operand of the matrix units: 32 rows (lane % 32) x 16 of K, eight per lane (halves lane / 32).  It is read as slabs of
+// 32 bytes of K, 16 bytes per lane: one slab in 16 bits, two in fp32.  Any assignment of K to the slots of a fragment gives
+// the same product as long as both operands use it.
+//
+// fp32 products by bf16 matrix instructions: x = h + m + l, each the nearest bf16 to what is left, h within 2^-9 of x, m
+// within 2^-9 of the rest, l 2^-9 again, so that 24 bits are there exactly.  Of the nine products the three smallest, below
+// 2^-25 of the whole together, are left out, half of what rounding each product to fp32 would cost; sums are fp32 as ever.
+// Six instructions of 32 cycles do 16 of K, for which the fp32 instruction takes 512 cycles; taking the operands apart, 11
+// vector instructions for two elements, runs beside them and bounds the product.  A training step of 4096 x 8000 x 512, a
+// tenth of the rows left out, 802 us instead of 1115, of 21577 x 4938 x 128 806 instead of 1372.  What rounds to an infinite
+// h (from 3.39e38 on) gives NaN.
+template <typename T> struct Fragment {
+    static constexpr int SLABS = 1, PRODUCTS = 1;                   // of K; matrix instructions per product of fragments
+    u32x4 v;
+    __device__ __forceinline__ void set(const u32x4 (&slab)[1]) { v = slab[0]; }
+};
+template <> struct Fragment<float> {
+    static constexpr int SLABS = 2, PRODUCTS = 6;
+    u32x4 h, m, l;
+    __device__ __forceinline__ void set(const u32x4 (&slab)[2]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x = u2f(slab[i >> 1][2 * (i & 1)]), y = u2f(slab[i >> 1][2 * (i & 1) + 1]), a, b;
+            h[i] = pack2(x, y, (const bf16_t*)nullptr);
+            unpack2(h[i], a, b, (const bf16_t*)nullptr);
+            x -= a;
+            y -= b;
+            m[i] = pack2(x, y, (const bf16_t*)nullptr);
+            unpack2(m[i], a, b, (const bf16_t*)nullptr);
+            l[i] = pack2(x - a, y - b, (const bf16_t*)nullptr);
+        }
     }
 };
-template <> struct Mma<_Float16> {
-    static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
-    }
-};
-template <> struct Mma<float> {
-    static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
-        const vec4f x = __builtin_bit_cast(vec4f, a), y = __builtin_bit_cast(vec4f, b);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.x, y.x, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.y, y.y, c, 0, 0, 0);
-        c = __builtin_amdgcn_mfma_f32_32x32x2f32(x.z, y.z, c, 0, 0, 0);
-        return __builtin_amdgcn_mfma_f32_32x32x2f32(x.w, y.w, c, 0, 0, 0);
-    }
-};
+
+__device__ __forceinline__ f32x16 mma_bf16(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const Fragment<bf16_t>& a, const Fragment<bf16_t>& b, f32x16 c) {
+    return mma_bf16(a.v, b.v, c);
+}
+__device__ __forceinline__ f32x16 mma(const Fragment<_Float16>& a, const Fragment<_Float16>& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a.v), __builtin_bit_cast(h16x8, b.v), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(const Fragment<float>& a, const Fragment<float>& b, f32x16 c) {
+    c = mma_bf16(a.l, b.h, c);                                      // the small ones first
+    c = mma_bf16(a.h, b.l, c);
+    c = mma_bf16(a.m, b.m, c);
+    c = mma_bf16(a.m, b.h, c);
+    c = mma_bf16(a.h, b.m, c);
+    return mma_bf16(a.h, b.h, c);
+}
 
 typedef __attribute__((address_space(3))) char lds_char;
 typedef const __attribute__((address_space(1))) uint32_t* global_words;
@@ -626,16 +655,18 @@ __device__ __forceinline__ void join_halves(float& m, float& s) {
     m = top;
 }
 
-// Rows of up to 1 KiB: a wave keeps the features of its 32 NF rows in registers for the whole sweep over the classes (128
-// VGPRs), and only tiles of CT classes stream through LDS, two of them in turn.  That takes 16 bytes per cycle and compute
-// unit out of L2 at full matrix rate where a 128 x 128 tile that streams both operands takes 64, all that L2 gives.  Two
-// workgroups per compute unit drift apart, so that one's exponentials run beside the other's products.
+// Rows of up to 1 KiB (fp32: 768 bytes, 1152 in three parts): a wave keeps the features of its 32 NF rows in registers for the
+// whole sweep over the classes (at most 144 VGPRs), and only tiles of CT classes stream through LDS, two of them in turn.
+// That takes 16 bytes per cycle and compute unit out of L2 at full matrix rate where a 128 x 128 tile that streams both
+// operands takes 64, all that L2 gives.  Two workgroups per compute unit drift apart, so that one's exponentials run beside
+// the other's products.
 template <typename T, int KS, bool GRAD>
 struct Resident {
     static constexpr int ROW = KS * 32;                             // bytes of a row
-    static constexpr int NF = KS <= 16 ? 2 : 1;                     // row fragments per wave
+    static constexpr int NF = KS <= (sizeof(T) == 4 ? 8 : 16) ? 2 : 1;  // row fragments per wave
     static constexpr int CT = KS <= 16 ? 64 : 32;                   // classes per tile
     static constexpr int ROWS = 4 * 32 * NF;                        // rows per workgroup
+    static constexpr int SLABS = Fragment<T>::SLABS, K = KS / SLABS;    // fragments of K
 };
 
 template <typename T, int KS, bool GRAD>
@@ -723,16 +754,23 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
         auto fetch_bias = [&](int t) { if (threadIdx.x < CT && t < t1) tile_bias = p.bias2[(long long)t * CT + threadIdx.x]; };
         fetch_bias(t0);
         stage(lds0, t0);
-        u32x4 rows[NF][KS];
+        constexpr int SLABS = S::SLABS;
+        Fragment<T> rows[NF][S::K];
 #pragma unroll
         for (int g = 0; g < NF; ++g)
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
-                rows[g][k] = *reinterpret_cast<const u32x4*>(p.features + (mine + g * 32) * ROW + k * 32 + 16 * h);
+            for (int k = 0; k < S::K; ++k) {
+                u32x4 slab[SLABS];
+#pragma unroll
+                for (int i = 0; i < SLABS; ++i)
+                    slab[i] =
+                        *reinterpret_cast<const u32x4*>(p.features + (mine + g * 32) * ROW + (k * SLABS + i) * 32 + 16 * h);
+                rows[g][k].set(slab);
+            }
         if (threadIdx.x < CT) s_bias[t0 & 1][threadIdx.x] = tile_bias;
         fetch_bias(t0 + 1);
 
-        auto step = [&](const char* now, char* next, int t) {
+        auto step = [&](const char* now, char* next, int t) __attribute__((always_inline)) {
             stage_barrier();
             if (threadIdx.x < CT) s_bias[(t + 1) & 1][threadIdx.x] = tile_bias;
             fetch_bias(t + 2);
@@ -751,17 +789,24 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
             // the wave that multiplies goes first, the one beside it fills in with its exponentials
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                u32x4 a[CF];
-                const char* from = now + ((first_chunk ^ (((2 * k) & FLIP) << 4)) + (((2 * k) & ~FLIP) << 4));
+            for (int k = 0; k < S::K; ++k) {
+                u32x4 raw[CF][SLABS];
 #pragma unroll
-                for (int f = 0; f < CF; ++f) a[f] = *reinterpret_cast<const u32x4*>(from + f * 32 * ROW);
+                for (int i = 0; i < SLABS; ++i) {
+                    const int chunk = 2 * (k * SLABS + i);
+                    const char* from = now + ((first_chunk ^ ((chunk & FLIP) << 4)) + ((chunk & ~FLIP) << 4));
+#pragma unroll
+                    for (int f = 0; f < CF; ++f) raw[f][i] = *reinterpret_cast<const u32x4*>(from + f * 32 * ROW);
+                }
+                Fragment<T> a[CF];
+#pragma unroll
+                for (int f = 0; f < CF; ++f) a[f].set(raw[f]);
 #pragma unroll
                 for (int f = 0; f < CF; ++f)
 #pragma unroll
-                    for (int g = 0; g < NF; ++g) acc[f][g] = Mma<T>::run(a[f], rows[g][k], acc[f][g]);
+                    for (int g = 0; g < NF; ++g) acc[f][g] = mma(a[f], rows[g][k], acc[f][g]);
             }
-            interleave<4 * CF, KS, CF * NF*(sizeof(T) == 4 ? 4 : 1), CF>();
+            interleave<4 * CF, S::K, CF * NF * Fragment<T>::PRODUCTS, CF * SLABS>();
             __builtin_amdgcn_s_setprio(0);
             const float* bias = s_bias[t & 1] + 16 * h;
             if (GRAD) store_dz<G, CF, NF>(acc, bias, p.scale, shift, on, out, lane_at, t * CT);
@@ -807,8 +852,10 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
     long long unit = uniform(share.start(worker));
     const long long end = uniform(share.start(worker + 1));
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, h = lane >> 5;
-    const int wc = F == 2 ? (wave & 1) * 64 : 0, wr = F == 2 ? (wave >> 1) * 64 : wave * 32;   // its classes and rows of a tile
+    // this wave's classes and rows of a tile
+    const int wc = F == 2 ? (wave & 1) * 64 : 0, wr = F == 2 ? (wave >> 1) * 64 : wave * 32;
     constexpr int KE = 128 / sizeof(T);
+    constexpr int SLABS = Fragment<T>::SLABS;
     const int ksteps = p.dim_pad / KE;
     typedef ChunkedOperand<CT, VT, true> Classes;
     typedef ChunkedOperand<TILE, VT, false> Rows;
@@ -860,28 +907,34 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
                 ++next_t;
             }
         };
-        auto multiply = [&](const char* now) {
+        auto multiply = [&](const char* now) __attribute__((always_inline)) {
             int at = lane;
             asm volatile("" : "+v"(at));                            // addresses are formed anew, see resident_kernel
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 a[F], b[F];
+            for (int j = 0; j < 4; j += SLABS) {
+                Fragment<T> a[F], b[F];
 #pragma unroll
                 for (int f = 0; f < F; ++f) {
-                    a[f] = Classes::frag(now, wc + f * 32, j, at);
-                    b[f] = Rows::frag(now + CLASS_STAGE, wr + f * 32, j, at);
+                    u32x4 x[SLABS], y[SLABS];
+#pragma unroll
+                    for (int i = 0; i < SLABS; ++i) {
+                        x[i] = Classes::frag(now, wc + f * 32, j + i, at);
+                        y[i] = Rows::frag(now + CLASS_STAGE, wr + f * 32, j + i, at);
+                    }
+                    a[f].set(x);
+                    b[f].set(y);
                 }
 #pragma unroll
                 for (int f = 0; f < F; ++f)
 #pragma unroll
-                    for (int g = 0; g < F; ++g) acc[f][g] = Mma<T>::run(a[f], b[g], acc[f][g]);
+                    for (int g = 0; g < F; ++g) acc[f][g] = mma(a[f], b[g], acc[f][g]);
             }
-            interleave<4 * F, 4, F * F * (sizeof(T) == 4 ? 4 : 1), 2 * F>();
+            interleave<4 * F, 4 / SLABS, F * F * Fragment<T>::PRODUCTS, 2 * F * SLABS>();
         };
         // The bias of a tile is fetched ahead of the tile's first stage (waiting for it later would wait for the stages behind
         // it as well) and written to LDS in its first step.  The two stages are variables of their own, used by turns in
         // straight code: the compiler then knows that reading one need not wait for the loads into the other.
-        auto step = [&](const char* now, char* next, int& t, int& k) {
+        auto step = [&](const char* now, char* next, int& t, int& k) __attribute__((always_inline)) {
             stage_barrier();
             if (k == 0 && threadIdx.x < CT) s_bias[threadIdx.x] = tile_bias;
             if (k + 1 == ksteps) fetch_bias(t + 1);
@@ -920,8 +973,8 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
             if (threadIdx.x < TILE) {
                 const float2 a = joined[0][threadIdx.x], b = joined[F - 1][threadIdx.x];
                 const float top = fmaxf(a.x, b.x);
-                p.part[segment * TILE + threadIdx.x] =
-                    F == 1 ? a : make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top));
+                const float sum = a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top);
+                p.part[segment * TILE + threadIdx.x] = F == 1 ? a : make_float2(top, sum);
             }
         }
         __syncthreads();                                            // the next segment writes to LDS what others still read
@@ -1272,7 +1325,7 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
     constexpr int THREADS = 2 * VT, DT = 64 * AF;
     constexpr int A_BYTES = DT * 128, B_BYTES = ROW_TILE * 128;
     __shared__ __align__(1024) char a0[A_BYTES], b0[B_BYTES], a1[A_BYTES], b1[B_BYTES];
-    constexpr int KE = 128 / sizeof(T);
+    constexpr int KE = 128 / sizeof(T), SLABS = Fragment<T>::SLABS;
     const int dtiles = (p.dim_pad + DT - 1) / DT;
     const int id = xcd_range(blockIdx.x, gridDim.x);
     const int d0 = (id % dtiles) * DT, member = id / dtiles;
@@ -1333,41 +1386,55 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
             if (ROWS) bc.stage(to_b, k * Dz<T>::BLOCK * (long long)sizeof(T));
             else bs.stage(to_b, k * KE);
         };
-        auto multiply = [&](const char* ta, const char* tb, long long k) {
+        auto multiply = [&](const char* ta, const char* tb, long long k) __attribute__((always_inline)) {
             int at = lane;
             asm volatile("" : "+v"(at));                            // addresses are formed anew, see resident_kernel
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4 x[AF], y[2];
+            for (int j = 0; j < 4; j += SLABS) {
+                u32x4 y[2][SLABS];
+                Fragment<T> b[2], x[AF];
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
-                    y[g] = ROWS ? BC::frag(tb, wcol + g * 32, j, at) : BS::Tile::frag(tb, wcol + g * 32, j, at);
+                for (int g = 0; g < 2; ++g) {
 #pragma unroll
-                for (int f = 0; f < AF; ++f) x[f] = A::frag(ta, wd + f * 32, j, at);
+                    for (int i = 0; i < SLABS; ++i)
+                        y[g][i] = ROWS ? BC::frag(tb, wcol + g * 32, j + i, at) : BS::Tile::frag(tb, wcol + g * 32, j + i, at);
+                    b[g].set(y[g]);
+                }
+#pragma unroll
+                for (int f = 0; f < AF; ++f) {
+                    u32x4 raw[SLABS];
+#pragma unroll
+                    for (int i = 0; i < SLABS; ++i) raw[i] = A::frag(ta, wd + f * 32, j + i, at);
+                    x[f].set(raw);
+                }
 #pragma unroll
                 for (int f = 0; f < AF; ++f)
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) acc[f][g] = Mma<T>::run(x[f], y[g], acc[f][g]);
+                    for (int g = 0; g < 2; ++g) acc[f][g] = mma(x[f], b[g], acc[f][g]);
                 if (want_bias) {
-                    constexpr int E = 16 / sizeof(T);                   // a lane's K of slab j: E from (2 j + h) E on
-                    const u32x4 mine = (wave & 1) ? y[1] : y[0];        // the two waves of these columns take one fragment each
-                    if (p.row_weight) {
-                        const float* weight = p.row_weight + k * KE + (2 * j + h) * E;
+                    constexpr int E = 16 / sizeof(T);               // a lane's K of slab j: E from (2 j + h) E on
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            if constexpr (sizeof(T) == 2) {
-                                float lo, hi;
-                                unpack2(mine[w], lo, hi, (const T*)nullptr);
-                                bias += lo * weight[2 * w] + hi * weight[2 * w + 1];
-                            } else {
-                                bias += u2f(mine[w]) * weight[w];
+                    for (int i = 0; i < SLABS; ++i) {
+                        const u32x4 first = y[0][i], second = y[1][i];  // the two waves of these columns take one each
+                        const u32x4 mine = (wave & 1) ? second : first;
+                        if (p.row_weight) {
+                            const float* weight = p.row_weight + k * KE + (2 * (j + i) + h) * E;
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) {
+                                if constexpr (sizeof(T) == 2) {
+                                    float lo, hi;
+                                    unpack2(mine[w], lo, hi, (const T*)nullptr);
+                                    bias += lo * weight[2 * w] + hi * weight[2 * w + 1];
+                                } else {
+                                    bias += u2f(mine[w]) * weight[w];
+                                }
                             }
-                        }
-                    } else {
+                        } else {
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            if constexpr (sizeof(T) == 2) bias = sum_pair(mine[w], bias);
-                            else bias += u2f(mine[w]);
+                            for (int w = 0; w < 4; ++w) {
+                                if constexpr (sizeof(T) == 2) bias = sum_pair(mine[w], bias);
+                                else bias += u2f(mine[w]);
+                            }
                         }
                     }
                 }
@@ -1376,11 +1443,11 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
         auto order = [&] {
             constexpr int PER = sizeof(T) == 4 ? 4 : 2;                 // LDS reads of a transposed fragment
             constexpr int READS = AF * PER + 2 * (ROWS ? 1 : PER);
-            interleave<(sizeof(T) == 4 ? 1 : 2) * READS, 4, 2 * AF * (sizeof(T) == 4 ? 4 : 1), READS>();
+            interleave<(sizeof(T) == 4 ? 1 : 2) * READS, 4 / SLABS, 2 * AF * Fragment<T>::PRODUCTS, READS * SLABS>();
         };
         if (k_first < k_end) stage(a0, b0, k_first);
-        auto sweep = [&](auto works) {
-            auto work = [&](const char* ta, const char* tb, long long k) {
+        auto sweep = [&](auto works) __attribute__((always_inline)) {
+            auto work = [&](const char* ta, const char* tb, long long k) __attribute__((always_inline)) {
                 if constexpr (decltype(works)::value) {
                     multiply(ta, tb, k);
                     order();
@@ -1438,7 +1505,8 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
                     const int d = d0 + wd + chunk * 4;
                     if (cls < p.classes && d < p.dim) {
                         if (sizeof(T) == 2 && p.bf16_result)
-                            finish_line<bf16_t>(v, exponent, common, p.dim, d, (bf16_t*)p.result, (bf16_t*)p.result + cls * p.dim);
+                            finish_line<bf16_t>(v, exponent, common, p.dim, d, (bf16_t*)p.result,
+                                                (bf16_t*)p.result + cls * p.dim);
                         else finish_line<T>(v, exponent, common, p.dim, d, (T*)p.result, (T*)p.result + cls * p.dim);
                     }
                 } else if (d0 + wd + chunk * 4 < p.dim_pad) {           // dim_pad is a multiple of four
@@ -1584,12 +1652,13 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.classes = classes;
     p.classes_pad = up(classes, ROW_TILE);
     p.dim = dim;
-    // resident rows of 128, 256, 384, 512, 768 or 1024 bytes; wider ones stream in stages of 128
+    // resident rows of 128, 256, 384, 512, 768 or (16-bit) 1024 bytes; wider ones stream in stages of 128
     long long bytes = up((long long)dim * p.size, 128);
-    if (bytes > 512 && bytes <= 1024) bytes = up(bytes, 256);
+    const int resident = dtype == OD_DTYPE_F32 ? 768 : 1024;        // three parts of 1 KiB do not fit the registers
+    if (bytes > 512 && bytes <= resident) bytes = up(bytes, 256);
     p.dim_pad = (int)(bytes / p.size);
-    p.slabs = bytes <= 1024 ? (int)(bytes / 32) : 0;
-    p.row_tile = p.slabs > 0 && p.slabs <= 16 ? 256 : 128;
+    p.slabs = bytes <= resident ? (int)(bytes / 32) : 0;
+    p.row_tile = p.slabs > 0 && p.slabs <= (dtype == OD_DTYPE_F32 ? 8 : 16) ? 256 : 128;
     p.row_tiles = (int)((most(rows, 1) + p.row_tile - 1) / p.row_tile);
     p.class_tile = p.slabs == 0 ? (p.row_tiles * (p.classes_pad / TILE) < SLOTS / 4 ? 32 : TILE) : p.slabs <= 16 ? 64 : 32;
     // one thread per 16 bytes of both packed operands, fewer than 2^32 threads in a launch
@@ -1755,10 +1824,14 @@ int launch_product(const Call& c, int kernel, const ProductArgs& a) {
         OD_PRODUCT(12);
         OD_PRODUCT(16);
         OD_PRODUCT(24);
-        OD_PRODUCT(32);
 #undef OD_PRODUCT
+        case 32:
+            if constexpr (sizeof(T) == 2)
+                OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, 32, GRAD>), grid, dim3(VT), 0, c.stream, a);
+            break;
         default:
-            if (c.p.class_tile == TILE) OD_LAUNCH_KERNEL(kernel, (product_kernel<T, GRAD, TILE>), grid, dim3(VT), 0, c.stream, a);
+            if (c.p.class_tile == TILE)
+                OD_LAUNCH_KERNEL(kernel, (product_kernel<T, GRAD, TILE>), grid, dim3(VT), 0, c.stream, a);
             else OD_LAUNCH_KERNEL(kernel, (product_kernel<T, GRAD, 32>), grid, dim3(VT), 0, c.stream, a);
             break;
     }

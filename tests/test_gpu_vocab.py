@@ -331,6 +331,18 @@ def test_rows_left_out_in_any_number(device, N, V, D, keep, dtype):
     _check_ce(f, w, b, t)
 
 
+@pytest.mark.parametrize("D", [100, 300])
+@pytest.mark.parametrize("up,down", [(90, -94), (-100, 97), (-30, 24)])
+def test_fp32_operands_of_any_size(device, D, up, down):
+    """Products taken apart into bf16 keep fp32's accuracy wherever the parts are normal numbers; sizes also differ by 2^12
+    within each operand."""
+    f, w, b, t = _inputs(device, 200, 400, D, torch.float32, True, seed=41)
+    gen = torch.Generator().manual_seed(42)
+    f = f * 2.0 ** up * torch.exp2(-12 * torch.rand(f.shape, generator=gen)).to(device)
+    w = w * 2.0 ** down * torch.exp2(-12 * torch.rand(w.shape, generator=gen)).to(device)
+    _check_ce(f, w, b, t)
+
+
 def test_strides_alignment_and_shapes(device):
     f, w, b, t = _inputs(device, 24, 150, 64, torch.bfloat16, True, seed=13)
     want = det_utils.vocabulary_cross_entropy(f, w, t, bias=b, reduction="none")
