@@ -248,7 +248,7 @@ __device__ __forceinline__ int xcd_range(int id, int total) {
 }
 
 // ---- preparation --------------------------------------------------------------------------------------------------
-// Number of valid rows, their list and each row's place in it, in row order, by one workgroup; clears row_loss.
+// Number of valid rows, their list and each row's place in it, in row order; clears row_loss.
 // A row is valid if its flag is set (distillation) or its target is not negative.
 struct RowLists {
     int* count;
@@ -256,32 +256,89 @@ struct RowLists {
     int* place;                         // [rows] index into row_of, or -1
 };
 
-__global__ __launch_bounds__(1024) void list_rows_kernel(const long long* __restrict__ targets,
-                                                         const unsigned char* __restrict__ flags, int rows, RowLists lists,
-                                                         float* __restrict__ row_loss) {
-    __shared__ int sums[1024];
-    const int per = (rows + 1023) / 1024;
-    const int a = min(rows, (int)threadIdx.x * per), b = min(rows, a + per);
-    int n = 0;
-#pragma unroll 8
-    for (int r = a; r < b; ++r) n += flags ? flags[r] : (targets[r] >= 0);
-    sums[threadIdx.x] = n;
+__device__ __forceinline__ bool row_counts(const long long* targets, const unsigned char* flags, long long r) {
+    return flags ? flags[r] != 0 : targets[r] >= 0;
+}
+
+// PER consecutive rows per thread from `first` on, by one workgroup: lists them behind `before` others.  `write`: whether the
+// lists are wanted in memory; s_row_of, if not null, gets them too.  Returns the number of valid ones.
+template <int PER>
+__device__ __forceinline__ int list_rows(const long long* targets, const unsigned char* flags, long long first, int rows,
+                                         int before, const RowLists& lists, float* row_loss, bool write, int* s_row_of) {
+    __shared__ int s_sum[VT / 64];
+    bool on[PER];
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const long long r = first + threadIdx.x * PER + i;
+        on[i] = r < rows && row_counts(targets, flags, r);
+        mine += on[i] ? 1 : 0;
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int upto = (int)wave_scan_incl((uint32_t)mine);
+    if (lane == 63) s_sum[wave] = upto;
     __syncthreads();
-    for (int o = 1; o < 1024; o <<= 1) {                            // inclusive scan
-        const int v = (int)threadIdx.x >= o ? sums[threadIdx.x - o] : 0;
-        __syncthreads();
-        sums[threadIdx.x] += v;
-        __syncthreads();
+    int at = before + upto - mine, count = 0;
+#pragma unroll
+    for (int w = 0; w < VT / 64; ++w) {
+        if (w < wave) at += s_sum[w];
+        count += s_sum[w];
     }
-    int at = sums[threadIdx.x] - n;
-#pragma unroll 8
-    for (int r = a; r < b; ++r) {
-        const bool on = flags ? flags[r] != 0 : targets[r] >= 0;
-        lists.place[r] = on ? at : -1;
-        if (on) lists.row_of[at++] = r;
-        row_loss[r] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const long long r = first + threadIdx.x * PER + i;
+        if (write && r < rows) {
+            lists.place[r] = on[i] ? at : -1;
+            row_loss[r] = 0.0f;
+        }
+        if (on[i]) {
+            if (s_row_of) s_row_of[at] = (int)r;
+            if (write) lists.row_of[at] = (int)r;
+            ++at;
+        }
     }
-    if (threadIdx.x == 1023) *lists.count = sums[1023];
+    return count;
+}
+
+// Many rows: 4096 per workgroup, counted by a first launch and listed by a second (32768 rows: 21 us; one workgroup for
+// all of them took 99).
+constexpr int LIST_ROWS = 16 * VT;
+
+__global__ __launch_bounds__(VT) void count_rows_kernel(const long long* __restrict__ targets,
+                                                        const unsigned char* __restrict__ flags, int rows,
+                                                        int* __restrict__ counts) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < LIST_ROWS / VT; ++i) {
+        const long long r = (long long)blockIdx.x * LIST_ROWS + i * VT + threadIdx.x;
+        n += r < rows && row_counts(targets, flags, r) ? 1 : 0;
+    }
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+    __shared__ int s_sum[VT / 64];
+    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < VT / 64; ++w) n += s_sum[w];
+        counts[blockIdx.x] = n;
+    }
+}
+
+__global__ __launch_bounds__(VT) void list_rows_kernel(const long long* __restrict__ targets,
+                                                       const unsigned char* __restrict__ flags, int rows,
+                                                       const int* __restrict__ counts, RowLists lists,
+                                                       float* __restrict__ row_loss) {
+    __shared__ int s_before;
+    if (threadIdx.x == 0) s_before = 0;
+    __syncthreads();
+    int before = 0;
+    for (int b = threadIdx.x; b < (int)blockIdx.x; b += VT) before += counts[b];
+    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o, 64);
+    if ((threadIdx.x & 63) == 0 && before > 0) atomicAdd(&s_before, before);
+    __syncthreads();
+    before = s_before;
+    const int n = list_rows<LIST_ROWS / VT>(targets, flags, (long long)blockIdx.x * LIST_ROWS, rows, before, lists, row_loss,
+                                            true, nullptr);
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *lists.count = before + n;
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -427,40 +484,9 @@ __global__ __launch_bounds__(VT) void prepare_kernel(PrepareArgs p) {
     unsigned block = blockIdx.x;
     if (block < p.feature_blocks) {
         __shared__ int s_row_of[SCAN ? SCAN * VT : 1];
-        __shared__ int s_sum[VT / 64];
-        int count = 0;
-        if (SCAN) {
-            bool on[SCAN ? SCAN : 1];
-            int mine = 0;
-#pragma unroll
-            for (int i = 0; i < SCAN; ++i) {
-                const int r = threadIdx.x * SCAN + i;
-                on[i] = r < p.rows && (p.flags ? p.flags[r] != 0 : p.targets[r] >= 0);
-                mine += on[i] ? 1 : 0;
-            }
-            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-            int upto = (int)wave_scan_incl((uint32_t)mine);
-            if (lane == 63) s_sum[wave] = upto;
-            __syncthreads();
-            int before = 0;
-            for (int w = 0; w < VT / 64; ++w) {
-                if (w < wave) before += s_sum[w];
-                count += s_sum[w];
-            }
-            int at = before + upto - mine;
-#pragma unroll
-            for (int i = 0; i < SCAN; ++i) {
-                const int r = threadIdx.x * SCAN + i;
-                if (block == 0 && r < p.rows) {
-                    p.lists.place[r] = on[i] ? at : -1;
-                    p.row_loss[r] = 0.0f;
-                }
-                if (on[i]) {
-                    s_row_of[at] = r;
-                    if (block == 0) p.lists.row_of[at] = r;
-                    ++at;
-                }
-            }
+        int count;
+        if constexpr (SCAN > 0) {
+            count = list_rows<SCAN>(p.targets, p.flags, 0, p.rows, 0, p.lists, p.row_loss, block == 0, s_row_of);
             if (block == 0 && threadIdx.x == 0) *p.lists.count = count;
             __syncthreads();
         } else {
@@ -1077,6 +1103,7 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
                                                         float* __restrict__ loss) {
     __shared__ double red[1024];
     double v = 0.0;
+#pragma unroll 8
     for (int r = threadIdx.x; r < rows; r += 1024) v += (double)row_loss[r];
     red[threadIdx.x] = v;
     __syncthreads();
@@ -1633,7 +1660,7 @@ struct Plan {
     // saved buffer
     size_t o_count, o_row_of, o_place, o_lse, o_logit, o_prob, o_packed, o_weight, saved;
     // forward's scratch
-    size_t f_weight, f_bias, f_part, f_ends, f_entropy, f_flags, forward;
+    size_t f_weight, f_bias, f_part, f_ends, f_entropy, f_flags, f_counts, forward;
     // backward's scratch
     size_t b_weight, b_bias, b_row_weight, b_scales, b_scaled_f, b_scaled_w, b_dz, b_part_f, b_ends, b_part_w, b_part_b;
     size_t backward;
@@ -1698,6 +1725,7 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.f_ends = take(at, 8ll * groups_of(p.classes_pad / p.class_tile, p.row_tiles) * p.row_tiles);
     p.f_entropy = take(at, 4 * p.rows_pad);
     p.f_flags = take(at, p.rows_pad);
+    p.f_counts = take(at, 4 * (p.rows / LIST_ROWS + 1));
     p.forward = at;
 
     at = 0;
@@ -1774,10 +1802,14 @@ int prepare(const Call& c, bool with_features, const unsigned char* flags, size_
         a.flags = flags;
         a.rows = (int)p.rows;
         a.row_loss = c.row_loss;
-        scan = p.rows <= 4 * VT ? 4 : p.rows <= 16 * VT ? 16 : 0;
+        scan = p.rows <= 4 * VT ? 4 : p.rows <= LIST_ROWS ? LIST_ROWS / VT : 0;
         if (scan == 0) {
-            hipLaunchKernelGGL(list_rows_kernel, dim3(1), dim3(1024), 0, c.stream, c.targets, flags, (int)p.rows, a.lists,
-                               c.row_loss);
+            int* counts = (int*)(c.ws + p.f_counts);
+            const dim3 grid(blocks_of(p.rows, LIST_ROWS));
+            hipLaunchKernelGGL(count_rows_kernel, grid, dim3(VT), 0, c.stream, c.targets, flags, (int)p.rows, counts);
+            OD_LAUNCH_CHECK();
+            hipLaunchKernelGGL(list_rows_kernel, grid, dim3(VT), 0, c.stream, c.targets, flags, (int)p.rows, (const int*)counts,
+                               a.lists, c.row_loss);
             OD_LAUNCH_CHECK();
         }
     }
