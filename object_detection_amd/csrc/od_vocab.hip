@@ -1132,6 +1132,7 @@ __global__ __launch_bounds__(1024) void row_weights_kernel(const float* __restri
     __shared__ float red[1024];
     const int count = *lists.count;
     float top = 0.0f;
+#pragma unroll 8
     for (int i = threadIdx.x; i < count; i += 1024) {
         const float g = fabsf(upstream[lists.row_of[i]]);
         if (g < __builtin_inff()) top = fmaxf(top, g);             // infinities and NaN go through as they are
@@ -1143,6 +1144,7 @@ __global__ __launch_bounds__(1024) void row_weights_kernel(const float* __restri
         __syncthreads();
     }
     top = red[0] > 0.0f ? red[0] : 1.0f;
+#pragma unroll 8
     for (long long i = threadIdx.x; i < rows_pad; i += 1024)
         weight[i] = i < count ? upstream[lists.row_of[i]] / top : 0.0f;
     if (threadIdx.x == 0) {
@@ -1317,7 +1319,7 @@ struct GradArgs {
     int accumulate;
     float* bias_out;                    // [splits][cols] weighted sums of dz over K, or null
     const float* row_weight;            // [rows_pad], or null: ones
-    // DIRECT: [classes][dim], instead of `out`
+    // DIRECT: [classes][dim] instead of `out`, or null where only the bias is wanted
     void* result;
     int bf16_result, dim, scaled;
     long long classes;
@@ -1530,7 +1532,7 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
                 if constexpr (DIRECT) {
                     const long long cls = c0 + wcol + g * 32 + c;
                     const int d = d0 + wd + chunk * 4;
-                    if (cls < p.classes && d < p.dim) {
+                    if (p.result && cls < p.classes && d < p.dim) {
                         if (sizeof(T) == 2 && p.bf16_result)
                             finish_line<bf16_t>(v, exponent, common, p.dim, d, (bf16_t*)p.result,
                                                 (bf16_t*)p.result + cls * p.dim);
@@ -1738,7 +1740,7 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     p.b_dz = take(at, p.rows_pad * p.piece * p.size);
     p.b_part_f = take(at, 4 * (p.workers_f * (long long)ROW_TILE + p.rows_pad) * p.dim_pad);
     p.b_ends = take(at, 8 * (p.rows_pad / ROW_TILE));
-    p.b_part_w = take(at, 4 * p.piece * p.dim_pad * p.splits_w);
+    p.b_part_w = take(at, p.splits_w > 1 ? 4 * p.piece * p.dim_pad * p.splits_w : 0);
     p.b_part_b = take(at, 4 * p.piece * p.splits_w);
     p.backward = at;
     return true;
@@ -2054,16 +2056,17 @@ int backward_typed(const Call& c) {
             g.accumulate = 0;
             g.bias_out = c.dbias ? (float*)(c.ws + p.b_part_b) : nullptr;
             g.row_weight = weighted ? row_weight : nullptr;
-            if (p.splits_w == 1 && c.dweight) {
-                g.result = (T*)c.dweight + first * p.dim;
+            const bool direct = p.splits_w == 1;
+            if (direct) {
+                g.result = c.dweight ? (T*)c.dweight + first * p.dim : nullptr;
                 g.bf16_result = BF16;
                 g.dim = p.dim;
                 g.scaled = scale_f;
                 g.classes = least(p.piece, p.classes - first);
                 g.scales = scales;
             }
-            rc = g.result ? launch_grad<G, false, true>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g)
-                          : launch_grad<G, false>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g);
+            rc = direct ? launch_grad<G, false, true>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g)
+                        : launch_grad<G, false>(c, OD_KERNEL_VOCAB_GRAD_CLASSES, g);
             if (rc != OD_OK) return rc;
         }
         FinishArgs f = {};

@@ -51,8 +51,10 @@ def _to_anchor_major(x: Tensor, per_anchor: int) -> Tensor:
     return x.view(B, -1, per_anchor, H, W).permute(0, 3, 4, 1, 2).reshape(B, -1, per_anchor)
 
 
-def _is_channels_last(x: Tensor) -> bool:
-    return not x.is_contiguous() and x.is_contiguous(memory_format=torch.channels_last)
+def _are_channels_last(maps: List[Tensor]) -> bool:
+    """Maps of one channel or one pixel are in both orders at once."""
+    return not all(m.is_contiguous() for m in maps) and \
+        all(m.is_contiguous(memory_format=torch.channels_last) for m in maps)
 
 
 class RetinaNetClassificationHead(nn.Module):
@@ -391,7 +393,7 @@ def postprocess_batched(cls_levels, reg_levels, anchors, image_shapes, score_thr
     dev = cls_levels[0].device
     hw = _image_hw_tensor(image_shapes, dev)
     K = int(topk_candidates)
-    if planar_classes is not None and all(map(_is_channels_last, [*cls_levels, *reg_levels, *(ctr_levels or [])])):
+    if planar_classes is not None and _are_channels_last([*cls_levels, *reg_levels, *(ctr_levels or [])]):
         # channels-last maps hold their anchors' rows already: read as [B, H*W*A, K] without a copy
         cls_levels = [_to_anchor_major(m, planar_classes) for m in cls_levels]
         reg_levels = [_to_anchor_major(m, 4) for m in reg_levels]

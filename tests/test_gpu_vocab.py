@@ -377,8 +377,9 @@ def test_strides_alignment_and_shapes(device):
     assert torch.equal(g, g24.sum(0, keepdim=True))
 
 
-def test_partial_gradients_and_repeated_results(device):
-    f, w, b, t = _inputs(device, 300, 700, 128, torch.bfloat16, True, seed=15)
+@pytest.mark.parametrize("N,dtype", [(300, torch.bfloat16), (40, torch.bfloat16), (40, torch.float32)])
+def test_partial_gradients_and_repeated_results(device, N, dtype):
+    f, w, b, t = _inputs(device, N, 700, 128, dtype, True, seed=15)
     def grads(which):
         leaves = [x.clone().requires_grad_(k in which) for k, x in zip("fwb", (f, w, b))]
         out = det_utils.vocabulary_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
