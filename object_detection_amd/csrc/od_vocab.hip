@@ -260,47 +260,45 @@ __device__ __forceinline__ bool row_counts(const long long* targets, const unsig
     return flags ? flags[r] != 0 : targets[r] >= 0;
 }
 
-// PER consecutive rows per thread from `first` on, by one workgroup: lists them behind `before` others.  `write`: whether the
-// lists are wanted in memory; s_row_of, if not null, gets them too.  Returns the number of valid ones.
+// PER * VT rows from `first` on, by one workgroup: lists them behind `before` others.  `write`: whether the lists are wanted in
+// memory; s_row_of, if not null, gets them too.  Returns the number of valid ones.
 template <int PER>
 __device__ __forceinline__ int list_rows(const long long* targets, const unsigned char* flags, long long first, int rows,
                                          int before, const RowLists& lists, float* row_loss, bool write, int* s_row_of) {
-    __shared__ int s_sum[VT / 64];
-    bool on[PER];
-    int mine = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const long long r = first + threadIdx.x * PER + i;
-        on[i] = r < rows && row_counts(targets, flags, r);
-        mine += on[i] ? 1 : 0;
-    }
+    constexpr int WAVES = VT / 64;
+    static_assert(PER * WAVES <= 64, "one lane per 64 rows");
+    __shared__ int s_count[PER * WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int upto = (int)wave_scan_incl((uint32_t)mine);
-    if (lane == 63) s_sum[wave] = upto;
-    __syncthreads();
-    int at = before + upto - mine, count = 0;
-#pragma unroll
-    for (int w = 0; w < VT / 64; ++w) {
-        if (w < wave) at += s_sum[w];
-        count += s_sum[w];
-    }
+    unsigned long long valid[PER];                                  // of 64 neighbouring rows
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const long long r = first + threadIdx.x * PER + i;
+        const long long r = first + i * VT + threadIdx.x;
+        valid[i] = __ballot(r < rows && row_counts(targets, flags, r));
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        if (lane == 0) s_count[i * WAVES + wave] = __popcll(valid[i]);
+    __syncthreads();
+    const int n = lane < PER * WAVES ? s_count[lane] : 0;
+    const int upto = (int)wave_scan_incl((uint32_t)n);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const long long r = first + i * VT + threadIdx.x;
+        const int at = before + __shfl(upto - n, i * WAVES + wave, 64) + __popcll(valid[i] & ((1ull << lane) - 1));
+        const bool on = (valid[i] >> lane) & 1;
         if (write && r < rows) {
-            lists.place[r] = on[i] ? at : -1;
+            lists.place[r] = on ? at : -1;
             row_loss[r] = 0.0f;
         }
-        if (on[i]) {
+        if (on) {
             if (s_row_of) s_row_of[at] = (int)r;
             if (write) lists.row_of[at] = (int)r;
-            ++at;
         }
     }
-    return count;
+    return __shfl(upto, 63, 64);
 }
 
-// Many rows: 4096 per workgroup, counted by a first launch and listed by a second (32768 rows: 21 us; one workgroup for
+// Many rows: 4096 per workgroup, counted by a first launch and listed by a second (32768 rows: 17 us; one workgroup for
 // all of them took 99).
 constexpr int LIST_ROWS = 16 * VT;
 
