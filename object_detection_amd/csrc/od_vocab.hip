@@ -14,8 +14,9 @@
 // its target entries are corrected, and the two products that read it, dF and dW, accumulate in fp32.
 // Operands of those two products, for 16-bit inputs: dz, features and weight in fp16, dz times 2^14 and the others (bf16, or
 // weighted by a gradient per row) under one power of two each, which brings the largest value to [2^13, 2^14).  fp16 keeps
-// three bits of dz more than bf16 (gradients 1.05 instead of 1.5 final roundings from the exact ones), and bf16 values no
-// more than 2^27 times smaller than the largest come through unchanged; the powers of two leave in the fp32 results.
+// three bits of dz more than bf16 (gradients 1.05 instead of 1.5 final roundings from the exact ones) down to 2^-28 of a
+// row's gradient and none below 2^-39, and bf16 values no more than 2^27 times smaller than the largest come through
+// unchanged; the powers of two leave in the fp32 results.
 //
 // Rows without a target (negative class; no finite teacher entry) are left out at the start: the valid rows are listed in
 // order and their features packed densely, so that masked rows cost nothing and whatever they hold (infinities, NaN)
@@ -1144,10 +1145,17 @@ __device__ __forceinline__ int exponent_of(uint32_t max_bits) {
     return min(max(14 - e, -100), 100);
 }
 
-// A gradient per row: weight[place] = upstream of the row / the largest |upstream|, zero behind the last valid row; and the
-// scalars.
+// A gradient per row, over the largest of them: g = mantissa * weight, mantissa in [1, 2) and weight a power of two with the
+// gradient's sign.  The mantissa becomes part of dz (whose exponentials take it with lse) and is rounded with it; the power
+// of two goes exactly onto the features (dW) and the results (dF), so that rows of small gradients keep their digits and no
+// operand is rounded a second time.  Zero behind the last valid row.  And the scalars.
+struct RowWeights {
+    float *weight, *mantissa, *lse2;    // [rows_pad]; lse2 less log2 of the mantissa
+};
+
 __global__ __launch_bounds__(1024) void row_weights_kernel(const float* __restrict__ upstream, RowLists lists,
-                                                           long long rows_pad, float temperature, float* __restrict__ weight,
+                                                           long long rows_pad, float temperature,
+                                                           const float* __restrict__ lse2, RowWeights out,
                                                            Scales* __restrict__ scales) {
     __shared__ float red[1024];
     const int count = *lists.count;
@@ -1164,9 +1172,18 @@ __global__ __launch_bounds__(1024) void row_weights_kernel(const float* __restri
         __syncthreads();
     }
     top = red[0] > 0.0f ? red[0] : 1.0f;
-#pragma unroll 8
-    for (long long i = threadIdx.x; i < rows_pad; i += 1024)
-        weight[i] = i < count ? upstream[lists.row_of[i]] / top : 0.0f;
+#pragma unroll 4
+    for (long long i = threadIdx.x; i < rows_pad; i += 1024) {
+        float g = i < count ? upstream[lists.row_of[i]] / top : 0.0f, m = 1.0f;
+        if (g != 0.0f && fabsf(g) < __builtin_inff()) {
+            int e;
+            m = 2.0f * frexpf(fabsf(g), &e);
+            g = copysignf(ldexpf(1.0f, e - 1), g);
+        }
+        out.weight[i] = g;
+        out.mantissa[i] = m;
+        out.lse2[i] = lse2[i] - log2f(m);
+    }
     if (threadIdx.x == 0) {
         scales->common = top * temperature;
         scales->features_max = 0;
@@ -1259,7 +1276,8 @@ template <typename G>
 __global__ __launch_bounds__(VT) void correct_targets_kernel(const long long* __restrict__ targets, int top,
                                                              const float* __restrict__ prob, RowLists lists,
                                                              const float* __restrict__ lse2,
-                                                             const float* __restrict__ target_logit, long long first_class,
+                                                             const float* __restrict__ target_logit,
+                                                             const float* __restrict__ mantissa, long long first_class,
                                                              long long piece, long long classes, float scale,
                                                              G* __restrict__ dz) {
     const int n = top > 0 ? top : 1;
@@ -1274,7 +1292,7 @@ __global__ __launch_bounds__(VT) void correct_targets_kernel(const long long* __
     if (p == 0.0f) return;                                          // what the product wrote is q already
     const float log_q = target_logit[at] - lse2[place] * LN2;
     const float v = p > 0.5f ? expm1f(log_q) + (1.0f - p) : expf(log_q) - p;
-    dz[Dz<G>::at(place, c - first_class, piece)] = Elem<G>::from_float(v * scale);
+    dz[Dz<G>::at(place, c - first_class, piece)] = Elem<G>::from_float(v * (mantissa ? mantissa[place] * scale : scale));
 }
 
 // 256 classes of KE rows of dz as an operand with K strided: four (fp32: eight) blocks side by side.
@@ -1754,7 +1772,7 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     at = 0;
     p.b_weight = take(at, dim == p.dim_pad ? p.classes * p.dim_pad * p.size : 0);
     p.b_bias = take(at, 4 * p.classes_pad + 4 * p.piece);
-    p.b_row_weight = take(at, 4 * p.rows_pad);
+    p.b_row_weight = take(at, 3 * 4 * p.rows_pad);
     p.b_scales = take(at, sizeof(Scales));
     p.b_scaled_f = take(at, p.rows_pad * p.dim_pad * p.size);
     p.b_scaled_w = take(at, dtype == OD_DTYPE_BF16 ? p.classes * p.dim_pad * p.size : 0);
@@ -1985,10 +2003,12 @@ int backward_typed(const Call& c) {
     const RowLists lists = lists_of(c);
     const bool weighted = c.reduction == OD_REDUCE_NONE;
     float* row_weight = (float*)(c.ws + p.b_row_weight);
+    const RowWeights weights = {row_weight, row_weight + p.rows_pad, row_weight + 2 * p.rows_pad};
+    const float* lse2 = (const float*)(c.saved + p.o_lse);
     Scales* scales = (Scales*)(c.ws + p.b_scales);
     if (weighted) {
         hipLaunchKernelGGL(row_weights_kernel, dim3(1), dim3(1024), 0, c.stream, c.upstream, lists, p.rows_pad, c.temperature,
-                           row_weight, scales);
+                           lse2, weights, scales);
         OD_LAUNCH_CHECK();
     }
     ProductArgs a = {};
@@ -2036,7 +2056,7 @@ int backward_typed(const Call& c) {
     a.groups = groups_of(a.tiles, p.row_tiles);
     a.row_tiles = p.row_tiles;
     a.scale = LOG2E / c.temperature;
-    a.lse2 = (const float*)(c.saved + p.o_lse);
+    a.lse2 = weighted ? weights.lse2 : lse2;
     a.dz = c.ws + p.b_dz;
     a.piece = p.piece;
     const int ke = 128 / p.size;
@@ -2047,8 +2067,9 @@ int backward_typed(const Call& c) {
         rc = launch_product<T, true>(c, OD_KERNEL_VOCAB_DZ, a);
         if (rc != OD_OK) return rc;
         hipLaunchKernelGGL(correct_targets_kernel<G>, dim3(blocks_of(p.rows * p.n, VT)), dim3(VT), 0, c.stream, c.targets,
-                           c.top, (const float*)(c.saved + p.o_prob), lists, a.lse2, (const float*)(c.saved + p.o_logit),
-                           first, p.piece, p.classes, (float)(1 << GradOf<T>::LOG2_DZ), (G*)(c.ws + p.b_dz));
+                           c.top, (const float*)(c.saved + p.o_prob), lists, lse2, (const float*)(c.saved + p.o_logit),
+                           weighted ? weights.mantissa : (const float*)nullptr, first, p.piece, p.classes,
+                           (float)(1 << GradOf<T>::LOG2_DZ), (G*)(c.ws + p.b_dz));
         OD_LAUNCH_CHECK();
         GradArgs g = {};
         g.dz = c.ws + p.b_dz;

@@ -190,6 +190,16 @@ def test_other_reductions(device, reduction, dtype):
     _check_kd(f, w, b, tl, tc, 2.0, reduction, scale)
 
 
+@pytest.mark.parametrize("N,V,D", [(3, 50, 1), (929, 7067, 5), (40, 300, 2)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_gradient_per_row_is_rounded_once(device, N, V, D, dtype):
+    """Few terms a sum, so that roundings do not average out: dz takes one, the row's gradient adds none."""
+    for seed in range(4):
+        f, w, b, t = _inputs(device, N, V, D, dtype, True, seed=50 + seed)
+        _check_ce(f, w, b, t, reduction="none")
+        _check_kd(f, w, b, *reversed(_teacher(device, N, V, 3, seed=seed)), 1.0, reduction="none")
+
+
 def test_teacher_entries_that_are_missing_repeated_or_without_weight(device):
     f, w, b, _ = _inputs(device, 12, 200, 64, torch.bfloat16, True, seed=4)
     tc, tl = _teacher(device, 12, 200, 6, seed=5)
