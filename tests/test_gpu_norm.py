@@ -113,6 +113,38 @@ def test_many_images_of_many_groups(device):
            "silu")
 
 
+def test_offsets_past_32_bits(device):
+    """An image of 2.3 G elements: a thread adds 6000 * 6000 / 256 / 32 = 4395 pixels, so that many half steps of fp32 more
+    in the statistics (twice, by the thread's own shift) and in the sums of the gradients."""
+    C, side, groups = 64, 6000, 4
+    gen = torch.Generator(device=device).manual_seed(2)
+    x = torch.empty((1, side, side, C), dtype=torch.bfloat16, device=device).normal_(0.5, 1.0, generator=gen)
+    x = x.permute(0, 3, 1, 2).requires_grad_(True)
+    y = group_norm_act(x, groups, None, None, 1e-5, "silu")
+    dx = torch.autograd.grad(y, x, torch.ones_like(y))[0]
+    per = C // groups
+    chain = CHAIN + 2 * 4395 * U32
+    for g in (0, groups - 1):
+        v = x.detach()[:, g * per:(g + 1) * per]
+        mean = v.mean(dtype=torch.float64)
+        parts = [v[:, c].double() for c in range(per)]
+        rstd = (sum((q - mean).pow(2).sum() for q in parts) / (per * side * side) + 1e-5).rsqrt()
+        a = b = 0.0
+        for q in parts:
+            h = (q - mean) * rstd
+            s = torch.sigmoid(h)
+            du = s * (1 + h * (1 - s))
+            a, b = a + du.sum() / (per * side * side), b + (du * h).sum() / (per * side * side)
+        for rows in (slice(0, 2), slice(side - 2, side)):
+            h = (v[:, :, rows].double() - mean) * rstd
+            s = torch.sigmoid(h)
+            _close(y.detach()[:, g * per:(g + 1) * per, rows], h * s,
+                   2.0 ** -8 * (h * s).abs() * 1.01 + (chain + 2.0 ** -20) * (h.abs() + 1), "y")
+            want = rstd * (s * (1 + h * (1 - s)) - a - h * b)
+            _close(dx[:, g * per:(g + 1) * per, rows], want,
+                   2.0 ** -8 * want.abs() * 1.01 + (chain + 2.0 ** -18) * rstd * (1 + h.abs()) * 3, "dx")
+
+
 @pytest.mark.parametrize("pdtype", [torch.float16, torch.bfloat16])
 def test_parameter_types_and_memory_orders(device, pdtype):
     x, dy, gamma, beta = _case(device, 2, 64, 12, 10, 8, "relu", torch.bfloat16, True, seed=5, pdtype=pdtype)

@@ -353,6 +353,45 @@ def test_fp32_operands_of_any_size(device, D, up, down):
     _check_ce(f, w, b, t)
 
 
+def test_offsets_past_32_bits(device):
+    """A weight of 4.6 GB, read in place and gradient written: losses, dF and the first and last classes' dW.  bf16 dz is
+    rounded to fp16, half a step of 2^-11 at most, and to zero below 2^-39; sums as in _definition."""
+    N, V, D = 32, 4_500_000, 512
+    gen = torch.Generator(device=device).manual_seed(1)
+    w = torch.empty((V, D), dtype=torch.bfloat16, device=device).normal_(0, D ** -0.5, generator=gen).requires_grad_(True)
+    t = torch.randint(0, V, (N,), generator=gen, device=device)
+    t[:4] = torch.tensor([0, V - 1, V - 2, V // 2], device=device)
+    f = (torch.randn((N, D), generator=gen, device=device) + 6 * w.detach()[t].float()).to(torch.bfloat16).requires_grad_(True)
+    loss = det_utils.vocabulary_cross_entropy(f, w, t, reduction="sum")
+    df, dw = torch.autograd.grad(loss, (f, w))
+    F, size = f.detach().double(), 0.0
+    z = torch.empty((N, V), dtype=torch.float64, device=device)
+    for a in range(0, V, 500_000):
+        W = w.detach()[a:a + 500_000].double()
+        z[:, a:a + 500_000] = torch.mm(F, W.t())
+        size = max(size, float(torch.mm(F.abs(), W.abs().t()).max()))
+    lse = torch.logsumexp(z, dim=1)
+    e_z = (D + 4) * U * size + 2.0 ** -18
+    row = lse - z.gather(1, t[:, None]).squeeze(1)
+    assert float((loss.detach().double() - row.sum()).abs()) <= N * (2 * e_z + 8 * U * float(lse.abs().max()))
+    z -= lse[:, None]
+    dz = z.exp_()
+    dz[torch.arange(N, device=device), t] -= 1.0
+    e_dz = dz.abs() * (2 * e_z + 2.0 ** -11) + 2.0 ** -39
+    # partial sums: 64 classes a step, at most V / 64 steps one after the other
+    steps = V / 64 * U
+    want = torch.zeros((N, D), dtype=torch.float64, device=device)
+    tol = torch.zeros_like(want)
+    for a in range(0, V, 500_000):
+        W = w.detach()[a:a + 500_000].double()
+        want += torch.mm(dz[:, a:a + 500_000], W)
+        tol += torch.mm(e_dz[:, a:a + 500_000] + steps * dz[:, a:a + 500_000].abs(), W.abs())
+    _close(df, want, tol + 2.0 ** -8 * 1.01 * want.abs(), "dF")
+    for part in (slice(0, 1000), slice(V - 1000, V), slice(V // 2 - 500, V // 2 + 500)):
+        want = torch.mm(dz[:, part].t(), F)
+        _close(dw[part], want, torch.mm(e_dz[:, part].t() + 8 * U, F.abs()) + 2.0 ** -8 * 1.01 * want.abs(), "dW")
+
+
 def test_strides_alignment_and_shapes(device):
     f, w, b, t = _inputs(device, 24, 150, 64, torch.bfloat16, True, seed=13)
     want = det_utils.vocabulary_cross_entropy(f, w, t, bias=b, reduction="none")
