@@ -686,18 +686,21 @@ __device__ __forceinline__ void join_halves(float& m, float& s) {
 // operands takes 64, all that L2 gives.  Two workgroups per compute unit drift apart, so that one's exponentials run beside
 // the other's products.  Forward, a tenth of the rows left out: 4096 x 32000 x 256 bf16 72 us (840 TFLOP/s), 32768 x 65536 x
 // 512 1800 us (1100, at 1.84 GHz; the largest library products reach 1300).
-template <typename T, int KS, bool GRAD>
+// SMALL: calls of few tiles, whose time is that of one tile's loads, products and exponentials one after the other: forward
+// with 64 x 1204 x 256 bf16 13.1 us instead of 15.9, 64 x 32000 (500 wide tiles) 18.8 instead of 22.5, 64 x 1204 x 128 fp32
+// 13.9 instead of 15.0, but 1000 x 4000 x 128 fp32 (256 tiles) 21.6 instead of 19.4.
+template <typename T, int KS, bool GRAD, bool SMALL>
 struct Resident {
     static constexpr int ROW = KS * 32;                             // bytes of a row
-    static constexpr int NF = KS <= (sizeof(T) == 4 ? 8 : 16) ? 2 : 1;  // row fragments per wave
-    static constexpr int CT = KS <= 16 ? 64 : 32;                   // classes per tile
+    static constexpr int NF = !SMALL && KS <= (sizeof(T) == 4 ? 8 : 16) ? 2 : 1;    // row fragments per wave
+    static constexpr int CT = !SMALL && KS <= 16 ? 64 : 32;         // classes per tile
     static constexpr int ROWS = 4 * 32 * NF;                        // rows per workgroup
     static constexpr int SLABS = Fragment<T>::SLABS, K = KS / SLABS;    // fragments of K
 };
 
-template <typename T, int KS, bool GRAD>
+template <typename T, int KS, bool GRAD, bool SMALL>
 __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
-    typedef Resident<T, KS, GRAD> S;
+    typedef Resident<T, KS, GRAD, SMALL> S;
     typedef typename GradOf<T>::type G;
     constexpr int ROW = S::ROW, NF = S::NF, CT = S::CT, CF = CT / 32, CHUNKS = ROW / 16, PASSES = CT * CHUNKS / VT;
     __shared__ __align__(1024) char lds0[CT * ROW], lds1[CT * ROW];
@@ -1695,6 +1698,7 @@ struct Plan {
     int dim, dim_pad, size, n;                  // n: targets per row
     int slabs;                                  // 32-byte slabs of a row where the rows are resident, 0 where they stream
     int row_tile, class_tile, row_tiles;        // of the product
+    bool small;                                 // see Resident
     int workgroups;                             // of the product
     long long piece;                            // classes per piece
     int pieces, grad_tile, workers_f, splits_w; // backward; grad_tile: columns of dim per workgroup, workers_f: for each
@@ -1726,9 +1730,12 @@ bool plan_of(long long rows, long long classes, int dim, int top, int dtype, Pla
     if (bytes > 512 && bytes <= resident) bytes = up(bytes, 256);
     p.dim_pad = (int)(bytes / p.size);
     p.slabs = bytes <= resident ? (int)(bytes / 32) : 0;
-    p.row_tile = p.slabs > 0 && p.slabs <= (dtype == OD_DTYPE_F32 ? 8 : 16) ? 256 : 128;
+    const long long wide_tiles = (most(rows, 1) + 255) / 256 * (p.classes_pad / 64);
+    p.small = p.slabs > 0 && p.slabs <= 16 && wide_tiles <= (p.size == 2 ? SLOTS : SLOTS / 4);
+    p.row_tile = p.slabs > 0 && p.slabs <= (dtype == OD_DTYPE_F32 ? 8 : 16) && !p.small ? 256 : 128;
     p.row_tiles = (int)((most(rows, 1) + p.row_tile - 1) / p.row_tile);
-    p.class_tile = p.slabs == 0 ? (p.row_tiles * (p.classes_pad / TILE) < SLOTS / 4 ? 32 : TILE) : p.slabs <= 16 ? 64 : 32;
+    p.class_tile = p.slabs == 0 ? (p.row_tiles * (p.classes_pad / TILE) < SLOTS / 4 ? 32 : TILE)
+                                : p.slabs <= 16 && !p.small ? 64 : 32;
     // one thread per 16 bytes of both packed operands, fewer than 2^32 threads in a launch
     if (most(p.rows_pad, p.classes_pad) * p.dim_pad * p.size / 16 > (1ll << 30)) return false;
     p.n = top > 0 ? top : 1;
@@ -1890,17 +1897,20 @@ template <typename T, bool GRAD>
 int launch_product(const Call& c, int kernel, const ProductArgs& a) {
     const dim3 grid((unsigned)c.p.workgroups);
     switch (c.p.slabs) {
-#define OD_PRODUCT(KS) \
-    case KS: OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, KS, GRAD>), grid, dim3(VT), 0, c.stream, a); break
+#define OD_PRODUCT(KS)                                                                                        \
+    case KS:                                                                                                  \
+        if (c.p.small) OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, KS, GRAD, true>), grid, dim3(VT), 0, c.stream, a); \
+        else OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, KS, GRAD, false>), grid, dim3(VT), 0, c.stream, a);  \
+        break
         OD_PRODUCT(4);
         OD_PRODUCT(8);
         OD_PRODUCT(12);
         OD_PRODUCT(16);
-        OD_PRODUCT(24);
 #undef OD_PRODUCT
+        case 24: OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, 24, GRAD, false>), grid, dim3(VT), 0, c.stream, a); break;
         case 32:
             if constexpr (sizeof(T) == 2)
-                OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, 32, GRAD>), grid, dim3(VT), 0, c.stream, a);
+                OD_LAUNCH_KERNEL(kernel, (resident_kernel<T, 32, GRAD, false>), grid, dim3(VT), 0, c.stream, a);
             break;
         default:
             if (c.p.class_tile == TILE)
