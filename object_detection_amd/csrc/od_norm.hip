@@ -15,10 +15,11 @@
 // Statistics: a thread sums x - k and (x - k)^2 with k its own first value of the channel, which bounds what the
 // subtraction of the two sums can lose by the number of its pixels whatever the mean of the map is: four pixels in 32 bits,
 // the fours in 64.  Everything above a thread is merged in 64 bits as (count, mean, M2) in two passes, M2 = sum M2_i + n_i
-// (mean_i - mean)^2.  Fixed order, no atomics.  The 64-bit sums cost the statistics of 16 x 64 x 64 x 256 bf16 12.0 us instead
-// of 11.2 and those of 16 x 256 x 256 x 256 nothing; with sums in 32 bits one in twenty of such maps had a channel whose
-// pixels on the rectifier's corner fell to the other side than by 64 bits throughout, with them one in five hundred.  Mean and 1/std stay 64-bit: a rectifier's gradient is all or nothing, and since a 16-bit map holds few different
-// values, hundreds of pixels of a channel lie on its corner together; where fp32 cannot tell the side, 64 bits decide.
+// (mean_i - mean)^2.  Fixed order, no atomics.  Mean and 1/std stay 64-bit: a rectifier's gradient is all or nothing, and
+// since a 16-bit map holds few different values, hundreds of pixels of a channel lie on its corner together; where fp32
+// cannot tell the side, 64 bits decide.  The sums in 64 bits cost the statistics of 16 x 64 x 64 x 256 bf16 12.0 us instead of
+// 11.2 and those of 16 x 256 x 256 x 256 nothing; with sums in 32 bits one in twenty of the large maps had a channel whose
+// corner fell to the other side than by 64 bits throughout, with them one in five hundred.
 #include "od_common.h"
 #include "../../include/od_boxes.h"
 #include "od_elem.h"
