@@ -435,7 +435,7 @@ int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int
  *   upstream     : fp32 gradient of row_loss [rows] (OD_REDUCE_NONE) or of loss [1]
  *   dfeatures    : [rows, dim] dense, dweight [classes, dim] dense, dbias [classes], all of dtype; any may be null
  *   workspace    : od_vocab_loss_workspace_bytes(..., backward = 0 or 1), 256-byte aligned
- * Sums are fp32 in a fixed order.  fp32 operands are taken apart into bf16 values, three that hold all of their 24 bits; a
+ * Sums are fp32 (that of a softmax: 64 bits above a tile of classes) in a fixed order.  fp32 operands are taken apart into bf16 values, three that hold all of their 24 bits; a
  * feature or weight from 3.39e38 on then makes its logits NaN.  16-bit gradients are rounded once at the end, and the logits'
  * gradients, an operand of the products, once before, to fp16 under a power of two: whole down to 2^-28 of the gradient of
  * the row, gone below 2^-39.  bf16 features and weights enter those products as fp16 under one power of two for all of them:

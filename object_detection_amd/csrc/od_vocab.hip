@@ -612,8 +612,11 @@ template <typename G> struct Dz {
 
 // Folds a tile's logits into the running maximum and sum of NF rows of this lane.  acc[f][g][i]: class 32 f + 16 h + i of
 // the tile; bias: at class 16 h.
+// A lane may sweep the whole vocabulary, and terms of one size are rounded to the same side again and again (a fresh head,
+// whose logits are nearly equal, lost 1e-4 of its sum over 16384 terms): a tile's 16 or 32 terms are added in fp32, four by
+// four, and the tiles in 64 bits, which costs 0.5 % at most (kd 16384 x 65001 x 256, a step 3328 -> 3345 us).
 template <int CF, int NF>
-__device__ __forceinline__ void fold(f32x16 (&acc)[CF][NF], const float* bias, float scale, float (&m)[NF], float (&s)[NF]) {
+__device__ __forceinline__ void fold(f32x16 (&acc)[CF][NF], const float* bias, float scale, float (&m)[NF], double (&s)[NF]) {
     float top[NF];
 #pragma unroll
     for (int g = 0; g < NF; ++g) top[g] = m[g];
@@ -633,13 +636,18 @@ __device__ __forceinline__ void fold(f32x16 (&acc)[CF][NF], const float* bias, f
         }
 #pragma unroll
     for (int g = 0; g < NF; ++g) {
-        float sum = s[g] * __builtin_amdgcn_exp2f(m[g] - top[g]);
+        float sum = 0.0f;
 #pragma unroll
         for (int f = 0; f < CF; ++f)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(acc[f][g][i] - top[g]);
+            for (int i = 0; i < 16; i += 4) {
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[k] = __builtin_amdgcn_exp2f(acc[f][g][i + k] - top[g]);
+                sum += (e[0] + e[1]) + (e[2] + e[3]);
+            }
+        s[g] = s[g] * (double)__builtin_amdgcn_exp2f(m[g] - top[g]) + (double)sum;
         m[g] = top[g];
-        s[g] = sum;
     }
 }
 
@@ -672,12 +680,11 @@ __device__ __forceinline__ void store_dz(const f32x16 (&acc)[CF][NF], const floa
     }
 }
 
-// Joins the two lanes that share a row; lane < 32 then holds it.
-__device__ __forceinline__ void join_halves(float& m, float& s) {
-    const float om = __shfl_xor(m, 32, 64), os = __shfl_xor(s, 32, 64);
+// (maximum, sum) of a row from the two lanes that share it; both get it.
+__device__ __forceinline__ float2 join_halves(float m, double s) {
+    const float sum = (float)s, om = __shfl_xor(m, 32, 64), os = __shfl_xor(sum, 32, 64);
     const float top = fmaxf(m, om);
-    s = s * __builtin_amdgcn_exp2f(m - top) + os * __builtin_amdgcn_exp2f(om - top);
-    m = top;
+    return make_float2(top, sum * __builtin_amdgcn_exp2f(m - top) + os * __builtin_amdgcn_exp2f(om - top));
 }
 
 // Rows of up to 1 KiB (fp32: 768 bytes, 1152 in three parts): a wave keeps the features of its 32 NF rows in registers for the
@@ -766,12 +773,13 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
         const int t1 = min(share.first_tile + share.tiles, t0 + (int)min(end - unit, (long long)share.tiles));
         unit += t1 - t0;
         const long long mine = row_tile * S::ROWS + wave * 32 * NF + (lane & 31);       // this lane's first row
-        float m[NF], s[NF], shift[NF];
+        float m[NF], shift[NF];
+        double s[NF];
         bool on[NF];
 #pragma unroll
         for (int g = 0; g < NF; ++g) {
             m[g] = LOWEST;
-            s[g] = 0.0f;
+            s[g] = 0.0;
             if (GRAD) {
                 shift[g] = p.lse2[mine + g * 32] - GradOf<T>::LOG2_DZ;
                 on[g] = mine + g * 32 < count;
@@ -853,8 +861,8 @@ __global__ __launch_bounds__(VT, 2) void resident_kernel(ProductArgs p) {
             if (threadIdx.x == 0) share.mark(p.ends + (long long)group * p.row_tiles + row_tile, segment, t0, t1);
 #pragma unroll
             for (int g = 0; g < NF; ++g) {
-                join_halves(m[g], s[g]);
-                if (h == 0) part[wave * 32 * NF + g * 32 + lane] = make_float2(m[g], s[g]);
+                const float2 row = join_halves(m[g], s[g]);
+                if (h == 0) part[wave * 32 * NF + g * 32 + lane] = row;
             }
         }
         __syncthreads();                                            // the next segment writes to LDS what others still read
@@ -897,12 +905,13 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
         Classes cls;
         rows.init(p.features, (long long)p.dim_pad * sizeof(T), r0, r0 + TILE);
 
-        float m[F], s[F], shift[F];
+        float m[F], shift[F];
+        double s[F];
         bool on[F];
 #pragma unroll
         for (int g = 0; g < F; ++g) {
             m[g] = LOWEST;
-            s[g] = 0.0f;
+            s[g] = 0.0;
             if (GRAD) {
                 const long long row = r0 + wr + g * 32 + (lane & 31);
                 shift[g] = p.lse2[row] - GradOf<T>::LOG2_DZ;
@@ -993,8 +1002,8 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
             // a row's classes lie in two lanes and, of a wide tile, two waves
 #pragma unroll
             for (int g = 0; g < F; ++g) {
-                join_halves(m[g], s[g]);
-                if (h == 0) joined[F == 2 ? wave & 1 : 0][wr + g * 32 + lane] = make_float2(m[g], s[g]);
+                const float2 row = join_halves(m[g], s[g]);
+                if (h == 0) joined[F == 2 ? wave & 1 : 0][wr + g * 32 + lane] = row;
             }
             __syncthreads();
             const long long segment = Share::segment(group, per_group, p.row_tiles, worker, row_tile);

@@ -625,3 +625,26 @@ def test_head_over_a_vocabulary_trains_through_tower_and_losses(device):
     assert abs(float(loss_a.detach()) - float(loss_b.detach())) <= 1e-3 * abs(float(loss_b.detach()))
     for p_, q_ in zip(ga, gb):
         assert float((p_ - q_).abs().max()) <= 1e-2 * float(q_.abs().max()) + 1e-7
+
+
+@pytest.mark.parametrize("dtype,D,V", [(torch.float32, 16, 262144), (torch.float32, 200, 65536), (torch.bfloat16, 64, 262144),
+                                       (torch.float16, 256, 262144), (torch.bfloat16, 600, 262144)])
+@pytest.mark.parametrize("spread", [0.0, 0.01])
+def test_nearly_equal_logits_over_a_large_vocabulary(device, dtype, D, V, spread):
+    """A fresh head: weights of zero and a bias that hardly differs, but for a few classes one higher, so that every lane's
+    terms are e^-1 next to its own maximum.  Terms of one size are rounded to one side: a sum that is not split up drifts.  A
+    lane sweeps V / 8 classes of a row tile here.  Off the definition: the bias' value and its scaling, three half steps of
+    its size; the exponential, 2^-23; a tile's sum, 32 terms in fours, 12 half steps; joining lanes, splits and waves, in turns
+    of at most 64 additions; log, the maximum's share and the value of lse itself, six half steps of its size."""
+    N = 32768
+    gen = torch.Generator().manual_seed(61)
+    f = torch.randn((N, D), generator=gen).to(device, dtype)
+    w = torch.zeros((V, D), device=device, dtype=dtype)
+    b = (torch.randn((V,), generator=gen) * spread).to(device, dtype)
+    b[::V // 64] = 1.0
+    b[16::V // 64] = 1.0
+    t = torch.randint(0, V, (N,), generator=gen).to(device)
+    rows = det_utils.vocabulary_cross_entropy(f, w, t, bias=b, reduction="none")
+    lse = torch.logsumexp(b.double(), 0)
+    tol = 3 * U + 2.0 ** -23 + (12 + 64) * U + 6 * U * float(lse)
+    assert float((rows.double() - (lse - b.double()[t])).abs().max()) <= tol
