@@ -1458,7 +1458,7 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
             for (int g = 0; g < 2; ++g)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[f][g][i] = 0.0f;
-        float bias = 0.0f;
+        double bias = 0.0;                                          // a stage's rows are added in fp32, the stages in 64 bits
         const bool want_bias = !ROWS && p.bias_out && d0 == 0;
 
         auto stage = [&](char* to_a, char* to_b, long long k) {
@@ -1469,6 +1469,7 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
         auto multiply = [&](const char* ta, const char* tb, long long k) __attribute__((always_inline)) {
             int at = lane;
             asm volatile("" : "+v"(at));                            // addresses are formed anew, see resident_kernel
+            float stage_bias = 0.0f;
 #pragma unroll
             for (int j = 0; j < 4; j += SLABS) {
                 u32x4 y[2][SLABS];
@@ -1504,21 +1505,22 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
                                 if constexpr (sizeof(T) == 2) {
                                     float lo, hi;
                                     unpack2(mine[w], lo, hi, (const T*)nullptr);
-                                    bias += lo * weight[2 * w] + hi * weight[2 * w + 1];
+                                    stage_bias += lo * weight[2 * w] + hi * weight[2 * w + 1];
                                 } else {
-                                    bias += u2f(mine[w]) * weight[w];
+                                    stage_bias += u2f(mine[w]) * weight[w];
                                 }
                             }
                         } else {
 #pragma unroll
                             for (int w = 0; w < 4; ++w) {
-                                if constexpr (sizeof(T) == 2) bias = sum_pair(mine[w], bias);
-                                else bias += u2f(mine[w]);
+                                if constexpr (sizeof(T) == 2) stage_bias = sum_pair(mine[w], stage_bias);
+                                else stage_bias += u2f(mine[w]);
                             }
                         }
                     }
                 }
             }
+            if (want_bias) bias += (double)stage_bias;
         };
         auto order = [&] {
             constexpr int PER = sizeof(T) == 4 ? 4 : 2;                 // LDS reads of a transposed fragment
@@ -1598,7 +1600,7 @@ __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
         if (want_bias) {
-            const float sum = bias + __shfl_xor(bias, 32, 64);
+            const float half = (float)bias, sum = half + __shfl_xor(half, 32, 64);
             if (h == 0) p.bias_out[line + wcol + (wave & 1) * 32 + lane] = sum;
         }
         if (ROWS) __syncthreads();                                  // the next segment writes to LDS what others still read

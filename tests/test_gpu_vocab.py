@@ -648,3 +648,18 @@ def test_nearly_equal_logits_over_a_large_vocabulary(device, dtype, D, V, spread
     lse = torch.logsumexp(b.double(), 0)
     tol = 3 * U + 2.0 ** -23 + (12 + 64) * U + 6 * U * float(lse)
     assert float((rows.double() - (lse - b.double()[t])).abs().max()) <= tol
+
+
+def test_bias_gradient_of_very_many_equal_rows(device):
+    """2 M rows of equal logits: the gradient of a class without targets is N / V, a sum of equal terms.  Off it: lse and its
+    scaling to log2 units and back, eight half steps of its size; two for the exponential; a stage of 32 rows, 16; its 64
+    partial sums, 64."""
+    N, V = 2_000_000, 50
+    f = torch.zeros((N, 4), device=device)
+    w = torch.zeros((V, 4), device=device)
+    b = torch.zeros(V, device=device, requires_grad=True)
+    t = torch.arange(N, device=device) % 25
+    db = torch.autograd.grad(det_utils.vocabulary_cross_entropy(f, w, t, bias=b, reduction="sum"), b)[0].double()
+    tol = (8 * math.log(V) + 2 + 16 + 64) * U * N / V
+    assert float((db[25:] - N / V).abs().max()) <= tol
+    assert float((db[:25] - (N / V - N / 25)).abs().max()) <= 2 * tol
