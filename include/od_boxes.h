@@ -426,7 +426,8 @@ int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int
  *                  teacher_logits [rows, top] of teacher_dtype; p = softmax(teacher_logits / temperature) over a row's
  *                  entries, entries of one class added up; entries with a logit of -inf have no weight; a row without
  *                  any entry of weight is left out
- *                  row loss = temperature^2 * (sum p log p - sum p z[class] + log sum exp z)
+ *                  row loss = temperature^2 * (sum p log p - sum p z[class] + log sum exp z);  temperature within
+ *                  2^-63 and 2^63, so that its square is a normal number
  *   A class >= classes is not followed: it makes the row's loss and its gradients NaN.  Rows left out have loss and
  *   gradient zero whatever their features hold.
  *   row_loss     : fp32 [rows];  loss: fp32 [1], by OD_REDUCE_*: not written, sum / max(1, rows not left out), or sum

@@ -1808,7 +1808,8 @@ int check_call(int64_t rows, int64_t classes, int32_t dim, int32_t top, int32_t 
     if (dtype < OD_DTYPE_F32 || dtype > OD_DTYPE_BF16 || teacher_dtype < OD_DTYPE_F32 || teacher_dtype > OD_DTYPE_BF16)
         return OD_ERR_ARG;
     if (rows < 0 || classes <= 0 || dim <= 0 || top < 0) return OD_ERR_ARG;
-    if (!(temperature > 0.0f) || temperature > 3.0e38f || (top == 0 && temperature != 1.0f)) return OD_ERR_ARG;
+    // its square scales the loss: 2^-126 to 2^126
+    if (!(temperature >= 0x1p-63f && temperature <= 0x1p63f) || (top == 0 && temperature != 1.0f)) return OD_ERR_ARG;
     if (reduction < OD_REDUCE_NONE || reduction > OD_REDUCE_SUM) return OD_ERR_ARG;
     if (rows > OD_MAX_VOCAB_ROWS || classes > OD_MAX_VOCAB_CLASSES || dim > OD_MAX_VOCAB_DIM || top > OD_MAX_TEACHER_TOP)
         return OD_ERR_LIMIT;

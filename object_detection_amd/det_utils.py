@@ -317,7 +317,7 @@ def vocabulary_distillation(features: Tensor, weight: Tensor, teacher_logits: Te
     q = softmax((features @ weight.T + bias) / T) over all V classes and p = softmax(teacher_logits / T) over the K classes
     that the teacher names for the row.
 
-    teacher_logits [..., K] (fp32 / fp16 / bf16), teacher_classes int64 [..., K], K <= 256.  An entry with a negative class
+    teacher_logits [..., K] (fp32 / fp16 / bf16), teacher_classes int64 [..., K], K <= 256; 2^-63 <= T <= 2^63.  An entry with a negative class
     is not there, one with a logit of -inf has no weight, and entries of the same class are added up; a row without an
     entry of weight is left out.  A class >= V makes the row's loss and gradients NaN.  The rest as in
     ``vocabulary_cross_entropy``; the teacher gets no gradient."""
@@ -325,8 +325,8 @@ def vocabulary_distillation(features: Tensor, weight: Tensor, teacher_logits: Te
         raise TypeError(f"teacher_classes must be int64, got {teacher_classes.dtype}")
     if teacher_logits.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("vocabulary_distillation: the teacher's logits take no gradient (detach them)")
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 2.0 ** -63 <= temperature <= 2.0 ** 63:                  # its square scales the loss
+        raise ValueError(f"temperature must be between 2^-63 and 2^63, got {temperature}")
     if teacher_classes.dim() < 2 or teacher_logits.shape != teacher_classes.shape or teacher_classes.shape[-1] < 1:
         raise ValueError(f"teacher logits {tuple(teacher_logits.shape)} and classes {tuple(teacher_classes.shape)} must be "
                          f"[..., K], K >= 1")

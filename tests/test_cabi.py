@@ -196,3 +196,22 @@ def test_argument_errors_of_vocab_loss():
     assert fwd(top=4, tl=p256, temp=0.0) == -1 and fwd(top=4, tl=p256, temp=float("nan")) == -1
     assert fwd(top=4, tl=p256, td=5) == -1
     assert bwd(up=null) == -1 and bwd(rows=0) == 0
+
+
+def test_temperatures_whose_square_leaves_fp32_are_refused():
+    from object_detection_amd import det_utils
+    lib = _C.lib()
+    null, p256 = ctypes.c_void_p(0), ctypes.c_void_p(256)
+
+    def fwd(temp, nbytes):
+        return lib.od_vocab_loss_forward(p256, 64, p256, 64, null, 2, 10, 50, 64, p256, 4, p256, 2, temp, 1, p256, p256, p256,
+                                         nbytes, p256, nbytes, null)
+    for temp in (2.0 ** -64, 2.0 ** 64, 1e30, 1e-39, float("inf")):
+        assert fwd(temp, 1024) == -1, temp
+    for temp in (2.0 ** -63, 1.0, 2.0 ** 63):
+        assert fwd(temp, 1024) == -3, temp                                      # stops at the workspace's size only
+    features, weight = torch.zeros((2, 8)), torch.zeros((5, 8))
+    logits, classes = torch.zeros((2, 3)), torch.zeros((2, 3), dtype=torch.int64)
+    for temp in (0.0, -1.0, 1e30, 1e-30, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            det_utils.vocabulary_distillation(features, weight, logits, classes, temperature=temp)
