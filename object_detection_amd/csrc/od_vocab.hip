@@ -1149,12 +1149,12 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
 
 // ---- backward ------------------------------------------------------------------------------------------------------
 // Power of two under which an operand with this largest size lies in [2^13, 2^14): what is 2^27 times smaller is still a
-// normal fp16 number, what is 2^37 times smaller vanishes.
+// normal fp16 number, what is 2^37 times smaller vanishes.  From -114 to 162: no fp32 number for itself, an exponent to add.
 __device__ __forceinline__ int exponent_of(uint32_t max_bits) {
     if (max_bits == 0) return 0;
     int e = 0;
     (void)frexpf(u2f(max_bits), &e);                                // max = f * 2^e, f in [0.5, 1)
-    return min(max(14 - e, -100), 100);
+    return 14 - e;
 }
 
 // A gradient per row, over the largest of them: g = mantissa * weight, mantissa in [1, 2) and weight a power of two with the
@@ -1273,11 +1273,11 @@ __global__ __launch_bounds__(VT) void scale_kernel(Operands ops) {
     const int c = (int)(at % chunks) * E;
     float v[E];
     load_vec<T, E>((const T*)o.x + r * o.pitch + c, v);
-    const float f = o.max_bits ? ldexpf(1.0f, exponent_of(*o.max_bits)) : 1.0f;
+    const int exponent = o.max_bits ? exponent_of(*o.max_bits) : 0;
     const float w = o.weight ? o.weight[r] : 1.0f;
     const bool on = !o.count || r < *o.count;
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = on ? v[i] * f * w : 0.0f;
+    for (int i = 0; i < E; ++i) v[i] = on ? ldexpf(v[i], exponent) * w : 0.0f;
     store_vec<G, E>((G*)o.out + r * ops.dim_pad + c, v);
 }
 
@@ -1341,8 +1341,8 @@ __device__ __forceinline__ vec4f sum_parts(const float* part, long long step, in
 }
 template <typename T>
 __device__ __forceinline__ void finish_line(vec4f v, int exponent, float factor, int dim, int d, T* out, T* line) {
-    v *= ldexpf(1.0f, -exponent - GradOf<T>::LOG2_DZ);
-    v *= factor;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ldexpf(v[i], -exponent - GradOf<T>::LOG2_DZ) * factor;
     T* to = line + d;
     if (dim % 4 == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0) {
         const float f[4] = {v.x, v.y, v.z, v.w};

@@ -663,3 +663,15 @@ def test_bias_gradient_of_very_many_equal_rows(device):
     tol = (8 * math.log(V) + 2 + 16 + 64) * U * N / V
     assert float((db[25:] - N / V).abs().max()) <= tol
     assert float((db[:25] - (N / V - N / 25)).abs().max()) <= 2 * tol
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("up,down", [(116, -116), (-116, 116), (60, -60)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_operands_near_the_ends_of_the_range(device, dtype, up, down, reduction):
+    """Features and weights whose products are ordinary but which lie themselves near the largest or the smallest numbers."""
+    if dtype == torch.float32 and abs(up) > 100:
+        pytest.skip("the parts of fp32 operands leave the normal numbers there")
+    f, w, b, t = _inputs(device, 200, 400, 256, dtype, True, seed=43)
+    t[::7] = -1
+    _check_ce(f * 2.0 ** up, w * 2.0 ** down, b, t, reduction, scale=16.0)
