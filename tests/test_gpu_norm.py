@@ -371,3 +371,40 @@ def test_channels_last_maps_are_selected_in_place(device, arch):
     assert sum(int(d["scores"].numel()) for d in last) > 0
     for p, q in zip(plain, last):
         assert all(torch.equal(p[k], q[k]) for k in p)
+
+
+@pytest.mark.parametrize("gamma,beta,value", [(0.0, 0.0, None), (0.0, 0.5, None), (0.0, -0.5, None), (1.0, 0.0, 0.0),
+                                              (1.0, 0.0, 0.375), (-0.5, 0.0, None)])
+def test_fresh_parameters_and_constant_maps(device, gamma, beta, value):
+    """A zero-initialised norm and a map of one value put every pixel on the rectifier's corner: the gradients are those of the
+    definition, and the backward pass does not go over the map once more for it."""
+    gen = torch.Generator().manual_seed(41)
+    C, groups = 256, 32
+    x = torch.randn((16, C, 64, 64), generator=gen).to(device, torch.bfloat16)
+    if value is not None:
+        x.fill_(value)
+    x = x.contiguous(memory_format=torch.channels_last)
+    dy = torch.randn((16, C, 64, 64), generator=gen).to(device, torch.bfloat16).contiguous(memory_format=torch.channels_last)
+    g, b = torch.full((C,), gamma, device=device), torch.full((C,), beta, device=device)
+    if gamma < 0:
+        # away from the corner: a value next to it may fall on either side
+        r = _ref(x, groups, g, b, 1e-5, "relu")
+        dy = torch.where(r["u"].abs() < 1e-3 * r["scale"], torch.zeros_like(dy), dy)
+    _check(x, dy, groups, g, b, "relu")
+
+    def spent(g, b, x):
+        leaves = [t.detach().clone(memory_format=torch.preserve_format).requires_grad_(True) for t in (x, g, b)]
+        y = group_norm_act(*leaves[:1], groups, *leaves[1:])
+        times = []
+        for _ in range(6):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            start.record()
+            for _ in range(20):
+                torch.autograd.grad(y, leaves, dy, retain_graph=True)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        return min(times)
+    ordinary = spent(torch.linspace(0.5, 1.5, C, device=device), torch.linspace(-0.3, 0.4, C, device=device),
+                     torch.randn((16, C, 64, 64), device=device).to(x).contiguous(memory_format=torch.channels_last))
+    assert spent(g, b, x) < 2 * ordinary                            # the second sweep: 3 times and more
