@@ -444,13 +444,11 @@ struct Channels {
         for (int i = 0; i < VEC; ++i) {
             mean[i] = (float)v[i].x;
             rstd[i] = (float)v[i].y;
-            const bool flat = a[i] == 0.0f;
             a[i] = (float)(v[i].y * (double)a[i]);
-            // u is off by a few half steps of its terms, |x - mean| |a| = |beta| where it is zero, and of mean * a
-            corner[i] = 5.0e-7f * (fabsf(beta[i]) + fabsf(mean[i] * a[i]));
-            // fp32 has u, or its sign, exactly: u = beta, or x - mean that beta does not shift.  A fresh norm (gamma and beta
-            // zero) or a constant map would ask at every pixel: 16 x 128 x 128 x 256 bf16 634 us backward instead of 143.
-            if (flat || (beta[i] == 0.0f && (double)mean[i] == v[i].x)) corner[i] = -1.0f;
+            // u is off by a few half steps of its terms, |x - mean| |a| = |beta| where it is zero, and by what the mean lost.
+            // Zero: fp32 has the side exactly, and nothing is near.  Else a fresh norm (gamma and beta zero) or a map of one
+            // value would ask at every pixel: 16 x 128 x 128 x 256 bf16 634 us backward instead of 139.
+            corner[i] = 5.0e-7f * fabsf(beta[i]) + 2.0f * fabsf((float)(v[i].x - (double)mean[i]) * a[i]);
         }
     }
     // d = x - mean and du, from x and dy; whether some du has to be decided again, see decide()
@@ -461,7 +459,7 @@ struct Channels {
             d[i] = x[i] - mean[i];
             const float u = fmaf(d[i], a[i], beta[i]);
             du[i] = act_grad<ACT>(u, dy[i]);
-            if (ACT == OD_ACT_RELU) near = near || fabsf(u) <= corner[i];
+            if (ACT == OD_ACT_RELU) near = near || fabsf(u) < corner[i];
         }
         return near;
     }
@@ -472,7 +470,7 @@ struct Channels {
         asm volatile("" : "+v"(c));                                 // keeps what is loaded here out of the loops around
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            if (fabsf(fmaf(d[i], a[i], beta[i])) <= corner[i]) {
+            if (fabsf(fmaf(d[i], a[i], beta[i])) < corner[i]) {
                 const double2 v = stats[(c + i) / per_group];
                 const double u = ((double)x[i] - v.x) * v.y * (double)param(weight, pdtype, c + i, 1.0f)
                                  + (double)param(bias, pdtype, c + i, 0.0f);
