@@ -346,9 +346,18 @@ def select_candidates(cls_levels: Sequence[Tensor], reg_levels: Sequence[Tensor]
     """
     L = len(cls_levels)
     dev = cls_levels[0].device
-    _require_gpu(cls_levels[0], "cls_logits")
     B, C = cls_levels[0].shape[0], cls_levels[0].shape[-1]
     sizes = [int(t.shape[1]) for t in cls_levels]
+    for what, levels, inner in (("class logits", cls_levels, C), ("box deltas", reg_levels, 4), ("anchors", anchor_levels, 4),
+                                ("centerness", ctr_levels, 1)):
+        if levels is None:
+            continue
+        if len(levels) != L:
+            raise ValueError(f"{what} of {len(levels)} levels, class logits of {L}")
+        for t, n in zip(levels, sizes):                      # the kernels read what the class logits' sizes say
+            if t.shape[-2:] != (n, inner) or (t.dim() == 3 and t.shape[0] != B):
+                raise ValueError(f"{what} of shape {tuple(t.shape)} do not hold {n} anchors x {inner} for {B} images")
+    _require_gpu(cls_levels[0], "cls_logits")
     key = (dev.index, tuple(sizes), B, C)
     plan = _plans.get(key)
     if plan is None:

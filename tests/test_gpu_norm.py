@@ -408,3 +408,20 @@ def test_fresh_parameters_and_constant_maps(device, gamma, beta, value):
     ordinary = spent(torch.linspace(0.5, 1.5, C, device=device), torch.linspace(-0.3, 0.4, C, device=device),
                      torch.randn((16, C, 64, 64), device=device).to(x).contiguous(memory_format=torch.channels_last))
     assert spent(g, b, x) < 2 * ordinary                            # the second sweep: 3 times and more
+
+
+def test_channels_last_maps_that_do_not_belong_together_are_refused(device):
+    """As in NCHW memory: a box map smaller than its class map, or anchors of another size, raise before anything is read."""
+    from object_detection_amd.retinanet import postprocess_batched
+    last = torch.channels_last
+
+    def call(side, anchors, memory):
+        cls = [torch.zeros((2, 3 * 5, 8, 8), device=device).contiguous(memory_format=memory)]
+        reg = [torch.zeros((2, 3 * 4, side, side), device=device).contiguous(memory_format=memory)]
+        return postprocess_batched(cls, reg, [[torch.zeros((anchors, 4), device=device)]] * 2, [(64, 64)] * 2, 0.05, 100, 0.5, 10,
+                                   0, 4.0, planar_classes=5)
+    assert len(call(8, 192, last)) == len(call(8, 192, torch.contiguous_format)) == 2
+    for side, anchors in ((4, 192), (8, 100)):
+        for memory in (last, torch.contiguous_format):
+            with pytest.raises((ValueError, _C.OdBoxesError)):
+                call(side, anchors, memory)

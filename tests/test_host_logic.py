@@ -182,3 +182,25 @@ def test_checkpoint_wire_format_roundtrip(tmp_path):
     torch.save([1, 2, 3], path)
     with pytest.raises(ValueError):
         checkpoint.load_checkpoint(path)
+
+
+def test_candidate_selection_checks_its_levels_before_it_reads_them():
+    """Levels that do not belong together are refused on the host, whatever device they are on: the kernels read as many rows
+    as the class logits have."""
+    from object_detection_amd import kernels
+    B, C, sizes = 2, 5, (12, 3)
+    cls = [torch.zeros((B, n, C)) for n in sizes]
+    reg, ctr = [torch.zeros((B, n, 4)) for n in sizes], [torch.zeros((B, n, 1)) for n in sizes]
+    anchors = [torch.zeros((n, 4)) for n in sizes]
+    hw = torch.zeros((B, 2), dtype=torch.int32)
+
+    def call(cls=cls, reg=reg, anchors=anchors, ctr=ctr):
+        return kernels.select_candidates(cls, reg, anchors, hw, 0.1, 10, 0, 4.0, ctr_levels=ctr)
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        call()
+    short = [torch.zeros((B, 11, 4)), reg[1]]
+    for bad in (dict(reg=short), dict(reg=reg[:1]), dict(reg=[r[:1] for r in reg]), dict(reg=[r[..., :3] for r in reg]),
+                dict(anchors=[anchors[0][:5], anchors[1]]), dict(anchors=[torch.zeros((1, n, 4)) for n in sizes]),
+                dict(ctr=[ctr[0], ctr[1][:, :2]]), dict(ctr=ctr[:1]), dict(cls=[cls[0], cls[1][..., :4]])):
+        with pytest.raises(ValueError, match="levels|do not hold"):
+            call(**bad)
