@@ -59,20 +59,21 @@ variable_list once(variable_list grads) {
     return out;
 }
 
-// A step recorded into a graph must not share leaves with an earlier step whose results still live: its backward pass would
-// have to wait for the stream on which the leaves' accumulators came to be, which a recording cannot, and the process would
-// end there.  Such a call is refused before it records anything.
+// A step recorded into a graph must not share leaves with an earlier step on the default stream whose results still live: its
+// backward pass would make that stream, on which the leaves' accumulators came to be, wait for the recorded one.  The default
+// stream cannot become part of a recording, and the process would end there.  Such a call is refused before it records
+// anything.  A stream of another kind becomes part of the recording and is joined at the end of the backward pass.
 void check_recording(const Tensor& on, std::initializer_list<const Tensor*> inputs) {
     if (!at::GradMode::is_enabled() || !on.is_cuda()) return;
-    const c10::Stream stream = c10::impl::VirtualGuardImpl(on.device().type()).getStream(on.device());
+    const c10::Stream refused = c10::impl::VirtualGuardImpl(on.device().type()).getDefaultStream(on.device());
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing((hipStream_t)stream_of(on), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
     for (const Tensor* t : inputs) {
         if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
         const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (accumulator && accumulator->stream() && *accumulator->stream() != stream)
+        if (accumulator && accumulator->stream() && *accumulator->stream() == refused)
             TORCH_CHECK(false, "a training step cannot be recorded while results of an earlier one with the same parameters, on "
-                               "another stream, are alive: drop them first");
+                               "the default stream, are alive: drop them first");
     }
 }
 

@@ -304,7 +304,7 @@ def vocabulary_cross_entropy(features: Tensor, weight: Tensor, targets: Tensor, 
     rows left out.  The logits are formed in pieces of the vocabulary, once forward and once backward; sums are fp32, and
     fp32 inputs keep fp32's accuracy.  bf16: features or weights 2^27 times smaller than the largest lose bits in the
     gradients.  Differentiable once in features, weight and bias.  A step that is recorded into a graph must not share these
-    with a live eager one on another stream (raises)."""
+    with a live eager one on the default stream (raises)."""
     if targets.dtype != torch.int64:
         raise TypeError(f"targets must be int64, got {targets.dtype}")
     flat = targets if targets.dim() == 1 else targets.reshape(-1)

@@ -675,3 +675,42 @@ def test_operands_near_the_ends_of_the_range(device, dtype, up, down, reduction)
     f, w, b, t = _inputs(device, 200, 400, 256, dtype, True, seed=43)
     t[::7] = -1
     _check_ce(f * 2.0 ** up, w * 2.0 ** down, b, t, reduction, scale=16.0)
+
+
+def test_a_recorded_step_may_share_leaves_with_a_live_one_on_a_side_stream(device):
+    """The usual warm-up: an eager step on a side stream, its loss still bound to a name, then the recording."""
+    from object_detection_amd.graph_step import capture
+    from object_detection_amd.norm import group_norm_act
+    f, w, b, t = _inputs(device, 300, 513, 64, torch.bfloat16, True, seed=27)
+    leaves = [x.detach().clone().requires_grad_(True) for x in (f, w, b)]
+    maps = [torch.randn((2, 32, 8, 8), device=device).contiguous(memory_format=torch.channels_last).requires_grad_(True)]
+    up = torch.randn_like(maps[0])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+
+    def loss_of():
+        return det_utils.vocabulary_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2])
+
+    def map_of():
+        return group_norm_act(maps[0], 8, None, None, 1e-5, "relu")
+    for forward, inputs, grad in ((loss_of, leaves, None), (map_of, maps, up)):
+        def step():
+            y = forward()
+            return [y.detach()] + list(torch.autograd.grad(y, inputs, grad))
+        with torch.cuda.stream(side):
+            alive = forward()
+        side.synchronize()
+        recorded = capture(step, device)
+        with torch.cuda.stream(side):
+            want = [alive.detach().clone()] + list(torch.autograd.grad(alive, inputs, grad))
+        side.synchronize()
+        for k in range(3):
+            with torch.no_grad():
+                inputs[0].mul_(1.0 if k == 0 else 0.5)
+            got = [x.clone() for x in recorded.replay()]
+            torch.cuda.synchronize()
+            if k > 0:
+                with torch.cuda.stream(side):
+                    want = step()
+                side.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(got, want)), k
