@@ -893,7 +893,7 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
     const int wc = F == 2 ? (wave & 1) * 64 : 0, wr = F == 2 ? (wave >> 1) * 64 : wave * 32;
     constexpr int KE = 128 / sizeof(T);
     constexpr int SLABS = Fragment<T>::SLABS;
-    const int ksteps = p.dim_pad / KE;
+    const int ksteps = p.dim_pad / KE;                              // at least seven: narrower rows are resident
     typedef ChunkedOperand<CT, VT, true> Classes;
     typedef ChunkedOperand<TILE, VT, false> Rows;
     while (unit < end) {
@@ -979,7 +979,6 @@ __global__ __launch_bounds__(VT, 2) void product_kernel(ProductArgs p) {
             stage_next(next);
             multiply(now);
             if (++k == ksteps) {
-                if (ksteps == 1) __syncthreads();                   // s_bias was written in this very step
                 const float* bias = s_bias + wc + 16 * h;
                 if (GRAD) store_dz<G, F, F>(acc, bias, p.scale, shift, on, out, lane_at, t * CT + wc);
                 else fold<F, F>(acc, bias, p.scale, m, s);

@@ -714,3 +714,124 @@ def test_a_recorded_step_may_share_leaves_with_a_live_one_on_a_side_stream(devic
                     want = step()
                 side.synchronize()
             assert all(torch.equal(x, y) for x, y in zip(got, want)), k
+
+
+# What a row takes, padded to 128 bytes, and the kernel that this picks: the features resident as 4, 8, 12, 16, 24 or 32 slabs of
+# 32 bytes, wide or (up to 16) small tiles; or streamed, by tiles of 128 or 32 classes.
+@pytest.mark.parametrize("N,V", [(6000, 5100), (150, 500)])        # nearly four times as many wide tiles as small calls have; few
+@pytest.mark.parametrize("dtype,D", [(dtype, D) for dtype in (torch.float16, torch.bfloat16)
+                                     for D in (60, 128, 160, 256, 384, 512, 600)]
+                         + [(torch.float32, D) for D in (30, 60, 80, 128, 150, 300)])
+def test_every_form_of_the_product(device, N, V, dtype, D):
+    f, w, b, t = _inputs(device, N, V, D, dtype, True, seed=N + D)
+    t[torch.rand((N,), generator=torch.Generator().manual_seed(71)).to(device) < 0.3] = -1
+    scale = 1024.0 if dtype == torch.float16 else 1.0
+    _check_ce(f, w, b, t, scale=scale)
+    tc, tl = _teacher(device, N, V, 3, seed=72)
+    tc[::5] = -1
+    _check_kd(f, w, b, tl, tc, 2.0, scale=scale)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weight_gradient_without_a_split(device, dtype, D):
+    """Few rows against many classes: dW leaves its product directly, in tiles of 64, 128 and 256 columns."""
+    f, w, b, t = _inputs(device, 40, 70000, D, dtype, True, seed=D)
+    t[::6] = -1
+    _check_ce(f, w, b, t, scale=256.0 if dtype == torch.float16 else 1.0)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_distillation_in_more_than_one_piece(device, dtype, reduction):
+    """Rows listed by the teacher's entries, by more than one workgroup; each row's classes spread over the pieces, some next to
+    their borders (multiples of 256), some repeated, some missing."""
+    N, V, K = (12000, 7001, 9) if dtype == torch.float32 else (20000, 9000, 9)
+    assert N * V * dtype.itemsize > 256 << 20
+    f, w, b, _ = _inputs(device, N, V, 64, dtype, True, seed=81)
+    gen = torch.Generator().manual_seed(82)
+    tc = torch.randint(0, V, (N, K), generator=gen)
+    edge = 256 * torch.randint(1, V // 256 + 1, (N,), generator=gen)
+    tc[:, 1], tc[:, 2] = edge - 1, edge
+    tc[::7, 3] = tc[::7, 1]
+    tc[::9, 5] = tc[::9, 0]
+    tc[::4, 6] = -1
+    tc[::11] = -2
+    tl = torch.randn((N, K), generator=gen) * 2
+    tl[5::13] = -math.inf
+    tl[2::13, 4] = -math.inf
+    _check_kd(f, w, b, tl.to(device, dtype), tc.to(device), 2.0, reduction,
+              scale=4096.0 if dtype == torch.float16 and reduction == "mean" else 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_gradient_per_row_in_more_than_one_piece(device, dtype):
+    N, V = (20000, 9000) if dtype == torch.bfloat16 else (12000, 7001)
+    f, w, b, t = _inputs(device, N, V, 64, dtype, True, seed=12)
+    t[::10] = -1
+    _check_ce(f, w, b, t, "none")
+
+
+@pytest.mark.parametrize("dtype,most", [(torch.bfloat16, 1.15), (torch.float16, 1.6)])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_how_many_roundings_the_gradients_take(device, dtype, most, reduction):
+    """Error of the gradients over that of rounding the exact ones once, root mean squares.  dz is rounded to 11 bits and the
+    result to the type's own, independently, both relative; the sums of random terms are as large as their terms' root mean
+    square: sqrt(1 + 2^-6) for bf16 and sqrt(2) for fp16.  (dz in bf16 would give sqrt(2) for bf16.)"""
+    N, V, D = 1000, 2000, 128
+    f, w, b, t = _inputs(device, N, V, D, dtype, True, seed=91)
+    up = torch.full((), 64.0, device=device) if reduction == "sum" else 64 * (0.5 + torch.rand((N,), device=device))
+    leaves = [x.detach().requires_grad_(True) for x in (f, w, b)]
+    grads = torch.autograd.grad(det_utils.vocabulary_cross_entropy(leaves[0], leaves[1], t, bias=leaves[2], reduction=reduction),
+                                leaves, up)
+    F, W = f.double(), w.double()
+    dz = torch.softmax(torch.mm(F, W.t()) + b.double(), dim=1)
+    dz[torch.arange(N, device=device), t] -= 1
+    dz *= up.double().expand(N)[:, None]
+    for g, want, name in zip(grads, (torch.mm(dz, W), torch.mm(dz.t(), F)), ("dF", "dW")):
+        ratio = float((g.double() - want).norm() / (want.to(dtype).double() - want).norm())
+        assert ratio <= most, (name, ratio)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_smallest_gradients_of_the_logits(device, dtype):
+    """q = 2^-1 .. 2^-60, read through weights of one: 11 bits down to 2^-28, to the nearest 2^-38 below, zero below 2^-39."""
+    V, scale = 64, 2.0 ** 14
+    b = (-math.log(2.0) * torch.arange(V)).to(device, dtype)
+    f = torch.zeros((5, V), device=device, dtype=dtype, requires_grad=True)
+    w = torch.eye(V, device=device, dtype=dtype)
+    t = torch.zeros(5, dtype=torch.int64, device=device)
+    df = torch.autograd.grad(det_utils.vocabulary_cross_entropy(f, w, t, bias=b, reduction="sum"), f,
+                             torch.tensor(scale, device=device))[0][:, 1:].double() / scale
+    q = torch.softmax(b.double(), 0)[1:].expand(5, V - 1)
+    # logits up to 63 in units of log2: three half steps of them in the exponent
+    rel = 3 * 64 * U + 2.0 ** -18
+    tol = q * (rel + 1.01 * 2.0 ** -11 + 1.01 * HALF[dtype]) + (q < 2.0 ** -28) * 2.0 ** -39 * 1.01 \
+        + (TINY[dtype] / scale if dtype == torch.float16 else 0.0)
+    assert bool(((df - q).abs() <= tol).all())
+    assert not df[q < 2.0 ** -39.1].any() and bool((df[q > 2.0 ** -38] > 0).all())
+
+
+@pytest.mark.parametrize("side", ["weight", "features"])
+def test_smallest_bf16_operands_of_the_gradients(device, side):
+    """Operands of 1 .. 2^-60 in one tensor: exact down to 2^-27 of the largest, to the nearest 2^-37 (2^-24 under 2^13) below,
+    zero from 2^-38 on."""
+    V = 64
+    size = 2.0 ** -torch.arange(V, dtype=torch.float64, device=device)
+    if side == "weight":                            # dF[n, c] = dz[n, c] * 2^-c
+        f = torch.zeros((3, V), device=device, dtype=torch.bfloat16, requires_grad=True)
+        w = torch.diag(size).to(torch.bfloat16)
+        t = torch.full((3,), V - 1, device=device)
+        got = torch.autograd.grad(det_utils.vocabulary_cross_entropy(f, w, t, reduction="sum"), f)[0][0].double()
+        want = size / V
+    else:                                           # dW[c, d] = sum_n dz[n, c] f[n, d]: one row per dimension
+        f = torch.diag(size).to(torch.bfloat16)
+        w = torch.zeros((V, V), device=device, dtype=torch.bfloat16, requires_grad=True)
+        t = torch.full((V,), V - 1, device=device)
+        got = torch.autograd.grad(det_utils.vocabulary_cross_entropy(f, w, t, reduction="sum"), w)[0][0].double()
+        want = size / V
+    exact = size >= 2.0 ** -27
+    err = (got - want).abs()
+    assert bool((err[exact & (torch.arange(V, device=device) < V - 1)] <= 2.0 ** -16 * want[exact]).all())
+    assert bool((err[:V - 1] <= (2.0 ** -8 + 2.0 ** -11) * want[:V - 1] + 2.0 ** -38 / V)[~exact[:V - 1]].all())
+    assert not got[:V - 1][size[:V - 1] < 2.0 ** -38].any()
