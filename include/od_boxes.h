@@ -435,12 +435,17 @@ int od_group_norm_act_backward(const void* x, const void* dy, int32_t dtype, int
  *                  (which takes the same weight, bias, targets and sizes)
  *   upstream     : fp32 gradient of row_loss [rows] (OD_REDUCE_NONE) or of loss [1]
  *   dfeatures    : [rows, dim] dense, dweight [classes, dim] dense, dbias [classes], all of dtype; any may be null
- *   workspace    : od_vocab_loss_workspace_bytes(..., backward = 0 or 1), 256-byte aligned
- * Sums are fp32 (that of a softmax: 64 bits above a tile of classes) in a fixed order.  fp32 operands are taken apart into bf16 values, three that hold all of their 24 bits; a
- * feature or weight from 3.39e38 on then makes its logits NaN.  16-bit gradients are rounded once at the end, and the logits'
- * gradients, an operand of the products, once before, to fp16 under a power of two: whole down to 2^-28 of the gradient of
- * the row, gone below 2^-39.  bf16 features and weights enter those products as fp16 under one power of two for all of them:
- * what is 2^27 times smaller than the largest loses bits, 2^38 times smaller it counts as zero.
+ *   workspace    : od_vocab_loss_workspace_bytes(..., backward = 0 or 1), 256-byte aligned; backward most of it holds a
+ *                  piece of the logits' gradient, 256 MiB or 256 classes for all rows where that is more (4 GiB at the limit
+ *                  of rows, fp32 8), and for bf16 a copy of the weight
+ * The backward call leaves its outputs as they are where rows = 0.
+ * Sums are fp32 (that of a softmax: 64 bits above a tile of classes) in a fixed order.  fp32 operands are taken apart into
+ * bf16 values, three that hold all of their 24 bits; a feature or weight from 3.39e38 on then makes its logits NaN, one below
+ * 2^-102 may lose its last bits.  16-bit gradients are rounded once at the end, and the logits' gradients, an operand of the
+ * products, once before, to fp16 under a power of two: whole down to 2^-28 of the gradient of the row, gone below 2^-39.
+ * Gradients lie 1.0 (bf16) and 1.2 to 1.4 (fp16) final roundings off the exact ones, root mean squares.  bf16 features and
+ * weights enter those products as fp16 under one power of two for all of them: what is 2^27 times smaller than the largest
+ * loses bits, 2^38 times smaller it counts as zero.
  */
 #define OD_REDUCE_NONE 0
 #define OD_REDUCE_MEAN 1

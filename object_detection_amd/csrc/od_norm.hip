@@ -805,8 +805,9 @@ bool small_form(const NormShape& s, int slab, int size, int limit) { return s.pi
 
 // Statistics of an image's chunks, 16 bytes each, up to which the workgroups that normalise join them themselves: a launch
 // less for the host, which bounds a training step on such maps (77 -> 72 us with the parameters' gradients in the launch of
-// dx).  On the device the two are even at 1024 of them (16 x 64 x 64 x 256 in 32 groups, forward 23.8 us against 23.9), near
-// it at 2160 (14.6 against 14.1), not at 4096 (17.8 against 15.1).
+// dx).  Forward over maps of 64 x 64 in 1, 2, 4 or 8 images, joined here against by a launch of its own: 1024 statistics 13.4
+// us against 14.1, 2048 13.8 against 14.4 (eight images 18.0 against 17.6), 2304 15.3 against 15.2, 2560 15.3 against 15.0
+// (eight images 22.8 against 21.0), 3328 16.6 against 15.3, 4096 16.7 against 14.8.
 constexpr int APPLY_JOINS = 2304;
 
 NormShape shape_of(long long batch, long long pixels, int channels, int groups, float eps, int size) {

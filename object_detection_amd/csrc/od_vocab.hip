@@ -10,17 +10,22 @@
 // Forward: one product whose epilogue folds each tile of logits into a running maximum and sum per row, in the lane that
 // owns the row: nothing passes between lanes before the end.  The classes are split over workgroups; a second kernel joins
 // the splits and forms the few logits of the targets by dot products.
-// Backward: the classes are taken in pieces.  A piece's dz is recomputed from the saved lse into a buffer of 256 MB at most,
-// its target entries are corrected, and the two products that read it, dF and dW, accumulate in fp32.
+// Backward: the classes are taken in pieces.  A piece's dz is recomputed from the saved lse into a buffer of 256 MB, or of 256
+// classes for every row where that is more (from 524288 rows on in 16 bits, half of that in 32; 4 and 8 GiB at the limit of
+// rows); its target entries are corrected, and the two products that read it, dF and dW, accumulate in fp32.
 // Operands of those two products, for 16-bit inputs: dz, features and weight in fp16, dz times 2^14 and the others (bf16, or
-// weighted by a gradient per row) under one power of two each, which brings the largest value to [2^13, 2^14).  fp16 keeps
-// three bits of dz more than bf16 (gradients 1.05 instead of 1.5 final roundings from the exact ones) down to 2^-28 of a
-// row's gradient and none below 2^-39, and bf16 values no more than 2^27 times smaller than the largest come through
-// unchanged; the powers of two leave in the fp32 results.
+// weighted by a gradient per row) under one power of two each, which brings the largest value to [2^13, 2^14).  dz has 11
+// bits down to 2^-28 of a row's gradient and none below 2^-39.  Its rounding and the final one are independent: bf16 gradients
+// lie 1.00 final roundings off the exact ones (dz in bf16 would make it 1.4), fp16 gradients 1.2 to 1.4 (dz in fp32 would
+// make it 1.0, for twice the traffic of the buffer and a sixth of the matrix rate).  bf16 values no more than 2^27 times smaller
+// than the largest come through unchanged; the powers of two leave in the fp32 results.
 //
 // Rows without a target (negative class; no finite teacher entry) are left out at the start: the valid rows are listed in
-// order and their features packed densely, so that masked rows cost nothing and whatever they hold (infinities, NaN)
-// reaches no product.  All sums run in a fixed order; the only atomics are integer maxima, whose order changes nothing.
+// order and their features packed densely, so that whatever masked rows hold (infinities, NaN) reaches no product.  The
+// products cost what the valid rows cost; buffers and the width of a piece are sized for all rows, since the host does not
+// know how many are valid: where nearly all are masked, taking the valid rows out beforehand makes for fewer pieces (786240 x
+// 32000 x 256 bf16 with 0.2 % valid: 7.4 ms a step in 125 pieces, 0.4 with the rows taken out).  All sums run in a fixed
+// order; the only atomics are maxima and sums of integers, whose order changes nothing.
 //
 // A product of n rows, V classes and dim D costs 2 n V D operations, four times a training step (forward, dz again, dF, dW).
 #include "od_common.h"
@@ -691,8 +696,8 @@ __device__ __forceinline__ float2 join_halves(float m, double s) {
 // whole sweep over the classes (at most 144 VGPRs), and only tiles of CT classes stream through LDS, two of them in turn.
 // That takes 16 bytes per cycle and compute unit out of L2 at full matrix rate where a 128 x 128 tile that streams both
 // operands takes 64, all that L2 gives.  Two workgroups per compute unit drift apart, so that one's exponentials run beside
-// the other's products.  Forward, a tenth of the rows left out: 4096 x 32000 x 256 bf16 72 us (840 TFLOP/s), 32768 x 65536 x
-// 512 1800 us (1100, at 1.84 GHz; the largest library products reach 1300).
+// the other's products.  Forward, a tenth of the rows left out: 4096 x 32000 x 256 bf16 71 us (850 TFLOP/s of the valid rows),
+// 32768 x 65536 x 512 1830 us (1080; the largest library products reach 1300).
 // SMALL: calls of few tiles, whose time is that of one tile's loads, products and exponentials one after the other: forward
 // with 64 x 1204 x 256 bf16 13.1 us instead of 15.9, 64 x 32000 (500 wide tiles) 18.8 instead of 22.5, 64 x 1204 x 128 fp32
 // 13.9 instead of 15.0, but 1000 x 4000 x 128 fp32 (256 tiles) 21.6 instead of 19.4.
@@ -1396,8 +1401,9 @@ __device__ __forceinline__ float sum_pair(uint32_t w, float c) {
 // out[col][d] = sum_k dz(k, col) * a[k][d].  ROWS: columns are rows of dz and K runs over the classes of the piece (dF);
 // otherwise columns are classes and K runs over the valid rows (dW).  A workgroup of eight waves takes 64 AF columns d and
 // 256 columns of the result, 32 AF x 64 per wave: at AF = 4 a stage of 64 KiB feeds 2048 cycles of the matrix units, half
-// of what L2 gives per cycle.  4096 x 32000 x 256 with a tenth of the rows left out: dF 94 us, dW 83 (640 and 730 TFLOP/s),
-// of which reading 240 MB of dz takes 50.
+// of what L2 gives per cycle.  4096 x 32000 x 256 with a tenth of the rows left out: dF 94 us, dW 80 (640 and 750 TFLOP/s);
+// reading 240 MB of dz takes 50, and waves wait half (dF) and a third (dW) of their cycles for loads, since a stage ends with
+// a wait for all of them and no second workgroup fits beside 128 KiB of LDS.
 // DIRECT: dW of one split, written as it leaves.
 template <typename T, int AF, bool ROWS, bool DIRECT>
 __global__ __launch_bounds__(2 * VT, 2) void grad_kernel(GradArgs p) {

@@ -299,12 +299,17 @@ def vocabulary_cross_entropy(features: Tensor, weight: Tensor, targets: Tensor, 
     features [..., D] are the embeddings of anchors or locations (any strides; rows that are not contiguous are copied),
     weight [V, D] and bias [V] (or None) those of the classes, all of one type (fp32 / fp16 / bf16) on one GPU; targets
     int64 [...].  A negative target leaves its row out, so the indices of a matcher can be used as they are: -1 (no
-    object) and -2 (between the thresholds) take no part.  A target >= V makes the row's loss and gradients NaN.
+    object) and -2 (between the thresholds) take no part.  They reach no product, but buffers and the number of passes over the
+    classes follow all rows: where most of 10^5 rows and more are left out, take the others out first
+    (``features[targets >= 0]``).  A target >= V makes the row's loss and gradients NaN.
     reduction: "mean" over the rows that take part (0 if there are none), "sum", or "none": fp32 losses [...], zero for the
-    rows left out.  The logits are formed in pieces of the vocabulary, once forward and once backward; sums are fp32, and
-    fp32 inputs keep fp32's accuracy.  bf16: features or weights 2^27 times smaller than the largest lose bits in the
-    gradients.  Differentiable once in features, weight and bias.  A step that is recorded into a graph must not share these
-    with a live eager one on the default stream (raises)."""
+    rows left out.  The logits are formed in pieces of the vocabulary, once forward and once backward; sums are fp32 or more,
+    and fp32 inputs keep fp32's accuracy.  In 16 bits the logits' gradients are held in fp16: whole down to 2^-28 of the row's
+    gradient, gone below 2^-39; bf16 features or weights 2^27 times smaller than the largest lose bits in the gradients.
+    Memory beside the results: the features packed (forward to backward), 256 MB or 256 classes for all rows for the
+    backward pass, and for bf16 the weight once more.  Limits: 8388608 rows, 16777216 classes, 16384 dimensions, 16 GiB each of
+    features and weight.  Differentiable once in features, weight and bias.  A step that is recorded into a graph must not
+    share these with a live eager one on the default stream (raises)."""
     if targets.dtype != torch.int64:
         raise TypeError(f"targets must be int64, got {targets.dtype}")
     flat = targets if targets.dim() == 1 else targets.reshape(-1)
